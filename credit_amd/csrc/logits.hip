@@ -1,0 +1,1075 @@
+// Operators on language-model logits z [rows, cols], x = z / temperature:
+// log-probabilities of given tokens with the row's entropy and its most likely
+// alternatives (credit_token_logprob_*), and the divergence from a teacher's
+// top entries (credit_topk_distill_*), each with its gradient.
+//
+// The forwards read the logits once and write a few numbers a row: one
+// streaming pass keeps, per lane, a reference m, s = sum e^(x - m/T) and, for
+// the entropy, t = sum e^(x - m/T) (x - m/T) (in base 2: one v_exp_f32 an
+// element).  The reference is raised only where a term passes it by 2^8, so
+// that the usual batch does no rescaling; floating point keeps the same
+// relative precision wherever the reference lies.  The backwards are
+// elementwise given the forward's row statistics.
+//
+// Rows start at any element address and may be apart by more than cols: a row
+// is read in 16-byte vectors from the 16-byte line that its first element lies
+// in, and the elements of its first and last line that are not its own are
+// masked.
+#include <float.h>
+
+#include <type_traits>
+
+#include "api_internal.hpp"
+#include "common.hpp"
+#include "rows.hpp"
+
+namespace credit {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kNW = kThreads / kWave;
+constexpr int kLane = 32;                     // elements of a lane in a batch
+constexpr int kBatch = kThreads * kLane;      // elements of a workgroup in a batch
+constexpr int kMaxEntries = kThreads;         // tokens, alternatives or teacher entries a row
+constexpr int64_t kMaxCols = int64_t{1} << 29;  // a row's bytes fit 32-bit offsets
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kNaN = __builtin_nanf("");
+constexpr double kLn2 = 0.693147180559945309417232;
+
+template <class T>
+struct Elem;
+template <>
+struct Elem<float> {
+  static constexpr int kN = 4;  // elements of a 16-byte vector
+  __device__ static float get(const float* p) { return *p; }
+  __device__ static void put(float* p, float v) { *p = v; }
+};
+template <>
+struct Elem<uint16_t> {
+  static constexpr int kN = 8;
+  __device__ static float get(const uint16_t* p) { return bf16_to_f32(*p); }
+  __device__ static void put(uint16_t* p, float v) { *p = f32_to_bf16(v); }
+};
+template <class T>
+constexpr int kN = Elem<T>::kN;
+template <class T>
+constexpr int kU = kLane / kN<T>;  // vectors of a lane in a batch
+
+// A row from the start of its first 16-byte line on: element e of the frame is
+// column e - head, and the row's own are those in [head, end).
+struct Frame {
+  buffer_rsrc_t r;
+  int head, end;
+};
+template <class T>
+__device__ __forceinline__ Frame frame_of(const T* row, int cols) {
+  Frame f;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(row);
+  f.head = static_cast<int>((a & 15u) / sizeof(T));
+  f.end = f.head + cols;
+  // Whole dwords: the last one holds the row's last element.
+  f.r = make_rsrc(reinterpret_cast<const void*>(a & ~uintptr_t{15}),
+                  (static_cast<uint32_t>(f.end) * static_cast<uint32_t>(sizeof(T)) + 3u) & ~3u);
+  return f;
+}
+
+template <class T, int N>
+__device__ __forceinline__ void unpack(float (&f)[N * kN<T>], const u32x4 (&v)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t w = v[k][e];
+      if constexpr (std::is_same_v<T, float>) {
+        f[4 * k + e] = __builtin_bit_cast(float, w);
+      } else {
+        f[8 * k + 2 * e] = bf16_lo(w);
+        f[8 * k + 2 * e + 1] = bf16_hi(w);
+      }
+    }
+}
+// Element of the frame: the i-th of this lane in batch b.
+template <class T>
+__device__ __forceinline__ int elem_at(int b, int i) {
+  return ((b * kU<T> + i / kN<T>)*kThreads + static_cast<int>(threadIdx.x)) * kN<T> + i % kN<T>;
+}
+template <class T>
+__device__ __forceinline__ void load_batch(u32x4 (&v)[kU<T>], const Frame& f, int b) {
+#pragma unroll
+  for (int k = 0; k < kU<T>; ++k)
+    v[k] = buffer_load_nt(f.r, ((b * kU<T> + k) * kThreads + threadIdx.x) * 16u);
+}
+// The lane's elements of batch b, -inf in the place of what is not the row's.
+template <class T>
+__device__ __forceinline__ void row_values(float (&z)[kLane], const u32x4 (&v)[kU<T>],
+                                           const Frame& f, int b) {
+  unpack<T, kU<T>>(z, v);
+  if ((b == 0 && f.head != 0) || (b + 1) * kBatch > f.end) {
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) {
+      const int e = elem_at<T>(b, i);
+      z[i] = e >= f.head && e < f.end ? z[i] : kNegInf;
+    }
+  }
+}
+
+// ---------------------------------------------------------- streaming pass --
+// s and t of the values seen, about m in the exponent's base-2 units: s = sum
+// 2^((z - m) c), t = sum 2^((z - m) c) (z - m) c with c = log2(e) / T; mx their
+// maximum (NaN-propagating).
+struct Lane {
+  float m = -FLT_MAX, s = 0.0f, t = 0.0f, mx = kNegInf;
+};
+constexpr float kRaise = 8.0f;  // 2^8 x 2^29 columns is far from overflow
+
+template <bool ENT>
+__device__ __forceinline__ void absorb(Lane& a, const float (&z)[kLane], float c) {
+  float bm = fmax_nan(z[0], z[1]);
+#pragma unroll
+  for (int i = 2; i < kLane; i += 2) bm = fmax_nan(bm, fmax_nan(z[i], z[i + 1]));
+  a.mx = fmax_nan(a.mx, bm);
+  const bool raise = (bm - a.m) * c > kRaise;
+  if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+    const float d = raise ? (a.m - bm) * c : 0.0f;
+    const float f = __builtin_amdgcn_exp2f(d);
+    // s = 0: d may be infinite.
+    if (ENT) a.t = a.s == 0.0f ? 0.0f : f * __builtin_fmaf(d, a.s, a.t);
+    a.s *= f;
+    a.m = raise ? bm : a.m;
+  }
+  float s[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < kLane; ++i) {
+    const float x = (z[i] - a.m) * c;
+    const float e = __builtin_amdgcn_exp2f(x);
+    s[i & 1] += e;
+    // 2^-1000 is 0 as 2^-inf is, and 0 (-1000) is 0.
+    if (ENT) t[i & 1] = __builtin_fmaf(e, __builtin_fmaxf(x, -1000.0f), t[i & 1]);
+  }
+  a.s += s[0] + s[1];
+  if (ENT) a.t += t[0] + t[1];
+}
+
+// The workgroup's lanes joined, about the maximum of them all; every thread has
+// the result.  `slots`: one use between two barriers of the caller.
+struct Joined {
+  float m;
+  double s, t;
+};
+struct JoinSlots {
+  float m[kNW];
+  double st[2][kNW];
+};
+__device__ __forceinline__ Joined join_lanes(const Lane& a, float c, JoinSlots& slots) {
+  Joined j;
+  j.m = rows::block_max<kNW>(a.mx, slots.m);
+  j.s = j.t = 0.0;
+  if (a.s != 0.0f) {  // not of NaN: then s is NaN
+    const float d = (a.m - j.m) * c;
+    const double f = __builtin_amdgcn_exp2f(d);
+    j.s = f * a.s;
+    j.t = f * (static_cast<double>(a.t) + static_cast<double>(d) * a.s);
+    // A lane that is too far below the maximum to count.
+    if (f == 0.0) j.t = 0.0;
+  }
+  if (j.m != j.m) j.s = kNaN;
+  rows::block_sum2<kNW>(j.s, j.t, slots.st);
+  return j;
+}
+
+// ------------------------------------------------------------ the largest --
+// Order of the alternatives: by value, NaN above everything and -0 as 0, equal
+// ones by column.  key: as unsigned, the order of the values.
+__device__ __forceinline__ uint32_t key_of(float z) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, z + 0.0f);
+  const uint32_t k = (u >> 31) != 0 ? ~u : u | 0x80000000u;
+  return z != z ? 0xFFFFFFFFu : k;
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  if (key == 0xFFFFFFFFu) return kNaN;
+  return __builtin_bit_cast(float, (key >> 31) != 0 ? key & 0x7FFFFFFFu : ~key);
+}
+
+constexpr int kBins = 256;
+constexpr int kCands = 1024;
+struct TopSlots {
+  uint32_t hist[kBins];
+  uint64_t cand[kCands];  // key above ~column: larger is nearer the front
+  uint32_t n, bin, above, count;
+  uint32_t wave[kNW];
+};
+
+template <class T, class Fn>
+__device__ __forceinline__ void each_value(const Frame& f, Fn&& fn) {
+  const int vecs = (f.end + kN<T> - 1) / kN<T>;
+  for (int v = threadIdx.x; v < vecs; v += kThreads) {
+    const u32x4 raw[1] = {buffer_load(f.r, static_cast<uint32_t>(v) * 16u)};
+    float z[kN<T>];
+    unpack<T, 1>(z, raw);
+#pragma unroll
+    for (int i = 0; i < kN<T>; ++i) {
+      const int e = v * kN<T> + i;
+      if (e >= f.head && e < f.end) fn(e - f.head, key_of(z[i]));
+    }
+  }
+}
+
+// The bin that holds the `need`-th largest of the histogram (bin 0 the largest)
+// and what lies above it; every thread.
+__device__ __forceinline__ void find_bin(TopSlots& s, uint32_t need) {
+  if (threadIdx.x < kWave) {
+    const int lane = threadIdx.x;
+    uint32_t h[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += h[i] = s.hist[4 * lane + i];
+    uint32_t incl = sum;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+      const uint32_t up = __shfl_up(incl, d);
+      if (lane >= d) incl += up;
+    }
+    uint32_t above = incl - sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (above < need && above + h[i] >= need) {
+        s.bin = 4 * lane + i;
+        s.above = above;
+        s.count = h[i];
+      }
+      above += h[i];
+    }
+  }
+  __syncthreads();
+}
+
+// The `top` largest of the row.  The range that holds the last of them is
+// narrowed by histograms until what is at or above it fits the candidates, or
+// until it is a single value; the candidates are then ranked by counting.
+template <class T>
+__device__ __forceinline__ void write_top(const Frame& f, int top, TopSlots& s, float m, double ln_s,
+                                          float temperature, float* top_logp, int64_t* top_ids) {
+  const auto put = [&](int rank, uint32_t key, int col) {
+    const float z = value_of(key);
+    top_logp[rank] =
+        z == kNegInf && ln_s == ln_s ? kNegInf
+                     : static_cast<float>((static_cast<double>(z) - m) / temperature - ln_s);
+    top_ids[rank] = col;
+  };
+  uint32_t lo = 0, hi = 0xFFFFFFFFu, need = top, above = 0;
+  for (;;) {
+    const int bits = 32 - __builtin_clz((hi - lo) | 1u);
+    const int shift = bits > 8 ? bits - 8 : 0;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.hist[i] = 0;
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    each_value<T>(f, [&](int, uint32_t key) {
+      if (key >= lo && key <= hi) atomicAdd(&s.hist[(hi - key) >> shift], 1u);
+    });
+    __syncthreads();
+    find_bin(s, need);
+    const uint32_t bin = s.bin, in_bin = s.count;
+    above += s.above;
+    need -= s.above;
+    hi -= bin << shift;
+    const uint32_t span = (1u << shift) - 1u;
+    lo = hi - lo > span ? hi - span : lo;
+    __syncthreads();
+    if (above + in_bin <= kCands || lo == hi) {
+      // At or above lo there are above + in_bin values, at least `top`; where
+      // they are too many, lo is a single value and those above it too few.
+      const bool ties = above + in_bin > kCands;
+      each_value<T>(f, [&](int col, uint32_t key) {
+        if (ties ? key > hi : key >= lo)
+          s.cand[atomicAdd(&s.n, 1u)] =
+              static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(col));
+      });
+      __syncthreads();
+      const int n = static_cast<int>(s.n);
+      for (int i = threadIdx.x; i < n; i += kThreads) {
+        const uint64_t mine = s.cand[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += s.cand[j] > mine;
+        if (rank < top)
+          put(rank, static_cast<uint32_t>(mine >> 32),
+              static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(mine)));
+      }
+      if (ties) {
+        // The first columns that hold the value, in order.
+        int found = n;
+        const int vecs = (f.end + kN<T> - 1) / kN<T>;
+        for (int v0 = 0; v0 < vecs && found < top; v0 += kThreads) {
+          const int v = v0 + threadIdx.x;
+          const u32x4 raw[1] = {buffer_load(f.r, static_cast<uint32_t>(v) * 16u)};
+          float z[kN<T>];
+          unpack<T, 1>(z, raw);
+          uint32_t hit = 0;
+#pragma unroll
+          for (int i = 0; i < kN<T>; ++i) {
+            const int e = v * kN<T> + i;
+            if (e >= f.head && e < f.end && key_of(z[i]) == hi) hit |= 1u << i;
+          }
+          const uint32_t mine = __builtin_popcount(hit);
+          uint32_t incl = mine;
+          const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+#pragma unroll
+          for (int d = 1; d < kWave; d *= 2) {
+            const uint32_t up = __shfl_up(incl, d);
+            if (lane >= d) incl += up;
+          }
+          if (lane == kWave - 1) s.wave[wave] = incl;
+          __syncthreads();
+          int at = found + static_cast<int>(incl - mine), all = 0;
+          for (int w = 0; w < kNW; ++w) {
+            if (w < wave) at += s.wave[w];
+            all += s.wave[w];
+          }
+          for (; hit != 0 && at < top; hit &= hit - 1, ++at)
+            put(at, hi, v * kN<T> + __builtin_ctz(hit) - f.head);
+          found += all;
+          __syncthreads();
+        }
+      }
+      return;
+    }
+  }
+}
+
+// -------------------------------------------------------- token log-probs --
+template <class T>
+struct LogprobArgs {
+  const T* logits;
+  int64_t ld;
+  const int64_t* tokens;
+  float* logp;
+  float* stats;
+  float* entropy;
+  float* top_logp;
+  int64_t* top_ids;
+  int cols, n_tokens, n_top;
+  float temperature, c;  // c = log2(e) / temperature
+};
+
+template <class T, bool ENT>
+__device__ __forceinline__ void logprob_outputs(const LogprobArgs<T>& a, int64_t row, const T* z,
+                                                const Joined& j) {
+  const bool empty = j.m == kNegInf;
+  const double ln_s = empty ? 0.0 : ::log(j.s);
+  if (threadIdx.x == 0) {
+    a.stats[2 * row] = j.m;
+    a.stats[2 * row + 1] = static_cast<float>(j.s);
+    if (ENT) a.entropy[row] = empty ? 0.0f : static_cast<float>(ln_s - kLn2 * j.t / j.s);
+  }
+  for (int k = threadIdx.x; k < a.n_tokens; k += kThreads) {
+    const int64_t tok = a.tokens[row * a.n_tokens + k];
+    float lp = 0.0f;
+    if (tok >= a.cols) {
+      lp = kNaN;
+    } else if (tok >= 0) {
+      const float v = Elem<T>::get(z + tok);
+      lp = v == kNegInf && ln_s == ln_s
+               ? kNegInf
+               : static_cast<float>((static_cast<double>(v) - j.m) / a.temperature - ln_s);
+    }
+    a.logp[row * a.n_tokens + k] = lp;
+  }
+}
+
+template <class T, bool ENT, bool TOP>
+__global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs<T> a) {
+  __shared__ JoinSlots join;
+  const int64_t row = blockIdx.x;
+  const T* z = a.logits + row * a.ld;
+  const Frame f = frame_of(z, a.cols);
+  const int batches = (f.end + kBatch - 1) / kBatch;
+  Lane lane;
+  u32x4 v[kU<T>];
+  load_batch<T>(v, f, 0);
+  for (int b = 0; b < batches; ++b) {
+    u32x4 next[kU<T>];
+    load_batch<T>(next, f, b + 1);  // past the row: zeros, no access
+    float x[kLane];
+    row_values<T>(x, v, f, b);
+    absorb<ENT>(lane, x, a.c);
+#pragma unroll
+    for (int k = 0; k < kU<T>; ++k) v[k] = next[k];
+  }
+  const Joined j = join_lanes(lane, a.c, join);
+  logprob_outputs<T, ENT>(a, row, z, j);
+  if constexpr (TOP) {
+    __shared__ TopSlots top;
+    write_top<T>(f, a.n_top, top, j.m, j.m == kNegInf ? 0.0 : ::log(j.s), a.temperature,
+                 a.top_logp + row * a.n_top, a.top_ids + row * a.n_top);
+  }
+}
+
+// ------------------------------------------------------------- gradients --
+// A workgroup writes kGradVecs vectors a lane of a row's gradient.  The entries
+// that a row names (its tokens, the teacher's columns) get the elementwise
+// value like all others and then, once those stores are in memory, their own.
+constexpr int kGradVecs = 4;
+template <class T>
+constexpr int kGradBatch = kThreads * kGradVecs * kN<T>;
+
+// Stores the row's own elements of a vector; VEC: in and out lie alike in their
+// 16-byte lines.
+template <class T, bool VEC>
+__device__ __forceinline__ void store_grad(T* row, const Frame& f, int e, const float (&g)[kN<T>]) {
+  if (VEC && e >= f.head && e + kN<T> <= f.end) {
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, float>)
+        v[i] = __builtin_bit_cast(uint32_t, g[i]);
+      else
+        v[i] = pack_bf16x2(g[2 * i], g[2 * i + 1]);
+    }
+    store_nt(reinterpret_cast<u32x4*>(row + (e - f.head)), v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kN<T>; ++i)
+      if (e + i >= f.head && e + i < f.end) Elem<T>::put(row + (e + i - f.head), g[i]);
+  }
+}
+
+// value(z) over the workgroup's part of the row, z not read where `zero`.
+template <class T, bool VEC, class Fn>
+__device__ __forceinline__ void write_grad(const Frame& f, T* out, int part, bool zero,
+                                           Fn&& value) {
+  const int v0 = part * kGradVecs * kThreads + static_cast<int>(threadIdx.x);
+  u32x4 v[kGradVecs] = {};
+  if (!zero) {
+#pragma unroll
+    for (int k = 0; k < kGradVecs; ++k)
+      v[k] = buffer_load_nt(f.r, static_cast<uint32_t>(v0 + k * kThreads) * 16u);
+  }
+#pragma unroll
+  for (int k = 0; k < kGradVecs; ++k) {
+    const u32x4 raw[1] = {v[k]};
+    float g[kN<T>];
+    if (zero) {
+#pragma unroll
+      for (int i = 0; i < kN<T>; ++i) g[i] = 0.0f;
+    } else {
+      unpack<T, 1>(g, raw);
+#pragma unroll
+      for (int i = 0; i < kN<T>; ++i) g[i] = value(g[i]);
+    }
+    store_grad<T, VEC>(out, f, (v0 + k * kThreads) * kN<T>, g);
+  }
+}
+
+// Stores of this wave are in memory, then the workgroup meets.
+__device__ __forceinline__ void memory_barrier() {
+  publish_wait();
+  lds_barrier();
+}
+
+template <class T>
+struct LogprobGradArgs {
+  const T* logits;
+  int64_t ld;
+  const int64_t* tokens;
+  const float* stats;
+  const float* entropy;
+  const float* dlogp;
+  const float* dentropy;
+  T* dlogits;
+  int64_t ldd;
+  int64_t rows;
+  int cols, n_tokens;
+  float inv_t, c;
+};
+
+template <class T, bool ENT, bool VEC>
+__global__ __launch_bounds__(kThreads) void token_logprob_bwd_kernel(LogprobGradArgs<T> a) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int part = blockIdx.x;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const T* z = a.logits + row * a.ld;
+    T* out = a.dlogits + row * a.ldd;
+    const Frame f = frame_of(z, a.cols);
+    const int first = part * kGradBatch<T> - f.head;  // the part's first column
+    if (first >= a.cols) continue;
+    const int64_t* tokens = a.tokens + row * a.n_tokens;
+    const float* dlogp = a.dlogp + row * a.n_tokens;
+    // Every wave by itself: the tokens' weight, and whether one lies here.
+    double weight = 0.0;
+    bool live = false, here = false;
+    for (int k = lane; k < a.n_tokens; k += kWave) {
+      const int64_t tok = tokens[k];
+      const float g = dlogp[k];
+      if (tok < 0 || g == 0.0f) continue;
+      live = true;
+      weight += tok >= a.cols ? kNaN : g;
+      here |= tok < a.cols && tok >= first && tok - first < kGradBatch<T>;
+    }
+    const float gsum = static_cast<float>(wave_reduce_sum_f64(weight));
+    live = __builtin_amdgcn_ballot_w64(live) != 0;
+    here = __builtin_amdgcn_ballot_w64(here) != 0;
+    const float m = a.stats[2 * row], s = a.stats[2 * row + 1];
+    const float h = ENT ? a.dentropy[row] : 0.0f;
+    // dz = e^(x - m/T) (A + B log2 e^(x - m/T)).
+    const float k = a.inv_t / s;
+    float A = gsum, B = 0.0f;
+    if (ENT && h != 0.0f) {
+      live = true;
+      A += h * (a.entropy[row] - ::logf(s));
+      B = -h * static_cast<float>(kLn2) * k;
+    }
+    A *= -k;
+    const bool zero = !live || m == kNegInf;
+    const auto value = [&](float v) {
+      const float x = (v - m) * a.c;
+      const float e = __builtin_amdgcn_exp2f(x);
+      return ENT ? e * __builtin_fmaf(B, __builtin_fmaxf(x, -1000.0f), A) : e * A;
+    };
+    float own = 0.0f;
+    const bool patch = here && !zero;
+    const int mine = threadIdx.x < a.n_tokens ? static_cast<int>(threadIdx.x) : -1;
+    int64_t col = -1;
+    if (patch) {
+      if (mine >= 0) {
+        const int64_t tok = tokens[mine];
+        if (tok >= 0 && tok < a.cols && tok >= first && tok - first < kGradBatch<T>) {
+          col = tok;
+          double g = 0.0;
+          for (int j = 0; j < a.n_tokens; ++j)
+            if (tokens[j] == tok) g += dlogp[j];
+          own = static_cast<float>(g) * a.inv_t + value(Elem<T>::get(z + tok));
+        }
+      }
+      memory_barrier();  // dlogits may be logits: read before anything is written
+    }
+    write_grad<T, VEC>(f, out, part, zero, value);
+    if (patch) {
+      memory_barrier();
+      if (col >= 0) Elem<T>::put(out + col, own);
+    }
+  }
+}
+
+// ------------------------------------------------------------ distillation --
+// Columns of the frame that a row's entries name, a bit each, for the batches
+// of one segment: bit i of word (b, lane) is the lane's i-th element of batch b.
+constexpr int kSegBatches = 32;
+constexpr int kSegWords = kSegBatches * kThreads;
+
+template <class T>
+struct DistillArgs {
+  const T* logits;
+  int64_t ld;
+  const int64_t* ids;
+  const float* teacher;
+  float* loss;
+  float* stats;
+  int cols, n_top;
+  float temperature, c;
+};
+// Row statistics [rows, 8] for the backward.
+enum DistillStat { kMax, kSum, kTailMax, kTailSum, kMass, kTailGrad, kTeacherLse, kUnused };
+
+template <class T>
+__device__ __forceinline__ void mark(uint32_t* bits, int e, int seg) {
+  const int v = e / kN<T>;
+  const int b = v / (kThreads * kU<T>) - seg * kSegBatches;
+  if (b < 0 || b >= kSegBatches) return;
+  const int i = v / kThreads % kU<T> * kN<T> + e % kN<T>;
+  atomicOr(&bits[b * kThreads + v % kThreads], 1u << i);
+}
+
+template <class T, bool TAIL>
+__global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<T> a) {
+  __shared__ JoinSlots join;
+  __shared__ float max_slots[2][kNW];
+  __shared__ double sum_slots[4][2][kNW];
+  __shared__ int flags[kNW];
+  __shared__ int id_list[kMaxEntries];
+  const int64_t row = blockIdx.x;
+  const T* z = a.logits + row * a.ld;
+  const int k = threadIdx.x;
+  // The thread's entry.
+  int64_t id = -1;
+  float t = kNegInf;
+  if (k < a.n_top) {
+    id = a.ids[row * a.n_top + k];
+    t = a.teacher[row * a.n_top + k];
+  }
+  const bool live = id >= 0;
+  const bool bad = id >= a.cols;
+  id_list[k] = live && !bad ? static_cast<int>(id) : -1;
+  const uint64_t any_live = __builtin_amdgcn_ballot_w64(live);
+  const uint64_t any_bad = __builtin_amdgcn_ballot_w64(bad);
+  if ((threadIdx.x & (kWave - 1)) == 0)
+    flags[threadIdx.x / kWave] = (any_live != 0) | (any_bad != 0) << 1;
+  // The teacher's largest value (renormalised entries).
+  const float tm = rows::block_max<kNW>(live ? t : kNegInf, max_slots[0]);
+  int flag = 0;
+  for (int w = 0; w < kNW; ++w) flag |= flags[w];
+  float* stats = a.stats + 8 * row;
+  if ((flag & 1) == 0 || (!TAIL && tm == kNegInf)) {  // no entry to learn from
+    if (threadIdx.x == 0) a.loss[row] = 0.0f;
+    if (threadIdx.x < 8) stats[threadIdx.x] = 0.0f;
+    return;
+  }
+  const float zk = live && !bad ? Elem<T>::get(z + id) : kNegInf;
+
+  const Frame f = frame_of(z, a.cols);
+  const int batches = (f.end + kBatch - 1) / kBatch;
+  Lane lane;
+  if constexpr (TAIL) {
+    __shared__ uint32_t bits[kSegWords];
+    for (int seg = 0; seg * kSegBatches < batches; ++seg) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < kSegWords; i += kThreads) bits[i] = 0;
+      __syncthreads();
+      if (live && !bad) mark<T>(bits, static_cast<int>(id) + f.head, seg);
+      __syncthreads();
+      const int last = (seg + 1) * kSegBatches < batches ? (seg + 1) * kSegBatches : batches;
+      for (int b = seg * kSegBatches; b < last; ++b) {
+        u32x4 v[kU<T>];
+        load_batch<T>(v, f, b);
+        float x[kLane];
+        row_values<T>(x, v, f, b);
+        const uint32_t w = bits[(b - seg * kSegBatches) * kThreads + threadIdx.x];
+        if (__builtin_amdgcn_ballot_w64(w != 0) != 0) {
+#pragma unroll
+          for (int i = 0; i < kLane; ++i) x[i] = (w >> i & 1u) != 0 ? kNegInf : x[i];
+        }
+        absorb<false>(lane, x, a.c);
+      }
+    }
+  } else {
+    for (int b = 0; b < batches; ++b) {
+      u32x4 v[kU<T>];
+      load_batch<T>(v, f, b);
+      float x[kLane];
+      row_values<T>(x, v, f, b);
+      absorb<false>(lane, x, a.c);
+    }
+  }
+  const Joined j = join_lanes(lane, a.c, join);
+
+  // The row's maximum and sum; `tail` what the entries leave.
+  float m = j.m;
+  double s = j.s;
+  if constexpr (TAIL) {
+    m = fmax_nan(j.m, rows::block_max<kNW>(zk, max_slots[1]));
+    // Of entries that name one column the first counts.
+    bool first = live && !bad;
+    for (int i = 0; i < k && first; ++i) first = id_list[i] != static_cast<int>(id);
+    double e = 0.0, none = 0.0;
+    if (first && zk != kNegInf) e = ::exp((static_cast<double>(zk) - m) / a.temperature);
+    rows::block_sum2<kNW>(e, none, sum_slots[0]);
+    s = e;
+    if (j.s != 0.0) s += j.s * ::exp((static_cast<double>(j.m) - m) / a.temperature);
+  }
+  const bool empty = m == kNegInf;
+  const double ln_s = empty ? 0.0 : ::log(s);
+  // The teacher.
+  double ln_q = kNegInf, lse = 0.0;
+  if constexpr (TAIL) {
+    if (live) ln_q = t;
+  } else {
+    double total = 0.0, none = 0.0;
+    if (live) total = ::exp((static_cast<double>(t) - tm) / a.temperature);
+    rows::block_sum2<kNW>(total, none, sum_slots[1]);
+    lse = static_cast<double>(tm) / a.temperature + ::log(total);
+    if (live) ln_q = static_cast<double>(t) / a.temperature - lse;
+  }
+  double q = live ? ::exp(ln_q) : 0.0;
+  double loss = 0.0;
+  if (q != 0.0) {
+    const double ln_p = zk == kNegInf && ln_s == ln_s
+                            ? static_cast<double>(kNegInf)
+                            : (static_cast<double>(zk) - m) / a.temperature - ln_s;
+    loss = q * (ln_q - ln_p);
+  }
+  rows::block_sum2<kNW>(q, loss, sum_slots[2]);
+  double rest = 0.0, tail_grad = 0.0;
+  if constexpr (TAIL) {
+    rest = q < 1.0 ? 1.0 - q : (q == q ? 0.0 : q);
+    double share = 0.0;
+    // A tail without mass (every other column masked) adds nothing.
+    if (j.s != 0.0) {
+      const double ln_tail = (static_cast<double>(j.m) - m) / a.temperature + ::log(j.s) - ln_s;
+      share = ::exp(ln_tail);
+      if (rest != 0.0) loss += rest * (::log(rest) - ln_tail);
+    }
+    tail_grad = (q + rest) * share - rest;
+  }
+  if ((flag & 2) != 0) loss = q = kNaN;
+  if (threadIdx.x == 0) {
+    a.loss[row] = static_cast<float>(loss);
+    stats[kMax] = m;
+    stats[kSum] = static_cast<float>(s);
+    stats[kTailMax] = TAIL ? j.m : 0.0f;
+    stats[kTailSum] = TAIL ? static_cast<float>(j.s) : 0.0f;
+    stats[kMass] = static_cast<float>(q + rest);
+    stats[kTailGrad] = static_cast<float>((flag & 2) != 0 ? kNaN : tail_grad);
+    stats[kTeacherLse] = static_cast<float>(lse);
+    stats[kUnused] = 0.0f;
+  }
+}
+
+template <class T>
+struct DistillGradArgs {
+  const T* logits;
+  int64_t ld;
+  const int64_t* ids;
+  const float* teacher;
+  const float* stats;
+  const float* dloss;
+  T* dlogits;
+  int64_t ldd;
+  int64_t rows;
+  int cols, n_top;
+  float inv_t, c;
+};
+
+template <class T, bool TAIL, bool VEC>
+__global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradArgs<T> a) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int part = blockIdx.x;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const T* z = a.logits + row * a.ld;
+    T* out = a.dlogits + row * a.ldd;
+    const Frame f = frame_of(z, a.cols);
+    const int first = part * kGradBatch<T> - f.head;
+    if (first >= a.cols) continue;
+    const int64_t* ids = a.ids + row * a.n_top;
+    const float* teacher = a.teacher + row * a.n_top;
+    bool live = false, here = false;
+    for (int k = lane; k < a.n_top; k += kWave) {
+      const int64_t id = ids[k];
+      live |= id >= 0;
+      here |= id >= 0 && id < a.cols && id >= first && id - first < kGradBatch<T>;
+    }
+    live = __builtin_amdgcn_ballot_w64(live) != 0;
+    here = __builtin_amdgcn_ballot_w64(here) != 0;
+    const float* st = a.stats + 8 * row;
+    const float m = st[kMax], s = st[kSum], mass = st[kMass];
+    const float g = a.dloss[row] * a.inv_t;
+    const bool zero = !live || g == 0.0f || mass == 0.0f || m == kNegInf;
+    float ref = m, A = g * mass / s;
+    if (TAIL) {
+      const bool some = st[kTailSum] != 0.0f;  // else every column is named or without mass
+      ref = some ? st[kTailMax] : m;
+      A = some ? g * st[kTailGrad] / st[kTailSum] : g * st[kTailGrad];
+    }
+    const auto value = [&](float v) {
+      return __builtin_amdgcn_exp2f((v - ref) * a.c) * A;
+    };
+    const bool patch = here && !zero;
+    const int mine = threadIdx.x < a.n_top ? static_cast<int>(threadIdx.x) : -1;
+    int64_t col = -1;
+    float own = 0.0f;
+    if (patch) {
+      if (mine >= 0) {
+        const int64_t id = ids[mine];
+        if (id >= 0 && id < a.cols && id >= first && id - first < kGradBatch<T>) {
+          col = id;
+          float q = 0.0f;
+          for (int j = 0; j < a.n_top; ++j)
+            if (ids[j] == id)
+              q += exp_accurate(TAIL ? teacher[j] : teacher[j] * a.inv_t - st[kTeacherLse]);
+          const float p = exp_accurate((Elem<T>::get(z + id) - m) * a.inv_t) / s;
+          own = g * (mass * p - q);
+        }
+      }
+      memory_barrier();  // dlogits may be logits: read before anything is written
+    }
+    write_grad<T, VEC>(f, out, part, zero, value);
+    if (patch) {
+      memory_barrier();
+      if (col >= 0) Elem<T>::put(out + col, own);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host ----
+int check_logits(const void* p, const char* name, int64_t ld, int64_t rows, int64_t cols,
+                 size_t elem) {
+  CREDIT_TRY(check_row_ptr(p, name, rows));
+  CREDIT_TRY(check_aligned(p, elem, name));
+  if (rows > 1 && ld < cols)
+    return set_error(CREDIT_ERR_BAD_SHAPE, "%s: rows of %lld columns are %lld elements apart",
+                     name, static_cast<long long>(cols), static_cast<long long>(ld));
+  if (rows > 1 && ld > (int64_t{1} << 62) / (rows * 4))
+    return set_error(CREDIT_ERR_BAD_SHAPE, "%s: %lld rows %lld elements apart", name,
+                     static_cast<long long>(rows), static_cast<long long>(ld));
+  return CREDIT_OK;
+}
+int check_entries(int32_t n, int32_t least, int64_t most, const char* what) {
+  if (n < least || n > most)
+    return set_error(CREDIT_ERR_BAD_SHAPE, "%d %s a row: need %d to %lld", n, what, least,
+                     static_cast<long long>(most));
+  return CREDIT_OK;
+}
+int check_temperature(float t) {
+  if (!(t >= 1e-4f && t <= 1e4f))
+    return set_error(CREDIT_ERR_BAD_CONFIG, "temperature %g outside [1e-4, 1e4]",
+                     static_cast<double>(t));
+  return CREDIT_OK;
+}
+int check_variant(const credit_cfg* cfg) {
+  CREDIT_TRY(check_cfg(cfg));
+  const int v = cfg_variant(cfg);
+  if (v != CREDIT_VARIANT_AUTO && v != CREDIT_VARIANT_READ)
+    return set_error(CREDIT_ERR_UNSUPPORTED, "the logits operators have no variant %d", v);
+  return CREDIT_OK;
+}
+float log2e_over(float temperature) {
+  return static_cast<float>(1.44269504088896340736 / static_cast<double>(temperature));
+}
+// Whether rows of in and out lie alike in their 16-byte lines.
+bool alike(const void* in, int64_t ld, const void* out, int64_t ldd, int64_t rows, size_t elem) {
+  const uintptr_t d = reinterpret_cast<uintptr_t>(in) - reinterpret_cast<uintptr_t>(out);
+  return d % 16 == 0 && (rows == 1 || (ld - ldd) * static_cast<int64_t>(elem) % 16 == 0);
+}
+// In place, or apart: a workgroup's part of one may not be another's of the other.
+int check_overlap(const void* in, int64_t ld, const void* out, int64_t ldd, int64_t rows,
+                  int64_t cols, size_t elem) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(in), b = reinterpret_cast<uintptr_t>(out);
+  if (a == b && (rows == 1 || ld == ldd)) return CREDIT_OK;
+  const uintptr_t na = ((rows - 1) * ld + cols) * elem, nb = ((rows - 1) * ldd + cols) * elem;
+  if (a < b + nb && b < a + na)
+    return set_error(CREDIT_ERR_BAD_CONFIG, "dlogits overlaps logits without being it");
+  return CREDIT_OK;
+}
+template <class T>
+dim3 grad_grid(int64_t rows, int64_t cols) {
+  const int64_t parts = (cols + kN<T> - 1 + kGradBatch<T> - 1) / kGradBatch<T>;
+  return dim3(static_cast<unsigned>(parts), static_cast<unsigned>(rows < 65535 ? rows : 65535));
+}
+
+template <class T>
+int logprob_fwd(const T* logits, int64_t ld, const int64_t* tokens, float* logp, float* stats,
+                float* entropy, float* top_logp, int64_t* top_ids, int64_t rows, int64_t cols,
+                int32_t n_tokens, int32_t n_top, float temperature, const credit_cfg* cfg) {
+  CREDIT_TRY(check_shape(rows, cols, kMaxCols));
+  CREDIT_TRY(check_logits(logits, "logits", ld, rows, cols, sizeof(T)));
+  CREDIT_TRY(check_entries(n_tokens, 0, kMaxEntries, "tokens"));
+  CREDIT_TRY(check_entries(n_top, 0, cols < kMaxEntries ? cols : kMaxEntries, "alternatives"));
+  CREDIT_TRY(check_row_ptr(stats, "stats", rows));
+  if (n_tokens > 0) {
+    CREDIT_TRY(check_row_ptr(tokens, "tokens", rows));
+    CREDIT_TRY(check_row_ptr(logp, "logp", rows));
+  }
+  if (n_top > 0) {
+    CREDIT_TRY(check_row_ptr(top_logp, "top_logp", rows));
+    CREDIT_TRY(check_row_ptr(top_ids, "top_ids", rows));
+  }
+  CREDIT_TRY(check_temperature(temperature));
+  CREDIT_TRY(check_variant(cfg));
+  if (rows == 0) return CREDIT_OK;
+  const LogprobArgs<T> a{logits,
+                         ld,
+                         tokens,
+                         logp,
+                         stats,
+                         entropy,
+                         top_logp,
+                         top_ids,
+                         static_cast<int>(cols),
+                         n_tokens,
+                         n_top,
+                         temperature,
+                         log2e_over(temperature)};
+  const unsigned grid = static_cast<unsigned>(rows);
+  hipStream_t stream = cfg_stream(cfg);
+  const auto launch = [&](auto ent, auto top) {
+    token_logprob_fwd_kernel<T, decltype(ent)::value, decltype(top)::value>
+        <<<grid, kThreads, 0, stream>>>(a);
+  };
+  const auto with_top = [&](auto ent) {
+    n_top > 0 ? launch(ent, std::true_type{}) : launch(ent, std::false_type{});
+  };
+  entropy != nullptr ? with_top(std::true_type{}) : with_top(std::false_type{});
+  return check_launch("token_logprob_fwd_kernel");
+}
+
+template <class T>
+int logprob_bwd(const T* logits, int64_t ld, const int64_t* tokens, const float* stats,
+                const float* entropy, const float* dlogp, const float* dentropy, T* dlogits,
+                int64_t ldd, int64_t rows, int64_t cols, int32_t n_tokens, float temperature,
+                const credit_cfg* cfg) {
+  CREDIT_TRY(check_shape(rows, cols, kMaxCols));
+  CREDIT_TRY(check_logits(logits, "logits", ld, rows, cols, sizeof(T)));
+  CREDIT_TRY(check_logits(dlogits, "dlogits", ldd, rows, cols, sizeof(T)));
+  CREDIT_TRY(check_entries(n_tokens, 0, kMaxEntries, "tokens"));
+  CREDIT_TRY(check_row_ptr(stats, "stats", rows));
+  if (n_tokens > 0) {
+    CREDIT_TRY(check_row_ptr(tokens, "tokens", rows));
+    CREDIT_TRY(check_row_ptr(dlogp, "dlogp", rows));
+  }
+  if (dentropy != nullptr) CREDIT_TRY(check_row_ptr(entropy, "entropy", rows));
+  CREDIT_TRY(check_temperature(temperature));
+  CREDIT_TRY(check_variant(cfg));
+  if (rows == 0) return CREDIT_OK;
+  CREDIT_TRY(check_overlap(logits, ld, dlogits, ldd, rows, cols, sizeof(T)));
+  const LogprobGradArgs<T> a{logits,
+                             ld,
+                             tokens,
+                             stats,
+                             entropy,
+                             dlogp,
+                             dentropy,
+                             dlogits,
+                             ldd,
+                             rows,
+                             static_cast<int>(cols),
+                             n_tokens,
+                             1.0f / temperature,
+                             log2e_over(temperature)};
+  hipStream_t stream = cfg_stream(cfg);
+  const dim3 grid = grad_grid<T>(rows, cols);
+  const auto launch = [&](auto ent, auto vec) {
+    token_logprob_bwd_kernel<T, decltype(ent)::value, decltype(vec)::value>
+        <<<grid, kThreads, 0, stream>>>(a);
+  };
+  const bool vec = alike(logits, ld, dlogits, ldd, rows, sizeof(T));
+  const auto with_vec = [&](auto ent) {
+    vec ? launch(ent, std::true_type{}) : launch(ent, std::false_type{});
+  };
+  dentropy != nullptr ? with_vec(std::true_type{}) : with_vec(std::false_type{});
+  return check_launch("token_logprob_bwd_kernel");
+}
+
+template <class T>
+int distill_fwd(const T* logits, int64_t ld, const int64_t* ids, const float* teacher, float* loss,
+                float* stats, int64_t rows, int64_t cols, int32_t n_top, int32_t tail,
+                float temperature, const credit_cfg* cfg) {
+  CREDIT_TRY(check_shape(rows, cols, kMaxCols));
+  CREDIT_TRY(check_logits(logits, "logits", ld, rows, cols, sizeof(T)));
+  CREDIT_TRY(check_entries(n_top, 1, kMaxEntries, "teacher entries"));
+  CREDIT_TRY(check_row_ptr(ids, "teacher_ids", rows));
+  CREDIT_TRY(check_row_ptr(teacher, "teacher", rows));
+  CREDIT_TRY(check_row_ptr(loss, "loss", rows));
+  CREDIT_TRY(check_row_ptr(stats, "stats", rows));
+  CREDIT_TRY(check_temperature(temperature));
+  CREDIT_TRY(check_variant(cfg));
+  if (rows == 0) return CREDIT_OK;
+  const DistillArgs<T> a{logits, ld,    ids, teacher,     loss, stats, static_cast<int>(cols),
+                         n_top,  temperature, log2e_over(temperature)};
+  const unsigned grid = static_cast<unsigned>(rows);
+  hipStream_t stream = cfg_stream(cfg);
+  if (tail != 0)
+    topk_distill_fwd_kernel<T, true><<<grid, kThreads, 0, stream>>>(a);
+  else
+    topk_distill_fwd_kernel<T, false><<<grid, kThreads, 0, stream>>>(a);
+  return check_launch("topk_distill_fwd_kernel");
+}
+
+template <class T>
+int distill_bwd(const T* logits, int64_t ld, const int64_t* ids, const float* teacher,
+                const float* stats, const float* dloss, T* dlogits, int64_t ldd, int64_t rows,
+                int64_t cols, int32_t n_top, int32_t tail, float temperature,
+                const credit_cfg* cfg) {
+  CREDIT_TRY(check_shape(rows, cols, kMaxCols));
+  CREDIT_TRY(check_logits(logits, "logits", ld, rows, cols, sizeof(T)));
+  CREDIT_TRY(check_logits(dlogits, "dlogits", ldd, rows, cols, sizeof(T)));
+  CREDIT_TRY(check_entries(n_top, 1, kMaxEntries, "teacher entries"));
+  CREDIT_TRY(check_row_ptr(ids, "teacher_ids", rows));
+  CREDIT_TRY(check_row_ptr(teacher, "teacher", rows));
+  CREDIT_TRY(check_row_ptr(stats, "stats", rows));
+  CREDIT_TRY(check_row_ptr(dloss, "dloss", rows));
+  CREDIT_TRY(check_temperature(temperature));
+  CREDIT_TRY(check_variant(cfg));
+  if (rows == 0) return CREDIT_OK;
+  CREDIT_TRY(check_overlap(logits, ld, dlogits, ldd, rows, cols, sizeof(T)));
+  const DistillGradArgs<T> a{logits,
+                             ld,
+                             ids,
+                             teacher,
+                             stats,
+                             dloss,
+                             dlogits,
+                             ldd,
+                             rows,
+                             static_cast<int>(cols),
+                             n_top,
+                             1.0f / temperature,
+                             log2e_over(temperature)};
+  hipStream_t stream = cfg_stream(cfg);
+  const dim3 grid = grad_grid<T>(rows, cols);
+  const auto launch = [&](auto has_tail, auto vec) {
+    topk_distill_bwd_kernel<T, decltype(has_tail)::value, decltype(vec)::value>
+        <<<grid, kThreads, 0, stream>>>(a);
+  };
+  const bool vec = alike(logits, ld, dlogits, ldd, rows, sizeof(T));
+  const auto with_vec = [&](auto has_tail) {
+    vec ? launch(has_tail, std::true_type{}) : launch(has_tail, std::false_type{});
+  };
+  tail != 0 ? with_vec(std::true_type{}) : with_vec(std::false_type{});
+  return check_launch("topk_distill_bwd_kernel");
+}
+
+}  // namespace
+}  // namespace credit
+
+using namespace credit;
+
+extern "C" {
+
+int credit_token_logprob_fwd_f32(const float* logits, int64_t ld, const int64_t* tokens,
+                                 float* logp, float* stats, float* entropy, float* top_logp,
+                                 int64_t* top_ids, int64_t rows, int64_t cols, int32_t n_tokens,
+                                 int32_t n_top, float temperature, const credit_cfg* cfg) {
+  return logprob_fwd(logits, ld, tokens, logp, stats, entropy, top_logp, top_ids, rows, cols,
+                     n_tokens, n_top, temperature, cfg);
+}
+int credit_token_logprob_fwd_bf16(const uint16_t* logits, int64_t ld, const int64_t* tokens,
+                                  float* logp, float* stats, float* entropy, float* top_logp,
+                                  int64_t* top_ids, int64_t rows, int64_t cols, int32_t n_tokens,
+                                  int32_t n_top, float temperature, const credit_cfg* cfg) {
+  return logprob_fwd(logits, ld, tokens, logp, stats, entropy, top_logp, top_ids, rows, cols,
+                     n_tokens, n_top, temperature, cfg);
+}
+int credit_token_logprob_bwd_f32(const float* logits, int64_t ld, const int64_t* tokens,
+                                 const float* stats, const float* entropy, const float* dlogp,
+                                 const float* dentropy, float* dlogits, int64_t ldd, int64_t rows,
+                                 int64_t cols, int32_t n_tokens, float temperature,
+                                 const credit_cfg* cfg) {
+  return logprob_bwd(logits, ld, tokens, stats, entropy, dlogp, dentropy, dlogits, ldd, rows, cols,
+                     n_tokens, temperature, cfg);
+}
+int credit_token_logprob_bwd_bf16(const uint16_t* logits, int64_t ld, const int64_t* tokens,
+                                  const float* stats, const float* entropy, const float* dlogp,
+                                  const float* dentropy, uint16_t* dlogits, int64_t ldd,
+                                  int64_t rows, int64_t cols, int32_t n_tokens, float temperature,
+                                  const credit_cfg* cfg) {
+  return logprob_bwd(logits, ld, tokens, stats, entropy, dlogp, dentropy, dlogits, ldd, rows, cols,
+                     n_tokens, temperature, cfg);
+}
+int credit_topk_distill_fwd_f32(const float* logits, int64_t ld, const int64_t* teacher_ids,
+                                const float* teacher, float* loss, float* stats, int64_t rows,
+                                int64_t cols, int32_t n_top, int32_t tail, float temperature,
+                                const credit_cfg* cfg) {
+  return distill_fwd(logits, ld, teacher_ids, teacher, loss, stats, rows, cols, n_top, tail,
+                     temperature, cfg);
+}
+int credit_topk_distill_fwd_bf16(const uint16_t* logits, int64_t ld, const int64_t* teacher_ids,
+                                 const float* teacher, float* loss, float* stats, int64_t rows,
+                                 int64_t cols, int32_t n_top, int32_t tail, float temperature,
+                                 const credit_cfg* cfg) {
+  return distill_fwd(logits, ld, teacher_ids, teacher, loss, stats, rows, cols, n_top, tail,
+                     temperature, cfg);
+}
+int credit_topk_distill_bwd_f32(const float* logits, int64_t ld, const int64_t* teacher_ids,
+                                const float* teacher, const float* stats, const float* dloss,
+                                float* dlogits, int64_t ldd, int64_t rows, int64_t cols,
+                                int32_t n_top, int32_t tail, float temperature,
+                                const credit_cfg* cfg) {
+  return distill_bwd(logits, ld, teacher_ids, teacher, stats, dloss, dlogits, ldd, rows, cols,
+                     n_top, tail, temperature, cfg);
+}
+int credit_topk_distill_bwd_bf16(const uint16_t* logits, int64_t ld, const int64_t* teacher_ids,
+                                 const float* teacher, const float* stats, const float* dloss,
+                                 uint16_t* dlogits, int64_t ldd, int64_t rows, int64_t cols,
+                                 int32_t n_top, int32_t tail, float temperature,
+                                 const credit_cfg* cfg) {
+  return distill_bwd(logits, ld, teacher_ids, teacher, stats, dloss, dlogits, ldd, rows, cols,
+                     n_top, tail, temperature, cfg);
+}
+
+}  // extern "C"

@@ -58,6 +58,10 @@ OPS = {
     "weighted_var_backward": 13,
     "pearson_backward": 14,
     "rmsnorm_fwd_bwd": 15,
+    "token_logprob_fwd": 16,
+    "token_logprob_bwd": 17,
+    "topk_distill_fwd": 18,
+    "topk_distill_bwd": 19,
 }
 
 
@@ -103,6 +107,7 @@ class DeviceInfo(ctypes.Structure):
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
+_I32 = ctypes.c_int32
 _F = ctypes.c_float
 _CFG = ctypes.POINTER(CreditCfg)
 
@@ -124,6 +129,14 @@ SIGNATURES: dict[str, list] = {
     "credit_softmax_fwd_f32": [_P, _P, _P, _P, _I64, _I64, _CFG],
     "credit_softmax_bwd_f32": [_P, _P, _P, _I64, _I64, _CFG],
     "credit_softmax_logits_bwd_f32": [_P, _P, _P, _I64, _I64, _CFG],
+    **{f"credit_token_logprob_fwd_{t}": [_P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32,
+                                         _F, _CFG] for t in ("f32", "bf16")},
+    **{f"credit_token_logprob_bwd_{t}": [_P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32,
+                                         _F, _CFG] for t in ("f32", "bf16")},
+    **{f"credit_topk_distill_fwd_{t}": [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _F,
+                                        _CFG] for t in ("f32", "bf16")},
+    **{f"credit_topk_distill_bwd_{t}": [_P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32,
+                                        _I32, _F, _CFG] for t in ("f32", "bf16")},
     "credit_rowwise_quant_f32": [_P, _P, _P, _I64, _I64, _CFG],
     "credit_lars_momentum_f32": [_P, _P, _P, _P, _P, _I64, _I64, _CFG],
     "credit_weighted_var_bwd_f32": [_P, _P, _P, _P, _I64, _I64, _F, _CFG],
@@ -237,6 +250,14 @@ def make_cfg(
         cfg.workspace = workspace.data_ptr()
         cfg.workspace_bytes = workspace.numel() * workspace.element_size()
     return cfg
+
+
+def _cfg_ref(cfg: CreditCfg | None, device: int):
+    """The cfg argument of a call: the caller's, or the current stream alone."""
+    if cfg is None:
+        cfg = CreditCfg()
+        cfg.stream = torch.cuda.current_stream(device).cuda_stream or None
+    return ctypes.byref(cfg)
 
 
 def workspace_bytes(op: str, rows: int, cols: int, variant: str = "auto", split: int = 0) -> int:
@@ -571,6 +592,164 @@ def pearson_backward(x: torch.Tensor, y: torch.Tensor, grad: torch.Tensor, dx: t
             _ptr(dy, "dy", f32), rows, cols, eps, ctypes.byref(cfg)),
         "credit_pearson_bwd_f32",
     )
+
+
+# Operators on logits: most tokens, alternatives or teacher entries of a row.
+MAX_ENTRIES = 256
+_LOGITS_TYPES = {torch.float32: "f32", torch.bfloat16: "bf16"}
+
+
+def _logits_rows(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(rows, cols, elements from one row to the next) of a matrix whose rows
+    are contiguous but may be apart."""
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected a 2-D tensor, got shape {tuple(t.shape)}")
+    rows, cols = t.shape
+    ld, one = t.stride()
+    if one != 1 and cols > 1:
+        raise ValueError(f"{name}: the columns of a row must be contiguous")
+    return rows, cols, ld if rows > 1 else cols
+
+
+def _logits_call(op: str, logits: torch.Tensor) -> tuple[int, int, int, int, Callable[..., int]]:
+    """(rows, cols, ld, device, entry point) of a call on these logits."""
+    suffix = _LOGITS_TYPES.get(logits.dtype)
+    if suffix is None:
+        raise TypeError(f"logits: expected torch.float32 or torch.bfloat16, got {logits.dtype}")
+    rows, cols, ld = _logits_rows(logits, "logits")
+    device = logits.get_device()
+    if device < 0:
+        raise ValueError(f"logits: tensor must be on a GPU, got {logits.device}")
+    if device != torch.cuda.current_device():
+        raise ValueError(f"logits: on {logits.device}, which is not the current device")
+    return rows, cols, ld, device, getattr(load_library(), f"credit_{op}_{suffix}")
+
+
+def _operand(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, ...],
+             device: int) -> int:
+    """Address of a contiguous operand of exactly this type, shape and device."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: tensor must be contiguous")
+    if t.get_device() != device:
+        raise ValueError(f"{name}: expected a tensor on the logits' device, got {t.device}")
+    return t.data_ptr()
+
+
+def _gradient(dlogits: torch.Tensor, logits: torch.Tensor, device: int) -> tuple[int, int]:
+    """(address, ld) of the gradient for the logits."""
+    if dlogits.dtype is not logits.dtype:
+        raise TypeError(f"dlogits: expected {logits.dtype}, got {dlogits.dtype}")
+    if dlogits.shape != logits.shape:
+        raise ValueError(f"dlogits: expected shape {tuple(logits.shape)}, "
+                         f"got {tuple(dlogits.shape)}")
+    if dlogits.get_device() != device:
+        raise ValueError(f"dlogits: expected a tensor on the logits' device, got {dlogits.device}")
+    return dlogits.data_ptr(), _logits_rows(dlogits, "dlogits")[2]
+
+
+def token_logprob_fwd(logits: torch.Tensor, tokens: torch.Tensor, logp: torch.Tensor,
+                      stats: torch.Tensor, entropy: torch.Tensor | None = None,
+                      top_logp: torch.Tensor | None = None, top_ids: torch.Tensor | None = None,
+                      temperature: float = 1.0, cfg: CreditCfg | None = None) -> None:
+    """Log-probabilities of given tokens under softmax(logits / temperature).
+
+    logits [rows, cols] fp32 or bf16 (rows may be apart), tokens [rows, n]
+    int64 (negative: padding, log-probability 0; n may be 0).  Written: logp
+    [rows, n], stats [rows, 2] (maximum and sum of exponentials, for the
+    backward) and, where given, entropy [rows] and the most likely
+    alternatives, top_logp and top_ids (int64) [rows, k], in falling order,
+    equal ones by column.  All fp32 but the columns."""
+    rows, cols, ld, dev, fn = _logits_call("token_logprob_fwd", logits)
+    f32, i64 = torch.float32, torch.int64
+    if tokens.dim() != 2:
+        raise ValueError(f"tokens: expected a 2-D tensor, got shape {tuple(tokens.shape)}")
+    n = tokens.shape[1]
+    if (top_logp is None) != (top_ids is None):
+        raise ValueError("top_logp and top_ids come together")
+    top = 0 if top_ids is None else top_ids.shape[-1]
+    status = fn(
+        logits.data_ptr(), ld, _operand(tokens, "tokens", i64, (rows, n), dev),
+        _operand(logp, "logp", f32, (rows, n), dev), _operand(stats, "stats", f32, (rows, 2), dev),
+        None if entropy is None else _operand(entropy, "entropy", f32, (rows,), dev),
+        None if top_logp is None else _operand(top_logp, "top_logp", f32, (rows, top), dev),
+        None if top_ids is None else _operand(top_ids, "top_ids", i64, (rows, top), dev),
+        rows, cols, n, top, temperature, _cfg_ref(cfg, dev))
+    check(status, "credit_token_logprob_fwd")
+
+
+def token_logprob_bwd(logits: torch.Tensor, tokens: torch.Tensor, stats: torch.Tensor,
+                      dlogp: torch.Tensor, dlogits: torch.Tensor,
+                      entropy: torch.Tensor | None = None, dentropy: torch.Tensor | None = None,
+                      temperature: float = 1.0, cfg: CreditCfg | None = None) -> None:
+    """Gradient for the logits of sum(dlogp * logp) + sum(dentropy * entropy),
+    from token_logprob_fwd's stats (and entropy).  dlogits, of the logits' type
+    and shape, may be the logits themselves.  Rows without a weight other than
+    0 are written 0 whatever their logits hold."""
+    rows, cols, ld, dev, fn = _logits_call("token_logprob_bwd", logits)
+    f32 = torch.float32
+    if tokens.dim() != 2:
+        raise ValueError(f"tokens: expected a 2-D tensor, got shape {tuple(tokens.shape)}")
+    n = tokens.shape[1]
+    if (entropy is None) != (dentropy is None):
+        raise ValueError("entropy and dentropy come together")
+    out, ldd = _gradient(dlogits, logits, dev)
+    status = fn(
+        logits.data_ptr(), ld, _operand(tokens, "tokens", torch.int64, (rows, n), dev),
+        _operand(stats, "stats", f32, (rows, 2), dev),
+        None if entropy is None else _operand(entropy, "entropy", f32, (rows,), dev),
+        _operand(dlogp, "dlogp", f32, (rows, n), dev),
+        None if dentropy is None else _operand(dentropy, "dentropy", f32, (rows,), dev),
+        out, ldd, rows, cols, n, temperature, _cfg_ref(cfg, dev))
+    check(status, "credit_token_logprob_bwd")
+
+
+def topk_distill_fwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: torch.Tensor,
+                     loss: torch.Tensor, stats: torch.Tensor, tail: bool = True,
+                     temperature: float = 1.0, cfg: CreditCfg | None = None) -> None:
+    """KL(teacher || student) a row from the teacher's top entries.
+
+    logits as in token_logprob_fwd (the student's); teacher_ids int64 and
+    teacher fp32 [rows, k] (negative id: absent).  tail: teacher holds
+    log-probabilities at this temperature (token_logprob_fwd's top_logp) and
+    what they leave of 1 is held against the other columns together; without
+    it, logits over whose softmax the entries are all there is.  Written: loss
+    [rows], stats [rows, 8] for the backward."""
+    rows, cols, ld, dev, fn = _logits_call("topk_distill_fwd", logits)
+    f32 = torch.float32
+    if teacher_ids.dim() != 2:
+        raise ValueError(f"teacher_ids: expected a 2-D tensor, got {tuple(teacher_ids.shape)}")
+    k = teacher_ids.shape[1]
+    status = fn(
+        logits.data_ptr(), ld, _operand(teacher_ids, "teacher_ids", torch.int64, (rows, k), dev),
+        _operand(teacher, "teacher", f32, (rows, k), dev),
+        _operand(loss, "loss", f32, (rows,), dev), _operand(stats, "stats", f32, (rows, 8), dev),
+        rows, cols, k, bool(tail), temperature, _cfg_ref(cfg, dev))
+    check(status, "credit_topk_distill_fwd")
+
+
+def topk_distill_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: torch.Tensor,
+                     stats: torch.Tensor, dloss: torch.Tensor, dlogits: torch.Tensor,
+                     tail: bool = True, temperature: float = 1.0,
+                     cfg: CreditCfg | None = None) -> None:
+    """Gradient for the logits of sum(dloss * loss) of topk_distill_fwd (same
+    tail and temperature), from its stats.  dlogits, of the logits' type and
+    shape, may be the logits themselves."""
+    rows, cols, ld, dev, fn = _logits_call("topk_distill_bwd", logits)
+    f32 = torch.float32
+    if teacher_ids.dim() != 2:
+        raise ValueError(f"teacher_ids: expected a 2-D tensor, got {tuple(teacher_ids.shape)}")
+    k = teacher_ids.shape[1]
+    out, ldd = _gradient(dlogits, logits, dev)
+    status = fn(
+        logits.data_ptr(), ld, _operand(teacher_ids, "teacher_ids", torch.int64, (rows, k), dev),
+        _operand(teacher, "teacher", f32, (rows, k), dev),
+        _operand(stats, "stats", f32, (rows, 8), dev), _operand(dloss, "dloss", f32, (rows,), dev),
+        out, ldd, rows, cols, k, bool(tail), temperature, _cfg_ref(cfg, dev))
+    check(status, "credit_topk_distill_bwd")
 
 
 def layernorm_backward(x: torch.Tensor, dy: torch.Tensor, gamma: torch.Tensor,

@@ -117,6 +117,10 @@ typedef struct credit_cfg {
 #define CREDIT_OP_WEIGHTED_VAR_BWD 13
 #define CREDIT_OP_PEARSON_BWD 14
 #define CREDIT_OP_RMSNORM_FWD_BWD 15
+#define CREDIT_OP_TOKEN_LOGPROB_FWD 16
+#define CREDIT_OP_TOKEN_LOGPROB_BWD 17
+#define CREDIT_OP_TOPK_DISTILL_FWD 18
+#define CREDIT_OP_TOPK_DISTILL_BWD 19
 
 /* ------------------------------------------------------------ library --- */
 
@@ -308,6 +312,93 @@ int credit_softmax_bwd_f32(const float* p, const float* dy, float* dx, int64_t r
  * ((max, sum), then sum p*dy); READ streams three passes. */
 int credit_softmax_logits_bwd_f32(const float* logits, const float* dy, float* dx,
                                   int64_t rows, int64_t cols, const credit_cfg* cfg);
+
+/* ------------------------------- log-probabilities of given tokens ------
+ * Over logits z [rows, cols] (fp32 or bf16, row r at logits + r ld, ld >=
+ * cols; any column count up to 2^29, rows at any element address) at a
+ * temperature T in [1e-4, 1e4]:
+ *   stats [rows, 2]   = m = max_j z_j (the value itself; NaN-propagating) and
+ *                       S = sum_j e^((z_j - m)/T); lse = m/T + ln S
+ *   logp [rows, n_tokens] = (z_t - m)/T - ln S for the row's tokens t; a
+ *                       negative t is padding (0), t >= cols gives NaN
+ *   entropy [rows]    = -sum_j p_j ln p_j, p = softmax(z/T) (NULL: not wanted)
+ *   top_logp, top_ids [rows, n_top] = the n_top largest z's log-probabilities
+ *                       and columns in falling order, equal ones by column,
+ *                       NaN above everything (n_top 0: not wanted)
+ * A column of -inf has probability 0.  A row of nothing else: S = 0, logp
+ * -inf, entropy 0.  A row with NaN or +inf gives NaN.  n_tokens and n_top are
+ * at most 256 (n_top at most cols); n_tokens may be 0.  Variants: AUTO, READ.
+ * No counterpart in the reference, whose softmax (src/workloads/
+ * softmax_logits_backward.cu:314-476) emits no statistics. */
+int credit_token_logprob_fwd_f32(const float* logits, int64_t ld, const int64_t* tokens,
+                                 float* logp, float* stats, float* entropy, float* top_logp,
+                                 int64_t* top_ids, int64_t rows, int64_t cols, int32_t n_tokens,
+                                 int32_t n_top, float temperature, const credit_cfg* cfg);
+int credit_token_logprob_fwd_bf16(const uint16_t* logits, int64_t ld, const int64_t* tokens,
+                                  float* logp, float* stats, float* entropy, float* top_logp,
+                                  int64_t* top_ids, int64_t rows, int64_t cols, int32_t n_tokens,
+                                  int32_t n_top, float temperature, const credit_cfg* cfg);
+/* The gradient for the logits of sum_t dlogp_t logp_t + dentropy H:
+ *   dlogits_j = (sum_{t: token t = j} dlogp_t
+ *                - p_j (G + dentropy (ln p_j + H))) / T,  G = sum dlogp_t,
+ * over the tokens that are not padding, from the forward's stats and entropy
+ * (both entropy and dentropy NULL: none).  dlogits [rows, cols] in the logits'
+ * type, row r at dlogits + r ldd; it may be the logits themselves (same ld),
+ * otherwise the two may not overlap.  A weight of 0 counts as padding: rows
+ * without any other are written 0 and their logits not read, whatever they
+ * hold; so are rows of -inf alone.  A token >= cols of weight other than 0
+ * makes its row NaN.  Columns behind cols are left as they are. */
+int credit_token_logprob_bwd_f32(const float* logits, int64_t ld, const int64_t* tokens,
+                                 const float* stats, const float* entropy, const float* dlogp,
+                                 const float* dentropy, float* dlogits, int64_t ldd, int64_t rows,
+                                 int64_t cols, int32_t n_tokens, float temperature,
+                                 const credit_cfg* cfg);
+int credit_token_logprob_bwd_bf16(const uint16_t* logits, int64_t ld, const int64_t* tokens,
+                                  const float* stats, const float* entropy, const float* dlogp,
+                                  const float* dentropy, uint16_t* dlogits, int64_t ldd,
+                                  int64_t rows, int64_t cols, int32_t n_tokens, float temperature,
+                                  const credit_cfg* cfg);
+
+/* ------------------------- distillation from a teacher's top entries -----
+ * loss [rows] = KL(q || p), p = softmax(z/T) of the student's logits z (as in
+ * credit_token_logprob_fwd_*: types, ld, T), q from the n_top (1 to 256)
+ * entries a row that were kept of the teacher, teacher_ids and teacher
+ * [rows, n_top]; a negative id is an absent entry.
+ *   tail == 0: teacher holds logits, q = softmax(teacher/T) over the row's
+ *     entries (the other columns have q = 0);
+ *   tail != 0: teacher holds log-probabilities at T (top_logp of
+ *     credit_token_logprob_fwd_* at the same T), q_k = e^teacher_k, and the
+ *     rest 1 - sum q_k (0 if that is negative) is held against all other
+ *     columns' probability together, which is summed directly over them.
+ * Entries that name one column add up.  A row without entries (tail == 0: or
+ * with all of them -inf): loss 0, stats 0, the logits not read.  An id >= cols
+ * makes the loss NaN; p = 0 where q > 0 makes it +inf, but other columns that
+ * are all -inf add nothing to it.  stats [rows, 8] is what the backward takes:
+ * m and S as above, the same two of the columns outside the entries (tail),
+ * sum q, the tail's gradient, the teacher's log-sum, 0. */
+int credit_topk_distill_fwd_f32(const float* logits, int64_t ld, const int64_t* teacher_ids,
+                                const float* teacher, float* loss, float* stats, int64_t rows,
+                                int64_t cols, int32_t n_top, int32_t tail, float temperature,
+                                const credit_cfg* cfg);
+int credit_topk_distill_fwd_bf16(const uint16_t* logits, int64_t ld, const int64_t* teacher_ids,
+                                 const float* teacher, float* loss, float* stats, int64_t rows,
+                                 int64_t cols, int32_t n_top, int32_t tail, float temperature,
+                                 const credit_cfg* cfg);
+/* dlogits = dloss/T (Q p - q), Q = sum q (with tail: plus the rest), in every
+ * column outside the entries q being the rest's share there,
+ * rest p_j / (their probability).  ids, teacher, tail and T as the forward's,
+ * whose stats it takes; dlogits as in credit_token_logprob_bwd_*.  Rows
+ * without entries or with dloss 0 are written 0 and their logits not read. */
+int credit_topk_distill_bwd_f32(const float* logits, int64_t ld, const int64_t* teacher_ids,
+                                const float* teacher, const float* stats, const float* dloss,
+                                float* dlogits, int64_t ldd, int64_t rows, int64_t cols,
+                                int32_t n_top, int32_t tail, float temperature,
+                                const credit_cfg* cfg);
+int credit_topk_distill_bwd_bf16(const uint16_t* logits, int64_t ld, const int64_t* teacher_ids,
+                                 const float* teacher, const float* stats, const float* dloss,
+                                 uint16_t* dlogits, int64_t ldd, int64_t rows, int64_t cols,
+                                 int32_t n_top, int32_t tail, float temperature,
+                                 const credit_cfg* cfg);
 
 /* --------------------------------------- rowwise_quant (reference) -----
  * q = int8(clamp(rint(x * inv), -127, 127)), inv = (1 / max_j |x_j|) * 127

@@ -385,3 +385,133 @@ def pearson_backward_init(rows: int, cols: int):
     grad = np.float32(0.75) + (np.arange(rows) % 17).astype(np.float32) * np.float32(0.03125)
     return x.reshape(rows, cols), y.reshape(rows, cols), grad.astype(np.float32).reshape(rows, 1)
 
+
+
+# ------------------------------------------------- operators on logits -----
+
+
+def _log_softmax(z, temperature: float = 1.0):
+    """(x, m, S, ln p) of rows z / temperature; a row of -inf alone has S = 0
+    and ln p = -inf."""
+    z = f64(z)
+    m = z.max(axis=-1, keepdims=True)
+    with np.errstate(all="ignore"):
+        x = (z - m) / temperature
+        e = np.where(z == -np.inf, 0.0, np.exp(x))
+        e = np.where(np.isposinf(m) | np.isnan(m), np.nan, e)
+        total = e.sum(axis=-1, keepdims=True)
+        lp = np.where((z == -np.inf) & ~np.isnan(total), -np.inf, x - np.log(total))
+    return m, total, lp
+
+
+def token_logprob_fwd(z, tokens, top: int = 0, temperature: float = 1.0):
+    """(logp [rows, n], stats [rows, 2], entropy [rows], top log-probabilities
+    and top columns [rows, top]) of softmax(z / temperature)."""
+    z, tokens = f64(z), np.asarray(tokens)
+    m, total, lp = _log_softmax(z, temperature)
+    cols = z.shape[1]
+    inside = (tokens >= 0) & (tokens < cols)
+    logp = np.take_along_axis(lp, np.where(inside, tokens, 0), axis=1)
+    logp = np.where(tokens < 0, 0.0, np.where(inside, logp, np.nan))
+    with np.errstate(all="ignore"):
+        h = -np.where(lp == -np.inf, 0.0, np.exp(lp) * lp).sum(axis=1)
+    h = np.where(m[:, 0] == -np.inf, 0.0, h)
+    # NaN above everything, equal values by column: a stable sort of -rank.
+    order = np.argsort(np.where(np.isnan(z), -np.inf, -z), axis=1, kind="stable")
+    nan_first = np.argsort(~np.take_along_axis(np.isnan(z), order, axis=1), axis=1, kind="stable")
+    ids = np.take_along_axis(order, nan_first, axis=1)[:, :top]
+    return (logp, np.concatenate((m, total), axis=1), h, np.take_along_axis(lp, ids, axis=1),
+            ids.astype(np.int64))
+
+
+def token_logprob_bwd(z, tokens, dlogp, dentropy=None, temperature: float = 1.0):
+    """Gradient of sum(dlogp * logp) + sum(dentropy * entropy) for z."""
+    z, tokens, dlogp = f64(z), np.asarray(tokens), f64(dlogp)
+    m, _, lp = _log_softmax(z, temperature)
+    rows, cols = z.shape
+    out = np.zeros((rows, cols))
+    with np.errstate(all="ignore"):
+        for r in range(rows):
+            h = 0.0 if dentropy is None else float(dentropy[r])
+            weights = [(int(t), g) for t, g in zip(tokens[r], dlogp[r]) if t >= 0 and g != 0.0]
+            if (not weights and h == 0.0) or m[r, 0] == -np.inf:
+                continue
+            if any(t >= cols for t, _ in weights):
+                out[r] = np.nan
+                continue
+            p = np.exp(lp[r])
+            d = -p * sum(g for _, g in weights)
+            if h != 0.0:
+                plp = np.where(lp[r] == -np.inf, 0.0, p * lp[r])
+                d -= h * (plp - p * plp.sum())
+            for t, g in weights:
+                d[t] += g
+            out[r] = d / temperature
+    return out
+
+
+def _teacher_mass(ids, teacher, tail, temperature):
+    """(q of a row's live entries, the rest) or None without entries."""
+    t = f64(teacher)[ids >= 0]
+    if t.size == 0:
+        return None
+    if tail:
+        q = np.exp(t)
+        return q, max(0.0, 1.0 - q.sum()) if not np.isnan(q).any() else np.nan
+    if t.max() == -np.inf:
+        return None
+    q = np.exp((t - t.max()) / temperature)
+    return q / q.sum(), 0.0
+
+
+def topk_distill_fwd(z, ids, teacher, tail: bool = True, temperature: float = 1.0):
+    """KL(q || softmax(z / temperature)) a row from the teacher's entries."""
+    z, ids = f64(z), np.asarray(ids)
+    m, total, lp = _log_softmax(z, temperature)
+    rows, cols = z.shape
+    loss = np.zeros(rows)
+    with np.errstate(all="ignore"):
+        for r in range(rows):
+            mass = _teacher_mass(ids[r], teacher[r], tail, temperature)
+            if mass is None:
+                continue
+            q, rest = mass
+            at = ids[r][ids[r] >= 0]
+            if (at >= cols).any():
+                loss[r] = np.nan
+                continue
+            loss[r] = np.where(q == 0.0, 0.0, q * (np.log(q) - lp[r, at])).sum()
+            others = np.ones(cols, bool)
+            others[at] = False
+            if tail and rest != 0.0 and (z[r, others] != -np.inf).any():
+                o = lp[r, others]
+                loss[r] += rest * (np.log(rest) - (o.max() + np.log(np.exp(o - o.max()).sum())))
+    return loss
+
+
+def topk_distill_bwd(z, ids, teacher, dloss, tail: bool = True, temperature: float = 1.0):
+    """Gradient of sum(dloss * loss) for z."""
+    z, ids, dloss = f64(z), np.asarray(ids), f64(dloss)
+    m, _, lp = _log_softmax(z, temperature)
+    rows, cols = z.shape
+    out = np.zeros((rows, cols))
+    with np.errstate(all="ignore"):
+        for r in range(rows):
+            mass = _teacher_mass(ids[r], teacher[r], tail, temperature)
+            if mass is None or dloss[r] == 0.0 or m[r, 0] == -np.inf:
+                continue
+            q, rest = mass
+            at = ids[r][ids[r] >= 0]
+            if (at >= cols).any():
+                out[r] = np.nan
+                continue
+            target = np.zeros(cols)
+            np.add.at(target, at, q)
+            others = np.ones(cols, bool)
+            others[at] = False
+            if tail and (z[r, others] != -np.inf).any():
+                o = lp[r, others]
+                w = np.exp(o - o.max())
+                target[others] = rest * w / w.sum()
+            out[r] = (np.exp(lp[r]) * (q.sum() + rest) - target) * dloss[r] / temperature
+    return out

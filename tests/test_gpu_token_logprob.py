@@ -1,0 +1,285 @@
+"""credit_token_logprob_fwd / _bwd against the oracle in 64 bits: widths and
+alignments around the vectors, batches and parts a row is cut into, rows that a
+mask empties, ties, padding, rows apart in memory, gradients in place."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from credit_amd import hip_lib
+from oracle import reference as ref
+from tests.logits_cases import (DTYPES, EPS, as64, assert_within, entropy_error, generator,
+                                half_step, make_logits, placed, special_rows, sum_error)
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = [(1, 1), (3, 2), (2, 7), (5, 63), (4, 257), (3, 1000), (2, 4099), (3, 8192), (2, 8193),
+          (2, 16383), (7, 20003), (2, 50001), (1, 131072), (2, 262144), (300, 515)]
+
+
+def forward(z, tokens, top, entropy=True, temperature=1.0, cfg=None):
+    rows, cols = z.shape
+    f32 = dict(device=z.device, dtype=torch.float32)
+    logp = torch.full(tokens.shape, 7.0, **f32)
+    stats = torch.full((rows, 2), 7.0, **f32)
+    h = torch.full((rows,), 7.0, **f32) if entropy else None
+    top_logp = torch.full((rows, top), 7.0, **f32) if top else None
+    ids = torch.full((rows, top), -7, device=z.device, dtype=torch.int64) if top else None
+    hip_lib.token_logprob_fwd(z, tokens.to(z.device), logp, stats, h, top_logp, ids, temperature,
+                              cfg)
+    torch.cuda.synchronize()
+    return logp, stats, h, top_logp, ids
+
+
+def check_forward(z, tokens, top, got, temperature=1.0, what=""):
+    logp, stats, h, top_logp, ids = got
+    cols = z.shape[1]
+    e_logp, e_stats, e_h, e_top, e_ids = ref.token_logprob_fwd(as64(z), tokens.numpy(), top,
+                                                               temperature)
+    # ln S is off by S's relative error; the result is rounded once.
+    err = sum_error(cols)
+    with np.errstate(invalid="ignore"):
+        assert_within(as64(logp), e_logp, err + np.abs(e_logp) * EPS, what + " logp")
+        m = as64(stats)[:, 0]
+        assert np.array_equal(m, e_stats[:, 0], equal_nan=True), what + " max"
+        assert_within(as64(stats)[:, 1], e_stats[:, 1], e_stats[:, 1] * (err + EPS), what + " sum")
+        if h is not None:
+            assert_within(as64(h), e_h, entropy_error(cols) + np.abs(e_h) * EPS, what + " entropy")
+        if top:
+            assert np.array_equal(ids.cpu().numpy(), e_ids), what + " columns"
+            assert_within(as64(top_logp), e_top, err + np.abs(e_top) * EPS, what + " top")
+
+
+def random_tokens(rows, cols, n, seed):
+    tokens = torch.randint(0, cols, (rows, n), generator=generator(seed))
+    if n > 1:
+        tokens[0, 1] = tokens[0, 0]
+        tokens[-1, -1] = -100
+    return tokens
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_forward(gpu, rows, cols, dtype):
+    print(f"token_logprob_fwd {dtype} {rows}x{cols}", flush=True)
+    z = make_logits(rows, cols, dtype, 11)
+    tokens = random_tokens(rows, cols, 3, 12)
+    top = min(cols, 20)
+    got = forward(z.to(gpu), tokens, top, temperature=0.7)
+    check_forward(z, tokens, top, got, 0.7)
+
+
+@pytest.mark.parametrize("top", [0, 1, 2, 64, 255, 256])
+@pytest.mark.parametrize("entropy", [False, True])
+def test_forward_options(gpu, top, entropy):
+    print(f"token_logprob_fwd top {top} entropy {entropy}", flush=True)
+    for dtype in DTYPES:
+        z = make_logits(6, 9001, dtype, 13)
+        for n in (0, 1, 256):
+            tokens = random_tokens(6, 9001, n, 14) if n else torch.zeros((6, 0), dtype=torch.int64)
+            check_forward(z, tokens, top, forward(z.to(gpu), tokens, top, entropy),
+                          what=f"{dtype} {n} tokens")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [5, 300, 4099, 20001])
+@pytest.mark.parametrize("temperature", [1.0, 0.25, 8.0])
+def test_forward_special_rows(gpu, cols, dtype, temperature):
+    print(f"token_logprob_fwd special rows {dtype} {cols}", flush=True)
+    z, names = special_rows(cols, dtype, 15)
+    tokens = torch.tensor([[0, cols // 2, cols - 1, -1, cols, 1 << 40, -(1 << 62)]] * len(names))
+    top = min(cols, 40)
+    got = forward(z.to(gpu), tokens, top, temperature=temperature)
+    for i, name in enumerate(names):
+        check_forward(z[i:i + 1], tokens[i:i + 1], top, [t[i:i + 1] for t in got], temperature,
+                      name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset,gap", [(0, 1), (1, 0), (3, 5), (8, 8), (7, 57)])
+def test_forward_rows_apart(gpu, dtype, offset, gap):
+    """Rows at any element address, NaN around them."""
+    for rows, cols in ((4, 33), (3, 8191), (2, 30011)):
+        print(f"token_logprob_fwd {dtype} {rows}x{cols} offset {offset} gap {gap}", flush=True)
+        z = make_logits(rows, cols, dtype, 16)
+        tokens = random_tokens(rows, cols, 2, 17)
+        got = forward(placed(z, gpu, offset, gap), tokens, 9)
+        check_forward(z, tokens, 9, got)
+
+
+# ---------------------------------------------------------------- backward --
+
+
+def gradient_bound(z, tokens, dlogp, dent, temperature, dtype, want):
+    """e^x has 2 EPS and 3 EPS ln 2 |x| (|x| <= 126 bits: 2.7e-5/2), S its sum's
+    error twice (the forward's and its rounding); the weight G + h (ln p + H) a
+    few roundings and the entropy's error; a token's gradient is one sum.  An
+    exponential below fp32's least normal, 2^-126, is 0: off by at most that
+    times the weight (S >= 1)."""
+    _, _, lp = ref._log_softmax(as64(z), temperature)
+    err = 1.7e-5 + 2 * sum_error(z.shape[1])
+    with np.errstate(all="ignore"):
+        p = np.where(lp == -np.inf, 0.0, np.exp(lp))
+        live = as64(tokens) >= 0
+        weight = np.abs(as64(dlogp) * live).sum(1, keepdims=True)
+        if dent is not None:
+            h = np.abs(as64(dent))[:, None]
+            ent = -np.where(p == 0, 0.0, p * lp).sum(1, keepdims=True)
+            weight = weight + h * (np.abs(np.where(p == 0, 0.0, lp)) + ent
+                                   + entropy_error(z.shape[1]) / err)
+        one = np.zeros(z.shape)
+        for r in range(z.shape[0]):
+            for t, g in zip(tokens[r].tolist(), as64(dlogp)[r]):
+                if 0 <= t < z.shape[1]:
+                    one[r, t] += abs(g)
+        bound = (p * weight * err + one * 8 * EPS + 2.0 ** -126 * (weight + 1)) / temperature
+        return bound + np.abs(want) * half_step(dtype) * (1 + 1e-6)
+
+
+def backward(z, tokens, dlogp, dent, temperature, gpu, out=None, cfg=None):
+    _, stats, h, _, _ = forward(z, tokens, 0, dent is not None, temperature)
+    out = torch.full(z.shape, 7.0, dtype=z.dtype, device=gpu) if out is None else out
+    hip_lib.token_logprob_bwd(z, tokens.to(gpu), stats, dlogp.to(gpu), out, h,
+                              None if dent is None else dent.to(gpu), temperature, cfg)
+    torch.cuda.synchronize()
+    return out
+
+
+def check_backward(z, tokens, dlogp, dent, temperature, dtype, out, what=""):
+    want = ref.token_logprob_bwd(as64(z), tokens.numpy(), as64(dlogp),
+                                 None if dent is None else as64(dent), temperature)
+    bound = gradient_bound(z, tokens, dlogp, dent, temperature, dtype, want)
+    assert_within(as64(out), want, bound, what + " dlogits")
+
+
+@pytest.mark.parametrize("entropy", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_backward(gpu, rows, cols, dtype, entropy):
+    print(f"token_logprob_bwd {dtype} {rows}x{cols} entropy {entropy}", flush=True)
+    g = generator(21)
+    z = make_logits(rows, cols, dtype, 22)
+    tokens = random_tokens(rows, cols, 3, 23)
+    dlogp = torch.randn(tokens.shape, generator=g)
+    dent = torch.randn(rows, generator=g) if entropy else None
+    out = backward(z.to(gpu), tokens, dlogp, dent, 0.7, gpu)
+    check_backward(z, tokens, dlogp, dent, 0.7, dtype, out)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [5, 300, 20001])
+def test_backward_special_rows(gpu, cols, dtype):
+    print(f"token_logprob_bwd special rows {dtype} {cols}", flush=True)
+    z, names = special_rows(cols, dtype, 24)
+    g = generator(25)
+    tokens = torch.tensor([[0, cols // 2, cols // 2, cols - 1]] * len(names))
+    dlogp = torch.randn(tokens.shape, generator=g)
+    dent = torch.randn(len(names), generator=g)
+    out = backward(z.to(gpu), tokens, dlogp, dent, 1.0, gpu)
+    for i, name in enumerate(names):
+        s = slice(i, i + 1)
+        check_backward(z[s], tokens[s], dlogp[s], dent[s], 1.0, dtype, out[s], name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_backward_padding_is_zero_whatever_the_row_holds(gpu, dtype):
+    print(f"token_logprob_bwd padding {dtype}", flush=True)
+    rows, cols = 6, 9001
+    z = make_logits(rows, cols, dtype, 26).to(gpu)
+    z[2:] = math.nan
+    tokens = torch.randint(0, cols, (rows, 2), generator=generator(27))
+    dlogp = torch.ones((rows, 2))
+    tokens[2] = -1                       # padding alone
+    dlogp[3] = 0.0                       # weights of 0
+    tokens[4, 0], dlogp[4, 1] = -5, 0.0  # one of each
+    dent = torch.ones(rows)
+    dent[2:5] = 0.0
+    out = backward(z, tokens, dlogp, dent, 1.0, gpu)
+    assert (out[2:5] == 0).all() and torch.isnan(out[5]).all()
+    check_backward(z[:2].cpu(), tokens[:2], dlogp[:2], dent[:2], 1.0, dtype, out[:2])
+    # A column that is none: its row is NaN, unless its weight is 0.
+    tokens[0, 0], tokens[1, 1], dlogp[1, 1] = cols, 1 << 33, 0.0
+    out = backward(z, tokens, dlogp, None, 1.0, gpu)
+    assert torch.isnan(out[0]).all()
+    check_backward(z[1:2].cpu(), tokens[1:2], dlogp[1:2], None, 1.0, dtype, out[1:2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("zo,zg,do,dg", [(0, 0, 0, 3), (1, 0, 0, 0), (3, 5, 3, 5), (2, 6, 10, 14),
+                                         (0, 8, 0, 0)])
+def test_backward_rows_apart(gpu, dtype, zo, zg, do, dg):
+    """In and out at different offsets and distances; what lies between the
+    rows of the gradient is left as it was."""
+    for rows, cols in ((4, 33), (3, 8191), (2, 30011)):
+        print(f"token_logprob_bwd {dtype} {rows}x{cols} {zo, zg, do, dg}", flush=True)
+        z = make_logits(rows, cols, dtype, 28)
+        tokens = random_tokens(rows, cols, 2, 29)
+        dlogp = torch.randn(tokens.shape, generator=generator(30))
+        flat = torch.full((do + rows * (cols + dg) + 9,), 3.0, dtype=DTYPES[dtype], device=gpu)
+        out = flat[do:do + rows * (cols + dg)].view(rows, cols + dg)
+        zs = placed(z, gpu, zo, zg)
+        _, stats, _, _, _ = forward(zs, tokens, 0, False)
+        hip_lib.token_logprob_bwd(zs, tokens.to(gpu), stats, dlogp.to(gpu), out[:, :cols])
+        torch.cuda.synchronize()
+        check_backward(z, tokens, dlogp, None, 1.0, dtype, out[:, :cols])
+        assert (out[:, cols:] == 3).all() and (flat[:do] == 3).all() and (flat[-9:] == 3).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [100, 8193, 40003])
+def test_backward_in_place(gpu, dtype, cols):
+    """The gradient over the logits themselves: the same bits."""
+    print(f"token_logprob_bwd in place {dtype} {cols}", flush=True)
+    rows = 5
+    z = make_logits(rows, cols, dtype, 31).to(gpu)
+    tokens = random_tokens(rows, cols, 40, 32)
+    dlogp = torch.randn(tokens.shape, generator=generator(33))
+    dent = torch.randn(rows, generator=generator(34))
+    apart = backward(z, tokens, dlogp, dent, 1.3, gpu)
+    over = z.clone()
+    backward(over, tokens, dlogp, dent, 1.3, gpu, out=over)
+    assert torch.equal(apart, over)
+
+
+def test_backward_against_differences(gpu):
+    """The kernels' own forward, differentiated numerically."""
+    rows, cols, step = 3, 37, 1e-2
+    z = make_logits(rows, cols, "f32", 35)
+    tokens = random_tokens(rows, cols, 2, 36)
+    dlogp = torch.randn(tokens.shape, generator=generator(37))
+    dent = torch.randn(rows, generator=generator(38))
+    out = as64(backward(z.to(gpu), tokens, dlogp, dent, 1.0, gpu))
+
+    def value(zz):
+        logp, _, h, _, _ = forward(zz.to(gpu), tokens.repeat(cols, 1), 0)
+        live = (tokens >= 0).repeat(cols, 1)
+        per_row = (logp.cpu().double() * live * dlogp.double().repeat(cols, 1)).sum(1)
+        return (per_row + h.cpu().double() * dent.double().repeat(cols)).view(cols, rows).t()
+
+    eye = torch.eye(cols)[:, None, :] * step
+    up, down = ((z[None] + s * eye).reshape(cols * rows, cols) for s in (1, -1))
+    numeric = ((value(up) - value(down)) / (2 * step)).numpy()
+    # Differences: the third derivative (at most 6 |weights|) times step^2 / 6,
+    # and the forward's errors over the step.
+    w = (np.abs(as64(dlogp)).sum(1) + 20 * np.abs(as64(dent)))[:, None]
+    bound = w * (step ** 2 + (sum_error(cols) + entropy_error(cols)) / step)
+    assert_within(out, numeric, bound, "differences")
+
+
+def test_offsets_beyond_32_bits(gpu):
+    """Rows whose elements lie more than 2^32 bytes and 2^31 elements into the
+    logits."""
+    rows, cols, ld = 5, 70001, (1 << 29) + 9
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    flat = torch.empty((rows - 1) * ld + cols, dtype=torch.bfloat16, device=gpu)
+    zs = torch.as_strided(flat, (rows, cols), (ld, 1))
+    z = make_logits(rows, cols, "bf16", 39)
+    zs.copy_(z)
+    tokens = random_tokens(rows, cols, 2, 40)
+    print("token_logprob far rows", flush=True)
+    check_forward(z, tokens, 7, forward(zs, tokens, 7))
+    dlogp = torch.randn(tokens.shape, generator=generator(41))
+    backward(zs, tokens, dlogp, None, 1.0, gpu, out=zs)
+    check_backward(z, tokens, dlogp, None, 1.0, "bf16", zs)
