@@ -122,8 +122,9 @@ struct Lane {
 };
 constexpr float kRaise = 8.0f;  // 2^8 x 2^29 columns is far from overflow
 
+// Returns the maximum of z.
 template <bool ENT>
-__device__ __forceinline__ void absorb(Lane& a, const float (&z)[kLane], float c) {
+__device__ __forceinline__ float absorb(Lane& a, const float (&z)[kLane], float c) {
   float bm = fmax_nan(z[0], z[1]);
 #pragma unroll
   for (int i = 2; i < kLane; i += 2) bm = fmax_nan(bm, fmax_nan(z[i], z[i + 1]));
@@ -148,6 +149,7 @@ __device__ __forceinline__ void absorb(Lane& a, const float (&z)[kLane], float c
   }
   a.s += s[0] + s[1];
   if (ENT) a.t += t[0] + t[1];
+  return bm;
 }
 
 // The workgroup's lanes joined, about the maximum of them all; every thread has
@@ -190,14 +192,30 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __builtin_bit_cast(float, (key >> 31) != 0 ? key & 0x7FFFFFFFu : ~key);
 }
 
+// While a row streams by, every lane leaves the maximum of its kLane elements of
+// each batch in LDS: a unit.  Afterwards the K-th largest of 512 group maxima
+// (each thread's units, even and odd batches) bounds the K-th largest element
+// from below, and closely: of n elements in G groups about G ln(1/(1 - K/G))
+// pass it (74 for K = 64, 355 for 256).  Only units that reach the bound are
+// read again.  What has no such bound (many equal values, a few huge units)
+// takes write_top_any, which reads the row several times.
 constexpr int kBins = 256;
 constexpr int kCands = 1024;
+constexpr int kUnitList = 1024;
+constexpr size_t kMaxUnitBytes = 32768;
 struct TopSlots {
   uint32_t hist[kBins];
-  uint64_t cand[kCands];  // key above ~column: larger is nearer the front
-  uint32_t n, bin, above, count;
+  uint16_t units[kUnitList];
+  uint32_t n, listed, bin, above, count;
   uint32_t wave[kNW];
+  float low[kNW];
+  uint64_t* cand;  // key above ~column: larger is nearer the front; over the units
 };
+// Units are kept in the logits' type, which holds them exactly.
+__device__ __forceinline__ void put_unit(float* u, float v) { *u = v; }
+__device__ __forceinline__ void put_unit(uint16_t* u, float v) {
+  *u = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, v) >> 16);
+}
 
 template <class T, class Fn>
 __device__ __forceinline__ void each_value(const Frame& f, Fn&& fn) {
@@ -242,96 +260,185 @@ __device__ __forceinline__ void find_bin(TopSlots& s, uint32_t need) {
   __syncthreads();
 }
 
-// The `top` largest of the row.  The range that holds the last of them is
-// narrowed by histograms until what is at or above it fits the candidates, or
-// until it is a single value; the candidates are then ranked by counting.
-template <class T>
-__device__ __forceinline__ void write_top(const Frame& f, int top, TopSlots& s, float m, double ln_s,
-                                          float temperature, float* top_logp, int64_t* top_ids) {
-  const auto put = [&](int rank, uint32_t key, int col) {
-    const float z = value_of(key);
-    top_logp[rank] =
-        z == kNegInf && ln_s == ln_s ? kNegInf
-                     : static_cast<float>((static_cast<double>(z) - m) / temperature - ln_s);
-    top_ids[rank] = col;
-  };
-  uint32_t lo = 0, hi = 0xFFFFFFFFu, need = top, above = 0;
+// Keys [lo, hi] narrowed around the `need`-th largest of what each() gives
+// (each(fn): fn(key) for the thread's keys; at least `need` lie in [lo, hi]):
+// afterwards `above` keys lie above hi and `in` in [lo, hi], together at most
+// `enough` unless lo = hi.
+struct Range {
+  uint32_t lo, hi, above, in;
+};
+template <class Each>
+__device__ __forceinline__ Range narrow(TopSlots& s, uint32_t lo, uint32_t hi, uint32_t need,
+                                        uint32_t enough, Each&& each) {
+  Range r{lo, hi, 0, 0};
   for (;;) {
-    const int bits = 32 - __builtin_clz((hi - lo) | 1u);
+    const int bits = 32 - __builtin_clz((r.hi - r.lo) | 1u);
     const int shift = bits > 8 ? bits - 8 : 0;
     for (int i = threadIdx.x; i < kBins; i += kThreads) s.hist[i] = 0;
-    if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
-    each_value<T>(f, [&](int, uint32_t key) {
-      if (key >= lo && key <= hi) atomicAdd(&s.hist[(hi - key) >> shift], 1u);
+    each([&](uint32_t key) {
+      if (key >= r.lo && key <= r.hi) atomicAdd(&s.hist[(r.hi - key) >> shift], 1u);
     });
     __syncthreads();
-    find_bin(s, need);
-    const uint32_t bin = s.bin, in_bin = s.count;
-    above += s.above;
-    need -= s.above;
-    hi -= bin << shift;
+    find_bin(s, need - r.above);
+    r.above += s.above;
+    r.in = s.count;
+    r.hi -= s.bin << shift;
     const uint32_t span = (1u << shift) - 1u;
-    lo = hi - lo > span ? hi - span : lo;
+    r.lo = r.hi - r.lo > span ? r.hi - span : r.lo;
     __syncthreads();
-    if (above + in_bin <= kCands || lo == hi) {
-      // At or above lo there are above + in_bin values, at least `top`; where
-      // they are too many, lo is a single value and those above it too few.
-      const bool ties = above + in_bin > kCands;
-      each_value<T>(f, [&](int col, uint32_t key) {
-        if (ties ? key > hi : key >= lo)
-          s.cand[atomicAdd(&s.n, 1u)] =
-              static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(col));
-      });
-      __syncthreads();
-      const int n = static_cast<int>(s.n);
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const uint64_t mine = s.cand[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += s.cand[j] > mine;
-        if (rank < top)
-          put(rank, static_cast<uint32_t>(mine >> 32),
-              static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(mine)));
-      }
-      if (ties) {
-        // The first columns that hold the value, in order.
-        int found = n;
-        const int vecs = (f.end + kN<T> - 1) / kN<T>;
-        for (int v0 = 0; v0 < vecs && found < top; v0 += kThreads) {
-          const int v = v0 + threadIdx.x;
-          const u32x4 raw[1] = {buffer_load(f.r, static_cast<uint32_t>(v) * 16u)};
-          float z[kN<T>];
-          unpack<T, 1>(z, raw);
-          uint32_t hit = 0;
+    if (r.above + r.in <= enough || r.lo == r.hi) return r;
+  }
+}
+
+// Ranks the candidates by counting; put(rank, key, column) for the first `top`.
+template <class Put>
+__device__ __forceinline__ void rank_candidates(const TopSlots& s, int n, int top, Put&& put) {
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t mine = s.cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += s.cand[j] > mine;
+    if (rank < top)
+      put(rank, static_cast<uint32_t>(mine >> 32),
+          static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(mine)));
+  }
+}
+__device__ __forceinline__ void add_candidate(TopSlots& s, uint32_t key, int col) {
+  const uint32_t at = atomicAdd(&s.n, 1u);
+  if (at < kCands)
+    s.cand[at] = static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(col));
+}
+
+// The `top` largest of any row: the range that holds the last of them is
+// narrowed until what is at or above it fits the candidates, or until it is a
+// single value, whose first columns are then taken in order.
+template <class T, class Put>
+__device__ __forceinline__ void write_top_any(const Frame& f, int top, TopSlots& s, Put&& put) {
+  const Range r = narrow(s, 0u, 0xFFFFFFFFu, top, kCands, [&](auto&& fn) {
+    each_value<T>(f, [&](int, uint32_t key) { fn(key); });
+  });
+  const bool ties = r.above + r.in > kCands;
+  if (threadIdx.x == 0) s.n = 0;
+  __syncthreads();
+  each_value<T>(f, [&](int col, uint32_t key) {
+    if (ties ? key > r.hi : key >= r.lo) add_candidate(s, key, col);
+  });
+  __syncthreads();
+  const int n = static_cast<int>(s.n);
+  rank_candidates(s, n, top, put);
+  if (!ties) return;
+  int found = n;
+  const int vecs = (f.end + kN<T> - 1) / kN<T>;
+  for (int v0 = 0; v0 < vecs && found < top; v0 += kThreads) {
+    const int v = v0 + threadIdx.x;
+    const u32x4 raw[1] = {buffer_load(f.r, static_cast<uint32_t>(v) * 16u)};
+    float z[kN<T>];
+    unpack<T, 1>(z, raw);
+    uint32_t hit = 0;
 #pragma unroll
-          for (int i = 0; i < kN<T>; ++i) {
-            const int e = v * kN<T> + i;
-            if (e >= f.head && e < f.end && key_of(z[i]) == hi) hit |= 1u << i;
-          }
-          const uint32_t mine = __builtin_popcount(hit);
-          uint32_t incl = mine;
-          const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    for (int i = 0; i < kN<T>; ++i) {
+      const int e = v * kN<T> + i;
+      if (e >= f.head && e < f.end && key_of(z[i]) == r.hi) hit |= 1u << i;
+    }
+    const uint32_t mine = __builtin_popcount(hit);
+    uint32_t incl = mine;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
 #pragma unroll
-          for (int d = 1; d < kWave; d *= 2) {
-            const uint32_t up = __shfl_up(incl, d);
-            if (lane >= d) incl += up;
-          }
-          if (lane == kWave - 1) s.wave[wave] = incl;
-          __syncthreads();
-          int at = found + static_cast<int>(incl - mine), all = 0;
-          for (int w = 0; w < kNW; ++w) {
-            if (w < wave) at += s.wave[w];
-            all += s.wave[w];
-          }
-          for (; hit != 0 && at < top; hit &= hit - 1, ++at)
-            put(at, hi, v * kN<T> + __builtin_ctz(hit) - f.head);
-          found += all;
-          __syncthreads();
-        }
+    for (int d = 1; d < kWave; d *= 2) {
+      const uint32_t up = __shfl_up(incl, d);
+      if (lane >= d) incl += up;
+    }
+    if (lane == kWave - 1) s.wave[wave] = incl;
+    __syncthreads();
+    int at = found + static_cast<int>(incl - mine), all = 0;
+    for (int w = 0; w < kNW; ++w) {
+      if (w < wave) at += s.wave[w];
+      all += s.wave[w];
+    }
+    for (; hit != 0 && at < top; hit &= hit - 1, ++at)
+      put(at, r.hi, v * kN<T> + __builtin_ctz(hit) - f.head);
+    found += all;
+    __syncthreads();
+  }
+}
+
+// The `top` largest of a row whose units (of 2^fold batches each, `groups` of
+// them a lane) and maximum m are known.  s.cand may share the units' memory.
+template <class T, class Put>
+__device__ __forceinline__ void write_top(const Frame& f, const T* units, int groups, int fold,
+                                          float m, int top, TopSlots& s, Put&& put) {
+  float g[2] = {kNegInf, kNegInf};
+  for (int u = 0; u < groups; ++u)
+    g[u & 1] = fmax_nan(g[u & 1], Elem<T>::get(units + u * kThreads + threadIdx.x));
+  // The least group maximum above -inf (NaN ones are the largest).
+  float low = __builtin_inff();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (g[i] > kNegInf) low = __builtin_fminf(low, g[i]);
+  int full = __builtin_popcountll(__builtin_amdgcn_ballot_w64(!(g[0] <= kNegInf))) +
+             __builtin_popcountll(__builtin_amdgcn_ballot_w64(!(g[1] <= kNegInf)));
+  low = -wave_reduce(-low, MaxOp{});
+  if ((threadIdx.x & (kWave - 1)) == 0) {
+    s.low[threadIdx.x / kWave] = low;
+    s.wave[threadIdx.x / kWave] = full;
+  }
+  if (threadIdx.x == 0) s.n = s.listed = 0;
+  __syncthreads();
+  full = 0;
+  for (int w = 0; w < kNW; ++w) {
+    low = __builtin_fminf(low, s.low[w]);
+    full += s.wave[w];
+  }
+  uint32_t bound = 0;
+  if (full >= top) {
+    const uint32_t hi = key_of(m), lo = key_of(low) < hi ? key_of(low) : hi;
+    bound = narrow(s, lo, hi, top, top + top / 8 + 8, [&](auto&& fn) {
+              fn(key_of(g[0]));
+              fn(key_of(g[1]));
+            }).lo;
+  }
+  for (int u = 0; u < groups; ++u)
+    if (key_of(Elem<T>::get(units + u * kThreads + threadIdx.x)) >= bound) {
+      const uint32_t at = atomicAdd(&s.listed, 1u);
+      if (at < kUnitList) s.units[at] = static_cast<uint16_t>(u * kThreads + threadIdx.x);
+    }
+  __syncthreads();
+  const int listed = static_cast<int>(s.listed);
+  if (listed > kUnitList) return write_top_any<T>(f, top, s, put);
+  const int per = kU<T> << fold;  // vectors of a unit
+  for (int i0 = 0; i0 < listed * per; i0 += 4 * kThreads) {
+    u32x4 raw[4];
+    int vec[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j * kThreads + static_cast<int>(threadIdx.x);
+      const int unit = i < listed * per ? s.units[i / per] : -1;
+      const int k = i % per;
+      vec[j] = unit < 0 ? -1
+                        : (((unit / kThreads << fold) * kU<T> + k) * kThreads + unit % kThreads);
+      raw[j] = buffer_load(f.r, static_cast<uint32_t>(vec[j]) * 16u);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (vec[j] < 0) continue;
+      const u32x4 one[1] = {raw[j]};
+      float z[kN<T>];
+      unpack<T, 1>(z, one);
+#pragma unroll
+      for (int e = 0; e < kN<T>; ++e) {
+        const int at = vec[j] * kN<T> + e;
+        const uint32_t key = key_of(z[e]);
+        if (key >= bound && at >= f.head && at < f.end) add_candidate(s, key, at - f.head);
       }
-      return;
     }
   }
+  __syncthreads();
+  const int n = static_cast<int>(s.n);
+  if (n > kCands) {
+    __syncthreads();
+    return write_top_any<T>(f, top, s, put);
+  }
+  rank_candidates(s, n, top, put);
 }
 
 // -------------------------------------------------------- token log-probs --
@@ -346,6 +453,7 @@ struct LogprobArgs {
   float* top_logp;
   int64_t* top_ids;
   int cols, n_tokens, n_top;
+  int fold;              // a unit is 2^fold batches of a lane
   float temperature, c;  // c = log2(e) / temperature
 };
 
@@ -376,7 +484,9 @@ __device__ __forceinline__ void logprob_outputs(const LogprobArgs<T>& a, int64_t
 
 template <class T, bool ENT, bool TOP>
 __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs<T> a) {
+  extern __shared__ __attribute__((aligned(16))) char dynamic_lds[];
   __shared__ JoinSlots join;
+  T* units = reinterpret_cast<T*>(dynamic_lds);
   const int64_t row = blockIdx.x;
   const T* z = a.logits + row * a.ld;
   const Frame f = frame_of(z, a.cols);
@@ -384,12 +494,18 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
   Lane lane;
   u32x4 v[kU<T>];
   load_batch<T>(v, f, 0);
+  float unit = kNegInf;
   for (int b = 0; b < batches; ++b) {
     u32x4 next[kU<T>];
     load_batch<T>(next, f, b + 1);  // past the row: zeros, no access
     float x[kLane];
     row_values<T>(x, v, f, b);
-    absorb<ENT>(lane, x, a.c);
+    const float bm = absorb<ENT>(lane, x, a.c);
+    if constexpr (TOP) {
+      unit = fmax_nan(unit, bm);
+      put_unit(units + (b >> a.fold) * kThreads + threadIdx.x, unit);
+      if (((b + 1) & ((1 << a.fold) - 1)) == 0) unit = kNegInf;
+    }
 #pragma unroll
     for (int k = 0; k < kU<T>; ++k) v[k] = next[k];
   }
@@ -397,8 +513,18 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
   logprob_outputs<T, ENT>(a, row, z, j);
   if constexpr (TOP) {
     __shared__ TopSlots top;
-    write_top<T>(f, a.n_top, top, j.m, j.m == kNegInf ? 0.0 : ::log(j.s), a.temperature,
-                 a.top_logp + row * a.n_top, a.top_ids + row * a.n_top);
+    if (threadIdx.x == 0) top.cand = reinterpret_cast<uint64_t*>(dynamic_lds);
+    const double ln_s = j.m == kNegInf ? 0.0 : ::log(j.s);
+    write_top<T>(f, units, (batches + (1 << a.fold) - 1) >> a.fold, a.fold, j.m, a.n_top, top,
+                 [&](int rank, uint32_t key, int col) {
+                   const float v = value_of(key);
+                   a.top_logp[row * a.n_top + rank] =
+                       v == kNegInf && ln_s == ln_s
+                           ? kNegInf
+                           : static_cast<float>(
+                                 (static_cast<double>(v) - j.m) / a.temperature - ln_s);
+                   a.top_ids[row * a.n_top + rank] = col;
+                 });
   }
 }
 
@@ -431,30 +557,26 @@ __device__ __forceinline__ void store_grad(T* row, const Frame& f, int e, const 
   }
 }
 
-// value(z) over the workgroup's part of the row, z not read where `zero`.
-template <class T, bool VEC, class Fn>
-__device__ __forceinline__ void write_grad(const Frame& f, T* out, int part, bool zero,
-                                           Fn&& value) {
-  const int v0 = part * kGradVecs * kThreads + static_cast<int>(threadIdx.x);
-  u32x4 v[kGradVecs] = {};
-  if (!zero) {
+// The workgroup's part of a row, and value(z) over it (0 where `zero`).
+template <class T>
+__device__ __forceinline__ void load_part(u32x4 (&v)[kGradVecs], const Frame& f, int part) {
 #pragma unroll
-    for (int k = 0; k < kGradVecs; ++k)
-      v[k] = buffer_load_nt(f.r, static_cast<uint32_t>(v0 + k * kThreads) * 16u);
-  }
+  for (int k = 0; k < kGradVecs; ++k)
+    v[k] = buffer_load_nt(f.r, ((part * kGradVecs + k) * kThreads + threadIdx.x) * 16u);
+}
+template <class T, bool VEC, class Fn>
+__device__ __forceinline__ void write_part(const u32x4 (&v)[kGradVecs], const Frame& f, T* out,
+                                           int part, bool zero, Fn&& value) {
 #pragma unroll
   for (int k = 0; k < kGradVecs; ++k) {
     const u32x4 raw[1] = {v[k]};
     float g[kN<T>];
-    if (zero) {
+    unpack<T, 1>(g, raw);
 #pragma unroll
-      for (int i = 0; i < kN<T>; ++i) g[i] = 0.0f;
-    } else {
-      unpack<T, 1>(g, raw);
-#pragma unroll
-      for (int i = 0; i < kN<T>; ++i) g[i] = value(g[i]);
-    }
-    store_grad<T, VEC>(out, f, (v0 + k * kThreads) * kN<T>, g);
+    for (int i = 0; i < kN<T>; ++i) g[i] = zero ? 0.0f : value(g[i]);
+    store_grad<T, VEC>(out, f,
+                       ((part * kGradVecs + k) * kThreads + static_cast<int>(threadIdx.x)) * kN<T>,
+                       g);
   }
 }
 
@@ -523,6 +645,8 @@ __global__ __launch_bounds__(kThreads) void token_logprob_bwd_kernel(LogprobGrad
       const float e = __builtin_amdgcn_exp2f(x);
       return ENT ? e * __builtin_fmaf(B, __builtin_fmaxf(x, -1000.0f), A) : e * A;
     };
+    u32x4 v[kGradVecs] = {};
+    if (!zero) load_part<T>(v, f, part);
     float own = 0.0f;
     const bool patch = here && !zero;
     const int mine = threadIdx.x < a.n_tokens ? static_cast<int>(threadIdx.x) : -1;
@@ -540,7 +664,7 @@ __global__ __launch_bounds__(kThreads) void token_logprob_bwd_kernel(LogprobGrad
       }
       memory_barrier();  // dlogits may be logits: read before anything is written
     }
-    write_grad<T, VEC>(f, out, part, zero, value);
+    write_part<T, VEC>(v, f, out, part, zero, value);
     if (patch) {
       memory_barrier();
       if (col >= 0) Elem<T>::put(out + col, own);
@@ -728,6 +852,10 @@ struct DistillGradArgs {
 
 template <class T, bool TAIL, bool VEC>
 __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradArgs<T> a) {
+  // The entries whose columns lie in this part, in their order.
+  __shared__ int here_col[kMaxEntries];
+  __shared__ float here_q[kMaxEntries];
+  __shared__ int here_n;
   const int lane = threadIdx.x & (kWave - 1);
   const int part = blockIdx.x;
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
@@ -736,53 +864,58 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
     const Frame f = frame_of(z, a.cols);
     const int first = part * kGradBatch<T> - f.head;
     if (first >= a.cols) continue;
-    const int64_t* ids = a.ids + row * a.n_top;
-    const float* teacher = a.teacher + row * a.n_top;
-    bool live = false, here = false;
-    for (int k = lane; k < a.n_top; k += kWave) {
-      const int64_t id = ids[k];
-      live |= id >= 0;
-      here |= id >= 0 && id < a.cols && id >= first && id - first < kGradBatch<T>;
-    }
-    live = __builtin_amdgcn_ballot_w64(live) != 0;
-    here = __builtin_amdgcn_ballot_w64(here) != 0;
     const float* st = a.stats + 8 * row;
     const float m = st[kMax], s = st[kSum], mass = st[kMass];
     const float g = a.dloss[row] * a.inv_t;
-    const bool zero = !live || g == 0.0f || mass == 0.0f || m == kNegInf;
+    // S = 0: a row without entries, or of -inf alone.
+    const bool zero = s == 0.0f || g == 0.0f || mass == 0.0f;
+    u32x4 v[kGradVecs] = {};
+    int n = 0, col = 0;
+    float own = 0.0f;
+    if (!zero) {
+      load_part<T>(v, f, part);
+      if (threadIdx.x < kWave) {
+        for (int k0 = 0; k0 < a.n_top; k0 += kWave) {
+          const int64_t id = k0 + lane < a.n_top ? a.ids[row * a.n_top + k0 + lane] : -1;
+          const bool here = id >= 0 && id < a.cols && id >= first && id - first < kGradBatch<T>;
+          const uint64_t mask = __builtin_amdgcn_ballot_w64(here);
+          if (here) {
+            const int at = n + __builtin_popcountll(mask & ((uint64_t{1} << lane) - 1));
+            const float t = a.teacher[row * a.n_top + k0 + lane];
+            here_col[at] = static_cast<int>(id);
+            here_q[at] = exp_accurate(TAIL ? t : t * a.inv_t - st[kTeacherLse]);
+          }
+          n += __builtin_popcountll(mask);
+        }
+        if (lane == 0) here_n = n;
+      }
+      lds_barrier();
+      n = here_n;
+    }
+    if (n != 0) {
+      if (threadIdx.x < n) {
+        col = here_col[threadIdx.x];
+        float q = 0.0f;
+        for (int j = 0; j < n; ++j)
+          if (here_col[j] == col) q += here_q[j];
+        const float p = exp_accurate((Elem<T>::get(z + col) - m) * a.inv_t) / s;
+        own = g * (mass * p - q);
+      }
+      memory_barrier();  // dlogits may be logits: read before anything is written
+    }
     float ref = m, A = g * mass / s;
     if (TAIL) {
       const bool some = st[kTailSum] != 0.0f;  // else every column is named or without mass
       ref = some ? st[kTailMax] : m;
       A = some ? g * st[kTailGrad] / st[kTailSum] : g * st[kTailGrad];
     }
-    const auto value = [&](float v) {
-      return __builtin_amdgcn_exp2f((v - ref) * a.c) * A;
-    };
-    const bool patch = here && !zero;
-    const int mine = threadIdx.x < a.n_top ? static_cast<int>(threadIdx.x) : -1;
-    int64_t col = -1;
-    float own = 0.0f;
-    if (patch) {
-      if (mine >= 0) {
-        const int64_t id = ids[mine];
-        if (id >= 0 && id < a.cols && id >= first && id - first < kGradBatch<T>) {
-          col = id;
-          float q = 0.0f;
-          for (int j = 0; j < a.n_top; ++j)
-            if (ids[j] == id)
-              q += exp_accurate(TAIL ? teacher[j] : teacher[j] * a.inv_t - st[kTeacherLse]);
-          const float p = exp_accurate((Elem<T>::get(z + id) - m) * a.inv_t) / s;
-          own = g * (mass * p - q);
-        }
-      }
-      memory_barrier();  // dlogits may be logits: read before anything is written
-    }
-    write_grad<T, VEC>(f, out, part, zero, value);
-    if (patch) {
+    write_part<T, VEC>(v, f, out, part, zero,
+                       [&](float x) { return __builtin_amdgcn_exp2f((x - ref) * a.c) * A; });
+    if (n != 0) {
       memory_barrier();
-      if (col >= 0) Elem<T>::put(out + col, own);
+      if (threadIdx.x < n) Elem<T>::put(out + col, own);
     }
+    if (row + gridDim.y < a.rows) lds_barrier();  // before the next row's list
   }
 }
 
@@ -862,6 +995,15 @@ int logprob_fwd(const T* logits, int64_t ld, const int64_t* tokens, float* logp,
   CREDIT_TRY(check_temperature(temperature));
   CREDIT_TRY(check_variant(cfg));
   if (rows == 0) return CREDIT_OK;
+  const int64_t batches = (cols + kN<T> - 1 + kBatch - 1) / kBatch;
+  int fold = 0;
+  const auto unit_bytes = [&] {
+    return static_cast<size_t>((batches + (int64_t{1} << fold) - 1) >> fold) * kThreads * sizeof(T);
+  };
+  while (unit_bytes() > kMaxUnitBytes) ++fold;
+  // The candidates take the units' place once those are listed.
+  const size_t lds = unit_bytes() < kCands * sizeof(uint64_t) ? kCands * sizeof(uint64_t)
+                                                               : unit_bytes();
   const LogprobArgs<T> a{logits,
                          ld,
                          tokens,
@@ -873,13 +1015,14 @@ int logprob_fwd(const T* logits, int64_t ld, const int64_t* tokens, float* logp,
                          static_cast<int>(cols),
                          n_tokens,
                          n_top,
+                         fold,
                          temperature,
                          log2e_over(temperature)};
   const unsigned grid = static_cast<unsigned>(rows);
   hipStream_t stream = cfg_stream(cfg);
   const auto launch = [&](auto ent, auto top) {
     token_logprob_fwd_kernel<T, decltype(ent)::value, decltype(top)::value>
-        <<<grid, kThreads, 0, stream>>>(a);
+        <<<grid, kThreads, n_top > 0 ? lds : 0, stream>>>(a);
   };
   const auto with_top = [&](auto ent) {
     n_top > 0 ? launch(ent, std::true_type{}) : launch(ent, std::false_type{});

@@ -15,7 +15,7 @@ from tests.logits_cases import (DTYPES, EPS, as64, assert_within, entropy_error,
 pytestmark = pytest.mark.gpu
 
 SHAPES = [(1, 1), (3, 2), (2, 7), (5, 63), (4, 257), (3, 1000), (2, 4099), (3, 8192), (2, 8193),
-          (2, 16383), (7, 20003), (2, 50001), (1, 131072), (2, 262144), (300, 515)]
+          (2, 16383), (7, 20003), (2, 50001), (1, 131072), (2, 262144), (2, 300007), (1, 1100001), (300, 515)]
 
 
 def forward(z, tokens, top, entropy=True, temperature=1.0, cfg=None):
@@ -265,6 +265,42 @@ def test_backward_against_differences(gpu):
     w = (np.abs(as64(dlogp)).sum(1) + 20 * np.abs(as64(dent)))[:, None]
     bound = w * (step ** 2 + (sum_error(cols) + entropy_error(cols)) / step)
     assert_within(out, numeric, bound, "differences")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_alternatives_that_crowd(gpu, dtype):
+    """The largest values side by side, in one lane's vectors, or too many equal
+    ones for any list."""
+    cols = 70001
+    z = make_logits(6, cols, dtype, 42)
+    g = generator(43)
+    z[0, 100:400] = torch.rand(300, generator=g).to(z.dtype) + 30
+    lane = torch.arange(0, cols - 8192, 8192)[:, None] + torch.arange(4)  # one lane's columns
+    z[1, lane.flatten()] = (torch.rand(lane.numel(), generator=g) + 30).to(z.dtype)
+    z[2, ::7] = 25.0
+    z[3, 5000:5000 + 1500] = torch.linspace(20, 40, 1500).to(z.dtype)
+    z[4] = z[4].clamp(max=2.0)
+    z[5, 64:] = -math.inf
+    tokens = random_tokens(6, cols, 1, 44)
+    for top in (1, 30, 64, 200, 256):
+        print(f"token_logprob_fwd crowd {dtype} top {top}", flush=True)
+        check_forward(z, tokens, top, forward(z.to(gpu), tokens, top), what=f"top {top}")
+
+
+def test_more_rows_than_a_grid_has(gpu):
+    rows, cols = 70001, 5
+    print("token_logprob many rows", flush=True)
+    z = make_logits(rows, cols, "f32", 45)
+    tokens = torch.randint(0, cols, (rows, 1), generator=generator(46))
+    check_forward(z, tokens, 3, forward(z.to(gpu), tokens, 3))
+    dlogp = torch.randn(tokens.shape, generator=generator(47))
+    out = backward(z.to(gpu), tokens, dlogp, None, 1.0, gpu)
+    want = torch.autograd.functional.vjp(
+        lambda x: torch.log_softmax(x, 1).gather(1, tokens), z.double(), dlogp.double())[1]
+    p = torch.softmax(z.double(), 1).numpy()
+    one = torch.zeros(z.shape, dtype=torch.float64).scatter_(1, tokens, dlogp.double().abs())
+    bound = p * dlogp.double().abs().numpy() * (1.7e-5 + 2 * sum_error(cols)) + one.numpy() * 8 * EPS
+    assert_within(as64(out), want.numpy(), bound, "dlogits")
 
 
 def test_offsets_beyond_32_bits(gpu):

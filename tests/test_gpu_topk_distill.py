@@ -206,6 +206,25 @@ def test_gradient_in_place(gpu, dtype, tail):
         assert torch.equal(apart, over)
 
 
+@pytest.mark.parametrize("tail", [False, True])
+def test_more_rows_than_a_grid_has(gpu, tail):
+    """Every row as it is alone: the rows beyond 65535 of one call against a
+    call of their own."""
+    rows, cols = 70001, 9
+    print(f"topk_distill many rows tail {tail}", flush=True)
+    z = make_logits(rows, cols, "f32", 72).to(gpu)
+    ids, teacher = make_teacher(z.cpu(), 4, tail, 1.0, 73)
+    ids[::3, 1] = ids[::3, 0]
+    dloss = torch.randn(rows, generator=generator(74))
+    loss, _ = forward(z, ids, teacher, tail, 1.0, gpu)
+    out = backward(z, ids, teacher, dloss, tail, 1.0, gpu)
+    for s in (slice(0, 100), slice(65436, 65636), slice(69901, rows)):
+        alone, _ = forward(z[s], ids[s], teacher[s], tail, 1.0, gpu)
+        assert torch.equal(loss[s], alone)
+        assert torch.equal(out[s], backward(z[s], ids[s], teacher[s], dloss[s], tail, 1.0, gpu))
+        check_loss(z[s].cpu(), ids[s], teacher[s], tail, 1.0, alone)
+
+
 def test_gradient_against_differences(gpu):
     rows, cols, step = 2, 37, 1e-2
     z = make_logits(rows, cols, "f32", 70)
