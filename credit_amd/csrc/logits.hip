@@ -4,11 +4,11 @@
 // top entries (credit_topk_distill_*), each with its gradient.
 //
 // The forwards read the logits once and write a few numbers a row: one
-// streaming pass keeps, per lane, a reference m, s = sum e^(x - m/T) and, for
-// the entropy, t = sum e^(x - m/T) (x - m/T) (in base 2: one v_exp_f32 an
-// element).  The reference is raised only where a term passes it by 2^8, so
-// that the usual batch does no rescaling; floating point keeps the same
-// relative precision wherever the reference lies.  The backwards are
+// streaming pass keeps, per lane, a reference r, s = sum e^(x - r) and, for the
+// entropy, t = sum e^(x - r) (x - r) (in base 2: one v_exp_f32 an element).  The
+// reference is raised only where a term passes it by 2^8, so that the usual
+// batch does no rescaling; floating point keeps the same relative precision
+// wherever the reference lies.  The backwards are
 // elementwise given the forward's row statistics.
 //
 // Rows start at any element address and may be apart by more than cols: a row
@@ -88,72 +88,122 @@ __device__ __forceinline__ void unpack(float (&f)[N * kN<T>], const u32x4 (&v)[N
       }
     }
 }
-// Element of the frame: the i-th of this lane in batch b.
-template <class T>
-__device__ __forceinline__ int elem_at(int b, int i) {
-  return ((b * kU<T> + i / kN<T>)*kThreads + static_cast<int>(threadIdx.x)) * kN<T> + i % kN<T>;
-}
 template <class T>
 __device__ __forceinline__ void load_batch(u32x4 (&v)[kU<T>], const Frame& f, int b) {
 #pragma unroll
   for (int k = 0; k < kU<T>; ++k)
     v[k] = buffer_load_nt(f.r, ((b * kU<T> + k) * kThreads + threadIdx.x) * 16u);
 }
-// The lane's elements of batch b, -inf in the place of what is not the row's.
+// The lane's elements of batch b that are not the row's, bit i the i-th.
 template <class T>
-__device__ __forceinline__ void row_values(float (&z)[kLane], const u32x4 (&v)[kU<T>],
-                                           const Frame& f, int b) {
-  unpack<T, kU<T>>(z, v);
-  if ((b == 0 && f.head != 0) || (b + 1) * kBatch > f.end) {
+__device__ __forceinline__ uint32_t outside(const Frame& f, int b) {
+  uint32_t drop = 0;
 #pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      const int e = elem_at<T>(b, i);
-      z[i] = e >= f.head && e < f.end ? z[i] : kNegInf;
+  for (int k = 0; k < kU<T>; ++k) {
+    const int e = ((b * kU<T> + k) * kThreads + static_cast<int>(threadIdx.x)) * kN<T>;
+    const int from = min(max(f.head - e, 0), kN<T>), to = min(max(f.end - e, 0), kN<T>);
+    const uint32_t own = (1u << to) - (1u << from);  // from > to: nothing is own
+    drop |= (to > from ? ~own & ((1u << kN<T>) - 1) : (1u << kN<T>) - 1) << (k * kN<T>);
+  }
+  return drop;
+}
+// -inf in the place of the elements that `drop` names, vector by vector where
+// any lane has one.
+template <class T>
+__device__ __forceinline__ void hide(u32x4 (&v)[kU<T>], uint32_t drop) {
+#pragma unroll
+  for (int k = 0; k < kU<T>; ++k) {
+    const uint32_t d = drop >> (k * kN<T>);
+    if (__builtin_amdgcn_ballot_w64((d & ((1u << kN<T>) - 1)) != 0) == 0) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t w = v[k][e];
+      if constexpr (std::is_same_v<T, float>) {
+        w = (d >> e & 1u) != 0 ? 0xFF800000u : w;
+      } else {
+        w = (d >> (2 * e) & 1u) != 0 ? (w & 0xFFFF0000u) | 0xFF80u : w;
+        w = (d >> (2 * e + 1) & 1u) != 0 ? (w & 0xFFFFu) | 0xFF800000u : w;
+      }
+      v[k][e] = w;
     }
   }
 }
 
 // ---------------------------------------------------------- streaming pass --
-// s and t of the values seen, about m in the exponent's base-2 units: s = sum
-// 2^((z - m) c), t = sum 2^((z - m) c) (z - m) c with c = log2(e) / T; mx their
-// maximum (NaN-propagating).
-struct Lane {
-  float m = -FLT_MAX, s = 0.0f, t = 0.0f, mx = kNegInf;
-};
+// s and t of the values a lane has seen, about a reference r in the exponent's
+// base-2 units: s = sum 2^(z c - r), t = sum 2^(z c - r) (z c - r), c = log2(e)/T;
+// mx their maximum (NaN-propagating).  One fused multiply-add makes an exponent,
+// exact but for its last rounding, as long as |z c| stays below kFar; a row
+// whose maximum does not (or one of lowest values alone) is streamed once more
+// in the CAREFUL form, whose reference is a logit: 2^((z - r) c).
+constexpr float kFar = 1048576.0f;
 constexpr float kRaise = 8.0f;  // 2^8 x 2^29 columns is far from overflow
+struct Lane {
+  float r, s = 0.0f, t = 0.0f, mx = kNegInf;
+};
+template <bool CAREFUL>
+__device__ __forceinline__ Lane new_lane() {
+  return Lane{CAREFUL ? -FLT_MAX : -2.0f * kFar};
+}
 
-// Returns the maximum of z.
-template <bool ENT>
-__device__ __forceinline__ float absorb(Lane& a, const float (&z)[kLane], float c) {
+template <bool ENT, bool CAREFUL, bool CLAMP>
+__device__ __forceinline__ void add_terms(float& s, float& t, const float (&z)[kLane], float r,
+                                          float c) {
+  float s2[2] = {0.0f, 0.0f}, t2[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < kLane; ++i) {
+    const float x = CAREFUL ? (z[i] - r) * c : __builtin_fmaf(z[i], c, -r);
+    const float e = __builtin_amdgcn_exp2f(x);
+    s2[i & 1] += e;
+    // 2^-1000 is 0 as 2^-inf is, and 0 (-1000) is 0.
+    if (ENT) t2[i & 1] = __builtin_fmaf(e, CLAMP ? __builtin_fmaxf(x, -1000.0f) : x, t2[i & 1]);
+  }
+  s = s2[0] + s2[1];
+  t = t2[0] + t2[1];
+}
+
+// Takes a batch; returns its maximum.  A column of -inf
+// makes the plain t NaN: then, and only then, the terms are formed again with
+// the exponent clamped (the clamp costs an eighth of the loop's instructions).
+template <class T, bool ENT, bool CAREFUL>
+__device__ __forceinline__ float absorb(Lane& a, float c, const u32x4 (&v)[kU<T>]) {
+  float z[kLane];
+  unpack<T, kU<T>>(z, v);
   float bm = fmax_nan(z[0], z[1]);
 #pragma unroll
   for (int i = 2; i < kLane; i += 2) bm = fmax_nan(bm, fmax_nan(z[i], z[i + 1]));
   a.mx = fmax_nan(a.mx, bm);
-  const bool raise = (bm - a.m) * c > kRaise;
-  if (__builtin_amdgcn_ballot_w64(raise) != 0) {
-    const float d = raise ? (a.m - bm) * c : 0.0f;
+  const float over = CAREFUL ? (bm - a.r) * c : __builtin_fmaf(bm, c, -a.r);
+  if (__builtin_amdgcn_ballot_w64(over > kRaise) != 0) {
+    const float r = over > kRaise ? (CAREFUL ? bm : bm * c) : a.r;
+    const float d = CAREFUL ? (a.r - r) * c : a.r - r;
     const float f = __builtin_amdgcn_exp2f(d);
     // s = 0: d may be infinite.
     if (ENT) a.t = a.s == 0.0f ? 0.0f : f * __builtin_fmaf(d, a.s, a.t);
     a.s *= f;
-    a.m = raise ? bm : a.m;
+    a.r = r;
   }
-  float s[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
+  float s, t;
+  add_terms<ENT, CAREFUL, CAREFUL>(s, t, z, a.r, c);
+  if (ENT && !CAREFUL && __builtin_amdgcn_ballot_w64(t != t) != 0) {
+    // From the packed values: what the first pass computed need not be kept.
+    u32x4 w[kU<T>];
 #pragma unroll
-  for (int i = 0; i < kLane; ++i) {
-    const float x = (z[i] - a.m) * c;
-    const float e = __builtin_amdgcn_exp2f(x);
-    s[i & 1] += e;
-    // 2^-1000 is 0 as 2^-inf is, and 0 (-1000) is 0.
-    if (ENT) t[i & 1] = __builtin_fmaf(e, __builtin_fmaxf(x, -1000.0f), t[i & 1]);
+    for (int k = 0; k < kU<T>; ++k) {
+      w[k] = v[k];
+      __asm__ volatile("" : "+v"(w[k]));
+    }
+    unpack<T, kU<T>>(z, w);
+    add_terms<ENT, CAREFUL, true>(s, t, z, a.r, c);
   }
-  a.s += s[0] + s[1];
-  if (ENT) a.t += t[0] + t[1];
+  a.s += s;
+  if (ENT) a.t += t;
   return bm;
 }
 
-// The workgroup's lanes joined, about the maximum of them all; every thread has
-// the result.  `slots`: one use between two barriers of the caller.
+// The workgroup's lanes joined, about the maximum m of them all: s = sum
+// e^((z - m)/T), t the same terms times their base-2 exponents; every thread has
+// the result.
 struct Joined {
   float m;
   double s, t;
@@ -162,12 +212,13 @@ struct JoinSlots {
   float m[kNW];
   double st[2][kNW];
 };
+template <bool CAREFUL>
 __device__ __forceinline__ Joined join_lanes(const Lane& a, float c, JoinSlots& slots) {
   Joined j;
   j.m = rows::block_max<kNW>(a.mx, slots.m);
   j.s = j.t = 0.0;
   if (a.s != 0.0f) {  // not of NaN: then s is NaN
-    const float d = (a.m - j.m) * c;
+    const float d = CAREFUL ? (a.r - j.m) * c : __builtin_fmaf(j.m, -c, a.r);
     const double f = __builtin_amdgcn_exp2f(d);
     j.s = f * a.s;
     j.t = f * (static_cast<double>(a.t) + static_cast<double>(d) * a.s);
@@ -178,6 +229,47 @@ __device__ __forceinline__ Joined join_lanes(const Lane& a, float c, JoinSlots& 
   rows::block_sum2<kNW>(j.s, j.t, slots.st);
   return j;
 }
+
+// Two results about their own maxima, as one (s alone).
+__device__ __forceinline__ Joined merge(const Joined& a, const Joined& b, float temperature) {
+  Joined j{fmax_nan(a.m, b.m), 0.0, 0.0};
+  if (a.s != 0.0) j.s += a.s * ::exp((static_cast<double>(a.m) - j.m) / temperature);
+  if (b.s != 0.0) j.s += b.s * ::exp((static_cast<double>(b.m) - j.m) / temperature);
+  return j;
+}
+
+// Batches [b0, b1) of a row: dropped(b) names further elements of batch b to
+// leave out, seen(b, m) takes the lane's maximum of each batch in order.
+template <class T, bool ENT, bool CAREFUL, class Dropped, class Seen>
+__device__ __forceinline__ Lane stream(const Frame& f, int b0, int b1, float c, Dropped&& dropped,
+                                       Seen&& seen) {
+  Lane lane = new_lane<CAREFUL>();
+  u32x4 v[2][kU<T>];
+  load_batch<T>(v[0], f, b0);
+  for (int b = b0; b < b1; b += 2) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = b + h;
+      if (h == 1 && at >= b1) break;
+      load_batch<T>(v[1 - h], f, at + 1);  // past the row: zeros, no access
+      uint32_t drop = dropped(at);
+      if ((at == 0 && f.head != 0) || (at + 1) * kBatch > f.end) drop |= outside<T>(f, at);
+      if (__builtin_amdgcn_ballot_w64(drop != 0) != 0) hide<T>(v[h], drop);
+      seen(at, absorb<T, ENT, CAREFUL>(lane, c, v[h]));
+    }
+  }
+  return lane;
+}
+template <class T, bool ENT, class Dropped, class Seen>
+__device__ __forceinline__ Joined scan(const Frame& f, int b0, int b1, float c, JoinSlots& slots,
+                                       Dropped&& dropped, Seen&& seen) {
+  const Joined j = join_lanes<false>(stream<T, ENT, false>(f, b0, b1, c, dropped, seen), c, slots);
+  if (__builtin_fabsf(j.m * c) <= kFar || __builtin_isinf(j.m) || j.m != j.m) return j;
+  __syncthreads();
+  return join_lanes<true>(stream<T, ENT, true>(f, b0, b1, c, dropped, seen), c, slots);
+}
+__device__ __forceinline__ uint32_t none_dropped(int) { return 0; }
+__device__ __forceinline__ void unseen(int, float) {}
 
 // ------------------------------------------------------------ the largest --
 // Order of the alternatives: by value, NaN above everything and -0 as 0, equal
@@ -209,8 +301,10 @@ struct TopSlots {
   uint32_t n, listed, bin, above, count;
   uint32_t wave[kNW];
   float low[kNW];
-  uint64_t* cand;  // key above ~column: larger is nearer the front; over the units
 };
+// A candidate: its key above ~column, so that the larger is nearer the front.
+// They lie where the units were.
+typedef uint64_t __attribute__((address_space(3))) * CandPtr;
 // Units are kept in the logits' type, which holds them exactly.
 __device__ __forceinline__ void put_unit(float* u, float v) { *u = v; }
 __device__ __forceinline__ void put_unit(uint16_t* u, float v) {
@@ -232,6 +326,18 @@ __device__ __forceinline__ void each_value(const Frame& f, Fn&& fn) {
   }
 }
 
+// Sum over this lane and those below it.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  int x = static_cast<int>(v);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1, 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31 to rows 2, 3
+  return static_cast<uint32_t>(x);
+}
+
 // The bin that holds the `need`-th largest of the histogram (bin 0 the largest)
 // and what lies above it; every thread.
 __device__ __forceinline__ void find_bin(TopSlots& s, uint32_t need) {
@@ -240,13 +346,7 @@ __device__ __forceinline__ void find_bin(TopSlots& s, uint32_t need) {
     uint32_t h[4], sum = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum += h[i] = s.hist[4 * lane + i];
-    uint32_t incl = sum;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-      const uint32_t up = __shfl_up(incl, d);
-      if (lane >= d) incl += up;
-    }
-    uint32_t above = incl - sum;
+    uint32_t above = wave_scan(sum) - sum;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (above < need && above + h[i] >= need) {
@@ -291,29 +391,35 @@ __device__ __forceinline__ Range narrow(TopSlots& s, uint32_t lo, uint32_t hi, u
   }
 }
 
-// Ranks the candidates by counting; put(rank, key, column) for the first `top`.
+// Ranks the n candidates by counting; put(rank, key, column) for the first `top`.
 template <class Put>
-__device__ __forceinline__ void rank_candidates(const TopSlots& s, int n, int top, Put&& put) {
+__device__ __forceinline__ void rank_candidates(CandPtr cand, int n, int top, Put&& put) {
+  const int padded = (n + 7) & ~7;  // zeros, which are larger than none
+  if (static_cast<int>(threadIdx.x) < padded - n) cand[n + threadIdx.x] = 0;
+  __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t mine = s.cand[i];
+    const uint64_t mine = cand[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += s.cand[j] > mine;
+    for (int j = 0; j < padded; j += 8)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) rank += cand[j + k] > mine;
     if (rank < top)
       put(rank, static_cast<uint32_t>(mine >> 32),
           static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(mine)));
   }
 }
-__device__ __forceinline__ void add_candidate(TopSlots& s, uint32_t key, int col) {
+__device__ __forceinline__ void add_candidate(TopSlots& s, CandPtr cand, uint32_t key, int col) {
   const uint32_t at = atomicAdd(&s.n, 1u);
   if (at < kCands)
-    s.cand[at] = static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(col));
+    cand[at] = static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(col));
 }
 
 // The `top` largest of any row: the range that holds the last of them is
 // narrowed until what is at or above it fits the candidates, or until it is a
 // single value, whose first columns are then taken in order.
 template <class T, class Put>
-__device__ __forceinline__ void write_top_any(const Frame& f, int top, TopSlots& s, Put&& put) {
+__device__ __forceinline__ void write_top_any(const Frame& f, int top, TopSlots& s, CandPtr cand,
+                                              Put&& put) {
   const Range r = narrow(s, 0u, 0xFFFFFFFFu, top, kCands, [&](auto&& fn) {
     each_value<T>(f, [&](int, uint32_t key) { fn(key); });
   });
@@ -321,11 +427,11 @@ __device__ __forceinline__ void write_top_any(const Frame& f, int top, TopSlots&
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
   each_value<T>(f, [&](int col, uint32_t key) {
-    if (ties ? key > r.hi : key >= r.lo) add_candidate(s, key, col);
+    if (ties ? key > r.hi : key >= r.lo) add_candidate(s, cand, key, col);
   });
   __syncthreads();
   const int n = static_cast<int>(s.n);
-  rank_candidates(s, n, top, put);
+  rank_candidates(cand, n, top, put);
   if (!ties) return;
   int found = n;
   const int vecs = (f.end + kN<T> - 1) / kN<T>;
@@ -341,13 +447,8 @@ __device__ __forceinline__ void write_top_any(const Frame& f, int top, TopSlots&
       if (e >= f.head && e < f.end && key_of(z[i]) == r.hi) hit |= 1u << i;
     }
     const uint32_t mine = __builtin_popcount(hit);
-    uint32_t incl = mine;
+    const uint32_t incl = wave_scan(mine);
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-      const uint32_t up = __shfl_up(incl, d);
-      if (lane >= d) incl += up;
-    }
     if (lane == kWave - 1) s.wave[wave] = incl;
     __syncthreads();
     int at = found + static_cast<int>(incl - mine), all = 0;
@@ -363,10 +464,10 @@ __device__ __forceinline__ void write_top_any(const Frame& f, int top, TopSlots&
 }
 
 // The `top` largest of a row whose units (of 2^fold batches each, `groups` of
-// them a lane) and maximum m are known.  s.cand may share the units' memory.
+// them a lane) and maximum m are known.
 template <class T, class Put>
-__device__ __forceinline__ void write_top(const Frame& f, const T* units, int groups, int fold,
-                                          float m, int top, TopSlots& s, Put&& put) {
+__device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPtr cand, int groups,
+                                          int fold, float m, int top, TopSlots& s, Put&& put) {
   float g[2] = {kNegInf, kNegInf};
   for (int u = 0; u < groups; ++u)
     g[u & 1] = fmax_nan(g[u & 1], Elem<T>::get(units + u * kThreads + threadIdx.x));
@@ -403,8 +504,9 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, int gr
       if (at < kUnitList) s.units[at] = static_cast<uint16_t>(u * kThreads + threadIdx.x);
     }
   __syncthreads();
-  const int listed = static_cast<int>(s.listed);
-  if (listed > kUnitList) return write_top_any<T>(f, top, s, put);
+  // Too many units that reach the bound: none is read, and s.n is past kCands.
+  if (threadIdx.x == 0 && s.listed > kUnitList) s.n = kCands + 1;
+  const int listed = s.listed > kUnitList ? 0 : static_cast<int>(s.listed);
   const int per = kU<T> << fold;  // vectors of a unit
   for (int i0 = 0; i0 < listed * per; i0 += 4 * kThreads) {
     u32x4 raw[4];
@@ -428,17 +530,16 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, int gr
       for (int e = 0; e < kN<T>; ++e) {
         const int at = vec[j] * kN<T> + e;
         const uint32_t key = key_of(z[e]);
-        if (key >= bound && at >= f.head && at < f.end) add_candidate(s, key, at - f.head);
+        if (key >= bound && at >= f.head && at < f.end) add_candidate(s, cand, key, at - f.head);
       }
     }
   }
   __syncthreads();
   const int n = static_cast<int>(s.n);
-  if (n > kCands) {
-    __syncthreads();
-    return write_top_any<T>(f, top, s, put);
-  }
-  rank_candidates(s, n, top, put);
+  if (n <= kCands)
+    rank_candidates(cand, n, top, put);
+  else
+    write_top_any<T>(f, top, s, cand, put);
 }
 
 // -------------------------------------------------------- token log-probs --
@@ -459,9 +560,8 @@ struct LogprobArgs {
 
 template <class T, bool ENT>
 __device__ __forceinline__ void logprob_outputs(const LogprobArgs<T>& a, int64_t row, const T* z,
-                                                const Joined& j) {
+                                                const Joined& j, double ln_s) {
   const bool empty = j.m == kNegInf;
-  const double ln_s = empty ? 0.0 : ::log(j.s);
   if (threadIdx.x == 0) {
     a.stats[2 * row] = j.m;
     a.stats[2 * row + 1] = static_cast<float>(j.s);
@@ -491,31 +591,21 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
   const T* z = a.logits + row * a.ld;
   const Frame f = frame_of(z, a.cols);
   const int batches = (f.end + kBatch - 1) / kBatch;
-  Lane lane;
-  u32x4 v[kU<T>];
-  load_batch<T>(v, f, 0);
   float unit = kNegInf;
-  for (int b = 0; b < batches; ++b) {
-    u32x4 next[kU<T>];
-    load_batch<T>(next, f, b + 1);  // past the row: zeros, no access
-    float x[kLane];
-    row_values<T>(x, v, f, b);
-    const float bm = absorb<ENT>(lane, x, a.c);
-    if constexpr (TOP) {
-      unit = fmax_nan(unit, bm);
-      put_unit(units + (b >> a.fold) * kThreads + threadIdx.x, unit);
-      if (((b + 1) & ((1 << a.fold) - 1)) == 0) unit = kNegInf;
-    }
-#pragma unroll
-    for (int k = 0; k < kU<T>; ++k) v[k] = next[k];
-  }
-  const Joined j = join_lanes(lane, a.c, join);
-  logprob_outputs<T, ENT>(a, row, z, j);
+  const Joined j = scan<T, ENT>(
+      f, 0, batches, a.c, join, none_dropped,
+      [&](int b, float bm) {
+        if constexpr (TOP) {
+          if ((b & ((1 << a.fold) - 1)) == 0) unit = kNegInf;
+          unit = fmax_nan(unit, bm);
+          put_unit(units + (b >> a.fold) * kThreads + threadIdx.x, unit);
+        }
+      });
+  const double ln_s = j.m == kNegInf ? 0.0 : ::log(j.s);
+  logprob_outputs<T, ENT>(a, row, z, j, ln_s);
   if constexpr (TOP) {
     __shared__ TopSlots top;
-    if (threadIdx.x == 0) top.cand = reinterpret_cast<uint64_t*>(dynamic_lds);
-    const double ln_s = j.m == kNegInf ? 0.0 : ::log(j.s);
-    write_top<T>(f, units, (batches + (1 << a.fold) - 1) >> a.fold, a.fold, j.m, a.n_top, top,
+    write_top<T>(f, units, (CandPtr)(dynamic_lds), (batches + (1 << a.fold) - 1) >> a.fold, a.fold, j.m, a.n_top, top,
                  [&](int rank, uint32_t key, int col) {
                    const float v = value_of(key);
                    a.top_logp[row * a.n_top + rank] =
@@ -675,7 +765,7 @@ __global__ __launch_bounds__(kThreads) void token_logprob_bwd_kernel(LogprobGrad
 // ------------------------------------------------------------ distillation --
 // Columns of the frame that a row's entries name, a bit each, for the batches
 // of one segment: bit i of word (b, lane) is the lane's i-th element of batch b.
-constexpr int kSegBatches = 32;
+constexpr int kSegBatches = 16;
 constexpr int kSegWords = kSegBatches * kThreads;
 
 template <class T>
@@ -692,22 +782,23 @@ struct DistillArgs {
 // Row statistics [rows, 8] for the backward.
 enum DistillStat { kMax, kSum, kTailMax, kTailSum, kMass, kTailGrad, kTeacherLse, kUnused };
 
+// Marks element e of the frame; whether it was marked before.
 template <class T>
-__device__ __forceinline__ void mark(uint32_t* bits, int e, int seg) {
+__device__ __forceinline__ bool mark(uint32_t* bits, int e, int seg) {
   const int v = e / kN<T>;
   const int b = v / (kThreads * kU<T>) - seg * kSegBatches;
-  if (b < 0 || b >= kSegBatches) return;
-  const int i = v / kThreads % kU<T> * kN<T> + e % kN<T>;
-  atomicOr(&bits[b * kThreads + v % kThreads], 1u << i);
+  if (b < 0 || b >= kSegBatches) return false;
+  const uint32_t bit = 1u << (v / kThreads % kU<T> * kN<T> + e % kN<T>);
+  return (atomicOr(&bits[b * kThreads + v % kThreads], bit) & bit) != 0;
 }
 
 template <class T, bool TAIL>
 __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<T> a) {
   __shared__ JoinSlots join;
   __shared__ float max_slots[2][kNW];
-  __shared__ double sum_slots[4][2][kNW];
+  __shared__ double sum_slots[4][kNW];
   __shared__ int flags[kNW];
-  __shared__ int id_list[kMaxEntries];
+  __shared__ int repeated;
   const int64_t row = blockIdx.x;
   const T* z = a.logits + row * a.ld;
   const int k = threadIdx.x;
@@ -718,99 +809,81 @@ __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<
     id = a.ids[row * a.n_top + k];
     t = a.teacher[row * a.n_top + k];
   }
-  const bool live = id >= 0;
   const bool bad = id >= a.cols;
-  id_list[k] = live && !bad ? static_cast<int>(id) : -1;
+  const bool live = id >= 0 && !bad;
   const uint64_t any_live = __builtin_amdgcn_ballot_w64(live);
   const uint64_t any_bad = __builtin_amdgcn_ballot_w64(bad);
   if ((threadIdx.x & (kWave - 1)) == 0)
     flags[threadIdx.x / kWave] = (any_live != 0) | (any_bad != 0) << 1;
-  // The teacher's largest value (renormalised entries).
-  const float tm = rows::block_max<kNW>(live ? t : kNegInf, max_slots[0]);
+  if (threadIdx.x == 0) repeated = 0;
+  const float tm = rows::block_max<kNW>(id >= 0 ? t : kNegInf, max_slots[0]);
   int flag = 0;
   for (int w = 0; w < kNW; ++w) flag |= flags[w];
   float* stats = a.stats + 8 * row;
-  if ((flag & 1) == 0 || (!TAIL && tm == kNegInf)) {  // no entry to learn from
+  if (flag == 0 || (!TAIL && tm == kNegInf)) {  // no entry to learn from
     if (threadIdx.x == 0) a.loss[row] = 0.0f;
     if (threadIdx.x < 8) stats[threadIdx.x] = 0.0f;
     return;
   }
-  const float zk = live && !bad ? Elem<T>::get(z + id) : kNegInf;
+  const float zk = live ? Elem<T>::get(z + id) : kNegInf;
 
   const Frame f = frame_of(z, a.cols);
   const int batches = (f.end + kBatch - 1) / kBatch;
-  Lane lane;
+  bool first = live;  // of the entries that name one column
+  Joined j;
   if constexpr (TAIL) {
     __shared__ uint32_t bits[kSegWords];
-    for (int seg = 0; seg * kSegBatches < batches; ++seg) {
+    // The segments' results joined as the lanes' are.
+    for (int b0 = 0; b0 < batches; b0 += kSegBatches) {
+      const int b1 = b0 + kSegBatches < batches ? b0 + kSegBatches : batches;
+      if (b0 != 0) __syncthreads();
+      for (int b = 0; b < b1 - b0; ++b) bits[b * kThreads + threadIdx.x] = 0;
       __syncthreads();
-      for (int i = threadIdx.x; i < kSegWords; i += kThreads) bits[i] = 0;
+      if (live && mark<T>(bits, static_cast<int>(id) + f.head, b0 / kSegBatches)) repeated = 1;
       __syncthreads();
-      if (live && !bad) mark<T>(bits, static_cast<int>(id) + f.head, seg);
+      const Joined p = scan<T, false>(
+          f, b0, b1, a.c, join, [&](int b) { return bits[(b - b0) * kThreads + threadIdx.x]; },
+          unseen);
+      j = b0 == 0 ? p : merge(j, p, a.temperature);
+    }
+    if (repeated != 0) {  // the lowest of those that name the column counts
+      __shared__ int ids[kMaxEntries];
+      ids[k] = live ? static_cast<int>(id) : -1;
       __syncthreads();
-      const int last = (seg + 1) * kSegBatches < batches ? (seg + 1) * kSegBatches : batches;
-      for (int b = seg * kSegBatches; b < last; ++b) {
-        u32x4 v[kU<T>];
-        load_batch<T>(v, f, b);
-        float x[kLane];
-        row_values<T>(x, v, f, b);
-        const uint32_t w = bits[(b - seg * kSegBatches) * kThreads + threadIdx.x];
-        if (__builtin_amdgcn_ballot_w64(w != 0) != 0) {
-#pragma unroll
-          for (int i = 0; i < kLane; ++i) x[i] = (w >> i & 1u) != 0 ? kNegInf : x[i];
-        }
-        absorb<false>(lane, x, a.c);
-      }
+      for (int i = 0; i < k && first; ++i) first = ids[i] != static_cast<int>(id);
     }
   } else {
-    for (int b = 0; b < batches; ++b) {
-      u32x4 v[kU<T>];
-      load_batch<T>(v, f, b);
-      float x[kLane];
-      row_values<T>(x, v, f, b);
-      absorb<false>(lane, x, a.c);
+    j = scan<T, false>(f, 0, batches, a.c, join, none_dropped, unseen);
+  }
+
+  // Over the entries, in one go: the mass that the row has outside the tail,
+  // and with w = q (tail) or q times its normalisation: w, w ln w, w ln(p S).
+  const float m = TAIL ? fmax_nan(j.m, rows::block_max<kNW>(zk, max_slots[1])) : j.m;
+  double sums[4] = {0.0, 0.0, 0.0, 0.0};
+  if (live) {
+    const double x = zk == kNegInf && m == m && m != __builtin_inff()
+                         ? static_cast<double>(kNegInf)
+                         : (static_cast<double>(zk) - m) / a.temperature;
+    const double ln_w =
+        TAIL ? static_cast<double>(t) : (static_cast<double>(t) - tm) / a.temperature;
+    if (TAIL && first && zk != kNegInf) sums[0] = ::exp(x);
+    sums[1] = ::exp(ln_w);
+    if (sums[1] != 0.0) {
+      sums[2] = sums[1] * ln_w;
+      sums[3] = sums[1] * x;
     }
   }
-  const Joined j = join_lanes(lane, a.c, join);
-
-  // The row's maximum and sum; `tail` what the entries leave.
-  float m = j.m;
+  block_reduce_sum_f64_multi<kNW, 4>(sums, sum_slots);
+  if (threadIdx.x >= kWave) return;
   double s = j.s;
-  if constexpr (TAIL) {
-    m = fmax_nan(j.m, rows::block_max<kNW>(zk, max_slots[1]));
-    // Of entries that name one column the first counts.
-    bool first = live && !bad;
-    for (int i = 0; i < k && first; ++i) first = id_list[i] != static_cast<int>(id);
-    double e = 0.0, none = 0.0;
-    if (first && zk != kNegInf) e = ::exp((static_cast<double>(zk) - m) / a.temperature);
-    rows::block_sum2<kNW>(e, none, sum_slots[0]);
-    s = e;
+  if (TAIL) {
+    s = sums[0];
     if (j.s != 0.0) s += j.s * ::exp((static_cast<double>(j.m) - m) / a.temperature);
   }
-  const bool empty = m == kNegInf;
-  const double ln_s = empty ? 0.0 : ::log(s);
-  // The teacher.
-  double ln_q = kNegInf, lse = 0.0;
+  const double ln_s = m == kNegInf ? 0.0 : ::log(s);
+  double q = sums[1], loss, rest = 0.0, tail_grad = 0.0, lse = 0.0;
   if constexpr (TAIL) {
-    if (live) ln_q = t;
-  } else {
-    double total = 0.0, none = 0.0;
-    if (live) total = ::exp((static_cast<double>(t) - tm) / a.temperature);
-    rows::block_sum2<kNW>(total, none, sum_slots[1]);
-    lse = static_cast<double>(tm) / a.temperature + ::log(total);
-    if (live) ln_q = static_cast<double>(t) / a.temperature - lse;
-  }
-  double q = live ? ::exp(ln_q) : 0.0;
-  double loss = 0.0;
-  if (q != 0.0) {
-    const double ln_p = zk == kNegInf && ln_s == ln_s
-                            ? static_cast<double>(kNegInf)
-                            : (static_cast<double>(zk) - m) / a.temperature - ln_s;
-    loss = q * (ln_q - ln_p);
-  }
-  rows::block_sum2<kNW>(q, loss, sum_slots[2]);
-  double rest = 0.0, tail_grad = 0.0;
-  if constexpr (TAIL) {
+    loss = sums[2] - sums[3] + q * ln_s;
     rest = q < 1.0 ? 1.0 - q : (q == q ? 0.0 : q);
     double share = 0.0;
     // A tail without mass (every other column masked) adds nothing.
@@ -820,8 +893,13 @@ __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<
       if (rest != 0.0) loss += rest * (::log(rest) - ln_tail);
     }
     tail_grad = (q + rest) * share - rest;
+  } else {
+    const double ln_w = ::log(q);
+    loss = (sums[2] - sums[3]) / q - ln_w + ln_s;
+    lse = static_cast<double>(tm) / a.temperature + ln_w;
+    q = q == q ? 1.0 : q;
   }
-  if ((flag & 2) != 0) loss = q = kNaN;
+  if ((flag & 2) != 0) loss = q = tail_grad = kNaN;
   if (threadIdx.x == 0) {
     a.loss[row] = static_cast<float>(loss);
     stats[kMax] = m;
@@ -829,7 +907,7 @@ __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<
     stats[kTailMax] = TAIL ? j.m : 0.0f;
     stats[kTailSum] = TAIL ? static_cast<float>(j.s) : 0.0f;
     stats[kMass] = static_cast<float>(q + rest);
-    stats[kTailGrad] = static_cast<float>((flag & 2) != 0 ? kNaN : tail_grad);
+    stats[kTailGrad] = static_cast<float>(tail_grad);
     stats[kTeacherLse] = static_cast<float>(lse);
     stats[kUnused] = 0.0f;
   }
