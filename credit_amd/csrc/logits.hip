@@ -244,19 +244,18 @@ template <class T, bool ENT, bool CAREFUL, class Dropped, class Seen>
 __device__ __forceinline__ Lane stream(const Frame& f, int b0, int b1, float c, Dropped&& dropped,
                                        Seen&& seen) {
   Lane lane = new_lane<CAREFUL>();
-  u32x4 v[2][kU<T>];
-  load_batch<T>(v[0], f, b0);
-  for (int b = b0; b < b1; b += 2) {
+  u32x4 v[kU<T>];
+  load_batch<T>(v, f, b0);
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) {
+    u32x4 next[kU<T>];
+    load_batch<T>(next, f, b + 1);  // past the row: zeros, no access
+    uint32_t drop = dropped(b);
+    if ((b == 0 && f.head != 0) || (b + 1) * kBatch > f.end) drop |= outside<T>(f, b);
+    if (__builtin_amdgcn_ballot_w64(drop != 0) != 0) hide<T>(v, drop);
+    seen(b, absorb<T, ENT, CAREFUL>(lane, c, v));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = b + h;
-      if (h == 1 && at >= b1) break;
-      load_batch<T>(v[1 - h], f, at + 1);  // past the row: zeros, no access
-      uint32_t drop = dropped(at);
-      if ((at == 0 && f.head != 0) || (at + 1) * kBatch > f.end) drop |= outside<T>(f, at);
-      if (__builtin_amdgcn_ballot_w64(drop != 0) != 0) hide<T>(v[h], drop);
-      seen(at, absorb<T, ENT, CAREFUL>(lane, c, v[h]));
-    }
+    for (int k = 0; k < kU<T>; ++k) v[k] = next[k];
   }
   return lane;
 }
@@ -285,12 +284,13 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 // While a row streams by, every lane leaves the maximum of its kLane elements of
-// each batch in LDS: a unit.  Afterwards the K-th largest of 512 group maxima
-// (each thread's units, even and odd batches) bounds the K-th largest element
-// from below, and closely: of n elements in G groups about G ln(1/(1 - K/G))
-// pass it (74 for K = 64, 355 for 256).  Only units that reach the bound are
-// read again.  What has no such bound (many equal values, a few huge units)
-// takes write_top_any, which reads the row several times.
+// each batch in LDS: a unit.  Afterwards every wave finds a bound that its share
+// of the K reaches among its 128 group maxima (a lane's units, even and odd
+// batches); the least of the waves' bounds is one that K elements of the row
+// reach, and not many more: of n elements in G groups about G ln(1/(1 - K/G))
+// pass the K-th largest group maximum (74 for K = 64 of 512).  Only units that
+// reach the bound are read again.  What has no such bound (many equal values, a
+// few crowded units) takes write_top_any, which reads the row several times.
 constexpr int kBins = 256;
 constexpr int kCands = 1024;
 constexpr int kUnitList = 1024;
@@ -299,8 +299,7 @@ struct TopSlots {
   uint32_t hist[kBins];
   uint16_t units[kUnitList];
   uint32_t n, listed, bin, above, count;
-  uint32_t wave[kNW];
-  float low[kNW];
+  uint32_t wave[kNW], bound[kNW];
 };
 // A candidate: its key above ~column, so that the larger is nearer the front.
 // They lie where the units were.
@@ -391,25 +390,37 @@ __device__ __forceinline__ Range narrow(TopSlots& s, uint32_t lo, uint32_t hi, u
   }
 }
 
-// Ranks the n candidates by counting; put(rank, key, column) for the first `top`.
+// Ranks the n candidates by counting, four lanes to a candidate; put(rank, key,
+// column) for the first `top`.
 template <class Put>
 __device__ __forceinline__ void rank_candidates(CandPtr cand, int n, int top, Put&& put) {
-  const int padded = (n + 7) & ~7;  // zeros, which are larger than none
+  const int padded = (n + 31) & ~31;  // zeros, which are larger than none
   if (static_cast<int>(threadIdx.x) < padded - n) cand[n + threadIdx.x] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t mine = cand[i];
+  const int quarter = threadIdx.x & 3;
+  for (int i0 = threadIdx.x / kWave * (kWave / 4); i0 < n; i0 += kThreads / 4) {
+    const int i = i0 + static_cast<int>(threadIdx.x & (kWave - 1)) / 4;
+    const uint64_t mine = i < n ? cand[i] : ~uint64_t{0};
     int rank = 0;
-    for (int j = 0; j < padded; j += 8)
+    for (int j = 0; j < padded; j += 32)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) rank += cand[j + k] > mine;
-    if (rank < top)
+      for (int k = 0; k < 8; ++k) rank += cand[j + 4 * k + quarter] > mine;
+    rank += __builtin_amdgcn_update_dpp(0, rank, kDppXor1, 0xf, 0xf, false);
+    rank += __builtin_amdgcn_update_dpp(0, rank, kDppXor2, 0xf, 0xf, false);
+    if (quarter == 0 && rank < top && i < n)
       put(rank, static_cast<uint32_t>(mine >> 32),
           static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(mine)));
   }
 }
-__device__ __forceinline__ void add_candidate(TopSlots& s, CandPtr cand, uint32_t key, int col) {
-  const uint32_t at = atomicAdd(&s.n, 1u);
+// The first place, in a list that *n counts, for each lane's `wanted` entries:
+// one atomic a wave.
+__device__ __forceinline__ uint32_t places(uint32_t* n, uint32_t wanted) {
+  const uint32_t upto = wave_scan(wanted);
+  uint32_t base = 0;
+  if ((threadIdx.x & (kWave - 1)) == kWave - 1) base = atomicAdd(n, upto);
+  return __builtin_amdgcn_readlane(base, kWave - 1) + upto - wanted;
+}
+__device__ __forceinline__ void put_candidate(CandPtr cand, uint32_t at, uint32_t key, int col) {
   if (at < kCands)
     cand[at] = static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(col));
 }
@@ -427,7 +438,7 @@ __device__ __forceinline__ void write_top_any(const Frame& f, int top, TopSlots&
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
   each_value<T>(f, [&](int col, uint32_t key) {
-    if (ties ? key > r.hi : key >= r.lo) add_candidate(s, cand, key, col);
+    if (ties ? key > r.hi : key >= r.lo) put_candidate(cand, atomicAdd(&s.n, 1u), key, col);
   });
   __syncthreads();
   const int n = static_cast<int>(s.n);
@@ -464,74 +475,99 @@ __device__ __forceinline__ void write_top_any(const Frame& f, int top, TopSlots&
 }
 
 // The `top` largest of a row whose units (of 2^fold batches each, `groups` of
-// them a lane) and maximum m are known.
+// them a lane) are known.  A row's end costs instructions, not traffic (five
+// workgroups a CU come to it together): hence masks and one scan for many units,
+// and vectors dealt out to whole waves.
 template <class T, class Put>
 __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPtr cand, int groups,
-                                          int fold, float m, int top, TopSlots& s, Put&& put) {
+                                          int fold, int top, TopSlots& s, Put&& put) {
+  const int wave = threadIdx.x / kWave;
   float g[2] = {kNegInf, kNegInf};
   for (int u = 0; u < groups; ++u)
     g[u & 1] = fmax_nan(g[u & 1], Elem<T>::get(units + u * kThreads + threadIdx.x));
-  // The least group maximum above -inf (NaN ones are the largest).
-  float low = __builtin_inff();
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (g[i] > kNegInf) low = __builtin_fminf(low, g[i]);
-  int full = __builtin_popcountll(__builtin_amdgcn_ballot_w64(!(g[0] <= kNegInf))) +
-             __builtin_popcountll(__builtin_amdgcn_ballot_w64(!(g[1] <= kNegInf)));
-  low = -wave_reduce(-low, MaxOp{});
-  if ((threadIdx.x & (kWave - 1)) == 0) {
-    s.low[threadIdx.x / kWave] = low;
-    s.wave[threadIdx.x / kWave] = full;
-  }
+  const uint32_t k0 = key_of(g[0]), k1 = key_of(g[1]);
+  const auto reach = [&](uint32_t t) {
+    return static_cast<uint32_t>(__builtin_popcountll(__builtin_amdgcn_ballot_w64(k0 >= t)) +
+                                 __builtin_popcountll(__builtin_amdgcn_ballot_w64(k1 >= t)));
+  };
+  // Groups of the wave that hold anything; its share of the row's `top`.
+  const uint32_t full = reach(key_of(kNegInf) + 1);
+  const float most = wave_reduce(fmax_nan(g[0], g[1]), MaxOp{});
+  // The least group maximum above -inf, of those that are no NaN.
+  const float few = -wave_reduce(fmax_nan(g[0] > kNegInf ? -g[0] : kNegInf,
+                                          g[1] > kNegInf ? -g[1] : kNegInf), MaxOp{});
+  if (threadIdx.x % kWave == 0) s.wave[wave] = full;
   if (threadIdx.x == 0) s.n = s.listed = 0;
   __syncthreads();
-  full = 0;
-  for (int w = 0; w < kNW; ++w) {
-    low = __builtin_fminf(low, s.low[w]);
-    full += s.wave[w];
-  }
+  uint32_t all = 0;
+  for (int w = 0; w < kNW; ++w) all += s.wave[w];
   uint32_t bound = 0;
-  if (full >= top) {
-    const uint32_t hi = key_of(m), lo = key_of(low) < hi ? key_of(low) : hi;
-    bound = narrow(s, lo, hi, top, top + top / 8 + 8, [&](auto&& fn) {
-              fn(key_of(g[0]));
-              fn(key_of(g[1]));
-            }).lo;
+  if (all >= static_cast<uint32_t>(top)) {
+    const uint32_t need = (top * full + all - 1) / all, enough = need + need / 4;
+    bound = 0xFFFFFFFFu;
+    if (need != 0) {
+      // Bit by bit below what the largest and the least group have in common.
+      const uint32_t hi = __builtin_amdgcn_readfirstlane(key_of(most));
+      const uint32_t lo = __builtin_amdgcn_readfirstlane(key_of(few));
+      uint32_t bit = most != most || lo > hi ? 0x80000000u
+                     : lo == hi              ? 0u
+                                             : 0x80000000u >> __builtin_clz(lo ^ hi);
+      bound = bit == 0 ? hi : hi & ~(bit | (bit - 1));
+#pragma unroll 1
+      for (uint32_t n = ~0u; n > enough && bit != 0; bit >>= 1) {
+        const uint32_t at = reach(bound | bit);
+        n = at >= need ? at : n;
+        bound |= at >= need ? bit : 0u;
+      }
+    }
+    if (threadIdx.x % kWave == 0) s.bound[wave] = bound;
+    __syncthreads();
+    for (int w = 0; w < kNW; ++w) bound = s.bound[w] < bound ? s.bound[w] : bound;
+    bound = __builtin_amdgcn_readfirstlane(bound);
   }
-  for (int u = 0; u < groups; ++u)
-    if (key_of(Elem<T>::get(units + u * kThreads + threadIdx.x)) >= bound) {
-      const uint32_t at = atomicAdd(&s.listed, 1u);
-      if (at < kUnitList) s.units[at] = static_cast<uint16_t>(u * kThreads + threadIdx.x);
+  // key >= bound, of values: all where the bound is a NaN's key or 0.
+  const float least = value_of(bound);
+  if (__builtin_amdgcn_ballot_w64(!(fmax_nan(g[0], g[1]) < least)) != 0)
+    for (int u0 = 0; u0 < groups; u0 += 32) {
+      uint32_t hits = 0;
+#pragma unroll 4
+      for (int j = 0; j < 32 && u0 + j < groups; ++j)
+        hits |= !(Elem<T>::get(units + (u0 + j) * kThreads + threadIdx.x) < least) ? 1u << j : 0u;
+      for (uint32_t at = places(&s.listed, __builtin_popcount(hits)); hits != 0;
+           hits &= hits - 1, ++at)
+        if (at < kUnitList)
+          s.units[at] =
+              static_cast<uint16_t>((u0 + __builtin_ctz(hits)) * kThreads + threadIdx.x);
     }
   __syncthreads();
   // Too many units that reach the bound: none is read, and s.n is past kCands.
   if (threadIdx.x == 0 && s.listed > kUnitList) s.n = kCands + 1;
-  const int listed = s.listed > kUnitList ? 0 : static_cast<int>(s.listed);
-  const int per = kU<T> << fold;  // vectors of a unit
-  for (int i0 = 0; i0 < listed * per; i0 += 4 * kThreads) {
-    u32x4 raw[4];
-    int vec[4];
+  constexpr int kPer = kU<T> == 4 ? 2 : 3;  // vectors of a lane in a batch: 4 or 8
+  static_assert(kU<T> == 1 << kPer);
+  const int per = kPer + fold;
+  const int vecs = (s.listed > kUnitList ? 0 : static_cast<int>(s.listed)) << per;
+#pragma unroll 1
+  for (int i0 = wave * kWave; i0 < vecs; i0 += kThreads) {
+    const int i = i0 + static_cast<int>(threadIdx.x & (kWave - 1));
+    const int unit = s.units[i < vecs ? i >> per : 0];
+    const int vec = ((unit / kThreads << per) + (i & ((1 << per) - 1))) * kThreads +
+                    unit % kThreads;
+    const u32x4 raw[1] = {buffer_load(f.r, static_cast<uint32_t>(vec) * 16u)};
+    const int e0 = vec * kN<T>;
+    float z[kN<T>];
+    unpack<T, 1>(z, raw);
+    uint32_t hits = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j * kThreads + static_cast<int>(threadIdx.x);
-      const int unit = i < listed * per ? s.units[i / per] : -1;
-      const int k = i % per;
-      vec[j] = unit < 0 ? -1
-                        : (((unit / kThreads << fold) * kU<T> + k) * kThreads + unit % kThreads);
-      raw[j] = buffer_load(f.r, static_cast<uint32_t>(vec[j]) * 16u);
-    }
+    for (int e = 0; e < kN<T>; ++e) hits |= !(z[e] < least) ? 1u << e : 0u;
+    // The row's own elements, of a vector that this lane has.
+    const int from = min(max(f.head - e0, 0), kN<T>), to = min(max(f.end - e0, 0), kN<T>);
+    hits = i < vecs && to > from ? hits & ((1u << to) - (1u << from)) : 0u;
+    for (uint32_t at = places(&s.n, __builtin_popcount(hits)); hits != 0; hits &= hits - 1, ++at) {
+      const int e = __builtin_ctz(hits);
+      float v = z[0];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (vec[j] < 0) continue;
-      const u32x4 one[1] = {raw[j]};
-      float z[kN<T>];
-      unpack<T, 1>(z, one);
-#pragma unroll
-      for (int e = 0; e < kN<T>; ++e) {
-        const int at = vec[j] * kN<T> + e;
-        const uint32_t key = key_of(z[e]);
-        if (key >= bound && at >= f.head && at < f.end) add_candidate(s, cand, key, at - f.head);
-      }
+      for (int k = 1; k < kN<T>; ++k) v = e == k ? z[k] : v;
+      put_candidate(cand, at, key_of(v), e0 + e - f.head);
     }
   }
   __syncthreads();
@@ -554,32 +590,18 @@ struct LogprobArgs {
   float* top_logp;
   int64_t* top_ids;
   int cols, n_tokens, n_top;
-  int fold;              // a unit is 2^fold batches of a lane
-  float temperature, c;  // c = log2(e) / temperature
+  int fold;      // a unit is 2^fold batches of a lane
+  float c;       // log2(e) / temperature
+  double inv_t;
 };
 
-template <class T, bool ENT>
-__device__ __forceinline__ void logprob_outputs(const LogprobArgs<T>& a, int64_t row, const T* z,
-                                                const Joined& j, double ln_s) {
-  const bool empty = j.m == kNegInf;
-  if (threadIdx.x == 0) {
-    a.stats[2 * row] = j.m;
-    a.stats[2 * row + 1] = static_cast<float>(j.s);
-    if (ENT) a.entropy[row] = empty ? 0.0f : static_cast<float>(ln_s - kLn2 * j.t / j.s);
-  }
-  for (int k = threadIdx.x; k < a.n_tokens; k += kThreads) {
-    const int64_t tok = a.tokens[row * a.n_tokens + k];
-    float lp = 0.0f;
-    if (tok >= a.cols) {
-      lp = kNaN;
-    } else if (tok >= 0) {
-      const float v = Elem<T>::get(z + tok);
-      lp = v == kNegInf && ln_s == ln_s
-               ? kNegInf
-               : static_cast<float>((static_cast<double>(v) - j.m) / a.temperature - ln_s);
-    }
-    a.logp[row * a.n_tokens + k] = lp;
-  }
+// ln s of s >= 1 to 4e-8: the exponent's part in 64 bits, that of a mantissa in
+// [1/sqrt 2, sqrt 2) by logf.
+__device__ __forceinline__ double ln_sum(double s) {
+  int e;
+  double m = ::frexp(s, &e);
+  if (m < 0.70710678118654752) m *= 2.0, e -= 1;
+  return e * kLn2 + static_cast<double>(::logf(static_cast<float>(m)));
 }
 
 template <class T, bool ENT, bool TOP>
@@ -589,6 +611,13 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
   T* units = reinterpret_cast<T*>(dynamic_lds);
   const int64_t row = blockIdx.x;
   const T* z = a.logits + row * a.ld;
+  // The thread's token, read ahead of the row.
+  int64_t token = -1;
+  float chosen = kNaN;  // a token >= cols
+  if (static_cast<int>(threadIdx.x) < a.n_tokens) {
+    token = a.tokens[row * a.n_tokens + threadIdx.x];
+    if (token >= 0 && token < a.cols) chosen = Elem<T>::get(z + token);
+  }
   const Frame f = frame_of(z, a.cols);
   const int batches = (f.end + kBatch - 1) / kBatch;
   float unit = kNegInf;
@@ -601,21 +630,35 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
           put_unit(units + (b >> a.fold) * kThreads + threadIdx.x, unit);
         }
       });
-  const double ln_s = j.m == kNegInf ? 0.0 : ::log(j.s);
-  logprob_outputs<T, ENT>(a, row, z, j, ln_s);
+  __shared__ double shared_ln_s;
+  if (threadIdx.x < kWave) {
+    const bool empty = j.m == kNegInf;
+    const double ln_s = empty ? 0.0 : j.s == j.s ? ln_sum(j.s) : j.s;
+    if (threadIdx.x == 0) {
+      shared_ln_s = ln_s;
+      a.stats[2 * row] = j.m;
+      a.stats[2 * row + 1] = static_cast<float>(j.s);
+      if (ENT) a.entropy[row] = empty ? 0.0f : static_cast<float>(ln_s - kLn2 * j.t / j.s);
+    }
+  }
+  const auto log_p = [&](float v) {
+    const double ln_s = shared_ln_s;
+    return v == kNegInf && ln_s == ln_s
+               ? kNegInf
+               : static_cast<float>((static_cast<double>(v) - j.m) * a.inv_t - ln_s);
+  };
   if constexpr (TOP) {
     __shared__ TopSlots top;
-    write_top<T>(f, units, (CandPtr)(dynamic_lds), (batches + (1 << a.fold) - 1) >> a.fold, a.fold, j.m, a.n_top, top,
-                 [&](int rank, uint32_t key, int col) {
-                   const float v = value_of(key);
-                   a.top_logp[row * a.n_top + rank] =
-                       v == kNegInf && ln_s == ln_s
-                           ? kNegInf
-                           : static_cast<float>(
-                                 (static_cast<double>(v) - j.m) / a.temperature - ln_s);
+    write_top<T>(f, units, (CandPtr)(dynamic_lds), (batches + (1 << a.fold) - 1) >> a.fold, a.fold,
+                 a.n_top, top, [&](int rank, uint32_t key, int col) {
+                   a.top_logp[row * a.n_top + rank] = log_p(value_of(key));
                    a.top_ids[row * a.n_top + rank] = col;
                  });
+  } else {
+    __syncthreads();
   }
+  if (static_cast<int>(threadIdx.x) < a.n_tokens)
+    a.logp[row * a.n_tokens + threadIdx.x] = token < 0 ? 0.0f : log_p(chosen);
 }
 
 // ------------------------------------------------------------- gradients --
@@ -1094,8 +1137,8 @@ int logprob_fwd(const T* logits, int64_t ld, const int64_t* tokens, float* logp,
                          n_tokens,
                          n_top,
                          fold,
-                         temperature,
-                         log2e_over(temperature)};
+                         log2e_over(temperature),
+                         1.0 / static_cast<double>(temperature)};
   const unsigned grid = static_cast<unsigned>(rows);
   hipStream_t stream = cfg_stream(cfg);
   const auto launch = [&](auto ent, auto top) {
