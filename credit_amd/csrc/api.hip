@@ -10,6 +10,7 @@
 
 #include "api_internal.hpp"
 #include "common.hpp"
+#include "logits_rules.hpp"
 #include "workspace_cache.hpp"
 
 namespace credit {
@@ -500,6 +501,12 @@ size_t credit_workspace_bytes(int32_t op, int64_t rows, int64_t cols,
       break;
     case CREDIT_OP_PEARSON_BWD:
       body = pearson_bwd_workspace(rows, cols, variant, split, cus);
+      break;
+    case CREDIT_OP_TOKEN_LOGPROB_FWD:
+    case CREDIT_OP_TOPK_DISTILL_FWD:
+      body = logits::workspace(rows, cols, variant == CREDIT_VARIANT_READ,
+                               variant == CREDIT_VARIANT_SPLIT ? split : 0,
+                               op == CREDIT_OP_TOKEN_LOGPROB_FWD);
       break;
     default:
       body = 0;

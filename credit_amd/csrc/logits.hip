@@ -21,6 +21,7 @@
 
 #include "api_internal.hpp"
 #include "common.hpp"
+#include "logits_rules.hpp"
 #include "rows.hpp"
 
 namespace credit {
@@ -267,6 +268,71 @@ __device__ __forceinline__ Joined scan(const Frame& f, int b0, int b1, float c, 
   __syncthreads();
   return join_lanes<true>(stream<T, ENT, true>(f, b0, b1, c, dropped, seen), c, slots);
 }
+// ------------------------------------------------ a row in several parts --
+// Few rows leave most CUs idle on a workgroup each, and one CU draws a row at 70
+// GB/s.  A row is then cut into parts of whole batches; each leaves its result
+// (and its units) in the workspace, and the part that finds all others arrived
+// joins them and goes on as a whole row's workgroup does.  Nothing waits for
+// another workgroup; the row's counter is 0 again afterwards.  Published and
+// read past the L2s, as the exchange of the SPLIT kernels (common.hpp).
+constexpr int kMaxParts = kWave;  // a lane each where they are joined
+constexpr int kPartValues = 4;    // m, s, t, whether a column was named twice
+struct Parts {
+  int n = 1, batches = 0;     // parts of a row, batches of a part
+  double* values = nullptr;   // [row][part][kPartValues]
+  float* units = nullptr;     // [row][batch][lane]
+  uint32_t* arrived = nullptr;  // kGroupCounterStride apart
+};
+// Every thread, with what the workgroup has published; true for the last part.
+__device__ __forceinline__ bool last_part(const Parts& p, int64_t row) {
+  __shared__ int last;
+  publish_wait();
+  lds_barrier();
+  if (threadIdx.x == 0) {
+    uint32_t* arrived = p.arrived + row * kGroupCounterStride;
+    last = arrive(arrived) == static_cast<uint32_t>(p.n - 1);
+    if (last) counter_reset(arrived);
+  }
+  __syncthreads();
+  return last != 0;
+}
+__device__ __forceinline__ void publish_part(const Parts& p, int64_t row, const Joined& j,
+                                             bool repeated) {
+  if (threadIdx.x != 0) return;
+  double* v = p.values + (row * p.n + blockIdx.x) * kPartValues;
+  publish(v, static_cast<double>(j.m));
+  publish(v + 1, j.s);
+  publish(v + 2, j.t);
+  publish(v + 3, repeated ? 1.0 : 0.0);
+}
+// All parts' results joined, in every thread.
+__device__ __forceinline__ Joined join_parts(const Parts& p, int64_t row, double inv_t,
+                                             bool* repeated) {
+  const int lane = threadIdx.x & (kWave - 1);
+  float m = kNegInf;
+  double s = 0.0, t = 0.0, twice = 0.0;
+  if (lane < p.n) {
+    const double* v = p.values + (row * p.n + lane) * kPartValues;
+    m = static_cast<float>(fetch(v));
+    s = fetch(v + 1);
+    t = fetch(v + 2);
+    twice = fetch(v + 3);
+  }
+  Joined j;
+  j.m = wave_reduce(m, MaxOp{});
+  if (s != 0.0) {
+    const double d = (static_cast<double>(m) - j.m) * inv_t;
+    const double f = ::exp(d);
+    t = f == 0.0 ? 0.0 : f * (t + d / kLn2 * s);
+    s *= f;
+  }
+  j.s = wave_reduce_sum_f64(s);
+  j.t = wave_reduce_sum_f64(t);
+  if (j.m != j.m) j.s = kNaN;
+  *repeated = __builtin_amdgcn_ballot_w64(twice != 0.0) != 0;
+  return j;
+}
+
 __device__ __forceinline__ uint32_t none_dropped(int) { return 0; }
 __device__ __forceinline__ void unseen(int, float) {}
 
@@ -593,6 +659,7 @@ struct LogprobArgs {
   int fold;      // a unit is 2^fold batches of a lane
   float c;       // log2(e) / temperature
   double inv_t;
+  Parts parts;
 };
 
 // ln s of s >= 1 to 4e-8: the exponent's part in 64 bits, that of a mantissa in
@@ -604,12 +671,12 @@ __device__ __forceinline__ double ln_sum(double s) {
   return e * kLn2 + static_cast<double>(::logf(static_cast<float>(m)));
 }
 
-template <class T, bool ENT, bool TOP>
+template <class T, bool ENT, bool TOP, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs<T> a) {
   extern __shared__ __attribute__((aligned(16))) char dynamic_lds[];
   __shared__ JoinSlots join;
   T* units = reinterpret_cast<T*>(dynamic_lds);
-  const int64_t row = blockIdx.x;
+  const int64_t row = SPLIT ? blockIdx.y : blockIdx.x;
   const T* z = a.logits + row * a.ld;
   // The thread's token, read ahead of the row.
   int64_t token = -1;
@@ -620,16 +687,44 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
   }
   const Frame f = frame_of(z, a.cols);
   const int batches = (f.end + kBatch - 1) / kBatch;
-  float unit = kNegInf;
-  const Joined j = scan<T, ENT>(
-      f, 0, batches, a.c, join, none_dropped,
-      [&](int b, float bm) {
-        if constexpr (TOP) {
+  const int groups = (batches + (1 << a.fold) - 1) >> a.fold;
+  Joined j;
+  if constexpr (SPLIT) {
+    const int b0 = blockIdx.x * a.parts.batches, b1 = min(b0 + a.parts.batches, batches);
+    float* out = a.parts.units + (row * a.parts.n * a.parts.batches) * kThreads + threadIdx.x;
+    j = scan<T, ENT>(f, b0, b1, a.c, join, none_dropped, [&](int b, float bm) {
+      if constexpr (TOP) publish(out + b * kThreads, bm);
+    });
+    publish_part(a.parts, row, j, false);
+    if (!last_part(a.parts, row)) return;
+    bool unused;
+    j = join_parts(a.parts, row, a.inv_t, &unused);
+    if constexpr (TOP) {
+      float unit = kNegInf;
+      for (int b0 = 0; b0 < batches; b0 += 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fetch(out + min(b0 + i, batches - 1) * kThreads);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int b = b0 + i;
+          if (b >= batches) break;
           if ((b & ((1 << a.fold) - 1)) == 0) unit = kNegInf;
-          unit = fmax_nan(unit, bm);
+          unit = fmax_nan(unit, v[i]);
           put_unit(units + (b >> a.fold) * kThreads + threadIdx.x, unit);
         }
-      });
+      }
+    }
+  } else {
+    float unit = kNegInf;
+    j = scan<T, ENT>(f, 0, batches, a.c, join, none_dropped, [&](int b, float bm) {
+      if constexpr (TOP) {
+        if ((b & ((1 << a.fold) - 1)) == 0) unit = kNegInf;
+        unit = fmax_nan(unit, bm);
+        put_unit(units + (b >> a.fold) * kThreads + threadIdx.x, unit);
+      }
+    });
+  }
   __shared__ double shared_ln_s;
   if (threadIdx.x < kWave) {
     const bool empty = j.m == kNegInf;
@@ -649,8 +744,7 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
   };
   if constexpr (TOP) {
     __shared__ TopSlots top;
-    write_top<T>(f, units, (CandPtr)(dynamic_lds), (batches + (1 << a.fold) - 1) >> a.fold, a.fold,
-                 a.n_top, top, [&](int rank, uint32_t key, int col) {
+    write_top<T>(f, units, (CandPtr)(dynamic_lds), groups, a.fold, a.n_top, top, [&](int rank, uint32_t key, int col) {
                    a.top_logp[row * a.n_top + rank] = log_p(value_of(key));
                    a.top_ids[row * a.n_top + rank] = col;
                  });
@@ -821,28 +915,30 @@ struct DistillArgs {
   float* stats;
   int cols, n_top;
   float temperature, c;
+  Parts parts;
 };
 // Row statistics [rows, 8] for the backward.
 enum DistillStat { kMax, kSum, kTailMax, kTailSum, kMass, kTailGrad, kTeacherLse, kUnused };
 
-// Marks element e of the frame; whether it was marked before.
+// Marks element e of the frame if it lies in batches [b0, b1); whether it was
+// marked before.
 template <class T>
-__device__ __forceinline__ bool mark(uint32_t* bits, int e, int seg) {
+__device__ __forceinline__ bool mark(uint32_t* bits, int e, int b0, int b1) {
   const int v = e / kN<T>;
-  const int b = v / (kThreads * kU<T>) - seg * kSegBatches;
-  if (b < 0 || b >= kSegBatches) return false;
+  const int b = v / (kThreads * kU<T>);
+  if (b < b0 || b >= b1) return false;
   const uint32_t bit = 1u << (v / kThreads % kU<T> * kN<T> + e % kN<T>);
-  return (atomicOr(&bits[b * kThreads + v % kThreads], bit) & bit) != 0;
+  return (atomicOr(&bits[(b - b0) * kThreads + v % kThreads], bit) & bit) != 0;
 }
 
-template <class T, bool TAIL>
+template <class T, bool TAIL, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<T> a) {
   __shared__ JoinSlots join;
   __shared__ float max_slots[2][kNW];
   __shared__ double sum_slots[4][kNW];
   __shared__ int flags[kNW];
   __shared__ int repeated;
-  const int64_t row = blockIdx.x;
+  const int64_t row = SPLIT ? blockIdx.y : blockIdx.x;
   const T* z = a.logits + row * a.ld;
   const int k = threadIdx.x;
   // The thread's entry.
@@ -864,6 +960,7 @@ __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<
   for (int w = 0; w < kNW; ++w) flag |= flags[w];
   float* stats = a.stats + 8 * row;
   if (flag == 0 || (!TAIL && tm == kNegInf)) {  // no entry to learn from
+    if (SPLIT && blockIdx.x != 0) return;
     if (threadIdx.x == 0) a.loss[row] = 0.0f;
     if (threadIdx.x < 8) stats[threadIdx.x] = 0.0f;
     return;
@@ -872,31 +969,40 @@ __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<
 
   const Frame f = frame_of(z, a.cols);
   const int batches = (f.end + kBatch - 1) / kBatch;
-  bool first = live;  // of the entries that name one column
-  Joined j;
+  const int first_batch = SPLIT ? blockIdx.x * a.parts.batches : 0;
+  const int end_batch = SPLIT ? min(first_batch + a.parts.batches, batches) : batches;
+  Joined j{kNegInf, 0.0, 0.0};  // of a part without batches
   if constexpr (TAIL) {
     __shared__ uint32_t bits[kSegWords];
     // The segments' results joined as the lanes' are.
-    for (int b0 = 0; b0 < batches; b0 += kSegBatches) {
-      const int b1 = b0 + kSegBatches < batches ? b0 + kSegBatches : batches;
-      if (b0 != 0) __syncthreads();
+    for (int b0 = first_batch; b0 < end_batch; b0 += kSegBatches) {
+      const int b1 = min(b0 + kSegBatches, end_batch);
+      if (b0 != first_batch) __syncthreads();
       for (int b = 0; b < b1 - b0; ++b) bits[b * kThreads + threadIdx.x] = 0;
       __syncthreads();
-      if (live && mark<T>(bits, static_cast<int>(id) + f.head, b0 / kSegBatches)) repeated = 1;
+      if (live && mark<T>(bits, static_cast<int>(id) + f.head, b0, b1)) repeated = 1;
       __syncthreads();
       const Joined p = scan<T, false>(
           f, b0, b1, a.c, join, [&](int b) { return bits[(b - b0) * kThreads + threadIdx.x]; },
           unseen);
-      j = b0 == 0 ? p : merge(j, p, a.temperature);
-    }
-    if (repeated != 0) {  // the lowest of those that name the column counts
-      __shared__ int ids[kMaxEntries];
-      ids[k] = live ? static_cast<int>(id) : -1;
-      __syncthreads();
-      for (int i = 0; i < k && first; ++i) first = ids[i] != static_cast<int>(id);
+      j = b0 == first_batch ? p : merge(j, p, a.temperature);
     }
   } else {
-    j = scan<T, false>(f, 0, batches, a.c, join, none_dropped, unseen);
+    j = scan<T, false>(f, first_batch, end_batch, a.c, join, none_dropped, unseen);
+  }
+  bool twice = TAIL && repeated != 0;
+  if constexpr (SPLIT) {
+    j.t = 0.0;
+    publish_part(a.parts, row, j, twice);
+    if (!last_part(a.parts, row)) return;
+    j = join_parts(a.parts, row, 1.0 / static_cast<double>(a.temperature), &twice);
+  }
+  bool first = live;  // of the entries that name one column: the lowest counts
+  if (TAIL && twice) {
+    __shared__ int ids[kMaxEntries];
+    ids[k] = live ? static_cast<int>(id) : -1;
+    __syncthreads();
+    for (int i = 0; i < k && first; ++i) first = ids[i] != static_cast<int>(id);
   }
 
   // Over the entries, in one go: the mass that the row has outside the tail,
@@ -1041,6 +1147,19 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
 }
 
 // ---------------------------------------------------------------- host ----
+using logits::kMaxSplitRows;
+using logits::part_values_bytes;
+using logits::parts_bytes;
+static_assert(kMaxSplitRows <= kMaxGroupsPerLaunch);
+static_assert(logits::kMaxParts == kMaxParts && logits::kPartValues == kPartValues &&
+              logits::kBatch == kBatch && logits::kThreads == kThreads);
+// Batches of the widest frame that a row of this alignment has.
+template <class T>
+int64_t row_batches(const T* logits, int64_t ld, int64_t rows, int64_t cols) {
+  const bool lines = reinterpret_cast<uintptr_t>(logits) % 16 == 0 &&
+                     (rows == 1 || ld * static_cast<int64_t>(sizeof(T)) % 16 == 0);
+  return (cols + (lines ? 0 : kN<T> - 1) + kBatch - 1) / kBatch;
+}
 int check_logits(const void* p, const char* name, int64_t ld, int64_t rows, int64_t cols,
                  size_t elem) {
   CREDIT_TRY(check_row_ptr(p, name, rows));
@@ -1065,11 +1184,42 @@ int check_temperature(float t) {
                      static_cast<double>(t));
   return CREDIT_OK;
 }
-int check_variant(const credit_cfg* cfg) {
+int check_variant(const credit_cfg* cfg, bool forward) {
   CREDIT_TRY(check_cfg(cfg));
   const int v = cfg_variant(cfg);
-  if (v != CREDIT_VARIANT_AUTO && v != CREDIT_VARIANT_READ)
-    return set_error(CREDIT_ERR_UNSUPPORTED, "the logits operators have no variant %d", v);
+  if (v == CREDIT_VARIANT_STAGED || (v == CREDIT_VARIANT_SPLIT && !forward))
+    return set_error(CREDIT_ERR_UNSUPPORTED, "this logits operator has no variant %d", v);
+  return CREDIT_OK;
+}
+
+// Parts of a row that the call takes (parts->n 1: one workgroup a row), with
+// their workspace.  `units`: also the units'.
+int plan_parts(const credit_cfg* cfg, int64_t rows, int64_t batches, bool units, Parts* parts) {
+  const int variant = cfg_variant(cfg);
+  const int64_t want = variant == CREDIT_VARIANT_READ ? 1
+                       : variant == CREDIT_VARIANT_SPLIT && cfg_split(cfg) > 0
+                           ? cfg_split(cfg)
+                           : logits::auto_parts(rows, batches, units);
+  const int64_t each = (batches + want - 1) / want;
+  const int64_t n = (batches + each - 1) / each;
+  if (n < 2 || rows > kMaxSplitRows) return CREDIT_OK;
+  if (cfg == nullptr || cfg->workspace == nullptr) {
+    // A graph replays on any stream, beside the eager calls of the one it was
+    // captured on: it may not share that one's workspace.
+    if (!keeps_scratch(cfg_stream(cfg))) {
+      if (variant == CREDIT_VARIANT_SPLIT)
+        return set_error(CREDIT_ERR_WORKSPACE,
+                         "SPLIT under capture or on the per-thread stream needs cfg->workspace");
+      return CREDIT_OK;
+    }
+  }
+  char* base = nullptr;
+  CREDIT_TRY(acquire_workspace(cfg, parts_bytes(rows, n, each, units), &base));
+  parts->n = static_cast<int>(n);
+  parts->batches = static_cast<int>(each);
+  parts->values = reinterpret_cast<double*>(ws_scratch(base));
+  parts->units = reinterpret_cast<float*>(ws_scratch(base) + part_values_bytes(rows, n));
+  parts->arrived = ws_counters(base) + kGroupCounterBase;
   return CREDIT_OK;
 }
 float log2e_over(float temperature) {
@@ -1096,6 +1246,17 @@ dim3 grad_grid(int64_t rows, int64_t cols) {
   return dim3(static_cast<unsigned>(parts), static_cast<unsigned>(rows < 65535 ? rows : 65535));
 }
 
+// fn(bool_constant...) for the values of `flags`.
+template <class Fn, class... Flags>
+void choose(Fn&& fn, bool flag, Flags... flags) {
+  if constexpr (sizeof...(flags) == 0) {
+    flag ? fn(std::true_type{}) : fn(std::false_type{});
+  } else {
+    choose([&](auto... rest) { flag ? fn(std::true_type{}, rest...) : fn(std::false_type{}, rest...); },
+           flags...);
+  }
+}
+
 template <class T>
 int logprob_fwd(const T* logits, int64_t ld, const int64_t* tokens, float* logp, float* stats,
                 float* entropy, float* top_logp, int64_t* top_ids, int64_t rows, int64_t cols,
@@ -1114,41 +1275,34 @@ int logprob_fwd(const T* logits, int64_t ld, const int64_t* tokens, float* logp,
     CREDIT_TRY(check_row_ptr(top_ids, "top_ids", rows));
   }
   CREDIT_TRY(check_temperature(temperature));
-  CREDIT_TRY(check_variant(cfg));
+  CREDIT_TRY(check_variant(cfg, true));
   if (rows == 0) return CREDIT_OK;
-  const int64_t batches = (cols + kN<T> - 1 + kBatch - 1) / kBatch;
-  int fold = 0;
+  LogprobArgs<T> a{logits,   ld,
+                   tokens,   logp,
+                   stats,    entropy,
+                   top_logp, top_ids,
+                   static_cast<int>(cols),
+                   n_tokens, n_top,
+                   0,        log2e_over(temperature),
+                   1.0 / static_cast<double>(temperature),
+                   Parts{}};
+  const int64_t batches = row_batches(logits, ld, rows, cols);
+  CREDIT_TRY(plan_parts(cfg, rows, batches, n_top > 0, &a.parts));
   const auto unit_bytes = [&] {
-    return static_cast<size_t>((batches + (int64_t{1} << fold) - 1) >> fold) * kThreads * sizeof(T);
+    return static_cast<size_t>((batches + (int64_t{1} << a.fold) - 1) >> a.fold) * kThreads *
+           sizeof(T);
   };
-  while (unit_bytes() > kMaxUnitBytes) ++fold;
+  while (unit_bytes() > kMaxUnitBytes) ++a.fold;
   // The candidates take the units' place once those are listed.
-  const size_t lds = unit_bytes() < kCands * sizeof(uint64_t) ? kCands * sizeof(uint64_t)
-                                                               : unit_bytes();
-  const LogprobArgs<T> a{logits,
-                         ld,
-                         tokens,
-                         logp,
-                         stats,
-                         entropy,
-                         top_logp,
-                         top_ids,
-                         static_cast<int>(cols),
-                         n_tokens,
-                         n_top,
-                         fold,
-                         log2e_over(temperature),
-                         1.0 / static_cast<double>(temperature)};
-  const unsigned grid = static_cast<unsigned>(rows);
+  const size_t lds = n_top > 0 ? std::max(unit_bytes(), size_t{kCands} * sizeof(uint64_t)) : 0;
   hipStream_t stream = cfg_stream(cfg);
-  const auto launch = [&](auto ent, auto top) {
-    token_logprob_fwd_kernel<T, decltype(ent)::value, decltype(top)::value>
-        <<<grid, kThreads, n_top > 0 ? lds : 0, stream>>>(a);
+  const auto launch = [&](auto ent, auto top, auto split) {
+    const dim3 grid = decltype(split)::value ? dim3(a.parts.n, static_cast<unsigned>(rows))
+                                             : dim3(static_cast<unsigned>(rows));
+    token_logprob_fwd_kernel<T, decltype(ent)::value, decltype(top)::value,
+                             decltype(split)::value><<<grid, kThreads, lds, stream>>>(a);
   };
-  const auto with_top = [&](auto ent) {
-    n_top > 0 ? launch(ent, std::true_type{}) : launch(ent, std::false_type{});
-  };
-  entropy != nullptr ? with_top(std::true_type{}) : with_top(std::false_type{});
+  choose(launch, entropy != nullptr, n_top > 0, a.parts.n > 1);
   return check_launch("token_logprob_fwd_kernel");
 }
 
@@ -1168,7 +1322,7 @@ int logprob_bwd(const T* logits, int64_t ld, const int64_t* tokens, const float*
   }
   if (dentropy != nullptr) CREDIT_TRY(check_row_ptr(entropy, "entropy", rows));
   CREDIT_TRY(check_temperature(temperature));
-  CREDIT_TRY(check_variant(cfg));
+  CREDIT_TRY(check_variant(cfg, false));
   if (rows == 0) return CREDIT_OK;
   CREDIT_TRY(check_overlap(logits, ld, dlogits, ldd, rows, cols, sizeof(T)));
   const LogprobGradArgs<T> a{logits,
@@ -1191,11 +1345,7 @@ int logprob_bwd(const T* logits, int64_t ld, const int64_t* tokens, const float*
     token_logprob_bwd_kernel<T, decltype(ent)::value, decltype(vec)::value>
         <<<grid, kThreads, 0, stream>>>(a);
   };
-  const bool vec = alike(logits, ld, dlogits, ldd, rows, sizeof(T));
-  const auto with_vec = [&](auto ent) {
-    vec ? launch(ent, std::true_type{}) : launch(ent, std::false_type{});
-  };
-  dentropy != nullptr ? with_vec(std::true_type{}) : with_vec(std::false_type{});
+  choose(launch, dentropy != nullptr, alike(logits, ld, dlogits, ldd, rows, sizeof(T)));
   return check_launch("token_logprob_bwd_kernel");
 }
 
@@ -1211,16 +1361,21 @@ int distill_fwd(const T* logits, int64_t ld, const int64_t* ids, const float* te
   CREDIT_TRY(check_row_ptr(loss, "loss", rows));
   CREDIT_TRY(check_row_ptr(stats, "stats", rows));
   CREDIT_TRY(check_temperature(temperature));
-  CREDIT_TRY(check_variant(cfg));
+  CREDIT_TRY(check_variant(cfg, true));
   if (rows == 0) return CREDIT_OK;
-  const DistillArgs<T> a{logits, ld,    ids, teacher,     loss, stats, static_cast<int>(cols),
-                         n_top,  temperature, log2e_over(temperature)};
-  const unsigned grid = static_cast<unsigned>(rows);
+  DistillArgs<T> a{logits, ld,    ids,         teacher,
+                   loss,   stats, static_cast<int>(cols),
+                   n_top,  temperature, log2e_over(temperature),
+                   Parts{}};
+  CREDIT_TRY(plan_parts(cfg, rows, row_batches(logits, ld, rows, cols), false, &a.parts));
   hipStream_t stream = cfg_stream(cfg);
-  if (tail != 0)
-    topk_distill_fwd_kernel<T, true><<<grid, kThreads, 0, stream>>>(a);
-  else
-    topk_distill_fwd_kernel<T, false><<<grid, kThreads, 0, stream>>>(a);
+  const auto launch = [&](auto has_tail, auto split) {
+    const dim3 grid = decltype(split)::value ? dim3(a.parts.n, static_cast<unsigned>(rows))
+                                             : dim3(static_cast<unsigned>(rows));
+    topk_distill_fwd_kernel<T, decltype(has_tail)::value, decltype(split)::value>
+        <<<grid, kThreads, 0, stream>>>(a);
+  };
+  choose(launch, tail != 0, a.parts.n > 1);
   return check_launch("topk_distill_fwd_kernel");
 }
 
@@ -1238,7 +1393,7 @@ int distill_bwd(const T* logits, int64_t ld, const int64_t* ids, const float* te
   CREDIT_TRY(check_row_ptr(stats, "stats", rows));
   CREDIT_TRY(check_row_ptr(dloss, "dloss", rows));
   CREDIT_TRY(check_temperature(temperature));
-  CREDIT_TRY(check_variant(cfg));
+  CREDIT_TRY(check_variant(cfg, false));
   if (rows == 0) return CREDIT_OK;
   CREDIT_TRY(check_overlap(logits, ld, dlogits, ldd, rows, cols, sizeof(T)));
   const DistillGradArgs<T> a{logits,
@@ -1260,11 +1415,7 @@ int distill_bwd(const T* logits, int64_t ld, const int64_t* ids, const float* te
     topk_distill_bwd_kernel<T, decltype(has_tail)::value, decltype(vec)::value>
         <<<grid, kThreads, 0, stream>>>(a);
   };
-  const bool vec = alike(logits, ld, dlogits, ldd, rows, sizeof(T));
-  const auto with_vec = [&](auto has_tail) {
-    vec ? launch(has_tail, std::true_type{}) : launch(has_tail, std::false_type{});
-  };
-  tail != 0 ? with_vec(std::true_type{}) : with_vec(std::false_type{});
+  choose(launch, tail != 0, alike(logits, ld, dlogits, ldd, rows, sizeof(T)));
   return check_launch("topk_distill_bwd_kernel");
 }
 

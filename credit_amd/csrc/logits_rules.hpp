@@ -1,0 +1,66 @@
+// How the forwards of the operators on logits (logits.hip) cut rows into parts,
+// and the workspace that takes.  Host arithmetic alone, so that the CPU tests
+// build it with g++ (tests/cpp/logits_rules_query.cpp).
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+namespace credit {
+namespace logits {
+
+constexpr int kThreads = 256;
+constexpr int kBatch = 8192;    // columns that a workgroup takes at once
+constexpr int kMaxParts = 64;   // of a row
+constexpr int kPartValues = 4;  // fp64 values a part leaves
+constexpr int64_t kMaxSplitRows = 1024;
+
+// Parts of a row of `batches` batches; 1: one workgroup a row.  As many as give
+// every CU a workgroup, where that saves a part four batches or more: a batch is
+// 0.5 us of a lone workgroup's time, the meeting of the parts 1.5 us.  us a call,
+// one workgroup a row -> parts:
+//   distillation with tail   1 x 131072 bf16 14.7 -> 7.5, 64 x 131072 16.3 -> 11.0,
+//                            128 x 131072 16.3 -> 13.6, 16 x 262144 fp32 28.6 -> 10.0
+//   but 64 x 32768 fp32 (4 batches) 8.9 -> 9.8; 256 rows of either, two parts: 17 -> 18
+// With alternatives the last part reads every lane's maxima back, which takes
+// more: 1 x 131072 15.1 -> 10.0, 64 x 131072 17.3 -> 15.3, 128 x 131072 17.6 ->
+// 18.6, 1 x 32768 fp32 8.6 -> 9.4.
+inline int64_t auto_parts(int64_t rows, int64_t batches, bool alternatives) {
+  if (alternatives && rows > 64) return 1;
+  const int64_t parts =
+      std::min<int64_t>({kMaxParts, batches, std::max<int64_t>(1, 256 / std::max<int64_t>(1, rows))});
+  const int64_t saved = batches - (batches + parts - 1) / parts;
+  return saved >= (alternatives ? 5 : 4) ? parts : 1;
+}
+
+inline size_t part_values_bytes(int64_t rows, int64_t parts) {
+  return (static_cast<size_t>(rows * parts) * kPartValues * sizeof(double) + 255) / 256 * 256;
+}
+// Scratch of a call whose rows are in `parts` of `batches` batches each.
+inline size_t parts_bytes(int64_t rows, int64_t parts, int64_t batches, bool alternatives) {
+  return part_values_bytes(rows, parts) +
+         (alternatives ? static_cast<size_t>(rows * parts * batches) * kThreads * sizeof(float)
+                       : 0);
+}
+
+// Scratch that any call of this shape can take, whatever its type and alignment:
+// a row's batches are at most one more than its columns fill, its parts at most
+// `split` (0: as AUTO takes them, with alternatives or without).
+inline size_t workspace(int64_t rows, int64_t cols, int variant_read, int64_t split,
+                        bool alternatives) {
+  size_t most = 0;
+  for (int64_t batches : {(cols + kBatch - 1) / kBatch, (cols + 7 + kBatch - 1) / kBatch})
+    for (bool top : {false, alternatives}) {
+      const int64_t want =
+          variant_read ? 1 : split > 0 ? split : auto_parts(rows, batches, top);
+      const int64_t each = (batches + want - 1) / want, n = (batches + each - 1) / each;
+      if (n >= 2 && rows <= kMaxSplitRows)
+        most = std::max(most, parts_bytes(rows, n, each, top));
+    }
+  return most;
+}
+
+}  // namespace logits
+}  // namespace credit

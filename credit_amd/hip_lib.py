@@ -252,12 +252,19 @@ def make_cfg(
     return cfg
 
 
+# The cfg argument of calls that give none: the stream alone, never written to.
+_STREAM_CFGS: dict[int, object] = {}
+
+
 def _cfg_ref(cfg: CreditCfg | None, device: int):
     """The cfg argument of a call: the caller's, or the current stream alone."""
-    if cfg is None:
-        cfg = CreditCfg()
-        cfg.stream = torch.cuda.current_stream(device).cuda_stream or None
-    return ctypes.byref(cfg)
+    if cfg is not None:
+        return ctypes.byref(cfg)
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    ref = _STREAM_CFGS.get(stream)
+    if ref is None:
+        ref = _STREAM_CFGS[stream] = ctypes.byref(CreditCfg(stream or None))
+    return ref
 
 
 def workspace_bytes(op: str, rows: int, cols: int, variant: str = "auto", split: int = 0) -> int:
@@ -622,21 +629,22 @@ def _logits_call(op: str, logits: torch.Tensor) -> tuple[int, int, int, int, Cal
         raise ValueError(f"logits: tensor must be on a GPU, got {logits.device}")
     if device != torch.cuda.current_device():
         raise ValueError(f"logits: on {logits.device}, which is not the current device")
-    return rows, cols, ld, device, getattr(load_library(), f"credit_{op}_{suffix}")
+    return rows, cols, ld, device, getattr(load_library(), op + suffix)
 
 
 def _operand(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, ...],
              device: int) -> int:
     """Address of a contiguous operand of exactly this type, shape and device."""
+    if (t.dtype is dtype and t.shape == shape and t.is_contiguous()
+            and t.get_device() == device):
+        return t.data_ptr()
     if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: tensor must be contiguous")
-    if t.get_device() != device:
-        raise ValueError(f"{name}: expected a tensor on the logits' device, got {t.device}")
-    return t.data_ptr()
+    raise ValueError(f"{name}: expected a tensor on the logits' device, got {t.device}")
 
 
 def _gradient(dlogits: torch.Tensor, logits: torch.Tensor, device: int) -> tuple[int, int]:
@@ -663,7 +671,7 @@ def token_logprob_fwd(logits: torch.Tensor, tokens: torch.Tensor, logp: torch.Te
     backward) and, where given, entropy [rows] and the most likely
     alternatives, top_logp and top_ids (int64) [rows, k], in falling order,
     equal ones by column.  All fp32 but the columns."""
-    rows, cols, ld, dev, fn = _logits_call("token_logprob_fwd", logits)
+    rows, cols, ld, dev, fn = _logits_call("credit_token_logprob_fwd_", logits)
     f32, i64 = torch.float32, torch.int64
     if tokens.dim() != 2:
         raise ValueError(f"tokens: expected a 2-D tensor, got shape {tuple(tokens.shape)}")
@@ -678,7 +686,8 @@ def token_logprob_fwd(logits: torch.Tensor, tokens: torch.Tensor, logp: torch.Te
         None if top_logp is None else _operand(top_logp, "top_logp", f32, (rows, top), dev),
         None if top_ids is None else _operand(top_ids, "top_ids", i64, (rows, top), dev),
         rows, cols, n, top, temperature, _cfg_ref(cfg, dev))
-    check(status, "credit_token_logprob_fwd")
+    if status:
+        check(status, fn.__name__)
 
 
 def token_logprob_bwd(logits: torch.Tensor, tokens: torch.Tensor, stats: torch.Tensor,
@@ -689,7 +698,7 @@ def token_logprob_bwd(logits: torch.Tensor, tokens: torch.Tensor, stats: torch.T
     from token_logprob_fwd's stats (and entropy).  dlogits, of the logits' type
     and shape, may be the logits themselves.  Rows without a weight other than
     0 are written 0 whatever their logits hold."""
-    rows, cols, ld, dev, fn = _logits_call("token_logprob_bwd", logits)
+    rows, cols, ld, dev, fn = _logits_call("credit_token_logprob_bwd_", logits)
     f32 = torch.float32
     if tokens.dim() != 2:
         raise ValueError(f"tokens: expected a 2-D tensor, got shape {tuple(tokens.shape)}")
@@ -704,7 +713,8 @@ def token_logprob_bwd(logits: torch.Tensor, tokens: torch.Tensor, stats: torch.T
         _operand(dlogp, "dlogp", f32, (rows, n), dev),
         None if dentropy is None else _operand(dentropy, "dentropy", f32, (rows,), dev),
         out, ldd, rows, cols, n, temperature, _cfg_ref(cfg, dev))
-    check(status, "credit_token_logprob_bwd")
+    if status:
+        check(status, fn.__name__)
 
 
 def topk_distill_fwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: torch.Tensor,
@@ -718,7 +728,7 @@ def topk_distill_fwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: t
     what they leave of 1 is held against the other columns together; without
     it, logits over whose softmax the entries are all there is.  Written: loss
     [rows], stats [rows, 8] for the backward."""
-    rows, cols, ld, dev, fn = _logits_call("topk_distill_fwd", logits)
+    rows, cols, ld, dev, fn = _logits_call("credit_topk_distill_fwd_", logits)
     f32 = torch.float32
     if teacher_ids.dim() != 2:
         raise ValueError(f"teacher_ids: expected a 2-D tensor, got {tuple(teacher_ids.shape)}")
@@ -728,7 +738,8 @@ def topk_distill_fwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: t
         _operand(teacher, "teacher", f32, (rows, k), dev),
         _operand(loss, "loss", f32, (rows,), dev), _operand(stats, "stats", f32, (rows, 8), dev),
         rows, cols, k, bool(tail), temperature, _cfg_ref(cfg, dev))
-    check(status, "credit_topk_distill_fwd")
+    if status:
+        check(status, fn.__name__)
 
 
 def topk_distill_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: torch.Tensor,
@@ -738,7 +749,7 @@ def topk_distill_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: t
     """Gradient for the logits of sum(dloss * loss) of topk_distill_fwd (same
     tail and temperature), from its stats.  dlogits, of the logits' type and
     shape, may be the logits themselves."""
-    rows, cols, ld, dev, fn = _logits_call("topk_distill_bwd", logits)
+    rows, cols, ld, dev, fn = _logits_call("credit_topk_distill_bwd_", logits)
     f32 = torch.float32
     if teacher_ids.dim() != 2:
         raise ValueError(f"teacher_ids: expected a 2-D tensor, got {tuple(teacher_ids.shape)}")
@@ -749,7 +760,8 @@ def topk_distill_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: t
         _operand(teacher, "teacher", f32, (rows, k), dev),
         _operand(stats, "stats", f32, (rows, 8), dev), _operand(dloss, "dloss", f32, (rows,), dev),
         out, ldd, rows, cols, k, bool(tail), temperature, _cfg_ref(cfg, dev))
-    check(status, "credit_topk_distill_bwd")
+    if status:
+        check(status, fn.__name__)
 
 
 def layernorm_backward(x: torch.Tensor, dy: torch.Tensor, gamma: torch.Tensor,
