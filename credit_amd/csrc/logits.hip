@@ -12,8 +12,8 @@
 // elementwise given the forward's row statistics.
 //
 // Rows start at any element address and may be apart by more than cols: a row
-// is read in 16-byte vectors from the 16-byte line that its first element lies
-// in, and the elements of its first and last line that are not its own are
+// is read in 16-byte vectors from the 128-byte line that its first element lies
+// in, and the elements of its first and last vector that are not its own are
 // masked.
 #include <float.h>
 
@@ -32,6 +32,7 @@ constexpr int kNW = kThreads / kWave;
 constexpr int kLane = 32;                     // elements of a lane in a batch
 constexpr int kBatch = kThreads * kLane;      // elements of a workgroup in a batch
 constexpr int kMaxEntries = kThreads;         // tokens, alternatives or teacher entries a row
+constexpr uintptr_t kLine = 128;              // bytes
 constexpr int64_t kMaxCols = int64_t{1} << 29;  // a row's bytes fit 32-bit offsets
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kNaN = __builtin_nanf("");
@@ -56,22 +57,34 @@ constexpr int kN = Elem<T>::kN;
 template <class T>
 constexpr int kU = kLane / kN<T>;  // vectors of a lane in a batch
 
-// A row from the start of its first 16-byte line on: element e of the frame is
-// column e - head, and the row's own are those in [head, end).
+// A row from the start of its first 128-byte line on: element e of the frame is
+// column e - head, and the row's own are those in [head, end).  Whole waves then
+// read and write whole lines, wherever the row starts.  Vectors wholly before
+// the row are not accessed: their offsets wrap around, past the buffer's end.
 struct Frame {
-  buffer_rsrc_t r;
+  buffer_rsrc_t r;  // from the 16 bytes that hold the row's first element
+  uint32_t skip;    // bytes of the frame before those
   int head, end;
 };
 template <class T>
 __device__ __forceinline__ Frame frame_of(const T* row, int cols) {
   Frame f;
   const uintptr_t a = reinterpret_cast<uintptr_t>(row);
-  f.head = static_cast<int>((a & 15u) / sizeof(T));
+  const uint32_t in_line = static_cast<uint32_t>(a & (kLine - 1));
+  f.skip = in_line & ~15u;
+  f.head = static_cast<int>(in_line / sizeof(T));
   f.end = f.head + cols;
   // Whole dwords: the last one holds the row's last element.
   f.r = make_rsrc(reinterpret_cast<const void*>(a & ~uintptr_t{15}),
-                  (static_cast<uint32_t>(f.end) * static_cast<uint32_t>(sizeof(T)) + 3u) & ~3u);
+                  (static_cast<uint32_t>(f.end) * static_cast<uint32_t>(sizeof(T)) + 3u & ~3u) -
+                      f.skip);
   return f;
+}
+__device__ __forceinline__ u32x4 load_vec(const Frame& f, int vec) {
+  return buffer_load(f.r, static_cast<uint32_t>(vec) * 16u - f.skip);
+}
+__device__ __forceinline__ u32x4 load_vec_nt(const Frame& f, int vec) {
+  return buffer_load_nt(f.r, static_cast<uint32_t>(vec) * 16u - f.skip);
 }
 
 template <class T, int N>
@@ -93,7 +106,7 @@ template <class T>
 __device__ __forceinline__ void load_batch(u32x4 (&v)[kU<T>], const Frame& f, int b) {
 #pragma unroll
   for (int k = 0; k < kU<T>; ++k)
-    v[k] = buffer_load_nt(f.r, ((b * kU<T> + k) * kThreads + threadIdx.x) * 16u);
+    v[k] = load_vec_nt(f, (b * kU<T> + k) * kThreads + static_cast<int>(threadIdx.x));
 }
 // The lane's elements of batch b that are not the row's, bit i the i-th.
 template <class T>
@@ -380,7 +393,7 @@ template <class T, class Fn>
 __device__ __forceinline__ void each_value(const Frame& f, Fn&& fn) {
   const int vecs = (f.end + kN<T> - 1) / kN<T>;
   for (int v = threadIdx.x; v < vecs; v += kThreads) {
-    const u32x4 raw[1] = {buffer_load(f.r, static_cast<uint32_t>(v) * 16u)};
+    const u32x4 raw[1] = {load_vec(f, v)};
     float z[kN<T>];
     unpack<T, 1>(z, raw);
 #pragma unroll
@@ -514,7 +527,7 @@ __device__ __forceinline__ void write_top_any(const Frame& f, int top, TopSlots&
   const int vecs = (f.end + kN<T> - 1) / kN<T>;
   for (int v0 = 0; v0 < vecs && found < top; v0 += kThreads) {
     const int v = v0 + threadIdx.x;
-    const u32x4 raw[1] = {buffer_load(f.r, static_cast<uint32_t>(v) * 16u)};
+    const u32x4 raw[1] = {load_vec(f, v)};
     float z[kN<T>];
     unpack<T, 1>(z, raw);
     uint32_t hit = 0;
@@ -618,7 +631,7 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPt
     const int unit = s.units[i < vecs ? i >> per : 0];
     const int vec = ((unit / kThreads << per) + (i & ((1 << per) - 1))) * kThreads +
                     unit % kThreads;
-    const u32x4 raw[1] = {buffer_load(f.r, static_cast<uint32_t>(vec) * 16u)};
+    const u32x4 raw[1] = {load_vec(f, vec)};
     const int e0 = vec * kN<T>;
     float z[kN<T>];
     unpack<T, 1>(z, raw);
@@ -789,7 +802,7 @@ template <class T>
 __device__ __forceinline__ void load_part(u32x4 (&v)[kGradVecs], const Frame& f, int part) {
 #pragma unroll
   for (int k = 0; k < kGradVecs; ++k)
-    v[k] = buffer_load_nt(f.r, ((part * kGradVecs + k) * kThreads + threadIdx.x) * 16u);
+    v[k] = load_vec_nt(f, (part * kGradVecs + k) * kThreads + static_cast<int>(threadIdx.x));
 }
 template <class T, bool VEC, class Fn>
 __device__ __forceinline__ void write_part(const u32x4 (&v)[kGradVecs], const Frame& f, T* out,
@@ -1156,9 +1169,10 @@ static_assert(logits::kMaxParts == kMaxParts && logits::kPartValues == kPartValu
 // Batches of the widest frame that a row of this alignment has.
 template <class T>
 int64_t row_batches(const T* logits, int64_t ld, int64_t rows, int64_t cols) {
-  const bool lines = reinterpret_cast<uintptr_t>(logits) % 16 == 0 &&
-                     (rows == 1 || ld * static_cast<int64_t>(sizeof(T)) % 16 == 0);
-  return (cols + (lines ? 0 : kN<T> - 1) + kBatch - 1) / kBatch;
+  const bool lines = reinterpret_cast<uintptr_t>(logits) % kLine == 0 &&
+                     (rows == 1 || ld * static_cast<int64_t>(sizeof(T)) % kLine == 0);
+  const int64_t head = lines ? 0 : kLine / sizeof(T) - 1;
+  return (cols + head + kBatch - 1) / kBatch;
 }
 int check_logits(const void* p, const char* name, int64_t ld, int64_t rows, int64_t cols,
                  size_t elem) {
@@ -1242,7 +1256,7 @@ int check_overlap(const void* in, int64_t ld, const void* out, int64_t ldd, int6
 }
 template <class T>
 dim3 grad_grid(int64_t rows, int64_t cols) {
-  const int64_t parts = (cols + kN<T> - 1 + kGradBatch<T> - 1) / kGradBatch<T>;
+  const int64_t parts = (cols + kLine / sizeof(T) - 1 + kGradBatch<T> - 1) / kGradBatch<T>;
   return dim3(static_cast<unsigned>(parts), static_cast<unsigned>(rows < 65535 ? rows : 65535));
 }
 

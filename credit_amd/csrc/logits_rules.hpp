@@ -46,12 +46,12 @@ inline size_t parts_bytes(int64_t rows, int64_t parts, int64_t batches, bool alt
 }
 
 // Scratch that any call of this shape can take, whatever its type and alignment:
-// a row's batches are at most one more than its columns fill, its parts at most
+// a row's batches start at a 128-byte line, at most one more than its columns fill, its parts at most
 // `split` (0: as AUTO takes them, with alternatives or without).
 inline size_t workspace(int64_t rows, int64_t cols, int variant_read, int64_t split,
                         bool alternatives) {
   size_t most = 0;
-  for (int64_t batches : {(cols + kBatch - 1) / kBatch, (cols + 7 + kBatch - 1) / kBatch})
+  for (int64_t batches : {(cols + kBatch - 1) / kBatch, (cols + 63 + kBatch - 1) / kBatch})
     for (bool top : {false, alternatives}) {
       const int64_t want =
           variant_read ? 1 : split > 0 ? split : auto_parts(rows, batches, top);

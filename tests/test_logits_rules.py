@@ -49,7 +49,7 @@ def test_the_workspace_covers_every_type_alignment_and_plan(rules):
             for split in (0, 1, 2, 5, 64):
                 for alternatives in (0, 1):
                     have = rules.logits_workspace(rows, cols, 0, split, alternatives)
-                    for slack in (0, 3, 7):
+                    for slack in (0, 3, 31, 63):
                         batches = (cols + slack + BATCH - 1) // BATCH
                         for top in range(alternatives + 1):
                             want = split or rules.logits_auto_parts(rows, batches, top)
