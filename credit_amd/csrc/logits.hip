@@ -176,16 +176,24 @@ __device__ __forceinline__ void add_terms(float& s, float& t, const float (&z)[k
   t = t2[0] + t2[1];
 }
 
-// Takes a batch; returns its maximum.  A column of -inf
+// Takes a batch; vm: the maxima of the lane's vectors.  A column of -inf
 // makes the plain t NaN: then, and only then, the terms are formed again with
 // the exponent clamped (the clamp costs an eighth of the loop's instructions).
 template <class T, bool ENT, bool CAREFUL>
-__device__ __forceinline__ float absorb(Lane& a, float c, const u32x4 (&v)[kU<T>]) {
+__device__ __forceinline__ void absorb(Lane& a, float c, const u32x4 (&v)[kU<T>],
+                                       float (&vm)[kU<T>]) {
   float z[kLane];
   unpack<T, kU<T>>(z, v);
-  float bm = fmax_nan(z[0], z[1]);
 #pragma unroll
-  for (int i = 2; i < kLane; i += 2) bm = fmax_nan(bm, fmax_nan(z[i], z[i + 1]));
+  for (int k = 0; k < kU<T>; ++k) {
+    const float* y = z + k * kN<T>;
+    vm[k] = fmax_nan(y[0], y[1]);
+#pragma unroll
+    for (int i = 2; i < kN<T>; i += 2) vm[k] = fmax_nan(vm[k], fmax_nan(y[i], y[i + 1]));
+  }
+  float bm = vm[0];
+#pragma unroll
+  for (int k = 1; k < kU<T>; ++k) bm = fmax_nan(bm, vm[k]);
   a.mx = fmax_nan(a.mx, bm);
   const float over = CAREFUL ? (bm - a.r) * c : __builtin_fmaf(bm, c, -a.r);
   if (__builtin_amdgcn_ballot_w64(over > kRaise) != 0) {
@@ -212,7 +220,6 @@ __device__ __forceinline__ float absorb(Lane& a, float c, const u32x4 (&v)[kU<T>
   }
   a.s += s;
   if (ENT) a.t += t;
-  return bm;
 }
 
 // The workgroup's lanes joined, about the maximum m of them all: s = sum
@@ -253,7 +260,8 @@ __device__ __forceinline__ Joined merge(const Joined& a, const Joined& b, float 
 }
 
 // Batches [b0, b1) of a row: dropped(b) names further elements of batch b to
-// leave out, seen(b, m) takes the lane's maximum of each batch in order.
+// leave out, seen(b, vm) takes the maxima of the lane's vectors of each batch in
+// order.
 template <class T, bool ENT, bool CAREFUL, class Dropped, class Seen>
 __device__ __forceinline__ Lane stream(const Frame& f, int b0, int b1, float c, Dropped&& dropped,
                                        Seen&& seen) {
@@ -267,7 +275,9 @@ __device__ __forceinline__ Lane stream(const Frame& f, int b0, int b1, float c, 
     uint32_t drop = dropped(b);
     if ((b == 0 && f.head != 0) || (b + 1) * kBatch > f.end) drop |= outside<T>(f, b);
     if (__builtin_amdgcn_ballot_w64(drop != 0) != 0) hide<T>(v, drop);
-    seen(b, absorb<T, ENT, CAREFUL>(lane, c, v));
+    float vm[kU<T>];
+    absorb<T, ENT, CAREFUL>(lane, c, v, vm);
+    seen(b, vm);
 #pragma unroll
     for (int k = 0; k < kU<T>; ++k) v[k] = next[k];
   }
@@ -347,7 +357,7 @@ __device__ __forceinline__ Joined join_parts(const Parts& p, int64_t row, double
 }
 
 __device__ __forceinline__ uint32_t none_dropped(int) { return 0; }
-__device__ __forceinline__ void unseen(int, float) {}
+constexpr auto unseen = [](int, auto&&) {};
 
 // ------------------------------------------------------------ the largest --
 // Order of the alternatives: by value, NaN above everything and -0 as 0, equal
@@ -362,24 +372,52 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __builtin_bit_cast(float, (key >> 31) != 0 ? key & 0x7FFFFFFFu : ~key);
 }
 
-// While a row streams by, every lane leaves the maximum of its kLane elements of
-// each batch in LDS: a unit.  Afterwards every wave finds a bound that its share
-// of the K reaches among its 128 group maxima (a lane's units, even and odd
-// batches); the least of the waves' bounds is one that K elements of the row
-// reach, and not many more: of n elements in G groups about G ln(1/(1 - K/G))
-// pass the K-th largest group maximum (74 for K = 64 of 512).  Only units that
-// reach the bound are read again.  What has no such bound (many equal values, a
-// few crowded units) takes write_top_any, which reads the row several times.
+// A unit is the 64 (bf16) or 128 (fp32) contiguous bytes that kU lanes read at
+// once; its maximum goes, while the row streams by, to the one of those lanes
+// whose number is the vector's: a lane leaves one unit a batch in LDS.
+// Afterwards every wave finds a bound that its share of the K reaches among its
+// 128 group maxima (a lane's units, even and odd batches); the least of the
+// waves' bounds is one that K elements of the row reach, and not many more: of n
+// elements in G groups about G ln(1/(1 - K/G)) pass the K-th largest group
+// maximum (74 for K = 64 of 512).  Only units that reach the bound are read
+// again (units of one lane's 32 elements, which lie in four or eight lines, took
+// a third of the row's traffic at 4096 x 65536 and K = 64).  What has no such
+// bound (many equal values, a few crowded units) takes write_top_any, which
+// reads the row several times.
 constexpr int kBins = 256;
 constexpr int kCands = 1024;
-constexpr int kUnitList = 1024;
+constexpr int kUnitList = 256;  // units that a wave lists
 constexpr size_t kMaxUnitBytes = 32768;
 struct TopSlots {
   uint32_t hist[kBins];
-  uint16_t units[kUnitList];
-  uint32_t n, listed, bin, above, count;
+  union {
+    uint16_t units[kNW][kUnitList];
+    uint64_t order[kMaxEntries];  // the first candidates, once the units are read
+  };
+  uint32_t n, bin, above, count;
   uint32_t wave[kNW], bound[kNW];
 };
+// The lane's unit of a batch, from the maxima of its vectors: the lanes of a unit
+// halve what they hold step by step, each sending its partner what that keeps.
+template <int CTRL, int N>
+__device__ __forceinline__ void halve(float* m, bool upper) {
+#pragma unroll
+  for (int k = 0; k < N / 2; ++k) {
+    const float keep = upper ? m[k + N / 2] : m[k], send = upper ? m[k] : m[k + N / 2];
+    m[k] = fmax_nan(keep, dpp_f32<CTRL>(send));
+  }
+}
+template <class T>
+__device__ __forceinline__ float unit_max(const float (&vm)[kU<T>]) {
+  float m[kU<T>];
+#pragma unroll
+  for (int k = 0; k < kU<T>; ++k) m[k] = vm[k];
+  // Partners lane ^ 7, ^ 2, ^ 1: those of a step hold the same vectors.
+  if constexpr (kU<T> == 8) halve<kDppHalfMirror, 8>(m, (threadIdx.x & 4) != 0);
+  halve<kDppXor2, 4>(m, (threadIdx.x & 2) != 0);
+  halve<kDppXor1, 2>(m, (threadIdx.x & 1) != 0);
+  return m[0];
+}
 // A candidate: its key above ~column, so that the larger is nearer the front.
 // They lie where the units were.
 typedef uint64_t __attribute__((address_space(3))) * CandPtr;
@@ -469,26 +507,33 @@ __device__ __forceinline__ Range narrow(TopSlots& s, uint32_t lo, uint32_t hi, u
   }
 }
 
-// Ranks the n candidates by counting, four lanes to a candidate; put(rank, key,
+// Orders the n candidates by counting, four lanes to a candidate; put(rank, key,
 // column) for the first `top`.
 template <class Put>
-__device__ __forceinline__ void rank_candidates(CandPtr cand, int n, int top, Put&& put) {
+__device__ __forceinline__ void rank_candidates(TopSlots& s, CandPtr cand, int n, int top,
+                                                Put&& put) {
   const int padded = (n + 31) & ~31;  // zeros, which are larger than none
   if (static_cast<int>(threadIdx.x) < padded - n) cand[n + threadIdx.x] = 0;
   __syncthreads();
   const int quarter = threadIdx.x & 3;
+#pragma unroll 1
   for (int i0 = threadIdx.x / kWave * (kWave / 4); i0 < n; i0 += kThreads / 4) {
     const int i = i0 + static_cast<int>(threadIdx.x & (kWave - 1)) / 4;
     const uint64_t mine = i < n ? cand[i] : ~uint64_t{0};
     int rank = 0;
+#pragma unroll 1
     for (int j = 0; j < padded; j += 32)
 #pragma unroll
       for (int k = 0; k < 8; ++k) rank += cand[j + 4 * k + quarter] > mine;
     rank += __builtin_amdgcn_update_dpp(0, rank, kDppXor1, 0xf, 0xf, false);
     rank += __builtin_amdgcn_update_dpp(0, rank, kDppXor2, 0xf, 0xf, false);
-    if (quarter == 0 && rank < top && i < n)
-      put(rank, static_cast<uint32_t>(mine >> 32),
-          static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(mine)));
+    if (quarter == 0 && rank < top && i < n) s.order[rank] = mine;
+  }
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < min(n, top)) {
+    const uint64_t c = s.order[threadIdx.x];
+    put(static_cast<int>(threadIdx.x), static_cast<uint32_t>(c >> 32),
+        static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(c)));
   }
 }
 // The first place, in a list that *n counts, for each lane's `wanted` entries:
@@ -521,7 +566,7 @@ __device__ __forceinline__ void write_top_any(const Frame& f, int top, TopSlots&
   });
   __syncthreads();
   const int n = static_cast<int>(s.n);
-  rank_candidates(cand, n, top, put);
+  rank_candidates(s, cand, n, top, put);
   if (!ties) return;
   int found = n;
   const int vecs = (f.end + kN<T> - 1) / kN<T>;
@@ -576,7 +621,7 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPt
   const float few = -wave_reduce(fmax_nan(g[0] > kNegInf ? -g[0] : kNegInf,
                                           g[1] > kNegInf ? -g[1] : kNegInf), MaxOp{});
   if (threadIdx.x % kWave == 0) s.wave[wave] = full;
-  if (threadIdx.x == 0) s.n = s.listed = 0;
+  if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
   uint32_t all = 0;
   for (int w = 0; w < kNW; ++w) all += s.wave[w];
@@ -606,31 +651,42 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPt
   }
   // key >= bound, of values: all where the bound is a NaN's key or 0.
   const float least = value_of(bound);
-  if (__builtin_amdgcn_ballot_w64(!(fmax_nan(g[0], g[1]) < least)) != 0)
+  // The wave's own units that reach it.
+  uint16_t* mine = s.units[wave];
+  int listed = 0;
+  if (__builtin_amdgcn_ballot_w64(!(fmax_nan(g[0], g[1]) < least)) != 0) {
+#pragma unroll 1
     for (int u0 = 0; u0 < groups; u0 += 32) {
       uint32_t hits = 0;
 #pragma unroll 4
       for (int j = 0; j < 32 && u0 + j < groups; ++j)
         hits |= !(Elem<T>::get(units + (u0 + j) * kThreads + threadIdx.x) < least) ? 1u << j : 0u;
-      for (uint32_t at = places(&s.listed, __builtin_popcount(hits)); hits != 0;
-           hits &= hits - 1, ++at)
+      const int count = __builtin_popcount(hits);
+      const int upto = static_cast<int>(wave_scan(count));
+      for (int at = listed + upto - count; hits != 0; hits &= hits - 1, ++at)
         if (at < kUnitList)
-          s.units[at] =
-              static_cast<uint16_t>((u0 + __builtin_ctz(hits)) * kThreads + threadIdx.x);
+          mine[at] = static_cast<uint16_t>((u0 + __builtin_ctz(hits)) * kThreads + threadIdx.x);
+      listed += __builtin_amdgcn_readlane(upto, kWave - 1);
     }
+  }
+  // Every wave has read the units: candidates may take their place.
   __syncthreads();
-  // Too many units that reach the bound: none is read, and s.n is past kCands.
-  if (threadIdx.x == 0 && s.listed > kUnitList) s.n = kCands + 1;
-  constexpr int kPer = kU<T> == 4 ? 2 : 3;  // vectors of a lane in a batch: 4 or 8
+  // Too many units that reach the bound: none is read, and s.n ends past kCands.
+  if (listed > kUnitList) {
+    if (threadIdx.x % kWave == 0) atomicAdd(&s.n, kCands + 1u);
+    listed = 0;
+  }
+  constexpr int kPer = kU<T> == 4 ? 2 : 3;  // vectors of a unit in a batch: 4 or 8
   static_assert(kU<T> == 1 << kPer);
-  const int per = kPer + fold;
-  const int vecs = (s.listed > kUnitList ? 0 : static_cast<int>(s.listed)) << per;
+  const int per = kPer + fold, vecs = listed << per;
 #pragma unroll 1
-  for (int i0 = wave * kWave; i0 < vecs; i0 += kThreads) {
+  for (int i0 = 0; i0 < vecs; i0 += kWave) {
     const int i = i0 + static_cast<int>(threadIdx.x & (kWave - 1));
-    const int unit = s.units[i < vecs ? i >> per : 0];
-    const int vec = ((unit / kThreads << per) + (i & ((1 << per) - 1))) * kThreads +
-                    unit % kThreads;
+    const int unit = mine[i < vecs ? i >> per : 0];
+    // Vector `first % kU` of lanes first / kU kU + [0, kU), in batch b.
+    const int b = (unit / kThreads << fold) + (i >> kPer & ((1 << fold) - 1));
+    const int first = unit % kThreads;
+    const int vec = (b * kU<T> + first % kU<T>)*kThreads + first / kU<T> * kU<T> + i % kU<T>;
     const u32x4 raw[1] = {load_vec(f, vec)};
     const int e0 = vec * kN<T>;
     float z[kN<T>];
@@ -643,16 +699,16 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPt
     hits = i < vecs && to > from ? hits & ((1u << to) - (1u << from)) : 0u;
     for (uint32_t at = places(&s.n, __builtin_popcount(hits)); hits != 0; hits &= hits - 1, ++at) {
       const int e = __builtin_ctz(hits);
-      float v = z[0];
+      float x = z[0];
 #pragma unroll
-      for (int k = 1; k < kN<T>; ++k) v = e == k ? z[k] : v;
-      put_candidate(cand, at, key_of(v), e0 + e - f.head);
+      for (int k = 1; k < kN<T>; ++k) x = e == k ? z[k] : x;
+      put_candidate(cand, at, key_of(x), e0 + e - f.head);
     }
   }
   __syncthreads();
   const int n = static_cast<int>(s.n);
   if (n <= kCands)
-    rank_candidates(cand, n, top, put);
+    rank_candidates(s, cand, n, top, put);
   else
     write_top_any<T>(f, top, s, cand, put);
 }
@@ -669,7 +725,7 @@ struct LogprobArgs {
   float* top_logp;
   int64_t* top_ids;
   int cols, n_tokens, n_top;
-  int fold;      // a unit is 2^fold batches of a lane
+  int fold;      // a unit has 2^fold batches
   float c;       // log2(e) / temperature
   double inv_t;
   Parts parts;
@@ -705,8 +761,8 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
   if constexpr (SPLIT) {
     const int b0 = blockIdx.x * a.parts.batches, b1 = min(b0 + a.parts.batches, batches);
     float* out = a.parts.units + (row * a.parts.n * a.parts.batches) * kThreads + threadIdx.x;
-    j = scan<T, ENT>(f, b0, b1, a.c, join, none_dropped, [&](int b, float bm) {
-      if constexpr (TOP) publish(out + b * kThreads, bm);
+    j = scan<T, ENT>(f, b0, b1, a.c, join, none_dropped, [&](int b, const float (&vm)[kU<T>]) {
+      if constexpr (TOP) publish(out + b * kThreads, unit_max<T>(vm));
     });
     publish_part(a.parts, row, j, false);
     if (!last_part(a.parts, row)) return;
@@ -730,10 +786,10 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
     }
   } else {
     float unit = kNegInf;
-    j = scan<T, ENT>(f, 0, batches, a.c, join, none_dropped, [&](int b, float bm) {
+    j = scan<T, ENT>(f, 0, batches, a.c, join, none_dropped, [&](int b, const float (&vm)[kU<T>]) {
       if constexpr (TOP) {
         if ((b & ((1 << a.fold) - 1)) == 0) unit = kNegInf;
-        unit = fmax_nan(unit, bm);
+        unit = fmax_nan(unit, unit_max<T>(vm));
         put_unit(units + (b >> a.fold) * kThreads + threadIdx.x, unit);
       }
     });
