@@ -298,6 +298,7 @@ __device__ __forceinline__ Joined scan(const Frame& f, int b0, int b1, float c, 
 // joins them and goes on as a whole row's workgroup does.  Nothing waits for
 // another workgroup; the row's counter is 0 again afterwards.  Published and
 // read past the L2s, as the exchange of the SPLIT kernels (common.hpp).
+constexpr int kBufferPastL2 = 16;  // cache-policy operand: sc1, as device-scope loads have
 constexpr int kMaxParts = kWave;  // a lane each where they are joined
 constexpr int kPartValues = 4;    // m, s, t, whether a column was named twice
 struct Parts {
@@ -328,31 +329,36 @@ __device__ __forceinline__ void publish_part(const Parts& p, int64_t row, const 
   publish(v + 2, j.t);
   publish(v + 3, repeated ? 1.0 : 0.0);
 }
-// All parts' results joined, in every thread.
-__device__ __forceinline__ Joined join_parts(const Parts& p, int64_t row, double inv_t,
-                                             bool* repeated) {
+// The lane's part of the row, read before the parts are joined.
+struct PartValues {
+  double m, s, t, twice;
+};
+__device__ __forceinline__ PartValues fetch_part(const Parts& p, int64_t row) {
   const int lane = threadIdx.x & (kWave - 1);
-  float m = kNegInf;
-  double s = 0.0, t = 0.0, twice = 0.0;
-  if (lane < p.n) {
-    const double* v = p.values + (row * p.n + lane) * kPartValues;
-    m = static_cast<float>(fetch(v));
-    s = fetch(v + 1);
-    t = fetch(v + 2);
-    twice = fetch(v + 3);
-  }
+  // Without a branch: loads that follow need not wait for these.
+  const double* v = p.values + (row * p.n + min(lane, p.n - 1)) * kPartValues;
+  return PartValues{fetch(v), fetch(v + 1), fetch(v + 2), fetch(v + 3)};
+}
+// All parts' results joined, in every thread.
+__device__ __forceinline__ Joined join_parts(const PartValues& p, int parts, float c,
+                                             bool* repeated) {
+  const bool mine = static_cast<int>(threadIdx.x & (kWave - 1)) < parts;
+  const float m = mine ? static_cast<float>(p.m) : kNegInf;
+  double s = mine ? p.s : 0.0, t = p.t;
   Joined j;
   j.m = wave_reduce(m, MaxOp{});
-  if (s != 0.0) {
-    const double d = (static_cast<double>(m) - j.m) * inv_t;
-    const double f = ::exp(d);
-    t = f == 0.0 ? 0.0 : f * (t + d / kLn2 * s);
+  if (s == 0.0) {
+    t = 0.0;
+  } else {
+    const float d = (m - j.m) * c;
+    const double f = __builtin_amdgcn_exp2f(d);
+    t = f == 0.0 ? 0.0 : f * (t + static_cast<double>(d) * s);
     s *= f;
   }
   j.s = wave_reduce_sum_f64(s);
   j.t = wave_reduce_sum_f64(t);
   if (j.m != j.m) j.s = kNaN;
-  *repeated = __builtin_amdgcn_ballot_w64(twice != 0.0) != 0;
+  *repeated = __builtin_amdgcn_ballot_w64(p.twice != 0.0) != 0;
   return j;
 }
 
@@ -607,8 +613,21 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPt
                                           int fold, int top, TopSlots& s, Put&& put) {
   const int wave = threadIdx.x / kWave;
   float g[2] = {kNegInf, kNegInf};
-  for (int u = 0; u < groups; ++u)
-    g[u & 1] = fmax_nan(g[u & 1], Elem<T>::get(units + u * kThreads + threadIdx.x));
+  // Sixteen of the lane's units at once, -inf past the last.
+  const auto sixteen = [&](float (&v)[16], int u0) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      v[j] = Elem<T>::get(units + min(u0 + j, groups - 1) * kThreads + threadIdx.x);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = u0 + j < groups ? v[j] : kNegInf;
+  };
+#pragma unroll 1
+  for (int u0 = 0; u0 < groups; u0 += 16) {
+    float v[16];
+    sixteen(v, u0);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) g[j & 1] = fmax_nan(g[j & 1], v[j]);
+  }
   const uint32_t k0 = key_of(g[0]), k1 = key_of(g[1]);
   const auto reach = [&](uint32_t t) {
     return static_cast<uint32_t>(__builtin_popcountll(__builtin_amdgcn_ballot_w64(k0 >= t)) +
@@ -627,7 +646,9 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPt
   for (int w = 0; w < kNW; ++w) all += s.wave[w];
   uint32_t bound = 0;
   if (all >= static_cast<uint32_t>(top)) {
-    const uint32_t need = (top * full + all - 1) / all, enough = need + need / 4;
+    const uint32_t need = full * kNW == all ? (static_cast<uint32_t>(top) + kNW - 1) / kNW
+                                            : (top * full + all - 1) / all;
+    const uint32_t enough = need + need / 4;
     bound = 0xFFFFFFFFu;
     if (need != 0) {
       // Bit by bit below what the largest and the least group have in common.
@@ -656,11 +677,13 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPt
   int listed = 0;
   if (__builtin_amdgcn_ballot_w64(!(fmax_nan(g[0], g[1]) < least)) != 0) {
 #pragma unroll 1
-    for (int u0 = 0; u0 < groups; u0 += 32) {
+    for (int u0 = 0; u0 < groups; u0 += 16) {
+      float v[16];
+      sixteen(v, u0);
       uint32_t hits = 0;
-#pragma unroll 4
-      for (int j = 0; j < 32 && u0 + j < groups; ++j)
-        hits |= !(Elem<T>::get(units + (u0 + j) * kThreads + threadIdx.x) < least) ? 1u << j : 0u;
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        hits |= !(v[j] < least) && u0 + j < groups ? 1u << j : 0u;
       const int count = __builtin_popcount(hits);
       const int upto = static_cast<int>(wave_scan(count));
       for (int at = listed + upto - count; hits != 0; hits &= hits - 1, ++at)
@@ -740,6 +763,32 @@ __device__ __forceinline__ double ln_sum(double s) {
   return e * kLn2 + static_cast<double>(::logf(static_cast<float>(m)));
 }
 
+// The row's units from all parts, in LDS, four lanes' to a load.  They come from
+// past the L2: 16 batches take 4000 cycles, as many as one does.
+template <class T>
+__device__ __forceinline__ void fetch_units(const Parts& p, int64_t row, int batches, int groups,
+                                            int fold, T* units) {
+  const int lanes = threadIdx.x % kWave * 4;
+  const size_t all = static_cast<size_t>(p.n) * p.batches * kThreads;
+  const buffer_rsrc_t r = make_rsrc(p.units + row * all, static_cast<uint32_t>(all * 4));
+#pragma unroll 4
+  for (int g = threadIdx.x / kWave; g < groups; g += kNW) {
+    float unit[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+    for (int b = g << fold; b < min((g + 1) << fold, batches); ++b) {
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, (b * kThreads + lanes) * 4, 0,
+                                                            kBufferPastL2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = v[i];
+        unit[i] = fmax_nan(unit[i], __builtin_bit_cast(float, w));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) put_unit(units + g * kThreads + lanes + i, unit[i]);
+  }
+  __syncthreads();
+}
+
 template <class T, bool ENT, bool TOP, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs<T> a) {
   extern __shared__ __attribute__((aligned(16))) char dynamic_lds[];
@@ -766,24 +815,10 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
     });
     publish_part(a.parts, row, j, false);
     if (!last_part(a.parts, row)) return;
+    const PartValues values = fetch_part(a.parts, row);
+    if constexpr (TOP) fetch_units<T>(a.parts, row, batches, groups, a.fold, units);
     bool unused;
-    j = join_parts(a.parts, row, a.inv_t, &unused);
-    if constexpr (TOP) {
-      float unit = kNegInf;
-      for (int b0 = 0; b0 < batches; b0 += 8) {
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fetch(out + min(b0 + i, batches - 1) * kThreads);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int b = b0 + i;
-          if (b >= batches) break;
-          if ((b & ((1 << a.fold) - 1)) == 0) unit = kNegInf;
-          unit = fmax_nan(unit, v[i]);
-          put_unit(units + (b >> a.fold) * kThreads + threadIdx.x, unit);
-        }
-      }
-    }
+    j = join_parts(values, a.parts.n, a.c, &unused);
   } else {
     float unit = kNegInf;
     j = scan<T, ENT>(f, 0, batches, a.c, join, none_dropped, [&](int b, const float (&vm)[kU<T>]) {
@@ -1064,7 +1099,7 @@ __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<
     j.t = 0.0;
     publish_part(a.parts, row, j, twice);
     if (!last_part(a.parts, row)) return;
-    j = join_parts(a.parts, row, 1.0 / static_cast<double>(a.temperature), &twice);
+    j = join_parts(fetch_part(a.parts, row), a.parts.n, a.c, &twice);
   }
   bool first = live;  // of the entries that name one column: the lowest counts
   if (TAIL && twice) {
