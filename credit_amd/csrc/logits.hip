@@ -33,6 +33,7 @@ constexpr int kLane = 32;                     // elements of a lane in a batch
 constexpr int kBatch = kThreads * kLane;      // elements of a workgroup in a batch
 constexpr int kMaxEntries = kThreads;         // tokens, alternatives or teacher entries a row
 constexpr uintptr_t kLine = 128;              // bytes
+constexpr int64_t kMaxGridRows = int64_t{1} << 23;  // a grid's threads fit 32 bits
 constexpr int64_t kMaxCols = int64_t{1} << 29;  // a row's bytes fit 32-bit offsets
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kNaN = __builtin_nanf("");
@@ -200,8 +201,8 @@ __device__ __forceinline__ void absorb(Lane& a, float c, const u32x4 (&v)[kU<T>]
     const float r = over > kRaise ? (CAREFUL ? bm : bm * c) : a.r;
     const float d = CAREFUL ? (a.r - r) * c : a.r - r;
     const float f = __builtin_amdgcn_exp2f(d);
-    // s = 0: d may be infinite.
-    if (ENT) a.t = a.s == 0.0f ? 0.0f : f * __builtin_fmaf(d, a.s, a.t);
+    // f = 0: d may be infinite.
+    if (ENT) a.t = f == 0.0f ? 0.0f : f * __builtin_fmaf(d, a.s, a.t);
     a.s *= f;
     a.r = r;
   }
@@ -387,9 +388,10 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 // elements in G groups about G ln(1/(1 - K/G)) pass the K-th largest group
 // maximum (74 for K = 64 of 512).  Only units that reach the bound are read
 // again (units of one lane's 32 elements, which lie in four or eight lines, took
-// a third of the row's traffic at 4096 x 65536 and K = 64).  What has no such
-// bound (many equal values, a few crowded units) takes write_top_any, which
-// reads the row several times.
+// a third of the row's traffic at 4096 x 65536 and K = 64).  A row with fewer
+// than K columns above its mask, or with many equal to the bound, gives those
+// above it and then the first that equal it.  What crowds a few units otherwise
+// takes write_top_any, which reads the row several times.
 constexpr int kBins = 256;
 constexpr int kCands = 1024;
 constexpr int kUnitList = 256;  // units that a wave lists
@@ -400,7 +402,7 @@ struct TopSlots {
     uint16_t units[kNW][kUnitList];
     uint64_t order[kMaxEntries];  // the first candidates, once the units are read
   };
-  uint32_t n, bin, above, count;
+  uint32_t n, bin, above, count, crowded[2];
   uint32_t wave[kNW], bound[kNW];
 };
 // The lane's unit of a batch, from the maxima of its vectors: the lanes of a unit
@@ -427,6 +429,7 @@ __device__ __forceinline__ float unit_max(const float (&vm)[kU<T>]) {
 // A candidate: its key above ~column, so that the larger is nearer the front.
 // They lie where the units were.
 typedef uint64_t __attribute__((address_space(3))) * CandPtr;
+typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 // Units are kept in the logits' type, which holds them exactly.
 __device__ __forceinline__ void put_unit(float* u, float v) { *u = v; }
 __device__ __forceinline__ void put_unit(uint16_t* u, float v) {
@@ -530,7 +533,10 @@ __device__ __forceinline__ void rank_candidates(TopSlots& s, CandPtr cand, int n
 #pragma unroll 1
     for (int j = 0; j < padded; j += 32)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) rank += cand[j + 4 * k + quarter] > mine;
+      for (int k = 0; k < 4; ++k) {
+        const u64x2 two = *(u64x2 __attribute__((address_space(3)))*)(cand + j + 8 * k + 2 * quarter);
+        rank += (two[0] > mine) + (two[1] > mine);
+      }
     rank += __builtin_amdgcn_update_dpp(0, rank, kDppXor1, 0xf, 0xf, false);
     rank += __builtin_amdgcn_update_dpp(0, rank, kDppXor2, 0xf, 0xf, false);
     if (quarter == 0 && rank < top && i < n) s.order[rank] = mine;
@@ -555,6 +561,39 @@ __device__ __forceinline__ void put_candidate(CandPtr cand, uint32_t at, uint32_
     cand[at] = static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(col));
 }
 
+// The first columns whose values have this key, from place `found` on up to `top`.
+template <class T, class Put>
+__device__ __forceinline__ void put_equal(const Frame& f, uint32_t key, int found, int top,
+                                          TopSlots& s, Put&& put) {
+  const int vecs = (f.end + kN<T> - 1) / kN<T>;
+  for (int v0 = 0; v0 < vecs && found < top; v0 += kThreads) {
+    const int v = v0 + threadIdx.x;
+    const u32x4 raw[1] = {load_vec(f, v)};
+    float z[kN<T>];
+    unpack<T, 1>(z, raw);
+    uint32_t hit = 0;
+#pragma unroll
+    for (int i = 0; i < kN<T>; ++i) {
+      const int e = v * kN<T> + i;
+      if (e >= f.head && e < f.end && key_of(z[i]) == key) hit |= 1u << i;
+    }
+    const uint32_t mine = __builtin_popcount(hit);
+    const uint32_t incl = wave_scan(mine);
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    if (lane == kWave - 1) s.wave[wave] = incl;
+    __syncthreads();
+    int at = found + static_cast<int>(incl - mine), all = 0;
+    for (int w = 0; w < kNW; ++w) {
+      if (w < wave) at += s.wave[w];
+      all += s.wave[w];
+    }
+    for (; hit != 0 && at < top; hit &= hit - 1, ++at)
+      put(at, key, v * kN<T> + __builtin_ctz(hit) - f.head);
+    found += all;
+    __syncthreads();
+  }
+}
+
 // The `top` largest of any row: the range that holds the last of them is
 // narrowed until what is at or above it fits the candidates, or until it is a
 // single value, whose first columns are then taken in order.
@@ -573,35 +612,7 @@ __device__ __forceinline__ void write_top_any(const Frame& f, int top, TopSlots&
   __syncthreads();
   const int n = static_cast<int>(s.n);
   rank_candidates(s, cand, n, top, put);
-  if (!ties) return;
-  int found = n;
-  const int vecs = (f.end + kN<T> - 1) / kN<T>;
-  for (int v0 = 0; v0 < vecs && found < top; v0 += kThreads) {
-    const int v = v0 + threadIdx.x;
-    const u32x4 raw[1] = {load_vec(f, v)};
-    float z[kN<T>];
-    unpack<T, 1>(z, raw);
-    uint32_t hit = 0;
-#pragma unroll
-    for (int i = 0; i < kN<T>; ++i) {
-      const int e = v * kN<T> + i;
-      if (e >= f.head && e < f.end && key_of(z[i]) == r.hi) hit |= 1u << i;
-    }
-    const uint32_t mine = __builtin_popcount(hit);
-    const uint32_t incl = wave_scan(mine);
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    if (lane == kWave - 1) s.wave[wave] = incl;
-    __syncthreads();
-    int at = found + static_cast<int>(incl - mine), all = 0;
-    for (int w = 0; w < kNW; ++w) {
-      if (w < wave) at += s.wave[w];
-      all += s.wave[w];
-    }
-    for (; hit != 0 && at < top; hit &= hit - 1, ++at)
-      put(at, r.hi, v * kN<T> + __builtin_ctz(hit) - f.head);
-    found += all;
-    __syncthreads();
-  }
+  if (ties) put_equal<T>(f, r.hi, n, top, s, put);
 }
 
 // The `top` largest of a row whose units (of 2^fold batches each, `groups` of
@@ -640,12 +651,13 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPt
   const float few = -wave_reduce(fmax_nan(g[0] > kNegInf ? -g[0] : kNegInf,
                                           g[1] > kNegInf ? -g[1] : kNegInf), MaxOp{});
   if (threadIdx.x % kWave == 0) s.wave[wave] = full;
-  if (threadIdx.x == 0) s.n = 0;
+  if (threadIdx.x == 0) s.n = s.crowded[0] = s.crowded[1] = 0;
   __syncthreads();
   uint32_t all = 0;
   for (int w = 0; w < kNW; ++w) all += s.wave[w];
-  uint32_t bound = 0;
-  if (all >= static_cast<uint32_t>(top)) {
+  uint32_t bound = key_of(kNegInf);  // any column reaches that
+  bool above = all < static_cast<uint32_t>(top);
+  if (!above) {
     const uint32_t need = full * kNW == all ? (static_cast<uint32_t>(top) + kNW - 1) / kNW
                                             : (top * full + all - 1) / all;
     const uint32_t enough = need + need / 4;
@@ -670,70 +682,85 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPt
     for (int w = 0; w < kNW; ++w) bound = s.bound[w] < bound ? s.bound[w] : bound;
     bound = __builtin_amdgcn_readfirstlane(bound);
   }
-  // key >= bound, of values: all where the bound is a NaN's key or 0.
-  const float least = value_of(bound);
-  // The wave's own units that reach it.
+  // Values that reach the bound, or that are above it and then the first columns
+  // that hold it: where a mask leaves fewer groups than `top`, and where more
+  // reach it than the lists take.  key >= k is !(z < value_of(k)), of the values'
+  // keys up to that of infinity.
+  constexpr uint32_t kInfKey = 0xFF800000u;
   uint16_t* mine = s.units[wave];
-  int listed = 0;
-  if (__builtin_amdgcn_ballot_w64(!(fmax_nan(g[0], g[1]) < least)) != 0) {
-#pragma unroll 1
-    for (int u0 = 0; u0 < groups; u0 += 16) {
-      float v[16];
-      sixteen(v, u0);
-      uint32_t hits = 0;
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        hits |= !(v[j] < least) && u0 + j < groups ? 1u << j : 0u;
-      const int count = __builtin_popcount(hits);
-      const int upto = static_cast<int>(wave_scan(count));
-      for (int at = listed + upto - count; hits != 0; hits &= hits - 1, ++at)
-        if (at < kUnitList)
-          mine[at] = static_cast<uint16_t>((u0 + __builtin_ctz(hits)) * kThreads + threadIdx.x);
-      listed += __builtin_amdgcn_readlane(upto, kWave - 1);
-    }
-  }
-  // Every wave has read the units: candidates may take their place.
-  __syncthreads();
-  // Too many units that reach the bound: none is read, and s.n ends past kCands.
-  if (listed > kUnitList) {
-    if (threadIdx.x % kWave == 0) atomicAdd(&s.n, kCands + 1u);
+  int listed;
+  bool crowded;
+  float least;
+  for (;;) {
+    least = value_of(bound + (above ? 1u : 0u));
     listed = 0;
+    if (__builtin_amdgcn_ballot_w64(!(fmax_nan(g[0], g[1]) < least)) != 0) {
+#pragma unroll 1
+      for (int u0 = 0; u0 < groups; u0 += 16) {
+        float v[16];
+        sixteen(v, u0);
+        uint32_t hits = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          hits |= !(v[j] < least) && u0 + j < groups ? 1u << j : 0u;
+        const int count = __builtin_popcount(hits);
+        const int upto = static_cast<int>(wave_scan(count));
+        for (int at = listed + upto - count; hits != 0; hits &= hits - 1, ++at)
+          if (at < kUnitList)
+            mine[at] = static_cast<uint16_t>((u0 + __builtin_ctz(hits)) * kThreads + threadIdx.x);
+        listed += __builtin_amdgcn_readlane(upto, kWave - 1);
+      }
+    }
+    if (listed > kUnitList && threadIdx.x % kWave == 0) s.crowded[above] = 1;
+    // Every wave has read the units: candidates may take their place.
+    __syncthreads();
+    crowded = s.crowded[above] != 0;
+    if (!crowded || above || bound >= kInfKey) break;
+    above = true;
   }
   constexpr int kPer = kU<T> == 4 ? 2 : 3;  // vectors of a unit in a batch: 4 or 8
   static_assert(kU<T> == 1 << kPer);
   const int per = kPer + fold, vecs = listed << per;
+  int n = kCands + 1;
+  while (!crowded) {
 #pragma unroll 1
-  for (int i0 = 0; i0 < vecs; i0 += kWave) {
-    const int i = i0 + static_cast<int>(threadIdx.x & (kWave - 1));
-    const int unit = mine[i < vecs ? i >> per : 0];
-    // Vector `first % kU` of lanes first / kU kU + [0, kU), in batch b.
-    const int b = (unit / kThreads << fold) + (i >> kPer & ((1 << fold) - 1));
-    const int first = unit % kThreads;
-    const int vec = (b * kU<T> + first % kU<T>)*kThreads + first / kU<T> * kU<T> + i % kU<T>;
-    const u32x4 raw[1] = {load_vec(f, vec)};
-    const int e0 = vec * kN<T>;
-    float z[kN<T>];
-    unpack<T, 1>(z, raw);
-    uint32_t hits = 0;
+    for (int i0 = 0; i0 < vecs; i0 += kWave) {
+      const int i = i0 + static_cast<int>(threadIdx.x & (kWave - 1));
+      const int unit = mine[i < vecs ? i >> per : 0];
+      // Vector `first % kU` of lanes first / kU kU + [0, kU), in batch b.
+      const int b = (unit / kThreads << fold) + (i >> kPer & ((1 << fold) - 1));
+      const int first = unit % kThreads;
+      const int vec = (b * kU<T> + first % kU<T>)*kThreads + first / kU<T> * kU<T> + i % kU<T>;
+      const u32x4 raw[1] = {load_vec(f, vec)};
+      const int e0 = vec * kN<T>;
+      float z[kN<T>];
+      unpack<T, 1>(z, raw);
+      uint32_t hits = 0;
 #pragma unroll
-    for (int e = 0; e < kN<T>; ++e) hits |= !(z[e] < least) ? 1u << e : 0u;
-    // The row's own elements, of a vector that this lane has.
-    const int from = min(max(f.head - e0, 0), kN<T>), to = min(max(f.end - e0, 0), kN<T>);
-    hits = i < vecs && to > from ? hits & ((1u << to) - (1u << from)) : 0u;
-    for (uint32_t at = places(&s.n, __builtin_popcount(hits)); hits != 0; hits &= hits - 1, ++at) {
-      const int e = __builtin_ctz(hits);
-      float x = z[0];
+      for (int e = 0; e < kN<T>; ++e) hits |= !(z[e] < least) ? 1u << e : 0u;
+      // The row's own elements, of a vector that this lane has.
+      const int from = min(max(f.head - e0, 0), kN<T>), to = min(max(f.end - e0, 0), kN<T>);
+      hits = i < vecs && to > from ? hits & ((1u << to) - (1u << from)) : 0u;
+      for (uint32_t at = places(&s.n, __builtin_popcount(hits)); hits != 0; hits &= hits - 1, ++at) {
+        const int e = __builtin_ctz(hits);
+        float x = z[0];
 #pragma unroll
-      for (int k = 1; k < kN<T>; ++k) x = e == k ? z[k] : x;
-      put_candidate(cand, at, key_of(x), e0 + e - f.head);
+        for (int k = 1; k < kN<T>; ++k) x = e == k ? z[k] : x;
+        put_candidate(cand, at, key_of(x), e0 + e - f.head);
+      }
     }
+    __syncthreads();
+    n = static_cast<int>(s.n);
+    if (n <= kCands || above || bound >= kInfKey) break;
+    above = true;
+    least = value_of(bound + 1u);
+    __syncthreads();
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
   }
-  __syncthreads();
-  const int n = static_cast<int>(s.n);
-  if (n <= kCands)
-    rank_candidates(s, cand, n, top, put);
-  else
-    write_top_any<T>(f, top, s, cand, put);
+  if (n > kCands) return write_top_any<T>(f, top, s, cand, put);
+  rank_candidates(s, cand, n, top, put);
+  if (n < top) put_equal<T>(f, bound, n, top, s, put);
 }
 
 // -------------------------------------------------------- token log-probs --
@@ -747,6 +774,7 @@ struct LogprobArgs {
   float* entropy;
   float* top_logp;
   int64_t* top_ids;
+  int64_t first = 0;  // row of the launch's first workgroup
   int cols, n_tokens, n_top;
   int fold;      // a unit has 2^fold batches
   float c;       // log2(e) / temperature
@@ -794,7 +822,7 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
   extern __shared__ __attribute__((aligned(16))) char dynamic_lds[];
   __shared__ JoinSlots join;
   T* units = reinterpret_cast<T*>(dynamic_lds);
-  const int64_t row = SPLIT ? blockIdx.y : blockIdx.x;
+  const int64_t row = SPLIT ? blockIdx.y : a.first + blockIdx.x;
   const T* z = a.logits + row * a.ld;
   // The thread's token, read ahead of the row.
   int64_t token = -1;
@@ -848,7 +876,8 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
   };
   if constexpr (TOP) {
     __shared__ TopSlots top;
-    write_top<T>(f, units, (CandPtr)(dynamic_lds), groups, a.fold, a.n_top, top, [&](int rank, uint32_t key, int col) {
+    write_top<T>(f, units, (CandPtr)(dynamic_lds), groups, a.fold, a.n_top, top,
+                 [&](int rank, uint32_t key, int col) {
                    a.top_logp[row * a.n_top + rank] = log_p(value_of(key));
                    a.top_ids[row * a.n_top + rank] = col;
                  });
@@ -1017,6 +1046,7 @@ struct DistillArgs {
   const float* teacher;
   float* loss;
   float* stats;
+  int64_t first = 0;  // row of the launch's first workgroup
   int cols, n_top;
   float temperature, c;
   Parts parts;
@@ -1042,7 +1072,7 @@ __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<
   __shared__ double sum_slots[4][kNW];
   __shared__ int flags[kNW];
   __shared__ int repeated;
-  const int64_t row = SPLIT ? blockIdx.y : blockIdx.x;
+  const int64_t row = SPLIT ? blockIdx.y : a.first + blockIdx.x;
   const T* z = a.logits + row * a.ld;
   const int k = threadIdx.x;
   // The thread's entry.
@@ -1351,6 +1381,12 @@ dim3 grad_grid(int64_t rows, int64_t cols) {
   return dim3(static_cast<unsigned>(parts), static_cast<unsigned>(rows < 65535 ? rows : 65535));
 }
 
+// A workgroup a row, or a part of one (of at most kMaxSplitRows rows).
+dim3 forward_grid(const Parts& parts, int64_t rows) {
+  if (parts.n > 1) return dim3(parts.n, static_cast<unsigned>(rows));
+  return dim3(static_cast<unsigned>(rows < kMaxGridRows ? rows : kMaxGridRows));
+}
+
 // fn(bool_constant...) for the values of `flags`.
 template <class Fn, class... Flags>
 void choose(Fn&& fn, bool flag, Flags... flags) {
@@ -1386,7 +1422,7 @@ int logprob_fwd(const T* logits, int64_t ld, const int64_t* tokens, float* logp,
                    tokens,   logp,
                    stats,    entropy,
                    top_logp, top_ids,
-                   static_cast<int>(cols),
+                   0,        static_cast<int>(cols),
                    n_tokens, n_top,
                    0,        log2e_over(temperature),
                    1.0 / static_cast<double>(temperature),
@@ -1402,10 +1438,10 @@ int logprob_fwd(const T* logits, int64_t ld, const int64_t* tokens, float* logp,
   const size_t lds = n_top > 0 ? std::max(unit_bytes(), size_t{kCands} * sizeof(uint64_t)) : 0;
   hipStream_t stream = cfg_stream(cfg);
   const auto launch = [&](auto ent, auto top, auto split) {
-    const dim3 grid = decltype(split)::value ? dim3(a.parts.n, static_cast<unsigned>(rows))
-                                             : dim3(static_cast<unsigned>(rows));
-    token_logprob_fwd_kernel<T, decltype(ent)::value, decltype(top)::value,
-                             decltype(split)::value><<<grid, kThreads, lds, stream>>>(a);
+    for (; a.first < rows; a.first += kMaxGridRows)
+      token_logprob_fwd_kernel<T, decltype(ent)::value, decltype(top)::value,
+                               decltype(split)::value>
+          <<<forward_grid(a.parts, rows - a.first), kThreads, lds, stream>>>(a);
   };
   choose(launch, entropy != nullptr, n_top > 0, a.parts.n > 1);
   return check_launch("token_logprob_fwd_kernel");
@@ -1469,16 +1505,15 @@ int distill_fwd(const T* logits, int64_t ld, const int64_t* ids, const float* te
   CREDIT_TRY(check_variant(cfg, true));
   if (rows == 0) return CREDIT_OK;
   DistillArgs<T> a{logits, ld,    ids,         teacher,
-                   loss,   stats, static_cast<int>(cols),
+                   loss,   stats, 0, static_cast<int>(cols),
                    n_top,  temperature, log2e_over(temperature),
                    Parts{}};
   CREDIT_TRY(plan_parts(cfg, rows, row_batches(logits, ld, rows, cols), false, &a.parts));
   hipStream_t stream = cfg_stream(cfg);
   const auto launch = [&](auto has_tail, auto split) {
-    const dim3 grid = decltype(split)::value ? dim3(a.parts.n, static_cast<unsigned>(rows))
-                                             : dim3(static_cast<unsigned>(rows));
-    topk_distill_fwd_kernel<T, decltype(has_tail)::value, decltype(split)::value>
-        <<<grid, kThreads, 0, stream>>>(a);
+    for (; a.first < rows; a.first += kMaxGridRows)
+      topk_distill_fwd_kernel<T, decltype(has_tail)::value, decltype(split)::value>
+          <<<forward_grid(a.parts, rows - a.first), kThreads, 0, stream>>>(a);
   };
   choose(launch, tail != 0, a.parts.n > 1);
   return check_launch("topk_distill_fwd_kernel");

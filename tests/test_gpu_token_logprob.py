@@ -287,6 +287,43 @@ def test_alternatives_that_crowd(gpu, dtype):
         check_forward(z, tokens, top, forward(z.to(gpu), tokens, top), what=f"top {top}")
 
 
+def masked_rows(cols, dtype, seed):
+    """Rows of which a mask leaves little, at random columns, in one place, or
+    behind everything else; equal values in few or all places."""
+    g = generator(seed)
+    low = torch.finfo(DTYPES[dtype]).min
+    base = make_logits(1, cols, dtype, seed + 1)[0]
+    rows = []
+    for fill in (-math.inf, low, -4.0):
+        for n in (0, 1, 10, 100, 1500):
+            z = torch.full((cols,), fill)
+            at = torch.randperm(cols, generator=g)[:n]
+            z[at] = base[at].float().abs()
+            rows.append(z)
+    rows.append(torch.full((cols,), -math.inf).index_fill(0, torch.arange(cols - 70, cols), 2.0))
+    rows.append(torch.where(torch.arange(cols) < cols - 9, 1.0, -1.0).index_fill(
+        0, torch.tensor([cols // 2]), 3.0))
+    rows.append(torch.where(torch.arange(cols) < cols - 300, low, 0.0))
+    rows.append(torch.full((cols,), math.inf))
+    rows.append(torch.full((cols,), -math.inf).index_fill(0, torch.arange(5, cols, 97), -0.0)
+                .index_fill(0, torch.arange(7, cols, 97), 0.0))
+    rows.append(torch.full((cols,), math.nan).index_fill(0, torch.arange(0, cols, 2), -math.inf))
+    return torch.stack(rows).to(DTYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("variant", ["read", "split"])
+@pytest.mark.parametrize("cols,offset", [(300, 0), (5003, 3), (70001, 1), (131072, 0)])
+def test_alternatives_of_masked_rows(gpu, dtype, variant, cols, offset):
+    z = masked_rows(cols, dtype, 49)
+    tokens = torch.randint(0, cols, (len(z), 2), generator=generator(50))
+    cfg = hip_lib.make_cfg(variant, 5 if variant == "split" else 0)
+    zs = placed(z, gpu, offset, offset)
+    for top in (1, 2, 20, 101, 256):
+        print(f"token_logprob masked {dtype} {variant} {cols} top {top}", flush=True)
+        check_forward(z, tokens, top, forward(zs, tokens, top, cfg=cfg), what=f"top {top}")
+
+
 def test_more_rows_than_a_grid_has(gpu):
     rows, cols = 70001, 5
     print("token_logprob many rows", flush=True)
@@ -301,6 +338,40 @@ def test_more_rows_than_a_grid_has(gpu):
     one = torch.zeros(z.shape, dtype=torch.float64).scatter_(1, tokens, dlogp.double().abs())
     bound = p * dlogp.double().abs().numpy() * (1.7e-5 + 2 * sum_error(cols)) + one.numpy() * 8 * EPS
     assert_within(as64(out), want.numpy(), bound, "dlogits")
+
+
+def test_more_threads_than_a_grid_has(gpu):
+    """2^24 workgroups have 2^32 threads: more rows than that, each as it is in
+    a call of its own."""
+    rows, cols = (1 << 24) + 5, 2
+    print("token_logprob 2^24 rows", flush=True)
+    z = torch.randn((rows, cols), generator=generator(48)).to(gpu)
+    tokens = torch.arange(rows, device=gpu).remainder(3)[:, None] - 1
+    got = forward(z, tokens, 1)
+    for s in (slice(0, 100), slice((1 << 23) - 50, (1 << 23) + 50), slice(rows - 100, rows)):
+        alone = forward(z[s], tokens[s], 1)
+        for a, b in zip(got, alone):
+            assert torch.equal(a[s], b)
+        check_forward(z[s].cpu(), tokens[s].cpu(), 1, alone)
+    assert not (got[0] == 7.0).any() and not (got[4] == -7).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("variant", ["read", "split"])
+def test_lowest_values_ahead_of_a_far_maximum(gpu, dtype, variant):
+    """A lane's first batches hold the type's lowest values alone, later ones
+    values beyond 2^20: from one to the other is further than fp32 goes."""
+    cols = 5 * 8192 + 77
+    print(f"token_logprob far maximum {dtype} {variant}", flush=True)
+    z = torch.full((3, cols), torch.finfo(DTYPES[dtype]).min)
+    z[0, 2 * 8192:] = 2.0 ** 22
+    z[1, 4 * 8192 + 5] = 2.0 ** 100
+    z[1, 4 * 8192 + 3000:] = -2.0 ** 100
+    z[2, 3 * 8192:] = 2.0 ** 23 + 2.0 ** 15 * (torch.arange(cols - 3 * 8192) % 3)
+    z = z.to(DTYPES[dtype])
+    tokens = torch.tensor([[0, cols - 1], [4 * 8192 + 5, 1], [cols - 2, cols - 3]])
+    cfg = hip_lib.make_cfg(variant, 3 if variant == "split" else 0)
+    check_forward(z, tokens, 9, forward(z.to(gpu), tokens, 9, cfg=cfg))
 
 
 def test_offsets_beyond_32_bits(gpu):

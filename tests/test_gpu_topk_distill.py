@@ -225,6 +225,19 @@ def test_more_rows_than_a_grid_has(gpu, tail):
         check_loss(z[s].cpu(), ids[s], teacher[s], tail, 1.0, alone)
 
 
+def test_more_threads_than_a_grid_has(gpu):
+    rows, cols = (1 << 24) + 5, 2
+    print("topk_distill 2^24 rows", flush=True)
+    z = torch.randn((rows, cols), generator=generator(75)).to(gpu)
+    ids = torch.arange(rows, device=gpu).remainder(2)[:, None].contiguous()
+    teacher = torch.full((rows, 1), -0.25)
+    loss, _ = forward(z, ids, teacher, True, 1.0, gpu)
+    for s in (slice(0, 100), slice((1 << 23) - 50, (1 << 23) + 50), slice(rows - 100, rows)):
+        alone, _ = forward(z[s], ids[s], teacher[s], True, 1.0, gpu)
+        assert torch.equal(loss[s], alone)
+        check_loss(z[s].cpu(), ids[s].cpu(), teacher[s], True, 1.0, alone)
+
+
 def test_gradient_against_differences(gpu):
     rows, cols, step = 2, 37, 1e-2
     z = make_logits(rows, cols, "f32", 70)
