@@ -46,8 +46,9 @@ inline size_t parts_bytes(int64_t rows, int64_t parts, int64_t batches, bool alt
 }
 
 // Scratch that any call of this shape can take, whatever its type and alignment:
-// a row's batches start at a 128-byte line, at most one more than its columns fill, its parts at most
-// `split` (0: as AUTO takes them, with alternatives or without).
+// a row's batches start at a 128-byte line, at most one more than its columns
+// fill, its parts at most `split` (0: as AUTO takes them, with alternatives or
+// without).
 inline size_t workspace(int64_t rows, int64_t cols, int variant_read, int64_t split,
                         bool alternatives) {
   size_t most = 0;

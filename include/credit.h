@@ -327,7 +327,17 @@ int credit_softmax_logits_bwd_f32(const float* logits, const float* dy, float* d
  *                       NaN above everything (n_top 0: not wanted)
  * A column of -inf has probability 0.  A row of nothing else: S = 0, logp
  * -inf, entropy 0.  A row with NaN or +inf gives NaN.  n_tokens and n_top are
- * at most 256 (n_top at most cols); n_tokens may be 0.  Variants: AUTO, READ.
+ * at most 256 (n_top at most cols); n_tokens may be 0.  Columns behind cols
+ * and what lies around them may hold anything.
+ * Variants: READ, a workgroup a row; SPLIT, rows (at most 1024 of them; more
+ * are not cut) in cfg->split parts of whole 8192 columns (0: as AUTO), which
+ * leave their results in the workspace; the last to arrive joins them and none
+ * waits for another, so co-residency is not needed and no watchdog is raised.
+ * AUTO cuts few wide rows as far as every CU has a part.  Values may differ by
+ * roundings between variants, never between calls of one.  Under capture and on
+ * hipStreamPerThread AUTO cuts rows only with a cfg->workspace, and SPLIT
+ * without one is refused (CREDIT_ERR_WORKSPACE); graphs that may run at the
+ * same time need a workspace each.
  * No counterpart in the reference, whose softmax (src/workloads/
  * softmax_logits_backward.cu:314-476) emits no statistics. */
 int credit_token_logprob_fwd_f32(const float* logits, int64_t ld, const int64_t* tokens,
@@ -347,7 +357,8 @@ int credit_token_logprob_fwd_bf16(const uint16_t* logits, int64_t ld, const int6
  * otherwise the two may not overlap.  A weight of 0 counts as padding: rows
  * without any other are written 0 and their logits not read, whatever they
  * hold; so are rows of -inf alone.  A token >= cols of weight other than 0
- * makes its row NaN.  Columns behind cols are left as they are. */
+ * makes its row NaN.  Columns behind cols are left as they are.  Variants:
+ * AUTO, READ.  Takes no workspace. */
 int credit_token_logprob_bwd_f32(const float* logits, int64_t ld, const int64_t* tokens,
                                  const float* stats, const float* entropy, const float* dlogp,
                                  const float* dentropy, float* dlogits, int64_t ldd, int64_t rows,
@@ -375,7 +386,8 @@ int credit_token_logprob_bwd_bf16(const uint16_t* logits, int64_t ld, const int6
  * makes the loss NaN; p = 0 where q > 0 makes it +inf, but other columns that
  * are all -inf add nothing to it.  stats [rows, 8] is what the backward takes:
  * m and S as above, the same two of the columns outside the entries (tail),
- * sum q, the tail's gradient, the teacher's log-sum, 0. */
+ * sum q, the tail's gradient, the teacher's log-sum, 0.  Variants and workspace
+ * as credit_token_logprob_fwd_*'s. */
 int credit_topk_distill_fwd_f32(const float* logits, int64_t ld, const int64_t* teacher_ids,
                                 const float* teacher, float* loss, float* stats, int64_t rows,
                                 int64_t cols, int32_t n_top, int32_t tail, float temperature,
@@ -388,7 +400,8 @@ int credit_topk_distill_fwd_bf16(const uint16_t* logits, int64_t ld, const int64
  * column outside the entries q being the rest's share there,
  * rest p_j / (their probability).  ids, teacher, tail and T as the forward's,
  * whose stats it takes; dlogits as in credit_token_logprob_bwd_*.  Rows
- * without entries or with dloss 0 are written 0 and their logits not read. */
+ * without entries or with dloss 0 are written 0 and their logits not read.
+ * Variants: AUTO, READ.  Takes no workspace. */
 int credit_topk_distill_bwd_f32(const float* logits, int64_t ld, const int64_t* teacher_ids,
                                 const float* teacher, const float* stats, const float* dloss,
                                 float* dlogits, int64_t ldd, int64_t rows, int64_t cols,
