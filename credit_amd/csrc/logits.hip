@@ -1289,11 +1289,11 @@ static_assert(logits::kMaxParts == kMaxParts && logits::kPartValues == kPartValu
               logits::kBatch == kBatch && logits::kThreads == kThreads);
 // Batches of the widest frame that a row of this alignment has.
 template <class T>
-int64_t row_batches(const T* logits, int64_t ld, int64_t rows, int64_t cols) {
+int64_t row_batches(const T* logits, int64_t ld, int64_t rows, int64_t cols, int batch = kBatch) {
   const bool lines = reinterpret_cast<uintptr_t>(logits) % kLine == 0 &&
                      (rows == 1 || ld * static_cast<int64_t>(sizeof(T)) % kLine == 0);
   const int64_t head = lines ? 0 : kLine / sizeof(T) - 1;
-  return (cols + head + kBatch - 1) / kBatch;
+  return (cols + head + batch - 1) / batch;
 }
 int check_logits(const void* p, const char* name, int64_t ld, int64_t rows, int64_t cols,
                  size_t elem) {
@@ -1376,8 +1376,8 @@ int check_overlap(const void* in, int64_t ld, const void* out, int64_t ldd, int6
   return CREDIT_OK;
 }
 template <class T>
-dim3 grad_grid(int64_t rows, int64_t cols) {
-  const int64_t parts = (cols + kLine / sizeof(T) - 1 + kGradBatch<T> - 1) / kGradBatch<T>;
+dim3 grad_grid(const T* logits, int64_t ld, int64_t rows, int64_t cols) {
+  const int64_t parts = row_batches(logits, ld, rows, cols, kGradBatch<T>);
   return dim3(static_cast<unsigned>(parts), static_cast<unsigned>(rows < 65535 ? rows : 65535));
 }
 
@@ -1481,7 +1481,7 @@ int logprob_bwd(const T* logits, int64_t ld, const int64_t* tokens, const float*
                              1.0f / temperature,
                              log2e_over(temperature)};
   hipStream_t stream = cfg_stream(cfg);
-  const dim3 grid = grad_grid<T>(rows, cols);
+  const dim3 grid = grad_grid(logits, ld, rows, cols);
   const auto launch = [&](auto ent, auto vec) {
     token_logprob_bwd_kernel<T, decltype(ent)::value, decltype(vec)::value>
         <<<grid, kThreads, 0, stream>>>(a);
@@ -1550,7 +1550,7 @@ int distill_bwd(const T* logits, int64_t ld, const int64_t* ids, const float* te
                              1.0f / temperature,
                              log2e_over(temperature)};
   hipStream_t stream = cfg_stream(cfg);
-  const dim3 grid = grad_grid<T>(rows, cols);
+  const dim3 grid = grad_grid(logits, ld, rows, cols);
   const auto launch = [&](auto has_tail, auto vec) {
     topk_distill_bwd_kernel<T, decltype(has_tail)::value, decltype(vec)::value>
         <<<grid, kThreads, 0, stream>>>(a);
