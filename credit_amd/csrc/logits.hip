@@ -8,8 +8,9 @@
 // entropy, t = sum e^(x - r) (x - r) (in base 2: one v_exp_f32 an element).  The
 // reference is raised only where a term passes it by 2^8, so that the usual
 // batch does no rescaling; floating point keeps the same relative precision
-// wherever the reference lies.  The backwards are
-// elementwise given the forward's row statistics.
+// wherever the reference lies.  The backwards are elementwise given the
+// forward's row statistics.  All of them are bound by HBM where the rows fill
+// the device and by latency, launch to last store, where they do not.
 //
 // Rows start at any element address and may be apart by more than cols: a row
 // is read in 16-byte vectors from the 128-byte line that its first element lies
@@ -262,7 +263,11 @@ __device__ __forceinline__ Joined merge(const Joined& a, const Joined& b, float 
 
 // Batches [b0, b1) of a row: dropped(b) names further elements of batch b to
 // leave out, seen(b, vm) takes the maxima of the lane's vectors of each batch in
-// order.
+// order.  A batch is 32 elements a lane (16 a lane, 512 or 1024 lanes, or two
+// batches ahead measured the same or slower), loaded while the one before is
+// absorbed: a wave spends some 30 cycles on 64 bf16 elements (unpack, multiply-
+// add, exponential at a quarter rate, add, two-input share of a maximum), two
+// thirds of the time that HBM takes for them, half of that for fp32.
 template <class T, bool ENT, bool CAREFUL, class Dropped, class Seen>
 __device__ __forceinline__ Lane stream(const Frame& f, int b0, int b1, float c, Dropped&& dropped,
                                        Seen&& seen) {
@@ -293,11 +298,11 @@ __device__ __forceinline__ Joined scan(const Frame& f, int b0, int b1, float c, 
   return join_lanes<true>(stream<T, ENT, true>(f, b0, b1, c, dropped, seen), c, slots);
 }
 // ------------------------------------------------ a row in several parts --
-// Few rows leave most CUs idle on a workgroup each, and one CU draws a row at 70
-// GB/s.  A row is then cut into parts of whole batches; each leaves its result
-// (and its units) in the workspace, and the part that finds all others arrived
-// joins them and goes on as a whole row's workgroup does.  Nothing waits for
-// another workgroup; the row's counter is 0 again afterwards.  Published and
+// Few rows leave most CUs idle on a workgroup each, and one workgroup draws a row
+// at 35 GB/s (bf16).  A row is then cut into parts of whole batches; each leaves
+// its result (and its units) in the workspace, and the part that finds all others
+// arrived joins them and goes on as a whole row's workgroup does.  Nothing waits
+// for another workgroup; the row's counter is 0 again afterwards.  Published and
 // read past the L2s, as the exchange of the SPLIT kernels (common.hpp).
 constexpr int kBufferPastL2 = 16;  // cache-policy operand: sc1, as device-scope loads have
 constexpr int kMaxParts = kWave;  // a lane each where they are joined
@@ -434,6 +439,7 @@ __device__ __forceinline__ float unit_max(const float (&vm)[kU<T>]) {
 // They lie where the units were.
 typedef uint64_t __attribute__((address_space(3))) * CandPtr;
 typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+typedef u64x2 __attribute__((address_space(3))) * Cand2Ptr;
 // Units are kept in the logits' type, which holds them exactly.
 __device__ __forceinline__ void put_unit(float* u, float v) { *u = v; }
 __device__ __forceinline__ void put_unit(uint16_t* u, float v) {
@@ -538,7 +544,7 @@ __device__ __forceinline__ void rank_candidates(TopSlots& s, CandPtr cand, int n
     for (int j = 0; j < padded; j += 32)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const u64x2 two = *(u64x2 __attribute__((address_space(3)))*)(cand + j + 8 * k + 2 * quarter);
+        const u64x2 two = *(Cand2Ptr)(cand + j + 8 * k + 2 * quarter);
         rank += (two[0] > mine) + (two[1] > mine);
       }
     rank += __builtin_amdgcn_update_dpp(0, rank, kDppXor1, 0xf, 0xf, false);
@@ -765,7 +771,8 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPt
       // The row's own elements, of a vector that this lane has.
       const int from = min(max(f.head - e0, 0), kN<T>), to = min(max(f.end - e0, 0), kN<T>);
       hits = i < vecs && to > from ? hits & ((1u << to) - (1u << from)) : 0u;
-      for (uint32_t at = places(&s.n, __builtin_popcount(hits)); hits != 0; hits &= hits - 1, ++at) {
+      uint32_t at = places(&s.n, __builtin_popcount(hits));
+      for (; hits != 0; hits &= hits - 1, ++at) {
         const int e = __builtin_ctz(hits);
         float x = z[0];
 #pragma unroll
@@ -841,6 +848,13 @@ __device__ __forceinline__ void fetch_units(const Parts& p, int64_t row, int bat
   __syncthreads();
 }
 
+// One read of the logits.  512 x 262144 fp32 with the entropy 77.6 us, 6.92 TB/s
+// (a kernel that reads alone reaches 7.08); 2048 x 131072 bf16 83 us without
+// alternatives (6.5 TB/s) and 95 with 64 (5.65): the workgroups that a CU holds
+// reach their rows' ends together, where a row's choice of alternatives, some
+// 9000 cycles of latency, has no loads to hide it.  64 x 131072 in four parts
+// each, K = 20: 13.6 us, of which the stream 4, the parts' meeting and the units
+// from past the L2 2.5, the choice 3.5.
 template <class T, bool ENT, bool TOP, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs<T> a) {
   extern __shared__ __attribute__((aligned(16))) char dynamic_lds[];
@@ -986,6 +1000,10 @@ struct LogprobGradArgs {
   float inv_t, c;
 };
 
+// One read, one write; a workgroup's part is four vectors a lane, all loaded
+// before the first is used.
+// 2048 x 131072 bf16 with the entropy's gradient 174 us, 6.17 TB/s (a kernel that
+// reads and writes as much and does nothing else reaches 6.37).
 template <class T, bool ENT, bool VEC>
 __global__ __launch_bounds__(kThreads) void token_logprob_bwd_kernel(LogprobGradArgs<T> a) {
   const int lane = threadIdx.x & (kWave - 1);
@@ -1089,6 +1107,11 @@ __device__ __forceinline__ bool mark(uint32_t* bits, int e, int b0, int b1) {
   return (atomicOr(&bits[(b - b0) * kThreads + v % kThreads], bit) & bit) != 0;
 }
 
+// The tail is summed directly, over the columns that no entry names (1 - sum p of
+// the named ones would lose it where it is small): their bits are marked in LDS
+// for 16 batches at a time.  2048 x 131072 bf16, K = 64, tail 87.8 us, 6.14 TB/s;
+// without it the same; 8192 x 32768 108 us against 85: 64 named columns in four
+// batches leave hardly a wave's batch without one to mask.
 template <class T, bool TAIL, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<T> a) {
   __shared__ JoinSlots join;
@@ -1235,6 +1258,8 @@ struct DistillGradArgs {
   float inv_t, c;
 };
 
+// One read, one write, as token_logprob_bwd_kernel: 2048 x 131072 bf16, K = 64
+// 175.6 us, 6.12 TB/s; 512 x 262144 fp32, K = 128, tail 176.1.
 template <class T, bool TAIL, bool VEC>
 __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradArgs<T> a) {
   // The entries whose columns lie in this part, in their order.
@@ -1417,8 +1442,10 @@ void choose(Fn&& fn, bool flag, Flags... flags) {
   if constexpr (sizeof...(flags) == 0) {
     flag ? fn(std::true_type{}) : fn(std::false_type{});
   } else {
-    choose([&](auto... rest) { flag ? fn(std::true_type{}, rest...) : fn(std::false_type{}, rest...); },
-           flags...);
+    const auto with = [&](auto... rest) {
+      flag ? fn(std::true_type{}, rest...) : fn(std::false_type{}, rest...);
+    };
+    choose(with, flags...);
   }
 }
 

@@ -21,16 +21,17 @@ constexpr int64_t kMaxSplitRows = 1024;
 // every CU a workgroup, where that saves a part four batches or more: a batch is
 // 0.5 us of a lone workgroup's time, the meeting of the parts 1.5 us.  us a call,
 // one workgroup a row -> parts:
-//   distillation with tail   1 x 131072 bf16 14.7 -> 7.5, 64 x 131072 16.3 -> 11.0,
-//                            128 x 131072 16.3 -> 13.6, 16 x 262144 fp32 28.6 -> 10.0
-//   but 64 x 32768 fp32 (4 batches) 8.9 -> 9.8; 256 rows of either, two parts: 17 -> 18
+//   distillation with tail   1 x 131072 bf16 14.6 -> 7.5, 64 x 131072 15.9 -> 10.2,
+//                            128 x 131072 16.3 -> 13.1, 16 x 262144 fp32 28.6 -> 9.6
+//   but 64 x 32768 fp32 (4 batches) 7.5 -> 7.4 (log-probabilities alone 7.4 -> 7.7);
+//   256 x 131072, two parts: 17.3 -> 18.3
 // With alternatives the last part reads every lane's maxima back, which takes
-// more: 1 x 131072 15.1 -> 10.0, 64 x 131072 17.3 -> 15.3, 128 x 131072 17.6 ->
-// 18.6, 1 x 32768 fp32 8.6 -> 9.4.
+// more (K = 20): 1 x 131072 15.2 -> 9.9, 64 x 131072 17.0 -> 14.0, 96 x 131072
+// 17.2 -> 17.0, 128 x 131072 17.3 -> 17.6, 1 x 32768 fp32 9.1 -> 9.4.
 inline int64_t auto_parts(int64_t rows, int64_t batches, bool alternatives) {
   if (alternatives && rows > 64) return 1;
-  const int64_t parts =
-      std::min<int64_t>({kMaxParts, batches, std::max<int64_t>(1, 256 / std::max<int64_t>(1, rows))});
+  const int64_t a_cu_each = std::max<int64_t>(1, 256 / std::max<int64_t>(1, rows));
+  const int64_t parts = std::min<int64_t>({kMaxParts, batches, a_cu_each});
   const int64_t saved = batches - (batches + parts - 1) / parts;
   return saved >= (alternatives ? 5 : 4) ? parts : 1;
 }

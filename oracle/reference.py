@@ -29,6 +29,10 @@ How each function is pinned (tests/test_oracle.py):
 * ``ffn_rmsnorm_gelu``       -- F.rms_norm -> matmul -> F.gelu(tanh) ->
                                 matmul in float64, and the GELU-tanh closed
                                 form at 0 and +-large.
+* ``token_logprob_*``, ``topk_distill_*``
+                             -- log_softmax, gather, topk, kl_div and
+                                autograd in float64, differences and special
+                                rows (tests/test_logits_oracle.py).
 * ``hash_lcg_*``             -- the reference's init kernels are closed
                                 integer forms; pinned by hand-computed
                                 values at idx = 0, 1 and 2^20.

@@ -15,7 +15,8 @@ from tests.logits_cases import (DTYPES, EPS, as64, assert_within, entropy_error,
 pytestmark = pytest.mark.gpu
 
 SHAPES = [(1, 1), (3, 2), (2, 7), (5, 63), (4, 257), (3, 1000), (2, 4099), (3, 8192), (2, 8193),
-          (2, 16383), (7, 20003), (2, 50001), (1, 131072), (2, 262144), (2, 300007), (1, 1100001), (300, 515)]
+          (2, 16383), (7, 20003), (2, 50001), (1, 131072), (2, 262144), (2, 300007),
+          (1, 1100001), (300, 515)]
 
 
 def forward(z, tokens, top, entropy=True, temperature=1.0, cfg=None):
@@ -336,7 +337,8 @@ def test_more_rows_than_a_grid_has(gpu):
         lambda x: torch.log_softmax(x, 1).gather(1, tokens), z.double(), dlogp.double())[1]
     p = torch.softmax(z.double(), 1).numpy()
     one = torch.zeros(z.shape, dtype=torch.float64).scatter_(1, tokens, dlogp.double().abs())
-    bound = p * dlogp.double().abs().numpy() * (1.7e-5 + 2 * sum_error(cols)) + one.numpy() * 8 * EPS
+    bound = p * dlogp.double().abs().numpy() * (1.7e-5 + 2 * sum_error(cols))
+    bound += one.numpy() * 8 * EPS
     assert_within(as64(out), want.numpy(), bound, "dlogits")
 
 
