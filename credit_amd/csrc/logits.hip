@@ -1265,7 +1265,7 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
   // The entries whose columns lie in this part, in their order.
   __shared__ int here_col[kMaxEntries];
   __shared__ float here_q[kMaxEntries];
-  __shared__ int here_n;
+  __shared__ int here_n[kNW];
   const int lane = threadIdx.x & (kWave - 1);
   const int part = blockIdx.x;
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
@@ -1283,31 +1283,36 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
     int n = 0, col = 0;
     float own = 0.0f;
     if (!zero) {
-      load_part<T>(v, f, part);
-      if (threadIdx.x < kWave) {
-        for (int k0 = 0; k0 < a.n_top; k0 += kWave) {
-          const int64_t id = k0 + lane < a.n_top ? a.ids[row * a.n_top + k0 + lane] : -1;
-          const bool here = id >= 0 && id < a.cols && id >= first && id - first < kGradBatch<T>;
-          const uint64_t mask = __builtin_amdgcn_ballot_w64(here);
-          if (here) {
-            const int at = n + __builtin_popcountll(mask & ((uint64_t{1} << lane) - 1));
-            const float t = a.teacher[row * a.n_top + k0 + lane];
-            here_col[at] = static_cast<int>(id);
-            here_q[at] = exp_accurate(TAIL ? t : t * a.inv_t - st[kTeacherLse]);
-          }
-          n += __builtin_popcountll(mask);
-        }
-        if (lane == 0) here_n = n;
+      // A thread an entry; all of the row's loads are in flight together.
+      const int k = threadIdx.x, wave = k / kWave;
+      int64_t id = -1;
+      float t = 0.0f;
+      if (k < a.n_top) {
+        id = a.ids[row * a.n_top + k];
+        t = a.teacher[row * a.n_top + k];
       }
+      load_part<T>(v, f, part);
+      const bool here = id >= 0 && id < a.cols && id >= first && id - first < kGradBatch<T>;
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(here);
+      if (lane == 0) here_n[wave] = __builtin_popcountll(mask);
       lds_barrier();
-      n = here_n;
+      int at = __builtin_popcountll(mask & ((uint64_t{1} << lane) - 1));
+      for (int w = 0; w < kNW; ++w) {
+        at += w < wave ? here_n[w] : 0;
+        n += here_n[w];
+      }
+      if (here) {
+        here_col[at] = static_cast<int>(id);
+        here_q[at] = exp_accurate(TAIL ? t : t * a.inv_t - st[kTeacherLse]);
+      }
+      if (n != 0) lds_barrier();
     }
     if (n != 0) {
       if (threadIdx.x < n) {
         col = here_col[threadIdx.x];
         float q = 0.0f;
-        for (int j = 0; j < n; ++j)
-          if (here_col[j] == col) q += here_q[j];
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) q += here_col[j] == col ? here_q[j] : 0.0f;
         const float p = exp_accurate((Elem<T>::get(z + col) - m) * a.inv_t) / s;
         own = g * (mass * p - q);
       }
