@@ -927,9 +927,10 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
 }
 
 // ------------------------------------------------------------- gradients --
-// A workgroup writes kGradVecs vectors a lane of a row's gradient.  The entries
-// that a row names (its tokens, the teacher's columns) get the elementwise
-// value like all others and then, once those stores are in memory, their own.
+// A workgroup writes kGradVecs vectors a lane of a row's gradient.  The teacher's
+// columns get their own value where the lane that holds them has it in registers;
+// the few tokens of a row get the elementwise value like all others and then,
+// once those stores are in memory, their own.
 constexpr int kGradVecs = 4;
 template <class T>
 constexpr int kGradBatch = kThreads * kGradVecs * kN<T>;
@@ -955,26 +956,36 @@ __device__ __forceinline__ void store_grad(T* row, const Frame& f, int e, const 
   }
 }
 
-// The workgroup's part of a row, and value(z) over it (0 where `zero`).
+// The workgroup's part of a row, and value(z) over it (0 where `zero`); own(column,
+// z) of the lane's elements that `named` has a bit for.
 template <class T>
 __device__ __forceinline__ void load_part(u32x4 (&v)[kGradVecs], const Frame& f, int part) {
 #pragma unroll
   for (int k = 0; k < kGradVecs; ++k)
     v[k] = load_vec_nt(f, (part * kGradVecs + k) * kThreads + static_cast<int>(threadIdx.x));
 }
-template <class T, bool VEC, class Fn>
+template <class T, bool VEC, class Fn, class Own>
 __device__ __forceinline__ void write_part(const u32x4 (&v)[kGradVecs], const Frame& f, T* out,
-                                           int part, bool zero, Fn&& value) {
+                                           int part, bool zero, uint32_t named, Fn&& value,
+                                           Own&& own) {
 #pragma unroll
   for (int k = 0; k < kGradVecs; ++k) {
     const u32x4 raw[1] = {v[k]};
-    float g[kN<T>];
-    unpack<T, 1>(g, raw);
+    float z[kN<T>], g[kN<T>];
+    unpack<T, 1>(z, raw);
 #pragma unroll
-    for (int i = 0; i < kN<T>; ++i) g[i] = zero ? 0.0f : value(g[i]);
-    store_grad<T, VEC>(out, f,
-                       ((part * kGradVecs + k) * kThreads + static_cast<int>(threadIdx.x)) * kN<T>,
-                       g);
+    for (int i = 0; i < kN<T>; ++i) g[i] = zero ? 0.0f : value(z[i]);
+    const int e = ((part * kGradVecs + k) * kThreads + static_cast<int>(threadIdx.x)) * kN<T>;
+    for (uint32_t d = named >> (k * kN<T>) & ((1u << kN<T>) - 1); d != 0; d &= d - 1) {
+      const int at = __builtin_ctz(d);
+      float x = z[0];
+#pragma unroll
+      for (int i = 1; i < kN<T>; ++i) x = at == i ? z[i] : x;
+      x = own(e + at - f.head, x);
+#pragma unroll
+      for (int i = 0; i < kN<T>; ++i) g[i] = at == i ? x : g[i];
+    }
+    store_grad<T, VEC>(out, f, e, g);
   }
 }
 
@@ -1066,7 +1077,7 @@ __global__ __launch_bounds__(kThreads) void token_logprob_bwd_kernel(LogprobGrad
       }
       memory_barrier();  // dlogits may be logits: read before anything is written
     }
-    write_part<T, VEC>(v, f, out, part, zero, value);
+    write_part<T, VEC>(v, f, out, part, zero, 0, value, [](int, float x) { return x; });
     if (patch) {
       memory_barrier();
       if (col >= 0) Elem<T>::put(out + col, own);
@@ -1262,10 +1273,13 @@ struct DistillGradArgs {
 // 175.6 us, 6.12 TB/s; 512 x 262144 fp32, K = 128, tail 176.1.
 template <class T, bool TAIL, bool VEC>
 __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradArgs<T> a) {
-  // The entries whose columns lie in this part, in their order.
+  // The entries whose columns lie in this part, in their order; a bit for each of a
+  // lane's elements that one names, and which; whether two name the same.
   __shared__ int here_col[kMaxEntries];
   __shared__ float here_q[kMaxEntries];
-  __shared__ int here_n[kNW];
+  __shared__ uint32_t here_bits[kThreads];
+  __shared__ uint8_t here_at[kGradBatch<T>];
+  __shared__ int here_n[kNW], here_twice;
   const int lane = threadIdx.x & (kWave - 1);
   const int part = blockIdx.x;
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
@@ -1280,8 +1294,8 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
     // S = 0: a row without entries, or of -inf alone.
     const bool zero = s == 0.0f || g == 0.0f || mass == 0.0f;
     u32x4 v[kGradVecs] = {};
-    int n = 0, col = 0;
-    float own = 0.0f;
+    int n = 0;
+    uint32_t named = 0;
     if (!zero) {
       // A thread an entry; all of the row's loads are in flight together.
       const int k = threadIdx.x, wave = k / kWave;
@@ -1295,6 +1309,8 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
       const bool here = id >= 0 && id < a.cols && id >= first && id - first < kGradBatch<T>;
       const uint64_t mask = __builtin_amdgcn_ballot_w64(here);
       if (lane == 0) here_n[wave] = __builtin_popcountll(mask);
+      here_bits[k] = 0;
+      if (k == 0) here_twice = 0;
       lds_barrier();
       int at = __builtin_popcountll(mask & ((uint64_t{1} << lane) - 1));
       for (int w = 0; w < kNW; ++w) {
@@ -1304,19 +1320,15 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
       if (here) {
         here_col[at] = static_cast<int>(id);
         here_q[at] = exp_accurate(TAIL ? t : t * a.inv_t - st[kTeacherLse]);
+        const int e = static_cast<int>(id) - first, vec = e / kN<T>;
+        const uint32_t bit = 1u << (vec / kThreads * kN<T> + e % kN<T>);
+        here_at[e] = static_cast<uint8_t>(at);
+        if ((atomicOr(&here_bits[vec % kThreads], bit) & bit) != 0) here_twice = 1;
       }
-      if (n != 0) lds_barrier();
-    }
-    if (n != 0) {
-      if (threadIdx.x < n) {
-        col = here_col[threadIdx.x];
-        float q = 0.0f;
-#pragma unroll 8
-        for (int j = 0; j < n; ++j) q += here_col[j] == col ? here_q[j] : 0.0f;
-        const float p = exp_accurate((Elem<T>::get(z + col) - m) * a.inv_t) / s;
-        own = g * (mass * p - q);
+      if (n != 0) {
+        lds_barrier();
+        named = here_bits[k];
       }
-      memory_barrier();  // dlogits may be logits: read before anything is written
     }
     float ref = m, A = g * mass / s;
     if (TAIL) {
@@ -1324,12 +1336,17 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
       ref = some ? st[kTailMax] : m;
       A = some ? g * st[kTailGrad] / st[kTailSum] : g * st[kTailGrad];
     }
-    write_part<T, VEC>(v, f, out, part, zero,
-                       [&](float x) { return __builtin_amdgcn_exp2f((x - ref) * a.c) * A; });
-    if (n != 0) {
-      memory_barrier();
-      if (threadIdx.x < n) Elem<T>::put(out + col, own);
-    }
+    write_part<T, VEC>(
+        v, f, out, part, zero, named,
+        [&](float x) { return __builtin_amdgcn_exp2f((x - ref) * a.c) * A; },
+        [&](int col, float x) {
+          float q = 0.0f;
+          if (here_twice == 0)
+            q = here_q[here_at[col - first]];
+          else
+            for (int j = 0; j < n; ++j) q += here_col[j] == col ? here_q[j] : 0.0f;
+          return g * (mass * exp_accurate((x - m) * a.inv_t) / s - q);
+        });
     if (row + gridDim.y < a.rows) lds_barrier();  // before the next row's list
   }
 }
