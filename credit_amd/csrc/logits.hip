@@ -927,10 +927,11 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
 }
 
 // ------------------------------------------------------------- gradients --
-// A workgroup writes kGradVecs vectors a lane of a row's gradient.  The teacher's
-// columns get their own value where the lane that holds them has it in registers;
-// the few tokens of a row get the elementwise value like all others and then,
-// once those stores are in memory, their own.
+// A workgroup writes kGradVecs vectors a lane of a row's gradient, in place too: a
+// lane writes what it has read.  The entries that a row names (its tokens, the
+// teacher's columns) get their own value in the registers of the lane that holds
+// them (patched in memory afterwards, 2048 x 131072 bf16 with 64 entries took
+// 173.6 us instead of 169.8, 8192 x 32768 with 256 260 instead of 176).
 constexpr int kGradVecs = 4;
 template <class T>
 constexpr int kGradBatch = kThreads * kGradVecs * kN<T>;
@@ -989,12 +990,6 @@ __device__ __forceinline__ void write_part(const u32x4 (&v)[kGradVecs], const Fr
   }
 }
 
-// Stores of this wave are in memory, then the workgroup meets.
-__device__ __forceinline__ void memory_barrier() {
-  publish_wait();
-  lds_barrier();
-}
-
 template <class T>
 struct LogprobGradArgs {
   const T* logits;
@@ -1013,8 +1008,8 @@ struct LogprobGradArgs {
 
 // One read, one write; a workgroup's part is four vectors a lane, all loaded
 // before the first is used.
-// 2048 x 131072 bf16 with the entropy's gradient 174 us, 6.17 TB/s (a kernel that
-// reads and writes as much and does nothing else reaches 6.37).
+// 2048 x 131072 bf16 with the entropy's gradient 173.2 us, 6.20 TB/s (a kernel
+// that reads and writes as much and does nothing else reaches 6.37).
 template <class T, bool ENT, bool VEC>
 __global__ __launch_bounds__(kThreads) void token_logprob_bwd_kernel(LogprobGradArgs<T> a) {
   const int lane = threadIdx.x & (kWave - 1);
@@ -1027,20 +1022,29 @@ __global__ __launch_bounds__(kThreads) void token_logprob_bwd_kernel(LogprobGrad
     if (first >= a.cols) continue;
     const int64_t* tokens = a.tokens + row * a.n_tokens;
     const float* dlogp = a.dlogp + row * a.n_tokens;
-    // Every wave by itself: the tokens' weight, and whether one lies here.
+    // Every wave by itself: the tokens' weight, and the lane's elements that they name.
     double weight = 0.0;
-    bool live = false, here = false;
-    for (int k = lane; k < a.n_tokens; k += kWave) {
-      const int64_t tok = tokens[k];
-      const float g = dlogp[k];
-      if (tok < 0 || g == 0.0f) continue;
-      live = true;
-      weight += tok >= a.cols ? kNaN : g;
-      here |= tok < a.cols && tok >= first && tok - first < kGradBatch<T>;
+    bool live = false;
+    uint32_t named = 0;
+    for (int k0 = 0; k0 < a.n_tokens; k0 += kWave) {
+      const int k = k0 + lane;
+      const int64_t tok = k < a.n_tokens ? tokens[k] : -1;
+      const float g = k < a.n_tokens ? dlogp[k] : 0.0f;
+      const bool counts = tok >= 0 && g != 0.0f;
+      live |= counts;
+      if (counts) weight += tok >= a.cols ? kNaN : g;
+      const int64_t e = tok - first;
+      uint64_t here = __builtin_amdgcn_ballot_w64(counts && tok < a.cols && e >= 0 &&
+                                                  e < kGradBatch<T>);
+      for (; here != 0; here &= here - 1) {
+        const int at = __builtin_amdgcn_readlane(static_cast<int>(e), __builtin_ctzll(here));
+        const int vec = at / kN<T>;
+        if (vec % kThreads == static_cast<int>(threadIdx.x))
+          named |= 1u << (vec / kThreads * kN<T> + at % kN<T>);
+      }
     }
     const float gsum = static_cast<float>(wave_reduce_sum_f64(weight));
     live = __builtin_amdgcn_ballot_w64(live) != 0;
-    here = __builtin_amdgcn_ballot_w64(here) != 0;
     const float m = a.stats[2 * row], s = a.stats[2 * row + 1];
     const float h = ENT ? a.dentropy[row] : 0.0f;
     // dz = e^(x - m/T) (A + B log2 e^(x - m/T)).
@@ -1060,28 +1064,13 @@ __global__ __launch_bounds__(kThreads) void token_logprob_bwd_kernel(LogprobGrad
     };
     u32x4 v[kGradVecs] = {};
     if (!zero) load_part<T>(v, f, part);
-    float own = 0.0f;
-    const bool patch = here && !zero;
-    const int mine = threadIdx.x < a.n_tokens ? static_cast<int>(threadIdx.x) : -1;
-    int64_t col = -1;
-    if (patch) {
-      if (mine >= 0) {
-        const int64_t tok = tokens[mine];
-        if (tok >= 0 && tok < a.cols && tok >= first && tok - first < kGradBatch<T>) {
-          col = tok;
-          double g = 0.0;
-          for (int j = 0; j < a.n_tokens; ++j)
-            if (tokens[j] == tok) g += dlogp[j];
-          own = static_cast<float>(g) * a.inv_t + value(Elem<T>::get(z + tok));
-        }
-      }
-      memory_barrier();  // dlogits may be logits: read before anything is written
-    }
-    write_part<T, VEC>(v, f, out, part, zero, 0, value, [](int, float x) { return x; });
-    if (patch) {
-      memory_barrier();
-      if (col >= 0) Elem<T>::put(out + col, own);
-    }
+    if (zero) named = 0;
+    write_part<T, VEC>(v, f, out, part, zero, named, value, [&](int col, float x) {
+      double g = 0.0;
+      for (int j = 0; j < a.n_tokens; ++j)
+        if (tokens[j] == col) g += dlogp[j];
+      return static_cast<float>(g) * a.inv_t + value(x);
+    });
   }
 }
 
@@ -1270,7 +1259,7 @@ struct DistillGradArgs {
 };
 
 // One read, one write, as token_logprob_bwd_kernel: 2048 x 131072 bf16, K = 64
-// 175.6 us, 6.12 TB/s; 512 x 262144 fp32, K = 128, tail 176.1.
+// 170.6 us, 6.30 TB/s; 512 x 262144 fp32, K = 128, tail 173.0.
 template <class T, bool TAIL, bool VEC>
 __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradArgs<T> a) {
   // The entries whose columns lie in this part, in their order; a bit for each of a
