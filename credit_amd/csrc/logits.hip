@@ -68,8 +68,9 @@ struct Frame {
   uint32_t skip;    // bytes of the frame before those
   int head, end;
 };
+// Of them, the loads reach those below `upto`.
 template <class T>
-__device__ __forceinline__ Frame frame_of(const T* row, int cols) {
+__device__ __forceinline__ Frame frame_of(const T* row, int cols, int upto = 0x7FFFFFFF) {
   Frame f;
   const uintptr_t a = reinterpret_cast<uintptr_t>(row);
   const uint32_t in_line = static_cast<uint32_t>(a & (kLine - 1));
@@ -78,8 +79,8 @@ __device__ __forceinline__ Frame frame_of(const T* row, int cols) {
   f.end = f.head + cols;
   // Whole dwords: the last one holds the row's last element.
   f.r = make_rsrc(reinterpret_cast<const void*>(a & ~uintptr_t{15}),
-                  (static_cast<uint32_t>(f.end) * static_cast<uint32_t>(sizeof(T)) + 3u & ~3u) -
-                      f.skip);
+                  (static_cast<uint32_t>(min(f.end, upto)) * static_cast<uint32_t>(sizeof(T)) + 3u &
+                   ~3u) - f.skip);
   return f;
 }
 __device__ __forceinline__ u32x4 load_vec(const Frame& f, int vec) {
@@ -875,8 +876,9 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
   Joined j;
   if constexpr (SPLIT) {
     const int b0 = blockIdx.x * a.parts.batches, b1 = min(b0 + a.parts.batches, batches);
+    const Frame own = frame_of(z, a.cols, b1 * kBatch);  // the next part's batch is not read ahead
     float* out = a.parts.units + (row * a.parts.n * a.parts.batches) * kThreads + threadIdx.x;
-    j = scan<T, ENT>(f, b0, b1, a.c, join, none_dropped, [&](int b, const float (&vm)[kU<T>]) {
+    j = scan<T, ENT>(own, b0, b1, a.c, join, none_dropped, [&](int b, const float (&vm)[kU<T>]) {
       if constexpr (TOP) publish(out + b * kThreads, unit_max<T>(vm));
     });
     publish_part(a.parts, row, j, false);
@@ -1152,6 +1154,7 @@ __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<
   const int batches = (f.end + kBatch - 1) / kBatch;
   const int first_batch = SPLIT ? blockIdx.x * a.parts.batches : 0;
   const int end_batch = SPLIT ? min(first_batch + a.parts.batches, batches) : batches;
+  const Frame own = SPLIT ? frame_of(z, a.cols, end_batch * kBatch) : f;
   Joined j{kNegInf, 0.0, 0.0};  // of a part without batches
   if constexpr (TAIL) {
     __shared__ uint32_t bits[kSegWords];
@@ -1164,12 +1167,12 @@ __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<
       if (live && mark<T>(bits, static_cast<int>(id) + f.head, b0, b1)) repeated = 1;
       __syncthreads();
       const Joined p = scan<T, false>(
-          f, b0, b1, a.c, join, [&](int b) { return bits[(b - b0) * kThreads + threadIdx.x]; },
+          own, b0, b1, a.c, join, [&](int b) { return bits[(b - b0) * kThreads + threadIdx.x]; },
           unseen);
       j = b0 == first_batch ? p : merge(j, p, a.temperature);
     }
   } else {
-    j = scan<T, false>(f, first_batch, end_batch, a.c, join, none_dropped, unseen);
+    j = scan<T, false>(own, first_batch, end_batch, a.c, join, none_dropped, unseen);
   }
   bool twice = TAIL && repeated != 0;
   if constexpr (SPLIT) {
