@@ -243,6 +243,25 @@ def test_backward_in_place(gpu, dtype, cols):
     assert torch.equal(apart, over)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols,offset", [(256, 0), (300, 5), (9001, 1), (131072, 0)])
+def test_backward_crowded_tokens(gpu, dtype, cols, offset):
+    """As many tokens as a row takes: neighbours, all of them one, the row's ends."""
+    print(f"token_logprob_bwd crowded {dtype} {cols}", flush=True)
+    z = make_logits(4, cols, dtype, 51)
+    tokens = torch.randint(0, cols, (4, 256), generator=generator(52))
+    tokens[0] = cols - 256 + torch.arange(256)
+    tokens[1] = cols // 2
+    tokens[2] = torch.arange(256) // 2 * 2
+    dlogp = torch.randn(tokens.shape, generator=generator(53))
+    dent = torch.randn(4, generator=generator(54))
+    apart = backward(placed(z, gpu, offset, offset), tokens, dlogp, dent, 0.9, gpu)
+    check_backward(z, tokens, dlogp, dent, 0.9, dtype, apart)
+    over = placed(z, gpu, offset, offset)
+    backward(over, tokens, dlogp, dent, 0.9, gpu, out=over)
+    assert torch.equal(apart, over)
+
+
 def test_backward_against_differences(gpu):
     """The kernels' own forward, differentiated numerically."""
     rows, cols, step = 3, 37, 1e-2

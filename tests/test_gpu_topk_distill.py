@@ -141,6 +141,30 @@ def test_absent_and_repeated_entries(gpu, dtype, tail):
 
 
 @pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols,offset", [(256, 0), (300, 5), (9001, 1), (131072, 0)])
+def test_crowded_entries(gpu, cols, offset, dtype, tail):
+    """As many entries as a row takes: neighbours, most of them one column, the
+    row's ends, each column twice."""
+    print(f"topk_distill crowded {dtype} {cols} tail {tail}", flush=True)
+    z = make_logits(4, cols, dtype, 76)
+    at = torch.arange(256)
+    ids = torch.stack([cols - 256 + at, torch.where(at < 3, at, cols // 2), at // 2 * 2,
+                       torch.randperm(cols, generator=generator(77))[:256]])
+    teacher = torch.randn(ids.shape, generator=generator(78))
+    if tail:
+        teacher = torch.log_softmax(teacher, 1) - 0.125
+    dloss = torch.randn(4, generator=generator(79))
+    zs = placed(z, gpu, offset, offset)
+    loss, _ = forward(zs, ids, teacher, tail, 0.9, gpu)
+    check_loss(z, ids, teacher, tail, 0.9, loss)
+    apart = backward(zs, ids, teacher, dloss, tail, 0.9, gpu)
+    check_gradient(z, ids, teacher, dloss, tail, 0.9, dtype, apart)
+    backward(zs, ids, teacher, dloss, tail, 0.9, gpu, out=zs)
+    assert torch.equal(apart, zs)
+
+
+@pytest.mark.parametrize("tail", [False, True])
 def test_rows_without_weight_are_not_read(gpu, tail):
     rows, cols = 4, 5003
     z = make_logits(rows, cols, "bf16", 60).to(gpu)
