@@ -1370,6 +1370,11 @@ int check_logits(const void* p, const char* name, int64_t ld, int64_t rows, int6
                      static_cast<long long>(rows), static_cast<long long>(ld));
   return CREDIT_OK;
 }
+// An operand with something for every row, its elements at their own alignment.
+int check_operand(const void* p, const char* name, int64_t rows, size_t elem) {
+  CREDIT_TRY(check_row_ptr(p, name, rows));
+  return check_aligned(p, elem, name);
+}
 int check_entries(int32_t n, int32_t least, int64_t most, const char* what) {
   if (n < least || n > most)
     return set_error(CREDIT_ERR_BAD_SHAPE, "%d %s a row: need %d to %lld", n, what, least,
@@ -1471,15 +1476,16 @@ int logprob_fwd(const T* logits, int64_t ld, const int64_t* tokens, float* logp,
   CREDIT_TRY(check_logits(logits, "logits", ld, rows, cols, sizeof(T)));
   CREDIT_TRY(check_entries(n_tokens, 0, kMaxEntries, "tokens"));
   CREDIT_TRY(check_entries(n_top, 0, cols < kMaxEntries ? cols : kMaxEntries, "alternatives"));
-  CREDIT_TRY(check_row_ptr(stats, "stats", rows));
+  CREDIT_TRY(check_operand(stats, "stats", rows, sizeof(float)));
   if (n_tokens > 0) {
-    CREDIT_TRY(check_row_ptr(tokens, "tokens", rows));
-    CREDIT_TRY(check_row_ptr(logp, "logp", rows));
+    CREDIT_TRY(check_operand(tokens, "tokens", rows, sizeof(int64_t)));
+    CREDIT_TRY(check_operand(logp, "logp", rows, sizeof(float)));
   }
   if (n_top > 0) {
-    CREDIT_TRY(check_row_ptr(top_logp, "top_logp", rows));
-    CREDIT_TRY(check_row_ptr(top_ids, "top_ids", rows));
+    CREDIT_TRY(check_operand(top_logp, "top_logp", rows, sizeof(float)));
+    CREDIT_TRY(check_operand(top_ids, "top_ids", rows, sizeof(int64_t)));
   }
+  CREDIT_TRY(check_aligned(entropy, sizeof(float), "entropy"));
   CREDIT_TRY(check_temperature(temperature));
   CREDIT_TRY(check_variant(cfg, true));
   if (rows == 0) return CREDIT_OK;
@@ -1521,12 +1527,15 @@ int logprob_bwd(const T* logits, int64_t ld, const int64_t* tokens, const float*
   CREDIT_TRY(check_logits(logits, "logits", ld, rows, cols, sizeof(T)));
   CREDIT_TRY(check_logits(dlogits, "dlogits", ldd, rows, cols, sizeof(T)));
   CREDIT_TRY(check_entries(n_tokens, 0, kMaxEntries, "tokens"));
-  CREDIT_TRY(check_row_ptr(stats, "stats", rows));
+  CREDIT_TRY(check_operand(stats, "stats", rows, sizeof(float)));
   if (n_tokens > 0) {
-    CREDIT_TRY(check_row_ptr(tokens, "tokens", rows));
-    CREDIT_TRY(check_row_ptr(dlogp, "dlogp", rows));
+    CREDIT_TRY(check_operand(tokens, "tokens", rows, sizeof(int64_t)));
+    CREDIT_TRY(check_operand(dlogp, "dlogp", rows, sizeof(float)));
   }
-  if (dentropy != nullptr) CREDIT_TRY(check_row_ptr(entropy, "entropy", rows));
+  if (dentropy != nullptr) {
+    CREDIT_TRY(check_operand(entropy, "entropy", rows, sizeof(float)));
+    CREDIT_TRY(check_aligned(dentropy, sizeof(float), "dentropy"));
+  }
   CREDIT_TRY(check_temperature(temperature));
   CREDIT_TRY(check_variant(cfg, false));
   if (rows == 0) return CREDIT_OK;
@@ -1562,10 +1571,10 @@ int distill_fwd(const T* logits, int64_t ld, const int64_t* ids, const float* te
   CREDIT_TRY(check_shape(rows, cols, kMaxCols));
   CREDIT_TRY(check_logits(logits, "logits", ld, rows, cols, sizeof(T)));
   CREDIT_TRY(check_entries(n_top, 1, kMaxEntries, "teacher entries"));
-  CREDIT_TRY(check_row_ptr(ids, "teacher_ids", rows));
-  CREDIT_TRY(check_row_ptr(teacher, "teacher", rows));
-  CREDIT_TRY(check_row_ptr(loss, "loss", rows));
-  CREDIT_TRY(check_row_ptr(stats, "stats", rows));
+  CREDIT_TRY(check_operand(ids, "teacher_ids", rows, sizeof(int64_t)));
+  CREDIT_TRY(check_operand(teacher, "teacher", rows, sizeof(float)));
+  CREDIT_TRY(check_operand(loss, "loss", rows, sizeof(float)));
+  CREDIT_TRY(check_operand(stats, "stats", rows, sizeof(float)));
   CREDIT_TRY(check_temperature(temperature));
   CREDIT_TRY(check_variant(cfg, true));
   if (rows == 0) return CREDIT_OK;
@@ -1593,10 +1602,10 @@ int distill_bwd(const T* logits, int64_t ld, const int64_t* ids, const float* te
   CREDIT_TRY(check_logits(logits, "logits", ld, rows, cols, sizeof(T)));
   CREDIT_TRY(check_logits(dlogits, "dlogits", ldd, rows, cols, sizeof(T)));
   CREDIT_TRY(check_entries(n_top, 1, kMaxEntries, "teacher entries"));
-  CREDIT_TRY(check_row_ptr(ids, "teacher_ids", rows));
-  CREDIT_TRY(check_row_ptr(teacher, "teacher", rows));
-  CREDIT_TRY(check_row_ptr(stats, "stats", rows));
-  CREDIT_TRY(check_row_ptr(dloss, "dloss", rows));
+  CREDIT_TRY(check_operand(ids, "teacher_ids", rows, sizeof(int64_t)));
+  CREDIT_TRY(check_operand(teacher, "teacher", rows, sizeof(float)));
+  CREDIT_TRY(check_operand(stats, "stats", rows, sizeof(float)));
+  CREDIT_TRY(check_operand(dloss, "dloss", rows, sizeof(float)));
   CREDIT_TRY(check_temperature(temperature));
   CREDIT_TRY(check_variant(cfg, false));
   if (rows == 0) return CREDIT_OK;

@@ -89,6 +89,23 @@ def test_staged_variant_and_bad_cfg(lib, op):
         assert call(lib, op, "f32", cfg=ctypes.byref(cfg)) == status
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("op", CALLS)
+def test_operands_off_their_alignment(lib, op, dtype):
+    """Every pointer at half an element: of 8 bytes the columns', of 4 the rest."""
+    columns = ("tokens", "teacher_ids", "top_ids")
+    for name, value in CALLS[op].items():
+        if value in (FAKE, 2 * FAKE):
+            off = 1 if name in ("logits", "dlogits") else 4 if name in columns else 2
+            assert call(lib, op, dtype, **{name: value + off}) == ALIGN, name
+
+
+@pytest.mark.parametrize("op", ["token_logprob_bwd", "topk_distill_bwd"])
+def test_gradients_have_no_parts(lib, op):
+    cfg = hip_lib.CreditCfg(None, hip_lib.VARIANTS["split"], 4, None, 0)
+    assert call(lib, op, "bf16", cfg=ctypes.byref(cfg)) == UNSUPPORTED
+
+
 @pytest.mark.parametrize("op", CALLS)
 def test_no_rows_is_a_noop(lib, op):
     nothing = {k: None for k, v in CALLS[op].items() if v is FAKE or v == 2 * FAKE}
