@@ -752,17 +752,26 @@ __device__ __forceinline__ void write_top(const Frame& f, const T* units, CandPt
   constexpr int kPer = kU<T> == 4 ? 2 : 3;  // vectors of a unit in a batch: 4 or 8
   static_assert(kU<T> == 1 << kPer);
   const int per = kPer + fold, vecs = listed << per;
+  // The lane's vector of the listed units' i0-th and following.
+  const auto vector_at = [&](int i0) {
+    const int i = i0 + static_cast<int>(threadIdx.x & (kWave - 1));
+    const int unit = mine[i < vecs ? i >> per : 0];
+    // Vector `first % kU` of lanes first / kU kU + [0, kU), in batch b.
+    const int b = (unit / kThreads << fold) + (i >> kPer & ((1 << fold) - 1));
+    const int first = unit % kThreads;
+    return (b * kU<T> + first % kU<T>)*kThreads + first / kU<T> * kU<T> + i % kU<T>;
+  };
   int n = kCands + 1;
   while (!crowded) {
+    int vec = 0, next_vec = 0;
+    u32x4 raw[1] = {}, next = {};
+    if (vecs != 0) next = load_vec(f, next_vec = vector_at(0));
 #pragma unroll 1
     for (int i0 = 0; i0 < vecs; i0 += kWave) {
       const int i = i0 + static_cast<int>(threadIdx.x & (kWave - 1));
-      const int unit = mine[i < vecs ? i >> per : 0];
-      // Vector `first % kU` of lanes first / kU kU + [0, kU), in batch b.
-      const int b = (unit / kThreads << fold) + (i >> kPer & ((1 << fold) - 1));
-      const int first = unit % kThreads;
-      const int vec = (b * kU<T> + first % kU<T>)*kThreads + first / kU<T> * kU<T> + i % kU<T>;
-      const u32x4 raw[1] = {load_vec(f, vec)};
+      raw[0] = next;
+      vec = next_vec;
+      if (i0 + kWave < vecs) next = load_vec(f, next_vec = vector_at(i0 + kWave));
       const int e0 = vec * kN<T>;
       float z[kN<T>];
       unpack<T, 1>(z, raw);
