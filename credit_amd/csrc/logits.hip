@@ -1267,7 +1267,7 @@ struct DistillGradArgs {
   int64_t ldd;
   int64_t rows;
   int cols, n_top;
-  float inv_t, c;
+  float temperature, c;
 };
 
 // One read, one write, as token_logprob_bwd_kernel: 2048 x 131072 bf16, K = 64
@@ -1281,6 +1281,7 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
   __shared__ uint32_t here_bits[kThreads];
   __shared__ uint8_t here_at[kGradBatch<T>];
   __shared__ int here_n[kNW], here_twice;
+  __shared__ float teacher_max[kNW], teacher_sum[kNW];
   const int lane = threadIdx.x & (kWave - 1);
   const int part = blockIdx.x;
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
@@ -1291,7 +1292,7 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
     if (first >= a.cols) continue;
     const float* st = a.stats + 8 * row;
     const float m = st[kMax], s = st[kSum], mass = st[kMass];
-    const float g = a.dloss[row] * a.inv_t;
+    const float g = a.dloss[row] / a.temperature;
     // S = 0: a row without entries, or of -inf alone.
     const bool zero = s == 0.0f || g == 0.0f || mass == 0.0f;
     u32x4 v[kGradVecs] = {};
@@ -1309,7 +1310,9 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
       load_part<T>(v, f, part);
       const bool here = id >= 0 && id < a.cols && id >= first && id - first < kGradBatch<T>;
       const uint64_t mask = __builtin_amdgcn_ballot_w64(here);
-      if (lane == 0) here_n[wave] = __builtin_popcountll(mask);
+      const bool live = id >= 0 && id < a.cols;
+      const float most = TAIL ? 0.0f : wave_reduce(live ? t : kNegInf, MaxOp{});
+      if (lane == 0) here_n[wave] = __builtin_popcountll(mask), teacher_max[wave] = most;
       here_bits[k] = 0;
       if (k == 0) here_twice = 0;
       lds_barrier();
@@ -1318,9 +1321,22 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
         at += w < wave ? here_n[w] : 0;
         n += here_n[w];
       }
+      // q about the teacher's maximum, as the forward has it: the log-sum of logits
+      // near 20 is off by 10^-6 in fp32, and with it every q formed from that.
+      float q = 0.0f;
+      if (n != 0 && live) {
+        float tm = kNegInf;
+        if (!TAIL)
+          for (int w = 0; w < kNW; ++w) tm = fmax_nan(tm, teacher_max[w]);
+        q = exp_accurate(TAIL ? t : (t - tm) / a.temperature);
+      }
+      if (!TAIL && n != 0) {
+        const float sum = wave_reduce(q, SumOp{});
+        if (lane == 0) teacher_sum[wave] = sum;
+      }
       if (here) {
         here_col[at] = static_cast<int>(id);
-        here_q[at] = exp_accurate(TAIL ? t : t * a.inv_t - st[kTeacherLse]);
+        here_q[at] = q;
         const int e = static_cast<int>(id) - first, vec = e / kN<T>;
         const uint32_t bit = 1u << (vec / kThreads * kN<T> + e % kN<T>);
         here_at[e] = static_cast<uint8_t>(at);
@@ -1346,7 +1362,12 @@ __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradA
             q = here_q[here_at[col - first]];
           else
             for (int j = 0; j < n; ++j) q += here_col[j] == col ? here_q[j] : 0.0f;
-          return g * (mass * exp_accurate((x - m) * a.inv_t) / s - q);
+          if (!TAIL) {
+            float sum = 0.0f;
+            for (int w = 0; w < kNW; ++w) sum += teacher_sum[w];
+            q /= sum;
+          }
+          return g * (mass * exp_accurate((x - m) / a.temperature) / s - q);
         });
     if (row + gridDim.y < a.rows) lds_barrier();  // before the next row's list
   }
@@ -1630,7 +1651,7 @@ int distill_bwd(const T* logits, int64_t ld, const int64_t* ids, const float* te
                              rows,
                              static_cast<int>(cols),
                              n_top,
-                             1.0f / temperature,
+                             temperature,
                              log2e_over(temperature)};
   hipStream_t stream = cfg_stream(cfg);
   const dim3 grid = grad_grid(logits, ld, rows, cols);
