@@ -860,10 +860,10 @@ __device__ __forceinline__ void fetch_units(const Parts& p, int64_t row, int bat
 
 // One read of the logits.  512 x 262144 fp32 with the entropy 77.6 us, 6.92 TB/s
 // (a kernel that reads alone reaches 7.08); 2048 x 131072 bf16 83 us without
-// alternatives (6.5 TB/s) and 95 with 64 (5.65): the workgroups that a CU holds
+// alternatives (6.5 TB/s) and 93 with 64 (5.78): the workgroups that a CU holds
 // reach their rows' ends together, where a row's choice of alternatives, some
 // 9000 cycles of latency, has no loads to hide it.  64 x 131072 in four parts
-// each, K = 20: 13.6 us, of which the stream 4, the parts' meeting and the units
+// each, K = 20: 13.4 us, of which the stream 4, the parts' meeting and the units
 // from past the L2 2.5, the choice 3.5.
 template <class T, bool ENT, bool TOP, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs<T> a) {
