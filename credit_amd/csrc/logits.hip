@@ -1228,8 +1228,11 @@ __global__ __launch_bounds__(kThreads) void topk_distill_fwd_kernel(DistillArgs<
     loss = sums[2] - sums[3] + q * ln_s;
     rest = q < 1.0 ? 1.0 - q : (q == q ? 0.0 : q);
     double share = 0.0;
-    // A tail without mass (every other column masked) adds nothing.
-    if (j.s != 0.0) {
+    // Without mass outside the entries (all of it masked) nothing is held against
+    // them: neither the loss nor its gradient has that term.
+    if (j.s == 0.0) {
+      rest = 0.0;
+    } else {
       const double ln_tail = (static_cast<double>(j.m) - m) / a.temperature + ::log(j.s) - ln_s;
       share = ::exp(ln_tail);
       if (rest != 0.0) loss += rest * (::log(rest) - ln_tail);

@@ -725,8 +725,8 @@ def topk_distill_fwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: t
     logits as in token_logprob_fwd (the student's); teacher_ids int64 and
     teacher fp32 [rows, k] (negative id: absent).  tail: teacher holds
     log-probabilities at this temperature (token_logprob_fwd's top_logp) and
-    what they leave of 1 is held against the other columns together; without
-    it, logits over whose softmax the entries are all there is.  Written: loss
+    what they leave of 1 is held against the other columns together, unless
+    those are masked altogether; without it, logits over whose softmax the entries are all there is.  Written: loss
     [rows], stats [rows, 8] for the backward."""
     rows, cols, ld, dev, fn = _logits_call("credit_topk_distill_fwd_", logits)
     f32 = torch.float32

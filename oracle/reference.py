@@ -517,5 +517,7 @@ def topk_distill_bwd(z, ids, teacher, dloss, tail: bool = True, temperature: flo
                 o = lp[r, others]
                 w = np.exp(o - o.max())
                 target[others] = rest * w / w.sum()
+            else:  # nothing is held against columns without mass
+                rest = 0.0
             out[r] = (np.exp(lp[r]) * (q.sum() + rest) - target) * dloss[r] / temperature
     return out
