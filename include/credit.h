@@ -381,8 +381,9 @@ int credit_token_logprob_bwd_bf16(const uint16_t* logits, int64_t ld, const int6
  *     credit_token_logprob_fwd_* at the same T), q_k = e^teacher_k, and the
  *     rest 1 - sum q_k (0 if that is negative) is held against all other
  *     columns' probability together, which is summed directly over them.
- * Entries that name one column add up.  A row without entries (tail == 0: or
- * with all of them -inf): loss 0, stats 0, the logits not read.  An id >= cols
+ * Entries that name one column add up: its q is their sum, in the loss too.  A
+ * row without entries (tail == 0: or with all of them -inf): loss 0, stats 0,
+ * the logits not read.  An id >= cols
  * makes the loss NaN; p = 0 where q > 0 makes it +inf, but where no column
  * outside the entries has mass (all of them -inf, or every column named) the
  * rest counts as 0, in the loss and in its gradient.  stats [rows, 8] is what

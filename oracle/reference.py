@@ -484,6 +484,9 @@ def topk_distill_fwd(z, ids, teacher, tail: bool = True, temperature: float = 1.
             if (at >= cols).any():
                 loss[r] = np.nan
                 continue
+            # Entries that name one column add up.
+            at, of = np.unique(at, return_inverse=True)
+            q = np.bincount(of, weights=q)
             loss[r] = np.where(q == 0.0, 0.0, q * (np.log(q) - lp[r, at])).sum()
             others = np.ones(cols, bool)
             others[at] = False
