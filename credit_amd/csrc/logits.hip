@@ -251,6 +251,9 @@ __device__ __forceinline__ Joined join_lanes(const Lane& a, float c, JoinSlots& 
   }
   if (j.m != j.m) j.s = kNaN;
   rows::block_sum2<kNW>(j.s, j.t, slots.st);
+  // The maximum's own e^0 is in the sum, formed as 2^d 2^-d of two roundings.
+  // Parts and segments keep this: the one with the maximum joins with a factor of 1.
+  if (j.m != kNegInf && j.s < 1.0) j.s = 1.0;
   return j;
 }
 
@@ -914,7 +917,10 @@ __global__ __launch_bounds__(kThreads) void token_logprob_fwd_kernel(LogprobArgs
       shared_ln_s = ln_s;
       a.stats[2 * row] = j.m;
       a.stats[2 * row + 1] = static_cast<float>(j.s);
-      if (ENT) a.entropy[row] = empty ? 0.0f : static_cast<float>(ln_s - kLn2 * j.t / j.s);
+      if (ENT) {
+        const float h = empty ? 0.0f : static_cast<float>(ln_s - kLn2 * j.t / j.s);
+        a.entropy[row] = h < 0.0f ? 0.0f : h;  // NaN stays
+      }
     }
   }
   const auto log_p = [&](float v) {

@@ -326,7 +326,8 @@ int credit_softmax_logits_bwd_f32(const float* logits, const float* dy, float* d
  *                       and columns in falling order, equal ones by column,
  *                       NaN above everything (n_top 0: not wanted)
  * A column of -inf has probability 0.  A row of nothing else: S = 0, logp
- * -inf, entropy 0.  A row with NaN or +inf gives NaN.  n_tokens and n_top are
+ * -inf, entropy 0.  A row with NaN or +inf gives NaN.  Of all others S >= 1,
+ * logp <= 0 and entropy >= 0, whatever the rounding.  n_tokens and n_top are
  * at most 256 (n_top at most cols); n_tokens may be 0.  Columns behind cols
  * and what lies around them may hold anything.
  * Variants: READ, a workgroup a row; SPLIT, rows (at most 1024 of them; more
