@@ -1511,15 +1511,12 @@ bool alike(const void* in, int64_t ld, const void* out, int64_t ldd, int64_t row
   const uintptr_t d = reinterpret_cast<uintptr_t>(in) - reinterpret_cast<uintptr_t>(out);
   return d % 16 == 0 && (rows == 1 || (ld - ldd) * static_cast<int64_t>(elem) % 16 == 0);
 }
-// In place, or apart: a workgroup's part of one may not be another's of the other.
 int check_overlap(const void* in, int64_t ld, const void* out, int64_t ldd, int64_t rows,
                   int64_t cols, size_t elem) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(in), b = reinterpret_cast<uintptr_t>(out);
-  if (a == b && (rows == 1 || ld == ldd)) return CREDIT_OK;
-  const uintptr_t na = ((rows - 1) * ld + cols) * elem, nb = ((rows - 1) * ldd + cols) * elem;
-  if (a < b + nb && b < a + na)
-    return set_error(CREDIT_ERR_BAD_CONFIG, "dlogits overlaps logits without being it");
-  return CREDIT_OK;
+  if (logits::may_share(reinterpret_cast<uintptr_t>(in), ld, reinterpret_cast<uintptr_t>(out), ldd,
+                        rows, cols, elem))
+    return CREDIT_OK;
+  return set_error(CREDIT_ERR_BAD_CONFIG, "dlogits overlaps logits without being it");
 }
 template <class T>
 dim3 grad_grid(const T* logits, int64_t ld, int64_t rows, int64_t cols) {

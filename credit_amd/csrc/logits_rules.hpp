@@ -1,6 +1,7 @@
 // How the forwards of the operators on logits (logits.hip) cut rows into parts,
-// and the workspace that takes.  Host arithmetic alone, so that the CPU tests
-// build it with g++ (tests/cpp/logits_rules_query.cpp).
+// the workspace that takes, and where a gradient may lie beside its logits.  Host
+// arithmetic alone, so that the CPU tests build it with g++
+// (tests/cpp/logits_rules_query.cpp, logits_overlap_query.cpp).
 #pragma once
 
 #include <stddef.h>
@@ -62,6 +63,21 @@ inline size_t workspace(int64_t rows, int64_t cols, int variant_read, int64_t sp
         most = std::max(most, parts_bytes(rows, n, each, top));
     }
   return most;
+}
+
+// Whether a gradient of `rows` rows at b, ldb elements apart, may be written while
+// logits at a, lda apart, are read: in place (a lane writes what it has read), or
+// where no element is in both: memory apart, or rows of one distance that lie
+// between each other's.  Rows of two distances whose spans meet are not looked at.
+inline bool may_share(uintptr_t a, int64_t lda, uintptr_t b, int64_t ldb, int64_t rows,
+                      int64_t cols, size_t elem) {
+  if (a == b && (rows == 1 || lda == ldb)) return true;
+  const uintptr_t width = cols * elem;
+  const uintptr_t na = (rows - 1) * lda * elem + width, nb = (rows - 1) * ldb * elem + width;
+  if (a >= b + nb || b >= a + na) return true;
+  if (rows == 1 || lda != ldb) return false;
+  const uintptr_t step = lda * elem, after = (a < b ? b - a : a - b) % step;
+  return after >= width && step - after >= width;
 }
 
 }  // namespace logits

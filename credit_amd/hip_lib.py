@@ -696,8 +696,9 @@ def token_logprob_bwd(logits: torch.Tensor, tokens: torch.Tensor, stats: torch.T
                       temperature: float = 1.0, cfg: CreditCfg | None = None) -> None:
     """Gradient for the logits of sum(dlogp * logp) + sum(dentropy * entropy),
     from token_logprob_fwd's stats (and entropy).  dlogits, of the logits' type
-    and shape, may be the logits themselves.  Rows without a weight other than
-    0 are written 0 whatever their logits hold."""
+    and shape, may be the logits themselves or another column range of their
+    buffer.  Rows without a weight other than 0 are written 0 whatever their
+    logits hold."""
     rows, cols, ld, dev, fn = _logits_call("credit_token_logprob_bwd_", logits)
     f32 = torch.float32
     if tokens.dim() != 2:
@@ -748,7 +749,8 @@ def topk_distill_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: t
                      cfg: CreditCfg | None = None) -> None:
     """Gradient for the logits of sum(dloss * loss) of topk_distill_fwd (same
     tail and temperature), from its stats.  dlogits, of the logits' type and
-    shape, may be the logits themselves."""
+    shape, may be the logits themselves or another column range of their
+    buffer."""
     rows, cols, ld, dev, fn = _logits_call("credit_topk_distill_bwd_", logits)
     f32 = torch.float32
     if teacher_ids.dim() != 2:

@@ -354,8 +354,9 @@ int credit_token_logprob_fwd_bf16(const uint16_t* logits, int64_t ld, const int6
  *                - p_j (G + dentropy (ln p_j + H))) / T,  G = sum dlogp_t,
  * over the tokens that are not padding, from the forward's stats and entropy
  * (both entropy and dentropy NULL: none).  dlogits [rows, cols] in the logits'
- * type, row r at dlogits + r ldd; it may be the logits themselves (same ld),
- * otherwise the two may not overlap.  A weight of 0 counts as padding: rows
+ * type, row r at dlogits + r ldd; it may be the logits themselves (same ld) or
+ * rows between theirs (same ld, no element in both: two column ranges of one
+ * buffer), otherwise the two may not overlap.  A weight of 0 counts as padding: rows
  * without any other are written 0 and their logits not read, whatever they
  * hold; so are rows of -inf alone.  A token >= cols of weight other than 0
  * makes its row NaN.  Columns behind cols are left as they are.  Variants:
