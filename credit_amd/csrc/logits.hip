@@ -861,9 +861,9 @@ __device__ __forceinline__ void fetch_units(const Parts& p, int64_t row, int bat
   __syncthreads();
 }
 
-// One read of the logits.  512 x 262144 fp32 with the entropy 77.6 us, 6.92 TB/s
+// One read of the logits.  512 x 262144 fp32 with the entropy 77.8 us, 6.90 TB/s
 // (a kernel that reads alone reaches 7.08); 2048 x 131072 bf16 83 us without
-// alternatives (6.5 TB/s) and 93 with 64 (5.78): the workgroups that a CU holds
+// alternatives (6.5 TB/s) and 93 with 64 (5.80): the workgroups that a CU holds
 // reach their rows' ends together, where a row's choice of alternatives, some
 // 9000 cycles of latency, has no loads to hide it.  64 x 131072 in four parts
 // each, K = 20: 13.4 us, of which the stream 4, the parts' meeting and the units
@@ -1110,7 +1110,8 @@ struct DistillArgs {
   float temperature, c;
   Parts parts;
 };
-// Row statistics [rows, 8] for the backward.
+// Row statistics [rows, 8] for the backward, which takes the teacher's softmax
+// about its maximum and leaves the log-sum to the caller.
 enum DistillStat { kMax, kSum, kTailMax, kTailSum, kMass, kTailGrad, kTeacherLse, kUnused };
 
 // Marks element e of the frame if it lies in batches [b0, b1); whether it was
@@ -1126,7 +1127,7 @@ __device__ __forceinline__ bool mark(uint32_t* bits, int e, int b0, int b1) {
 
 // The tail is summed directly, over the columns that no entry names (1 - sum p of
 // the named ones would lose it where it is small): their bits are marked in LDS
-// for 16 batches at a time.  2048 x 131072 bf16, K = 64, tail 87.8 us, 6.14 TB/s;
+// for 16 batches at a time.  2048 x 131072 bf16, K = 64, tail 87.6 us, 6.15 TB/s;
 // without it the same; 8192 x 32768 108 us against 85: 64 named columns in four
 // batches leave hardly a wave's batch without one to mask.
 // Rows whose entries repeat a column, found by their marks, sum its entries
@@ -1319,7 +1320,7 @@ struct DistillGradArgs {
 };
 
 // One read, one write, as token_logprob_bwd_kernel: 2048 x 131072 bf16, K = 64
-// 170.6 us, 6.30 TB/s; 512 x 262144 fp32, K = 128, tail 173.0.
+// 171.9 us, 6.25 TB/s; 512 x 262144 fp32, K = 128, tail 172.0.
 template <class T, bool TAIL, bool VEC>
 __global__ __launch_bounds__(kThreads) void topk_distill_bwd_kernel(DistillGradArgs<T> a) {
   // The entries whose columns lie in this part, in their order; a bit for each of a

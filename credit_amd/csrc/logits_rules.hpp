@@ -22,13 +22,19 @@ constexpr int64_t kMaxSplitRows = 1024;
 // every CU a workgroup, where that saves a part four batches or more: a batch is
 // 0.5 us of a lone workgroup's time, the meeting of the parts 1.5 us.  us a call,
 // one workgroup a row -> parts:
-//   distillation with tail   1 x 131072 bf16 14.6 -> 7.5, 64 x 131072 15.9 -> 10.2,
-//                            128 x 131072 16.3 -> 13.1, 16 x 262144 fp32 28.6 -> 9.6
-//   but 64 x 32768 fp32 (4 batches) 7.5 -> 7.4 (log-probabilities alone 7.4 -> 7.7);
-//   256 x 131072, two parts: 17.3 -> 18.3
+//   distillation with tail   1 x 131072 bf16 14.8 -> 7.4, 64 x 131072 16.0 -> 10.5,
+//                            128 x 131072 16.3 -> 13.4, 16 x 262144 fp32 28.5 -> 9.8
+//   but 64 x 32768 fp32 (4 batches) 9.0 -> 8.4 (log-probabilities alone 7.3 -> 7.5);
+//   256 x 131072, two parts: 17.4 -> 18.5
 // With alternatives the last part reads every lane's maxima back, which takes
-// more (K = 20): 1 x 131072 15.2 -> 9.9, 64 x 131072 17.0 -> 14.0, 96 x 131072
-// 17.2 -> 17.0, 128 x 131072 17.3 -> 17.6, 1 x 32768 fp32 9.1 -> 9.4.
+// more (K = 20): 1 x 131072 15.2 -> 9.8, 64 x 131072 17.2 -> 14.3, 96 x 131072, two
+// parts 17.2 -> 17.5, 128 x 131072 17.4 -> 18.1, 1 x 32768 fp32 9.2 -> 9.3.
+// Not the best choice above its limits in bf16 rows of more than 16 batches, which
+// keep whole rows: K = 20, 65 x 262144 27.8 -> 21.9 in four parts, 96 rows 27.9 ->
+// 23.7, 128 rows 28.3 -> 26.2 (fp32 29.8 -> 27.8, 31.1 -> 30.9, 32.0 -> 35.8; 65 x
+// 131072 bf16 17.2 -> 14.9, 200 x 262144 29.6 -> 37.0), and without alternatives
+// 130 x 262144 23.1 -> 15.6 in three parts, 200 x 262144 24.7 -> 20.7 in two (fp32
+// 27.0 -> 24.8, 31.9 -> 34.8).
 inline int64_t auto_parts(int64_t rows, int64_t batches, bool alternatives) {
   if (alternatives && rows > 64) return 1;
   const int64_t a_cu_each = std::max<int64_t>(1, 256 / std::max<int64_t>(1, rows));

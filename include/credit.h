@@ -390,8 +390,8 @@ int credit_token_logprob_bwd_bf16(const uint16_t* logits, int64_t ld, const int6
  * outside the entries has mass (all of them -inf, or every column named) the
  * rest counts as 0, in the loss and in its gradient.  stats [rows, 8] is what
  * the backward takes: m and S as above, the same two of the columns outside the
- * entries (tail), Q = sum q + rest, the tail's gradient, the teacher's log-sum,
- * 0.  Variants and workspace as credit_token_logprob_fwd_*'s. */
+ * entries (tail), Q = sum q + rest, the tail's gradient; then ln sum e^(teacher/T)
+ * (tail == 0), which it does not read, and 0.  Variants and workspace as credit_token_logprob_fwd_*'s. */
 int credit_topk_distill_fwd_f32(const float* logits, int64_t ld, const int64_t* teacher_ids,
                                 const float* teacher, float* loss, float* stats, int64_t rows,
                                 int64_t cols, int32_t n_top, int32_t tail, float temperature,
