@@ -1,0 +1,488 @@
+"""Performance cases of the operators around attention.
+
+``rope`` rotates queries and keys by their positions, ``qk_norm_rope_fwd`` takes
+the RMS norm of each head in the same pass and ``qk_norm_rope_bwd`` its gradients;
+``paged_append`` puts new keys and values into a paged cache, normed and rotated on
+the way, and ``paged_attention`` attends from a batch's new tokens to that cache.
+All of ``credit_amd.hip_lib``.
+
+The listed cases span the range in use: the decode step of one sequence and of a
+batch, chunks of prompts, training rows; odd head counts, head sizes and pages,
+both types and each direction.  ``draw`` gives more of the same ranges.
+
+``run`` makes the package's calls where ``own`` is true and computes the same in
+elementary torch operations where it is not; ``exact`` computes it in 64 bits.
+"""
+from __future__ import annotations
+
+import math
+import random
+
+import torch
+
+own = False
+
+F32, F64, I32, I64 = torch.float32, torch.float64, torch.int32, torch.int64
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+SIZE = {"f32": 4, "bf16": 2}
+EPS = 1e-6
+
+# Bounds of a drawn case, which the largest listed ones reach: bytes of the
+# queries, keys and values, and visible pairs of query and key over all heads.
+MOST_BYTES = 200 << 20
+MOST_PAIRS = 32 * 8192 * 8193 // 2
+
+
+def _heads(name, op, dtype, tokens, q_heads, kv_heads, dim, rot=None, layout="half", far=0,
+           packed=True, norm=True):
+    """packed: queries, keys and values are column ranges of one projection's
+    output.  far: positions start there, with frequencies scaled for it."""
+    return {"name": name, "op": op, "dtype": dtype, "tokens": tokens, "q_heads": q_heads,
+            "kv_heads": kv_heads, "dim": dim, "rot": dim if rot is None else rot,
+            "layout": layout, "far": far, "packed": packed, "norm": norm}
+
+
+def _append(name, tokens, q_heads, kv_heads, dim, page, pages, padded=False, far=0, norm=True):
+    case = _heads(name, "append", "bf16", tokens, q_heads, kv_heads, dim, far=far, norm=norm)
+    return {**case, "page": page, "pages": pages, "padded": padded}
+
+
+def _attention(name, batch, new, kv, q_heads, kv_heads, dim, page, ragged=False, window=0):
+    """new: most new tokens of a sequence; kv: its most positions, the new ones
+    among them; ragged: sequences of different lengths."""
+    return {"name": name, "op": "attention", "dtype": "bf16", "batch": batch, "new": new, "kv": kv,
+            "q_heads": q_heads, "kv_heads": kv_heads, "dim": dim, "page": page, "ragged": ragged,
+            "window": window}
+
+
+def listed() -> list[dict]:
+    return [
+        # One sequence's decode step: its token's queries and keys.
+        _heads("rope_one", "rope", "bf16", 1, 32, 8, 128),
+        # A prompt with interleaved pairs in half of each head, positions far out.
+        _heads("rope_far", "rope", "f32", 2048, 32, 8, 128, rot=64, layout="interleaved",
+               far=400000, packed=False),
+        # A batch's decode step with norms.
+        _heads("norm_rope_batch", "norm_rope_fwd", "bf16", 64, 32, 8, 128),
+        # The forward and the gradients of a training step's rows.
+        _heads("norm_rope_train", "norm_rope_fwd", "bf16", 16384, 32, 8, 128),
+        _heads("norm_rope_grad", "norm_rope_bwd", "bf16", 16384, 32, 8, 128),
+        # The gradients of an odd model in full precision.
+        _heads("norm_rope_grad_odd", "norm_rope_bwd", "f32", 1000, 14, 2, 80, rot=40, packed=False),
+        # A batch's decode step into its cache, some of its rows not in use.
+        _append("append_batch", 64, 32, 8, 128, 16, 2048, padded=True),
+        # A prompt's chunk into the cache.
+        _append("append_prompt", 8192, 32, 8, 128, 64, 256, far=131072),
+        # One sequence's decode step over what it has seen.
+        _attention("attend_one", 1, 1, 8192, 32, 8, 128, 16),
+        # A batch's decode step, sequences of different lengths.
+        _attention("attend_batch", 64, 1, 16384, 32, 8, 128, 64, ragged=True),
+        # Chunks of several prompts behind what is cached, pages of an odd size, a window.
+        _attention("attend_chunks", 6, 500, 6000, 14, 2, 80, 24, ragged=True, window=4096),
+        # A long prompt at once.
+        _attention("attend_prompt", 1, 8192, 8192, 32, 8, 128, 64),
+    ]
+
+
+def _log_int(rng, low: int, high: int) -> int:
+    return min(high, max(low, round(math.exp(rng.uniform(math.log(low), math.log(high))))))
+
+
+def _draw_heads(rng):
+    """(query heads, key and value heads, head size)."""
+    kv_heads = rng.choice((1, 2, 4, 8))
+    return kv_heads * rng.choice((1, 4, 7, 8)), kv_heads, rng.choice((64, 80, 96, 128, 128, 256))
+
+
+def draw(rng) -> dict:
+    op = rng.choice(("rope", "norm_rope_fwd", "norm_rope_bwd", "append", "attention", "attention"))
+    q_heads, kv_heads, dim = _draw_heads(rng)
+    if op == "attention":
+        batch = _log_int(rng, 1, 64)
+        kv = _log_int(rng, 16, 16384)
+        most = min(kv, MOST_PAIRS * 128 // (batch * q_heads * kv * dim))
+        new = 1 if rng.random() < 0.4 else _log_int(rng, 1, max(1, min(most, 4096)))
+        # The caches stay within a quarter of the listed batch's.
+        while batch * kv * kv_heads * dim > (1 << 29):
+            batch = (batch + 1) // 2
+            kv = max(new, kv // 2)
+        case = _attention("", batch, new, kv, q_heads, kv_heads, dim,
+                          rng.choice((16, 32, 64, 128, 24)), rng.random() < 0.6,
+                          rng.choice((0, 0, 0, 128, 1000)))
+        del case["name"]
+        return case
+    dtype = "bf16" if op == "append" else rng.choice(("f32", "bf16"))
+    row = (q_heads + 2 * kv_heads) * dim * SIZE[dtype]
+    tokens = _log_int(rng, 1, min(16384, MOST_BYTES // row))
+    far = rng.choice((0, 0, 100000, 500000))
+    rot, layout = rng.choice((dim, dim, dim // 2)), rng.choice(("half", "half", "interleaved"))
+    if op == "append":
+        page = rng.choice((16, 32, 64, 24))
+        case = _append("", tokens, q_heads, kv_heads, dim, page, tokens // page + 1
+                       + _log_int(rng, 1, 256), rng.random() < 0.3, far, rng.random() < 0.5)
+        case.update(rot=rot, layout=layout)
+    else:
+        case = _heads("", op, dtype, tokens, q_heads, kv_heads, dim, rot, layout, far,
+                      rng.random() < 0.5, op != "rope")
+    del case["name"]
+    return case
+
+
+def _lengths(case):
+    """New tokens and positions of each sequence: of the case alone."""
+    batch, new, kv = case["batch"], case["new"], case["kv"]
+    if not case["ragged"]:
+        return [new] * batch, [kv] * batch
+    rng = random.Random(f"{batch} {new} {kv} {case['page']}")
+    news = [new] + [rng.randint(1, new) for _ in range(batch - 1)]
+    kvs = [rng.randint(max(n, kv // 8), kv) for n in news[:-1]] + [kv]
+    return news, kvs
+
+
+# ------------------------------------------------------------------ inputs --
+
+
+def _frequencies(case):
+    """Radians a position for each pair; of far positions, long waves are
+    stretched by 8 and short ones kept, and the rotation's magnitude grows."""
+    rot = case["rot"]
+    f = torch.arange(0, rot, 2, dtype=F64).mul_(-math.log(500000.0) / rot).exp_()
+    if not case["far"]:
+        return f.to(F32).cuda(), 1.0
+    keep = ((f * 8192 / (2 * math.pi) - 1.0) / 31.0).clamp(0.0, 1.0)
+    return (f * keep + f / 8.0 * (1.0 - keep)).to(F32).cuda(), 0.1 * math.log(8.0) + 1.0
+
+
+def _projection(g, case, tensors):
+    """Queries, keys (and values) [tokens, heads, dim], heads of unlike scale."""
+    tokens, dim, dtype = case["tokens"], case["dim"], DTYPES[case["dtype"]]
+    heads = [case["q_heads"], case["kv_heads"], case["kv_heads"]][:tensors]
+    scale = torch.rand((sum(heads), 1), generator=g, device="cuda").mul_(2.0).add_(0.5)
+    x = torch.randn((tokens, sum(heads), dim), generator=g, device="cuda").mul_(scale).to(dtype)
+    parts = x.split(heads, 1)
+    return parts if case["packed"] else tuple(p.contiguous() for p in parts)
+
+
+def prepare(case: dict, seed: int) -> dict:
+    g = torch.Generator(device="cuda").manual_seed(int(seed))
+    if case["op"] == "attention":
+        return _prepare_attention(g, case)
+    tokens, dim, dtype = case["tokens"], case["dim"], DTYPES[case["dtype"]]
+    s = {"case": case}
+    s["freq"], s["magnitude"] = _frequencies(case)
+    start = torch.randint(0, 1000, (1,), generator=g, device="cuda") + case["far"]
+    s["positions"] = torch.arange(tokens, device="cuda") + start
+    if case["op"] == "append":
+        s["q"], s["k"], s["v"] = _projection(g, case, 3)
+    else:
+        s["q"], s["k"] = _projection(g, case, 3)[:2]
+        s["k_out"] = torch.empty(s["k"].shape, device="cuda", dtype=dtype)
+    s["q_out"] = torch.empty(s["q"].shape, device="cuda", dtype=dtype)
+    if case["norm"]:
+        s["wq"], s["wk"] = ((torch.randn(dim, generator=g, device="cuda") * 0.2 + 1.0).to(dtype)
+                            for _ in range(2))
+    if case["op"].startswith("norm_rope"):
+        s["rstd"] = torch.empty((tokens, case["q_heads"] + case["kv_heads"]), device="cuda")
+    if case["op"] == "norm_rope_bwd":
+        s["rstd"] = torch.cat((_rstd(s["q"].float()), _rstd(s["k"].float())), 1)[..., 0].contiguous()
+        s["gq"], s["gk"] = (torch.randn(s[n].shape, generator=g, device="cuda").to(dtype)
+                            for n in "qk")
+        s["dwq"], s["dwk"] = (torch.empty(dim, device="cuda") for _ in range(2))
+    if case["op"] == "append":
+        shape = (case["pages"], case["page"], case["kv_heads"], dim)
+        s["k_cache"], s["v_cache"] = (torch.randn(shape, generator=g, device="cuda").to(dtype)
+                                      for _ in range(2))
+        slots = torch.randperm(case["pages"] * case["page"], generator=g, device="cuda")[:tokens]
+        if case["padded"]:
+            slots[tokens - tokens // 8:] = -1
+        s["slots"] = slots
+    return s
+
+
+def _prepare_attention(g, case):
+    news, kvs = _lengths(case)
+    page, dim, kv_heads = case["page"], case["dim"], case["kv_heads"]
+    need = [-(-n // page) for n in kvs]
+    pages = sum(need) + 3
+    s = {"case": case, "news": news, "kvs": kvs}
+    order = torch.randperm(pages, generator=g, device="cuda").to(I32)
+    s["pages"] = torch.full((len(kvs), max(need)), -1, device="cuda", dtype=I32)
+    at = 0
+    for b, n in enumerate(need):
+        s["pages"][b, :n] = order[at:at + n]
+        at += n
+    starts = [0]
+    for n in news:
+        starts.append(starts[-1] + n)
+    s["q_start"] = torch.tensor(starts, device="cuda", dtype=I32)
+    s["kv_len"] = torch.tensor(kvs, device="cuda", dtype=I32)
+    shape = (starts[-1], case["q_heads"], dim)
+    bf16 = torch.bfloat16
+    s["q"] = torch.randn(shape, generator=g, device="cuda").mul_(1.5).to(bf16)
+    # A key in 64 stands out, as those that many tokens attend to do.
+    k = torch.randn((pages, page, kv_heads, dim), generator=g, device="cuda").to(bf16)
+    loud = torch.rand((pages, page, 1, 1), generator=g, device="cuda") < 1.0 / 64.0
+    s["k_cache"] = torch.where(loud, k * 2, k)
+    del k, loud
+    s["v_cache"] = torch.randn((pages, page, kv_heads, dim), generator=g, device="cuda").to(bf16)
+    s["out"] = torch.empty(shape, device="cuda", dtype=bf16)
+    s["lse"] = torch.empty(shape[:2], device="cuda")
+    return s
+
+
+# -------------------------------------------------------------- plain form --
+
+
+def _rstd(x):
+    return ((x * x).sum(-1, keepdim=True) / x.shape[-1] + EPS).rsqrt()
+
+
+def _angles(s, dtype):
+    """cos and sin [tokens, 1, rot / 2] of the angles, taken in 64 bits."""
+    a = s["positions"].double()[:, None, None] * s["freq"].double()
+    return ((a.cos() * s["magnitude"]).to(dtype), (a.sin() * s["magnitude"]).to(dtype))
+
+
+def _rotate(x, cos, sin, layout):
+    """x [tokens, heads, dim]: pairs of its first elements turned by the angles."""
+    rot = 2 * cos.shape[-1]
+    y, rest = x[..., :rot], x[..., rot:]
+    if layout == "half":
+        a, b = y[..., :rot // 2], y[..., rot // 2:]
+        return torch.cat((a * cos - b * sin, b * cos + a * sin, rest), -1)
+    a, b = y[..., 0::2], y[..., 1::2]
+    turned = torch.stack((a * cos - b * sin, b * cos + a * sin), -1).flatten(-2)
+    return torch.cat((turned, rest), -1)
+
+
+def _plain_side(s, x, weight, cos, sin):
+    """One tensor normed (where it has a weight) and rotated, and its rstd."""
+    y, r = x.float(), None
+    if weight is not None:
+        r = _rstd(y)
+        y = y * r * weight.float()
+    return _rotate(y, cos, sin, s["case"]["layout"]).to(x.dtype), r
+
+
+def _plain_grad(s, x, weight, rstd, dy, cos, sin):
+    """dx and the weight's gradient: dy turned back, then through the norm."""
+    x, w = x.float(), weight.float()
+    d = _rotate(dy.float(), cos, -sin, s["case"]["layout"])
+    n = x * rstd[..., None]
+    u = d * w
+    dx = rstd[..., None] * (u - n * ((u * n).sum(-1, keepdim=True) / x.shape[-1]))
+    return dx, (d * n).sum((0, 1))
+
+
+def _row_step(kv, heads):
+    """Query rows whose scores are held at once: at most 2 GiB of them."""
+    return max(1, (1 << 29) // (kv * heads))
+
+
+def _sequence(s, b, dtype):
+    """Keys and values [kv_heads, positions, dim] of sequence b."""
+    n, page = s["kvs"][b], s["case"]["page"]
+    at = s["pages"][b, :-(-n // page)].long()
+    return (s[c][at].flatten(0, 1)[:n].transpose(0, 1).to(dtype).contiguous()
+            for c in ("k_cache", "v_cache"))
+
+
+def _hidden(case, new, kv, first, rows):
+    """[rows, kv]: which positions the sequence's rows from `first` on cannot
+    see, the row of its last token seeing all (or the last `window`)."""
+    at = torch.arange(kv, device="cuda")
+    last = torch.arange(first, first + rows, device="cuda")[:, None] + (kv - new)
+    hidden = at > last
+    return hidden | (at <= last - case["window"]) if case["window"] else hidden
+
+
+def _plain_attention(s):
+    case = s["case"]
+    group = case["q_heads"] // case["kv_heads"]
+    scale = 1.0 / math.sqrt(case["dim"])
+    out, lse, first = [], [], 0
+    for b, (new, kv) in enumerate(zip(s["news"], s["kvs"])):
+        k, v = _sequence(s, b, F32)
+        kt = k.transpose(1, 2).contiguous()
+        step = _row_step(kv, case["q_heads"])
+        for i in range(0, new, step):
+            n = min(step, new - i)
+            q = s["q"][first + i:first + i + n].float()
+            # [kv_heads, n * group, dim]
+            q = q.view(n, case["kv_heads"], group, -1).transpose(0, 1).reshape(
+                case["kv_heads"], n * group, -1)
+            x = torch.matmul(q, kt).mul_(scale).view(case["kv_heads"], n, group, kv)
+            x.masked_fill_(_hidden(case, new, kv, i, n)[None, :, None], -math.inf)
+            m = x.amax(-1, keepdim=True)
+            p = x.sub_(m).exp_()
+            total = p.sum(-1, keepdim=True)
+            o = torch.matmul(p.view(case["kv_heads"], n * group, kv), v).view(
+                case["kv_heads"], n, group, -1) / total
+            out.append(o.transpose(0, 1).reshape(n, case["q_heads"], -1).to(s["q"].dtype))
+            lse.append((m + total.log()).transpose(0, 1).reshape(n, case["q_heads"]))
+            del x, p, o
+        first += new
+    return torch.cat(out), torch.cat(lse)
+
+
+def run(s: dict):
+    case = s["case"]
+    op = case["op"]
+    if own:
+        return _own(s)
+    if op == "attention":
+        return _plain_attention(s)
+    cos, sin = _angles(s, F32)
+    if op == "norm_rope_bwd":
+        heads = case["q_heads"]
+        dq, dwq = _plain_grad(s, s["q"], s["wq"], s["rstd"][:, :heads], s["gq"], cos, sin)
+        dk, dwk = _plain_grad(s, s["k"], s["wk"], s["rstd"][:, heads:], s["gk"], cos, sin)
+        return dq.to(s["q"].dtype), dk.to(s["k"].dtype), dwq, dwk
+    q, rq = _plain_side(s, s["q"], s.get("wq"), cos, sin)
+    k, rk = _plain_side(s, s["k"], s.get("wk"), cos, sin)
+    if op == "append":
+        live = s["slots"] >= 0
+        for cache, new in ((s["k_cache"], k), (s["v_cache"], s["v"])):
+            cache.flatten(0, 1)[s["slots"][live]] = new[live]
+        return q, s["k_cache"], s["v_cache"]
+    if op == "norm_rope_fwd":
+        return q, k, torch.cat((rq, rk), 1)[..., 0]
+    return q, k
+
+
+def _own(s):
+    from credit_amd import hip_lib
+
+    case = s["case"]
+    op = case["op"]
+    if op == "attention":
+        hip_lib.paged_attention(s["q"], s["k_cache"], s["v_cache"], s["pages"], s["q_start"],
+                                s["kv_len"], s["out"], s["lse"], window=case["window"])
+        return s["out"], s["lse"]
+    turn = {"layout": case["layout"], "magnitude": s["magnitude"]}
+    if op == "append":
+        hip_lib.paged_append(s["k"], s["v"], s["slots"], s["k_cache"], s["v_cache"],
+                             s["positions"], s["freq"], k_weight=s.get("wk"), q=s["q"],
+                             q_out=s["q_out"], q_weight=s.get("wq"), eps=EPS, **turn)
+        return s["q_out"], s["k_cache"], s["v_cache"]
+    if op == "rope":
+        hip_lib.rope(s["q"], s["positions"], s["freq"], s["q_out"], s["k"], s["k_out"], **turn)
+        return s["q_out"], s["k_out"]
+    if op == "norm_rope_fwd":
+        hip_lib.qk_norm_rope_fwd(s["q"], s["k"], s["wq"], s["wk"], s["positions"], s["freq"],
+                                 s["q_out"], s["k_out"], s["rstd"], eps=EPS, **turn)
+        return s["q_out"], s["k_out"], s["rstd"]
+    hip_lib.qk_norm_rope_bwd(s["q"], s["k"], s["wq"], s["wk"], s["positions"], s["freq"],
+                             s["rstd"], s["gq"], s["gk"], s["q_out"], s["k_out"], s["dwq"],
+                             s["dwk"], **turn)
+    return s["q_out"], s["k_out"], s["dwq"], s["dwk"]
+
+
+def _visible(case):
+    """Pairs of a new token and a position that it sees, of one head, and the
+    positions that any token of a sequence sees."""
+    pairs = seen = 0
+    for new, kv in zip(*_lengths(case)):
+        for i in range(new):
+            n = kv - new + i + 1
+            pairs += min(n, case["window"]) if case["window"] else n
+        seen += min(kv, new + case["window"] - 1) if case["window"] else kv
+    return pairs, seen
+
+
+def work(case: dict) -> dict:
+    size, dim = SIZE[case["dtype"]], case["dim"]
+    if case["op"] == "attention":
+        pairs, seen = _visible(case)
+        new = sum(_lengths(case)[0])
+        return {"bytes": 2 * seen * case["kv_heads"] * dim * size
+                + new * case["q_heads"] * (2 * dim * size + 4),
+                "flops": 4 * pairs * case["q_heads"] * dim}
+    heads, tokens = case["q_heads"] + case["kv_heads"], case["tokens"]
+    row, per = heads * dim * size, 3 * heads * case["rot"]
+    if case["op"] == "rope":
+        return {"bytes": tokens * (2 * row + 8), "flops": tokens * per}
+    if case["op"] == "norm_rope_fwd":
+        return {"bytes": tokens * (2 * row + 4 * heads + 8), "flops": tokens * (per + 4 * heads * dim)}
+    if case["op"] == "norm_rope_bwd":
+        return {"bytes": tokens * (3 * row + 4 * heads + 8), "flops": tokens * (per + 8 * heads * dim)}
+    live = tokens - (tokens // 8 if case["padded"] else 0)
+    kv = case["kv_heads"] * dim * size
+    return {"bytes": tokens * (2 * case["q_heads"] * dim * size + 16) + live * 4 * kv,
+            "flops": tokens * (per + 4 * heads * dim * case["norm"])}
+
+
+# ------------------------------------------------------------------- exact --
+
+
+def _exact_turn(s, x, back=False):
+    """The rotation as a product of complex numbers."""
+    case = s["case"]
+    rot, x = case["rot"], x.double()
+    a = s["positions"].double()[:, None] * s["freq"].double()
+    z = torch.polar(torch.full_like(a, s["magnitude"]), -a if back else a)[:, None]
+    if case["layout"] == "half":
+        pairs = torch.complex(x[..., :rot // 2], x[..., rot // 2:rot]) * z
+        return torch.cat((pairs.real, pairs.imag, x[..., rot:]), -1)
+    pairs = torch.view_as_complex(x[..., :rot].unflatten(-1, (-1, 2)).contiguous()) * z
+    return torch.cat((torch.view_as_real(pairs).flatten(-2), x[..., rot:]), -1)
+
+
+def _exact_norm(x):
+    return x.double() / (x.double().pow(2).mean(-1, keepdim=True) + EPS).sqrt()
+
+
+def _exact_attention(s):
+    case = s["case"]
+    group = case["q_heads"] // case["kv_heads"]
+    out = torch.empty(s["q"].shape, device="cuda", dtype=F64)
+    lse = torch.empty(s["q"].shape[:2], device="cuda", dtype=F64)
+    first = 0
+    for b, (new, kv) in enumerate(zip(s["news"], s["kvs"])):
+        k, v = _sequence(s, b, F64)
+        step = _row_step(kv, 4 * group)
+        for i in range(0, new, step):
+            n = min(step, new - i)
+            hidden = _hidden(case, new, kv, i, n)[:, None]
+            for h in range(case["kv_heads"]):
+                rows = slice(first + i, first + i + n), slice(h * group, (h + 1) * group)
+                x = s["q"][rows].double().reshape(n * group, -1) @ k[h].T.contiguous()
+                x = (x / math.sqrt(case["dim"])).view(n, group, kv).masked_fill(hidden, -math.inf)
+                lse[rows] = x.logsumexp(-1)
+                out[rows] = (torch.softmax(x, -1).view(n * group, kv) @ v[h]).view(n, group, -1)
+                del x
+        first += new
+    return out, lse
+
+
+def exact(case: dict, seed: int):
+    s = prepare(case, seed)
+    op = case["op"]
+    if op == "attention":
+        return _exact_attention(s)
+    if op == "norm_rope_bwd":
+        grads, weights = [], []
+        heads = case["q_heads"]
+        for x, w, r, dy in ((s["q"], s["wq"], s["rstd"][:, :heads], s["gq"]),
+                            (s["k"], s["wk"], s["rstd"][:, heads:], s["gk"])):
+            # The gradient at the norms that the forward left.
+            d = _exact_turn(s, dy, back=True)
+            n = x.double() * r.double()[..., None]
+            weights.append((d * n).sum((0, 1)))
+            d *= w.double()
+            grads.append((d - n * (d * n).mean(-1, keepdim=True)) * r.double()[..., None])
+        return (*grads, *weights)
+    q, k = s["q"], s["k"]
+    if case["norm"]:
+        q, k = _exact_norm(q) * s["wq"].double(), _exact_norm(k) * s["wk"].double()
+    q, k = _exact_turn(s, q), _exact_turn(s, k)
+    if op == "append":
+        caches = [s["k_cache"].double(), s["v_cache"].double()]
+        live = s["slots"] >= 0
+        for cache, new in zip(caches, (k, s["v"].double())):
+            cache.view(-1, *cache.shape[2:])[s["slots"][live]] = new[live]
+        return (q, *caches)
+    if op == "norm_rope_fwd":
+        ms = [x.double().pow(2).mean(-1) for x in (s["q"], s["k"])]
+        return q, k, (torch.cat(ms, 1) + EPS).rsqrt()
+    return q, k
