@@ -508,6 +508,9 @@ size_t credit_workspace_bytes(int32_t op, int64_t rows, int64_t cols,
                                variant == CREDIT_VARIANT_SPLIT ? split : 0,
                                op == CREDIT_OP_TOKEN_LOGPROB_FWD);
       break;
+    case CREDIT_OP_QK_NORM_ROPE_BWD:
+      body = qk_norm_rope_bwd_workspace(cols);
+      break;
     default:
       body = 0;
   }

@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include "../../include/credit.h"
+#include "heads_rules.hpp"
 #include "split_plan.hpp"
 
 namespace credit {
@@ -247,6 +248,7 @@ size_t rowwise_quant_workspace(int64_t rows, int64_t cols, int variant, int spli
 size_t lars_workspace(int64_t rows, int64_t cols, int variant, int split, int cu_count);
 size_t wvar_bwd_workspace(int64_t rows, int64_t cols, int variant, int split, int cu_count);
 size_t pearson_bwd_workspace(int64_t rows, int64_t cols, int variant, int split, int cu_count);
+size_t qk_norm_rope_bwd_workspace(int64_t dim);
 size_t rmsnorm_bwd_workspace(int64_t rows, int64_t cols, int variant, int split,
                              int cu_count);
 size_t rmsnorm_fused_workspace(int64_t rows, int64_t cols, int variant, int split,
@@ -267,6 +269,12 @@ int wide_layernorm_bwd(const T* x, const T* dy, const T* gamma, T* dx, int64_t r
 int wide_layernorm_fwd(const uint16_t* x, const uint16_t* gamma, const uint16_t* beta,
                        uint16_t* y, float* mean, float* rstd, int64_t rows, int64_t cols,
                        float eps, bool vec, const credit_cfg* cfg, bool* taken);
+
+// A paged cache's arguments, checked (heads.hip): the places of its pages and of
+// the slots of one, and two caches against each other.
+int check_cache(const credit_pages* cache, const char* name, int dim, size_t elem,
+                heads::Place* pages, heads::Place* slots);
+int check_caches_apart(const heads::Place& k, const heads::Place& v);
 
 // CU count of the current device, or 256 (MI355X) when none is visible.
 int cu_count_or_default();

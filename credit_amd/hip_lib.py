@@ -15,6 +15,7 @@ non-zero status raises.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import threading
 from dataclasses import dataclass
@@ -62,6 +63,7 @@ OPS = {
     "token_logprob_bwd": 17,
     "topk_distill_fwd": 18,
     "topk_distill_bwd": 19,
+    "qk_norm_rope_bwd": 20,
 }
 
 
@@ -105,11 +107,45 @@ class DeviceInfo(ctypes.Structure):
     ]
 
 
+class CreditHeads(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+    ]
+
+
+class CreditRotation(ctypes.Structure):
+    _fields_ = [
+        ("positions", ctypes.c_void_p),
+        ("inv_freq", ctypes.c_void_p),
+        ("rot", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("magnitude", ctypes.c_float),
+    ]
+
+
+class CreditPages(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("slot_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
 _F = ctypes.c_float
 _CFG = ctypes.POINTER(CreditCfg)
+_HEADS = ctypes.POINTER(CreditHeads)
+_ROTATION = ctypes.POINTER(CreditRotation)
+_PAGES = ctypes.POINTER(CreditPages)
 
 # name -> argument types (return type is int unless listed in _RESTYPES).
 SIGNATURES: dict[str, list] = {
@@ -137,6 +173,15 @@ SIGNATURES: dict[str, list] = {
                                         _CFG] for t in ("f32", "bf16")},
     **{f"credit_topk_distill_bwd_{t}": [_P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32,
                                         _I32, _F, _CFG] for t in ("f32", "bf16")},
+    **{f"credit_rope_{t}": [_HEADS, _HEADS, _ROTATION, _HEADS, _HEADS, _I64, _I32, _I32, _CFG]
+       for t in ("f32", "bf16")},
+    **{f"credit_qk_norm_rope_fwd_{t}": [_HEADS, _HEADS, _P, _P, _ROTATION, _HEADS, _HEADS, _P,
+                                        _I64, _I32, _F, _CFG] for t in ("f32", "bf16")},
+    **{f"credit_qk_norm_rope_bwd_{t}": [_HEADS, _HEADS, _P, _P, _ROTATION, _P, _HEADS, _HEADS,
+                                        _HEADS, _HEADS, _P, _P, _I64, _I32, _CFG]
+       for t in ("f32", "bf16")},
+    "credit_paged_append_bf16": [_HEADS, _HEADS, _HEADS, _P, _P, _ROTATION, _P, _PAGES, _PAGES,
+                                 _HEADS, _I64, _I32, _F, _CFG],
     "credit_rowwise_quant_f32": [_P, _P, _P, _I64, _I64, _CFG],
     "credit_lars_momentum_f32": [_P, _P, _P, _P, _P, _I64, _I64, _CFG],
     "credit_weighted_var_bwd_f32": [_P, _P, _P, _P, _I64, _I64, _F, _CFG],
@@ -633,7 +678,7 @@ def _logits_call(op: str, logits: torch.Tensor) -> tuple[int, int, int, int, Cal
 
 
 def _operand(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, ...],
-             device: int) -> int:
+             device: int, whose: str = "the logits'") -> int:
     """Address of a contiguous operand of exactly this type, shape and device."""
     if (t.dtype is dtype and t.shape == shape and t.is_contiguous()
             and t.get_device() == device):
@@ -644,7 +689,7 @@ def _operand(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, .
         raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: tensor must be contiguous")
-    raise ValueError(f"{name}: expected a tensor on the logits' device, got {t.device}")
+    raise ValueError(f"{name}: expected a tensor on {whose} device, got {t.device}")
 
 
 def _gradient(dlogits: torch.Tensor, logits: torch.Tensor, device: int) -> tuple[int, int]:
@@ -762,6 +807,229 @@ def topk_distill_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: t
         _operand(teacher, "teacher", f32, (rows, k), dev),
         _operand(stats, "stats", f32, (rows, 8), dev), _operand(dloss, "dloss", f32, (rows,), dev),
         out, ldd, rows, cols, k, bool(tail), temperature, _cfg_ref(cfg, dev))
+    if status:
+        check(status, fn.__name__)
+
+# ---------------------------------------------------- operators on heads --
+
+
+def _heads(t: torch.Tensor, name: str, dtype: torch.dtype, tokens: int, dim: int, device: int):
+    """A [tokens, heads, dim] tensor whose heads' elements are contiguous."""
+    if t.dim() != 3:
+        raise ValueError(f"{name}: expected [tokens, heads, dim], got shape {tuple(t.shape)}")
+    n, heads, d = t.shape
+    token, head, one = t.stride()
+    if t.dtype is not dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if n != tokens or d != dim:
+        raise ValueError(f"{name}: expected [{tokens}, heads, {dim}], got {tuple(t.shape)}")
+    if one != 1 and d > 1:
+        raise ValueError(f"{name}: the elements of a head must be contiguous")
+    if t.get_device() != device:
+        raise ValueError(f"{name}: expected a tensor on {_device_name(device)}, got {t.device}")
+    return ctypes.byref(CreditHeads(t.data_ptr(), token, head, heads))
+
+
+def _device_name(device: int) -> str:
+    return f"cuda:{device}"
+
+
+def _heads_call(op: str, q: torch.Tensor, name: str) -> tuple[int, int, int, Callable[..., int]]:
+    """(tokens, dim, device, entry point) of a call on these heads."""
+    suffix = _LOGITS_TYPES.get(q.dtype)
+    if suffix is None:
+        raise TypeError(f"{name}: expected torch.float32 or torch.bfloat16, got {q.dtype}")
+    if q.dim() != 3:
+        raise ValueError(f"{name}: expected [tokens, heads, dim], got shape {tuple(q.shape)}")
+    device = q.get_device()
+    if device < 0:
+        raise ValueError(f"{name}: tensor must be on a GPU, got {q.device}")
+    if device != torch.cuda.current_device():
+        raise ValueError(f"{name}: on {q.device}, which is not the current device")
+    return q.shape[0], q.shape[2], device, getattr(load_library(), op + suffix)
+
+
+_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+def _rotation(positions: torch.Tensor | None, inv_freq: torch.Tensor | None, layout: str,
+              magnitude: float, tokens: int, device: int):
+    interleaved = _LAYOUTS.get(layout)
+    if interleaved is None:
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    if (positions is None) != (inv_freq is None):
+        raise ValueError("positions and inv_freq come together")
+    if positions is None:
+        return None
+    pairs = inv_freq.shape[0] if inv_freq.dim() == 1 else -1
+    return ctypes.byref(CreditRotation(
+        _operand(positions, "positions", torch.int64, (tokens,), device, "the queries'"),
+        _operand(inv_freq, "inv_freq", torch.float32, (pairs,), device, "the queries'"),
+        2 * pairs, interleaved, magnitude))
+
+
+def rope_frequencies(rot: int, base: float = 10000.0, scaling: str | None = None,
+                     factor: float = 1.0, original_length: int = 8192, low: float = 1.0,
+                     high: float = 32.0) -> tuple[torch.Tensor, float]:
+    """inv_freq [rot / 2] (fp32, on the CPU) and magnitude of rotary positions.
+
+    base^(-2i/rot) radians a position for pair i; for contexts longer than the
+    trained ones by `factor`: scaling "linear" divides all of them (positions
+    interpolated); "ntk" takes the base to base factor^(rot/(rot-2)), which keeps
+    the shortest wave and stretches the longest by the factor; "yarn" divides those
+    that turn fewer than `low` times in original_length positions, keeps those that
+    turn more than `high` times and blends linearly in between, with a magnitude of
+    1 + ln(factor)/10."""
+    if rot < 2 or rot % 2:
+        raise ValueError(f"rot must be an even number of at least 2, got {rot}")
+    if not (base > 0.0 and factor > 0.0):
+        raise ValueError(f"base and factor must be positive, got {base}, {factor}")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling must be None, 'linear', 'ntk' or 'yarn', got {scaling!r}")
+    if scaling == "yarn" and not high > low:
+        raise ValueError(f"high must be above low, got {low}, {high}")
+    if scaling == "ntk" and rot > 2:
+        base = base * factor ** (rot / (rot - 2))
+    f = torch.tensor(base, dtype=torch.float64) ** (
+        -torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    magnitude = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        turns = f * original_length / (2.0 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+        magnitude = 1.0 + 0.1 * math.log(factor) if factor > 1.0 else 1.0
+    return f.to(torch.float32), magnitude
+
+
+def rope(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, q_out: torch.Tensor,
+         k: torch.Tensor | None = None, k_out: torch.Tensor | None = None, layout: str = "half",
+         magnitude: float = 1.0, transposed: bool = False, cfg: CreditCfg | None = None) -> None:
+    """Rotary positions: q_out (and k_out) from q (and k), [tokens, heads, dim]
+    fp32 or bf16, heads and tokens at any strides.
+
+    The first 2 len(inv_freq) elements of each head are turned by positions
+    (int64 [tokens]) times inv_freq (fp32, rope_frequencies) and scaled by
+    magnitude, in pairs that are half of them apart (layout "half") or neighbours
+    ("interleaved"); the others stay.  transposed: the gradient for q (and k) of
+    one for q_out (and k_out).  An output may be its own input."""
+    tokens, dim, dev, fn = _heads_call("credit_rope_", q, "q")
+    dt = q.dtype
+    if (k is None) != (k_out is None):
+        raise ValueError("k and k_out come together")
+    status = fn(_heads(q, "q", dt, tokens, dim, dev),
+                None if k is None else _heads(k, "k", dt, tokens, dim, dev),
+                _rotation(positions, inv_freq, layout, magnitude, tokens, dev),
+                _heads(q_out, "q_out", dt, tokens, dim, dev),
+                None if k_out is None else _heads(k_out, "k_out", dt, tokens, dim, dev),
+                tokens, dim, bool(transposed), _cfg_ref(cfg, dev))
+    if status:
+        check(status, fn.__name__)
+
+
+def qk_norm_rope_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
+                     k_weight: torch.Tensor, positions: torch.Tensor | None,
+                     inv_freq: torch.Tensor | None, q_out: torch.Tensor, k_out: torch.Tensor,
+                     rstd: torch.Tensor | None = None, eps: float = 1.0e-6, layout: str = "half",
+                     magnitude: float = 1.0, cfg: CreditCfg | None = None) -> None:
+    """RMS norm of each head of q and k (weights [dim] of their type), then the
+    rotation of rope(), in one pass.  rstd [tokens, q heads + k heads] fp32, where
+    given, gets what the backward takes.  positions and inv_freq None: the norms
+    alone.  An output may be its own input."""
+    tokens, dim, dev, fn = _heads_call("credit_qk_norm_rope_fwd_", q, "q")
+    dt = q.dtype
+    status = fn(_heads(q, "q", dt, tokens, dim, dev), _heads(k, "k", dt, tokens, dim, dev),
+                _operand(q_weight, "q_weight", dt, (dim,), dev, "the queries'"),
+                _operand(k_weight, "k_weight", dt, (dim,), dev, "the queries'"),
+                _rotation(positions, inv_freq, layout, magnitude, tokens, dev),
+                _heads(q_out, "q_out", dt, tokens, dim, dev),
+                _heads(k_out, "k_out", dt, tokens, dim, dev),
+                None if rstd is None else _operand(
+                    rstd, "rstd", torch.float32, (tokens, q.shape[1] + k.shape[1]), dev,
+                    "the queries'"),
+                tokens, dim, eps, _cfg_ref(cfg, dev))
+    if status:
+        check(status, fn.__name__)
+
+
+def qk_norm_rope_bwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
+                     k_weight: torch.Tensor, positions: torch.Tensor | None,
+                     inv_freq: torch.Tensor | None, rstd: torch.Tensor, dq_out: torch.Tensor,
+                     dk_out: torch.Tensor, dq: torch.Tensor, dk: torch.Tensor,
+                     dq_weight: torch.Tensor, dk_weight: torch.Tensor, layout: str = "half",
+                     magnitude: float = 1.0, cfg: CreditCfg | None = None) -> None:
+    """Gradients of qk_norm_rope_fwd from its inputs and rstd: dq and dk (the
+    inputs' type; they may be dq_out and dk_out, or q and k) and dq_weight,
+    dk_weight [dim] fp32.  Captured into a graph it takes its workspace from cfg."""
+    tokens, dim, dev, fn = _heads_call("credit_qk_norm_rope_bwd_", q, "q")
+    dt, f32 = q.dtype, torch.float32
+    status = fn(_heads(q, "q", dt, tokens, dim, dev), _heads(k, "k", dt, tokens, dim, dev),
+                _operand(q_weight, "q_weight", dt, (dim,), dev, "the queries'"),
+                _operand(k_weight, "k_weight", dt, (dim,), dev, "the queries'"),
+                _rotation(positions, inv_freq, layout, magnitude, tokens, dev),
+                _operand(rstd, "rstd", f32, (tokens, q.shape[1] + k.shape[1]), dev,
+                         "the queries'"),
+                _heads(dq_out, "dq_out", dt, tokens, dim, dev),
+                _heads(dk_out, "dk_out", dt, tokens, dim, dev),
+                _heads(dq, "dq", dt, tokens, dim, dev), _heads(dk, "dk", dt, tokens, dim, dev),
+                _operand(dq_weight, "dq_weight", f32, (dim,), dev, "the queries'"),
+                _operand(dk_weight, "dk_weight", f32, (dim,), dev, "the queries'"),
+                tokens, dim, _cfg_ref(cfg, dev))
+    if status:
+        check(status, fn.__name__)
+
+
+def _pages(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int, device: int):
+    """A cache [pages, slots of a page, heads, dim], at any strides but the last."""
+    if t.dim() != 4:
+        raise ValueError(f"{name}: expected [pages, page size, heads, dim], "
+                         f"got shape {tuple(t.shape)}")
+    pages, size, heads, d = t.shape
+    page, slot, head, one = t.stride()
+    if t.dtype is not dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if d != dim:
+        raise ValueError(f"{name}: expected heads of {dim}, got {tuple(t.shape)}")
+    if one != 1 and d > 1:
+        raise ValueError(f"{name}: the elements of a head must be contiguous")
+    if t.get_device() != device:
+        raise ValueError(f"{name}: expected a tensor on {_device_name(device)}, got {t.device}")
+    return ctypes.byref(CreditPages(t.data_ptr(), page, slot, head, pages, size, heads))
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
+                 v_cache: torch.Tensor, positions: torch.Tensor | None = None,
+                 inv_freq: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                 q: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                 q_weight: torch.Tensor | None = None, eps: float = 1.0e-6, layout: str = "half",
+                 magnitude: float = 1.0, cfg: CreditCfg | None = None) -> None:
+    """New keys and values [tokens, heads, dim] bf16 into the paged caches
+    [pages, page size, heads, dim] (any strides but the last), token t at
+    slots[t] (int64: page * page size + slot; negative: nowhere).
+
+    The keys are normed where k_weight [dim] is given and rotated as by rope()
+    where positions and inv_freq are; the values are put as they are.  q and q_out,
+    where given: the tokens' queries, normed (q_weight) and rotated in the same
+    launch; q_out may be q."""
+    if k.dtype is not torch.bfloat16:
+        raise TypeError(f"k: expected torch.bfloat16, got {k.dtype}")
+    tokens, dim, dev, fn = _heads_call("credit_paged_append_", k, "k")
+    dt = k.dtype
+    if (q is None) != (q_out is None):
+        raise ValueError("q and q_out come together")
+    status = fn(_heads(k, "k", dt, tokens, dim, dev), _heads(v, "v", dt, tokens, dim, dev),
+                None if q is None else _heads(q, "q", dt, tokens, dim, dev),
+                None if k_weight is None else _operand(k_weight, "k_weight", dt, (dim,), dev,
+                                                       "the keys'"),
+                None if q_weight is None else _operand(q_weight, "q_weight", dt, (dim,), dev,
+                                                       "the keys'"),
+                _rotation(positions, inv_freq, layout, magnitude, tokens, dev),
+                _operand(slots, "slots", torch.int64, (tokens,), dev, "the keys'"),
+                _pages(k_cache, "k_cache", dt, dim, dev),
+                _pages(v_cache, "v_cache", dt, dim, dev),
+                None if q_out is None else _heads(q_out, "q_out", dt, tokens, dim, dev),
+                tokens, dim, eps, _cfg_ref(cfg, dev))
     if status:
         check(status, fn.__name__)
 

@@ -121,6 +121,7 @@ typedef struct credit_cfg {
 #define CREDIT_OP_TOKEN_LOGPROB_BWD 17
 #define CREDIT_OP_TOPK_DISTILL_FWD 18
 #define CREDIT_OP_TOPK_DISTILL_BWD 19
+#define CREDIT_OP_QK_NORM_ROPE_BWD 20 /* rows = tokens, cols = dim */
 
 /* ------------------------------------------------------------ library --- */
 
@@ -416,6 +417,115 @@ int credit_topk_distill_bwd_bf16(const uint16_t* logits, int64_t ld, const int64
                                  uint16_t* dlogits, int64_t ldd, int64_t rows, int64_t cols,
                                  int32_t n_top, int32_t tail, float temperature,
                                  const credit_cfg* cfg);
+
+/* ------------------------------- queries, keys and values by heads ------
+ * Tokens of heads, each head dim contiguous elements, dim at most 512: head h
+ * of token t at data + t token_stride + h head_stride (strides in elements),
+ * so that queries and keys may be column ranges of one projection's output. */
+typedef struct credit_heads {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+  int32_t heads;
+} credit_heads;
+
+/* Rotary positions: pair i of a head is turned by the angle
+ * positions[t] inv_freq[i] and scaled by magnitude,
+ *   (a, b) -> magnitude (a cos - b sin, b cos + a sin),
+ * over its first rot elements (even, at most dim; 0: nothing is turned and the
+ * pointers are not read); the rest stays as it is.  The pairs are elements i and
+ * i + rot/2, or with interleaved != 0 elements 2i and 2i + 1.  The angle is taken
+ * in 64 bits from the fp32 inv_freq (radians a position), so that far positions
+ * keep their digits; long contexts scale inv_freq and magnitude. */
+typedef struct credit_rotation {
+  const int64_t* positions; /* [tokens] */
+  const float* inv_freq;    /* [rot / 2] */
+  int32_t rot;
+  int32_t interleaved;
+  float magnitude;
+} credit_rotation;
+
+/* A paged cache of keys or values: head h of slot s of page p at
+ * data + p page_stride + s slot_stride + h head_stride (elements). */
+typedef struct credit_pages {
+  void* data;
+  int64_t page_stride;
+  int64_t slot_stride;
+  int64_t head_stride;
+  int64_t pages;
+  int32_t page_size; /* slots of a page */
+  int32_t heads;
+} credit_pages;
+
+/* Rotates queries (and keys, unless k and k_out are NULL): q_out = R q, k_out =
+ * R k.  transposed != 0: the gradient for q and k of one for q_out and k_out
+ * (the angles turned the other way).  An output may be its own input (same data
+ * and strides); other tensors may share a buffer but no element with an output,
+ * as the column ranges of one projection.  No counterpart in the reference.
+ * Variants: AUTO.  Takes no workspace. */
+int credit_rope_f32(const credit_heads* q, const credit_heads* k, const credit_rotation* rotation,
+                    const credit_heads* q_out, const credit_heads* k_out, int64_t tokens,
+                    int32_t dim, int32_t transposed, const credit_cfg* cfg);
+int credit_rope_bf16(const credit_heads* q, const credit_heads* k,
+                     const credit_rotation* rotation, const credit_heads* q_out,
+                     const credit_heads* k_out, int64_t tokens, int32_t dim, int32_t transposed,
+                     const credit_cfg* cfg);
+
+/* RMS norm of each head of the queries and keys, then the rotation, in one pass:
+ *   n = x r, r = (mean(x^2) + eps)^(-1/2) over the head's dim elements,
+ *   q_out = R (n q_weight), k_out = R (n k_weight),
+ * computed in fp32 and rounded once.  Weights [dim] of the inputs' type; rstd
+ * [tokens, q heads + k heads] fp32 gets r, queries first (NULL: not wanted).
+ * Squares are summed in fp32: elements beyond 1e18 overflow it.  In place as
+ * credit_rope_*.  No counterpart in the reference.  Variants: AUTO. */
+int credit_qk_norm_rope_fwd_f32(const credit_heads* q, const credit_heads* k,
+                                const float* q_weight, const float* k_weight,
+                                const credit_rotation* rotation, const credit_heads* q_out,
+                                const credit_heads* k_out, float* rstd, int64_t tokens,
+                                int32_t dim, float eps, const credit_cfg* cfg);
+int credit_qk_norm_rope_fwd_bf16(const credit_heads* q, const credit_heads* k,
+                                 const uint16_t* q_weight, const uint16_t* k_weight,
+                                 const credit_rotation* rotation, const credit_heads* q_out,
+                                 const credit_heads* k_out, float* rstd, int64_t tokens,
+                                 int32_t dim, float eps, const credit_cfg* cfg);
+/* Its gradients, from the forward's inputs and rstd: with d = R^T dq_out,
+ *   dq = r (d w - n mean(d w n)),  dq_weight [dim] = sum of d n over all tokens
+ * and heads (fp32, in an order that is the same from call to call), and the same
+ * for the keys.  dq may be dq_out or q, dk dk_out or k (same data and strides).
+ * credit_workspace_bytes(CREDIT_OP_QK_NORM_ROPE_BWD, tokens, dim, ...) gives its
+ * workspace; under capture and on hipStreamPerThread cfg->workspace has to be
+ * set (CREDIT_ERR_WORKSPACE).  Variants: AUTO. */
+int credit_qk_norm_rope_bwd_f32(const credit_heads* q, const credit_heads* k,
+                                const float* q_weight, const float* k_weight,
+                                const credit_rotation* rotation, const float* rstd,
+                                const credit_heads* dq_out, const credit_heads* dk_out,
+                                const credit_heads* dq, const credit_heads* dk, float* dq_weight,
+                                float* dk_weight, int64_t tokens, int32_t dim,
+                                const credit_cfg* cfg);
+int credit_qk_norm_rope_bwd_bf16(const credit_heads* q, const credit_heads* k,
+                                 const uint16_t* q_weight, const uint16_t* k_weight,
+                                 const credit_rotation* rotation, const float* rstd,
+                                 const credit_heads* dq_out, const credit_heads* dk_out,
+                                 const credit_heads* dq, const credit_heads* dk,
+                                 float* dq_weight, float* dk_weight, int64_t tokens, int32_t dim,
+                                 const credit_cfg* cfg);
+
+/* Puts the keys and values of new tokens into a paged cache: slot slots[t]
+ * (page slots[t] / page_size, slot slots[t] % page_size) of k_cache gets the
+ * token's keys, normed where k_weight is not NULL and rotated, that of v_cache
+ * its values as they are.  A negative slot is padding, as is one behind the
+ * last page: the token's keys and values go nowhere.  Of two tokens with one slot
+ * it is not said whose elements are kept.  q and q_out (both NULL: none): the
+ * tokens' queries, normed where q_weight is not NULL and rotated in the same
+ * launch, padding too.  k and v have the caches' heads.  q_out may be q; the
+ * caches may not share an element with each other or with any input.  No
+ * counterpart in the reference.  Variants: AUTO.  Takes no workspace. */
+int credit_paged_append_bf16(const credit_heads* k, const credit_heads* v,
+                             const credit_heads* q, const uint16_t* k_weight,
+                             const uint16_t* q_weight, const credit_rotation* rotation,
+                             const int64_t* slots, const credit_pages* k_cache,
+                             const credit_pages* v_cache, const credit_heads* q_out,
+                             int64_t tokens, int32_t dim, float eps, const credit_cfg* cfg);
 
 /* --------------------------------------- rowwise_quant (reference) -----
  * q = int8(clamp(rint(x * inv), -127, 127)), inv = (1 / max_j |x_j|) * 127
