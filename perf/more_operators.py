@@ -366,7 +366,11 @@ def _own(s):
                              q_out=s["q_out"], q_weight=s.get("wq"), eps=EPS, **turn)
         return s["q_out"], s["k_cache"], s["v_cache"]
     if op == "rope":
-        hip_lib.rope(s["q"], s["positions"], s["freq"], s["q_out"], s["k"], s["k_out"], **turn)
+        if case["norm"]:
+            hip_lib.qk_norm_rope_fwd(s["q"], s["k"], s["wq"], s["wk"], s["positions"], s["freq"],
+                                     s["q_out"], s["k_out"], eps=EPS, **turn)
+        else:
+            hip_lib.rope(s["q"], s["positions"], s["freq"], s["q_out"], s["k"], s["k_out"], **turn)
         return s["q_out"], s["k_out"]
     if op == "norm_rope_fwd":
         hip_lib.qk_norm_rope_fwd(s["q"], s["k"], s["wq"], s["wk"], s["positions"], s["freq"],
