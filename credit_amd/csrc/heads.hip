@@ -509,52 +509,8 @@ __global__ __launch_bounds__(kSumCols* kSumRuns) void heads_dw_kernel(const SumA
 
 // ------------------------------------------------------------------- host --
 
-constexpr int64_t kMaxBytes = int64_t{1} << 60;
-
-// A tensor by tokens and heads, its place, checked.
-int check_heads(const credit_heads* h, const char* name, int64_t tokens, int dim, size_t elem,
-                Place* place) {
-  CREDIT_TRY(check_ptr(h, name));
-  if (h->heads < 1 || h->heads > (1 << 20))
-    return set_error(CREDIT_ERR_BAD_SHAPE, "%s: %d heads outside [1, 2^20]", name, h->heads);
-  CREDIT_TRY(check_row_ptr(h->data, name, tokens));
-  CREDIT_TRY(check_aligned(h->data, elem, name));
-  const double bytes = (static_cast<double>(tokens) * h->token_stride +
-                        static_cast<double>(h->heads) * h->head_stride + dim) *
-                       static_cast<double>(elem);
-  if (h->token_stride < 0 || h->head_stride < 0 || bytes > static_cast<double>(kMaxBytes))
-    return set_error(CREDIT_ERR_BAD_SHAPE, "%s: strides (%lld, %lld) negative or too large", name,
-                     static_cast<long long>(h->token_stride),
-                     static_cast<long long>(h->head_stride));
-  const int64_t e = static_cast<int64_t>(elem);
-  *place = Place{reinterpret_cast<uintptr_t>(h->data), h->token_stride * e, h->head_stride * e,
-                 tokens, h->heads, dim * e};
-  return CREDIT_OK;
-}
-int check_output(const credit_heads* h, const char* name, const credit_heads* in, int64_t tokens,
-                 int dim, size_t elem, Place* place) {
-  CREDIT_TRY(check_heads(h, name, tokens, dim, elem, place));
-  if (h->heads != in->heads)
-    return set_error(CREDIT_ERR_BAD_SHAPE, "%s: %d heads, its input has %d", name, h->heads,
-                     in->heads);
-  if (!heads::apart_within(*place))
-    return set_error(CREDIT_ERR_BAD_SHAPE, "%s: its heads overlap each other", name);
-  return CREDIT_OK;
-}
-int check_apart(const Place& out, const char* name, const Place& other, const char* other_name) {
-  if (heads::apart(out, other)) return CREDIT_OK;
-  return set_error(CREDIT_ERR_BAD_CONFIG, "%s overlaps %s", name, other_name);
-}
 int check_own(const Place& out, const char* name, const Place& in, const char* in_name) {
-  return heads::same(out, in) ? CREDIT_OK : check_apart(out, name, in, in_name);
-}
-int check_sizes(int64_t tokens, int32_t dim) {
-  if (tokens < 0 || tokens > (int64_t{1} << 31) - 1)
-    return set_error(CREDIT_ERR_BAD_SHAPE, "%lld tokens outside [0, 2^31)",
-                     static_cast<long long>(tokens));
-  if (dim < 1 || dim > kMaxDim)
-    return set_error(CREDIT_ERR_BAD_SHAPE, "dim %d outside [1, %d]", dim, kMaxDim);
-  return CREDIT_OK;
+  return heads::same(out, in) ? CREDIT_OK : check_places_apart(out, name, in, in_name);
 }
 int check_rotation(const credit_rotation* r, int64_t tokens, int dim, bool transposed,
                    Rotation* out) {
@@ -578,13 +534,6 @@ int check_eps(float eps) {
     return set_error(CREDIT_ERR_BAD_CONFIG, "eps %g is not a finite number >= 0", eps);
   return CREDIT_OK;
 }
-int check_auto(const credit_cfg* cfg) {
-  CREDIT_TRY(check_cfg(cfg));
-  if (cfg_variant(cfg) != CREDIT_VARIANT_AUTO || cfg_split(cfg) != 0)
-    return set_error(CREDIT_ERR_UNSUPPORTED, "only AUTO without a split is supported");
-  return CREDIT_OK;
-}
-
 // Whether units of n elements of `elem` bytes serve: every address and the
 // borders of the rotation lie on them.
 struct Shape {
@@ -685,7 +634,7 @@ int rotate(const credit_heads* q, const credit_heads* k, const T* q_weight, cons
            float* rstd, int64_t tokens, int32_t dim, float eps, bool norm, bool transposed,
            const credit_cfg* cfg) {
   constexpr size_t kElem = sizeof(T);
-  CREDIT_TRY(check_sizes(tokens, dim));
+  CREDIT_TRY(check_tokens(tokens, dim, kMaxDim));
   ForwardArgs<T> a{};
   CREDIT_TRY(check_rotation(rotation, tokens, dim, transposed, &a.r));
   Shape shape{dim, &a.r};
@@ -706,14 +655,14 @@ int rotate(const credit_heads* q, const credit_heads* k, const T* q_weight, cons
     CREDIT_TRY(check_eps(eps));
     shape.addresses |= reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight);
   }
-  CREDIT_TRY(check_auto(cfg));
+  CREDIT_TRY(check_only_auto(cfg));
   if (tokens == 0) return CREDIT_OK;
   CREDIT_TRY(check_own(out[0], "q_out", in[0], "q"));
   if (keys) {
     CREDIT_TRY(check_own(out[1], "k_out", in[1], "k"));
-    CREDIT_TRY(check_apart(out[0], "q_out", in[1], "k"));
-    CREDIT_TRY(check_apart(out[1], "k_out", in[0], "q"));
-    CREDIT_TRY(check_apart(out[0], "q_out", out[1], "k_out"));
+    CREDIT_TRY(check_places_apart(out[0], "q_out", in[1], "k"));
+    CREDIT_TRY(check_places_apart(out[1], "k_out", in[0], "q"));
+    CREDIT_TRY(check_places_apart(out[0], "q_out", out[1], "k_out"));
   }
   a.sides = keys ? 2 : 1;
   a.dim = dim;
@@ -741,7 +690,7 @@ int norm_rope_bwd(const credit_heads* q, const credit_heads* k, const T* q_weigh
                   const credit_heads* dk, float* dq_weight, float* dk_weight, int64_t tokens,
                   int32_t dim, const credit_cfg* cfg) {
   constexpr size_t kElem = sizeof(T);
-  CREDIT_TRY(check_sizes(tokens, dim));
+  CREDIT_TRY(check_tokens(tokens, dim, kMaxDim));
   GradArgs<T> a{};
   CREDIT_TRY(check_rotation(rotation, tokens, dim, true, &a.r));
   Shape shape{dim, &a.r};
@@ -774,14 +723,14 @@ int norm_rope_bwd(const credit_heads* q, const credit_heads* k, const T* q_weigh
   }
   CREDIT_TRY(check_row_ptr(rstd, "rstd", tokens));
   CREDIT_TRY(check_aligned(rstd, sizeof(float), "rstd"));
-  CREDIT_TRY(check_auto(cfg));
+  CREDIT_TRY(check_only_auto(cfg));
   for (int i = 0; i < 2 && tokens > 0; ++i) {
     CREDIT_TRY(check_own(pd[i], kNames[2][i], px[i], kNames[0][i]));
     CREDIT_TRY(check_own(pd[i], kNames[2][i], py[i], kNames[1][i]));
-    CREDIT_TRY(check_apart(pd[i], kNames[2][i], px[1 - i], kNames[0][1 - i]));
-    CREDIT_TRY(check_apart(pd[i], kNames[2][i], py[1 - i], kNames[1][1 - i]));
+    CREDIT_TRY(check_places_apart(pd[i], kNames[2][i], px[1 - i], kNames[0][1 - i]));
+    CREDIT_TRY(check_places_apart(pd[i], kNames[2][i], py[1 - i], kNames[1][1 - i]));
   }
-  if (tokens > 0) CREDIT_TRY(check_apart(pd[0], "dq", pd[1], "dk"));
+  if (tokens > 0) CREDIT_TRY(check_places_apart(pd[0], "dq", pd[1], "dk"));
   hipStream_t stream = cfg_stream(cfg);
   if ((cfg == nullptr || cfg->workspace == nullptr) && !keeps_scratch(stream))
     return set_error(CREDIT_ERR_WORKSPACE,
@@ -864,7 +813,7 @@ int append(const credit_heads* k, const credit_heads* v, const credit_heads* q,
            const credit_cfg* cfg) {
   using T = uint16_t;
   constexpr size_t kElem = sizeof(T);
-  CREDIT_TRY(check_sizes(tokens, dim));
+  CREDIT_TRY(check_tokens(tokens, dim, kMaxDim));
   ForwardArgs<T> a{};
   CREDIT_TRY(check_rotation(rotation, tokens, dim, false, &a.r));
   Shape shape{dim, &a.r};
@@ -887,22 +836,22 @@ int append(const credit_heads* k, const credit_heads* v, const credit_heads* q,
   CREDIT_TRY(check_aligned(k_weight, kElem, "k_weight"));
   CREDIT_TRY(check_aligned(q_weight, kElem, "q_weight"));
   CREDIT_TRY(check_eps(eps));
-  CREDIT_TRY(check_auto(cfg));
+  CREDIT_TRY(check_only_auto(cfg));
   if (tokens == 0) return CREDIT_OK;
-  CREDIT_TRY(check_caches_apart(kc, vc));
+  CREDIT_TRY(check_places_apart(kc, "k_cache", vc, "v_cache"));
   struct Named {
     const Place* place;
     const char* name;
   };
   const Named inputs[] = {{&pk, "k"}, {&pv, "v"}, {&pq, "q"}, {&po, "q_out"}};
   for (int i = 0; i < (queries ? 4 : 2); ++i) {
-    CREDIT_TRY(check_apart(kc, "k_cache", *inputs[i].place, inputs[i].name));
-    CREDIT_TRY(check_apart(vc, "v_cache", *inputs[i].place, inputs[i].name));
+    CREDIT_TRY(check_places_apart(kc, "k_cache", *inputs[i].place, inputs[i].name));
+    CREDIT_TRY(check_places_apart(vc, "v_cache", *inputs[i].place, inputs[i].name));
   }
   if (queries) {
     CREDIT_TRY(check_own(po, "q_out", pq, "q"));
-    CREDIT_TRY(check_apart(po, "q_out", pk, "k"));
-    CREDIT_TRY(check_apart(po, "q_out", pv, "v"));
+    CREDIT_TRY(check_places_apart(po, "q_out", pk, "k"));
+    CREDIT_TRY(check_places_apart(po, "q_out", pv, "v"));
   }
   a.dim = dim;
   a.eps = eps;
@@ -925,6 +874,59 @@ int append(const credit_heads* k, const credit_heads* v, const credit_heads* q,
 }
 
 }  // namespace
+
+namespace {
+constexpr int64_t kMaxBytes = int64_t{1} << 60;
+}  // namespace
+
+// A tensor by tokens and heads, its place, checked.
+int check_heads(const credit_heads* h, const char* name, int64_t tokens, int dim, size_t elem,
+                Place* place) {
+  CREDIT_TRY(check_ptr(h, name));
+  if (h->heads < 1 || h->heads > (1 << 20))
+    return set_error(CREDIT_ERR_BAD_SHAPE, "%s: %d heads outside [1, 2^20]", name, h->heads);
+  CREDIT_TRY(check_row_ptr(h->data, name, tokens));
+  CREDIT_TRY(check_aligned(h->data, elem, name));
+  const double bytes = (static_cast<double>(tokens) * h->token_stride +
+                        static_cast<double>(h->heads) * h->head_stride + dim) *
+                       static_cast<double>(elem);
+  if (h->token_stride < 0 || h->head_stride < 0 || bytes > static_cast<double>(kMaxBytes))
+    return set_error(CREDIT_ERR_BAD_SHAPE, "%s: strides (%lld, %lld) negative or too large", name,
+                     static_cast<long long>(h->token_stride),
+                     static_cast<long long>(h->head_stride));
+  const int64_t e = static_cast<int64_t>(elem);
+  *place = Place{reinterpret_cast<uintptr_t>(h->data), h->token_stride * e, h->head_stride * e,
+                 tokens, h->heads, dim * e};
+  return CREDIT_OK;
+}
+int check_output(const credit_heads* h, const char* name, const credit_heads* in, int64_t tokens,
+                 int dim, size_t elem, Place* place) {
+  CREDIT_TRY(check_heads(h, name, tokens, dim, elem, place));
+  if (h->heads != in->heads)
+    return set_error(CREDIT_ERR_BAD_SHAPE, "%s: %d heads, its input has %d", name, h->heads,
+                     in->heads);
+  if (!heads::apart_within(*place))
+    return set_error(CREDIT_ERR_BAD_SHAPE, "%s: its heads overlap each other", name);
+  return CREDIT_OK;
+}
+int check_places_apart(const Place& out, const char* name, const Place& other, const char* other_name) {
+  if (heads::apart(out, other)) return CREDIT_OK;
+  return set_error(CREDIT_ERR_BAD_CONFIG, "%s overlaps %s", name, other_name);
+}
+int check_tokens(int64_t tokens, int32_t dim, int32_t max_dim) {
+  if (tokens < 0 || tokens > (int64_t{1} << 31) - 1)
+    return set_error(CREDIT_ERR_BAD_SHAPE, "%lld tokens outside [0, 2^31)",
+                     static_cast<long long>(tokens));
+  if (dim < 1 || dim > max_dim)
+    return set_error(CREDIT_ERR_BAD_SHAPE, "dim %d outside [1, %d]", dim, max_dim);
+  return CREDIT_OK;
+}
+int check_only_auto(const credit_cfg* cfg) {
+  CREDIT_TRY(check_cfg(cfg));
+  if (cfg_variant(cfg) != CREDIT_VARIANT_AUTO || cfg_split(cfg) != 0)
+    return set_error(CREDIT_ERR_UNSUPPORTED, "only AUTO without a split is supported");
+  return CREDIT_OK;
+}
 
 // A cache's two levels: pages of heads, slots of heads.
 int check_cache(const credit_pages* c, const char* name, int dim, size_t elem, Place* pages,
@@ -955,10 +957,6 @@ int check_cache(const credit_pages* c, const char* name, int dim, size_t elem, P
     return set_error(CREDIT_ERR_BAD_SHAPE, "%s: its pages overlap each other", name);
   return CREDIT_OK;
 }
-int check_caches_apart(const Place& k, const Place& v) {
-  return check_apart(k, "k_cache", v, "v_cache");
-}
-
 size_t qk_norm_rope_bwd_workspace(int64_t dim) {
   return static_cast<size_t>(kMaxGradBlocks) * static_cast<size_t>(dim) * sizeof(float);
 }

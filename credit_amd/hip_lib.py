@@ -182,6 +182,9 @@ SIGNATURES: dict[str, list] = {
        for t in ("f32", "bf16")},
     "credit_paged_append_bf16": [_HEADS, _HEADS, _HEADS, _P, _P, _ROTATION, _P, _PAGES, _PAGES,
                                  _HEADS, _I64, _I32, _F, _CFG],
+    "credit_paged_attention_bf16": [_HEADS, _PAGES, _PAGES, _P, _I64, _I64, _P, _P, _HEADS, _P,
+                                    _I64, _I64, _I32, _F, _I32, _CFG],
+    "credit_paged_attention_workspace_bytes": [_I64, _I64, _I32, _I32, _I32, _I64],
     "credit_rowwise_quant_f32": [_P, _P, _P, _I64, _I64, _CFG],
     "credit_lars_momentum_f32": [_P, _P, _P, _P, _P, _I64, _I64, _CFG],
     "credit_weighted_var_bwd_f32": [_P, _P, _P, _P, _I64, _I64, _F, _CFG],
@@ -220,6 +223,7 @@ _RESTYPES = {
     "credit_status_string": ctypes.c_char_p,
     "credit_workspace_bytes": ctypes.c_size_t,
     "credit_ffn_bwd_workspace_bytes": ctypes.c_size_t,
+    "credit_paged_attention_workspace_bytes": ctypes.c_size_t,
 }
 
 _lib: ctypes.CDLL | None = None
@@ -1032,6 +1036,55 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
                 tokens, dim, eps, _cfg_ref(cfg, dev))
     if status:
         check(status, fn.__name__)
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    pages: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
+                    out: torch.Tensor, lse: torch.Tensor | None = None,
+                    scale: float | None = None, window: int = 0,
+                    cfg: CreditCfg | None = None) -> None:
+    """Attention of a batch's new tokens over a paged cache (causal).
+
+    q and out [tokens, q heads, dim] bf16, the caches [pages, page size, key heads,
+    dim] bf16 as paged_append fills them; pages int32 [batch, pages of a sequence at
+    most], q_start int32 [batch + 1] (the first token of each sequence), kv_len int32
+    [batch] (positions in the cache, the new tokens' among them).  lse [tokens, q
+    heads] fp32, where given, gets the log-sums.  scale: 1 / sqrt(dim) unless given.
+    window > 0: a token sees the last `window` positions up to its own.  Rows that
+    see nothing get 0 and -inf, tokens of no sequence are left as they are."""
+    if q.dtype is not torch.bfloat16:
+        raise TypeError(f"q: expected torch.bfloat16, got {q.dtype}")
+    tokens, dim, dev, fn = _heads_call("credit_paged_attention_", q, "q")
+    dt, i32 = q.dtype, torch.int32
+    if pages.dim() != 2:
+        raise ValueError(f"pages: expected [batch, pages], got shape {tuple(pages.shape)}")
+    batch, cols = pages.shape
+    ld, one = pages.stride()
+    if pages.dtype is not i32:
+        raise TypeError(f"pages: expected {i32}, got {pages.dtype}")
+    if one != 1 and cols > 1:
+        raise ValueError("pages: the entries of a sequence must be contiguous")
+    if pages.get_device() != dev:
+        raise ValueError(f"pages: expected a tensor on {_device_name(dev)}, got {pages.device}")
+    status = fn(_heads(q, "q", dt, tokens, dim, dev), _pages(k_cache, "k_cache", dt, dim, dev),
+                _pages(v_cache, "v_cache", dt, dim, dev), pages.data_ptr(),
+                ld if batch > 1 else cols, cols,
+                _operand(q_start, "q_start", i32, (batch + 1,), dev, "the queries'"),
+                _operand(kv_len, "kv_len", i32, (batch,), dev, "the queries'"),
+                _heads(out, "out", dt, tokens, dim, dev),
+                None if lse is None else _operand(lse, "lse", torch.float32,
+                                                  (tokens, q.shape[1]), dev, "the queries'"),
+                tokens, batch, dim, 1.0 / math.sqrt(dim) if scale is None else scale, window,
+                _cfg_ref(cfg, dev))
+    if status:
+        check(status, fn.__name__)
+
+
+def paged_attention_workspace_bytes(tokens: int, batch: int, q_heads: int, kv_heads: int,
+                                    dim: int, positions: int) -> int:
+    """Bytes of a workspace for paged_attention under capture; positions: the
+    columns of pages times the page size."""
+    return int(load_library().credit_paged_attention_workspace_bytes(
+        tokens, batch, q_heads, kv_heads, dim, positions))
 
 
 def layernorm_backward(x: torch.Tensor, dy: torch.Tensor, gamma: torch.Tensor,

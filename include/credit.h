@@ -527,6 +527,42 @@ int credit_paged_append_bf16(const credit_heads* k, const credit_heads* v,
                              const credit_pages* v_cache, const credit_heads* q_out,
                              int64_t tokens, int32_t dim, float eps, const credit_cfg* cfg);
 
+/* Attention of a batch's new tokens over a paged cache.  Sequence b has kv_len[b]
+ * positions in the cache, position j in slot j % page_size of page
+ * pages[b pages_ld + j / page_size], its new tokens among them as the last: tokens
+ * q_start[b] .. q_start[b + 1] - 1 of q (q_start [batch + 1] rising from row to
+ * row).  Token i of n new ones sees positions j <= kv_len[b] - n + i, with window
+ * > 0 only the last window of those:
+ *   out = sum_j p_j v_j, p = softmax(scale q k_j), lse = ln sum_j e^(scale q k_j)
+ * (lse [tokens, q heads] fp32; NULL: not wanted), head h of q with key head
+ * h / (q heads / key heads).  A row that sees nothing (kv_len[b] < n), or only
+ * scores of -inf: out 0, lse -inf.  What no row sees is not read for its values:
+ * NaN and infinities in hidden positions, in unused slots or behind the last
+ * sequence change nothing.  Rows that see an entry of pages outside [0, the
+ * cache's pages) become NaN.  kv_len beyond pages_cols page_size counts as that;
+ * tokens of no sequence are left as they are.
+ * Scores, maxima, sums and outputs are held in fp32, the weights rounded to bf16
+ * for their product with v, out once more.  dim: a multiple of 8 up to 256;
+ * addresses and strides of q, out and the caches: multiples of 16 bytes
+ * (CREDIT_ERR_ALIGNMENT).  out shares nothing with q or the caches.
+ * Few rows over many positions are cut into parts whose results meet in the
+ * workspace, credit_paged_attention_workspace_bytes(tokens, batch, q heads, key
+ * heads, dim, pages_cols page_size) bytes; under capture and on
+ * hipStreamPerThread only with a cfg->workspace, and graphs that may run at the
+ * same time need one each.  Values may differ by roundings with and without
+ * parts, never between calls of one kind.  No counterpart in the reference.
+ * Variants: AUTO. */
+int credit_paged_attention_bf16(const credit_heads* q, const credit_pages* k_cache,
+                                const credit_pages* v_cache, const int32_t* pages,
+                                int64_t pages_ld, int64_t pages_cols, const int32_t* q_start,
+                                const int32_t* kv_len, const credit_heads* out, float* lse,
+                                int64_t tokens, int64_t batch, int32_t dim, float scale,
+                                int32_t window, const credit_cfg* cfg);
+/* Bytes of a cfg->workspace with which the call above takes parts as it does
+ * without one (0: it takes none).  Plumbing of this ABI. */
+size_t credit_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int32_t q_heads,
+                                              int32_t kv_heads, int32_t dim, int64_t positions);
+
 /* --------------------------------------- rowwise_quant (reference) -----
  * q = int8(clamp(rint(x * inv), -127, 127)), inv = (1 / max_j |x_j|) * 127
  * (0 for an all-zero row), scale = max_j |x_j| / 127, fp32 in: the reference

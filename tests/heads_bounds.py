@@ -87,3 +87,52 @@ def norm_rope_bwd(x, weight, rstd, dy, positions, inv_freq, layout, magnitude):
     dn = np.abs(d) * n
     dw = (d_err * n + dn * E).sum((0, 1)) + (x.shape[0] * x.shape[1] + 2) * E * dn.sum((0, 1))
     return dx, dw
+
+
+RAISES = 16  # times that a row's maximum is raised, waves and parts joined
+
+
+def attention(q, k_cache, v_cache, pages, q_start, kv_len, scale, window=0):
+    """(bound of out in fp32 before its rounding, of lse).  A score: dim products,
+    exact in fp32, each addition off by at most a step (2 E).  A weight: the score's
+    error; the exponent's factor, base, and their fused product, each E of it; the
+    exponential, 2 E; the same for each time that it is rescaled; its rounding to
+    bf16, 2^-8.  Sums over the positions: a step (2 E) each.  Weights below the
+    smallest normal number count as 0."""
+    q, k_cache, v_cache = (np.asarray(t, np.float64) for t in (q, k_cache, v_cache))
+    tokens, heads, dim = q.shape
+    size, kv_heads = k_cache.shape[1:3]
+    out, lse = np.zeros(q.shape), np.zeros((tokens, heads))
+    for b, kv in enumerate(kv_len):
+        new = q_start[b + 1] - q_start[b]
+        for i in range(new):
+            t, last = q_start[b] + i, kv - new + i
+            at = np.arange(max(0, last - window + 1) if window else 0, max(0, last + 1))
+            if len(at) == 0:
+                continue
+            page = np.asarray(pages[b])[at // size]
+            if (page < 0).any() or (page >= k_cache.shape[0]).any():
+                continue
+            for h in range(heads):
+                g = h // (heads // kv_heads)
+                k, v = k_cache[page, at % size, g], np.abs(v_cache[page, at % size, g])
+                with np.errstate(all="ignore"):
+                    x = scale * (k @ q[t, h])
+                # A score of -inf makes a weight of exactly 0, which adds nothing
+                # and no error; a row of nothing else is written as it is, and one
+                # of +inf or NaN is NaN: no bound is asked for.
+                live = x > -np.inf
+                k, v, x = k[live], v[live], x[live]
+                if not live.any() or not np.isfinite(x).all():
+                    continue
+                w = np.exp(x - x.max())
+                total = w.sum()
+                w /= total
+                big = np.abs(x).max()
+                d = (scale * 2 * dim * E * (np.abs(k) @ np.abs(q[t, h]))
+                     + 4 * E * (np.abs(x) + big) + 2 * E + RAISES * (4 + 2 * big) * E)
+                wd, n = (w * d).sum(), 2 * (len(at) + RAISES) * E
+                out[t, h] = ((w * (2.0 ** -8 + d + n))[:, None] * v).sum(0) \
+                    + (w[:, None] * v).sum(0) * (wd + n + 3 * E) + 1e-36 * v.max()
+                lse[t, h] = wd + n + 4 * E * np.log(total) + 3 * E * (big + np.log(total))
+    return out, lse
