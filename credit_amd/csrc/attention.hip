@@ -159,6 +159,10 @@ __device__ __forceinline__ void clear(State<D>& s) {
 // are 0.
 __device__ __forceinline__ float base_of(float m) { return m == kNegInf ? 0.0f : m; }
 
+// The lane, opaque to the compiler: what is derived from it within a step is not
+// kept in registers from step to step.
+__device__ __forceinline__ int opaque_lane() { return opaque_lane_index() & (kWave - 1); }
+
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
 // The queries of a wave's rows: lane l holds elements 16 ks + 8 (l / 32) .. + 7 of
@@ -182,8 +186,7 @@ __device__ __forceinline__ void load_queries(bf16x8_t (&q)[D / 16], const Args& 
 // A fragment of V^T: column 32 db + l % 32 of the 16 positions from 16 ts on, in
 // the weights' order (element e: position 16 ts + 8 (e / 4) + 4 (l / 32) + e % 4).
 template <int D>
-__device__ __forceinline__ bf16x8_t value_fragment(const char* v, int db, int ts) {
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+__device__ __forceinline__ bf16x8_t value_fragment(const char* v, int lane, int db, int ts) {
   const int row = 16 * ts + 4 * (lane >> 5) + ((lane & 15) >> 2);
   const int column = 32 * db + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   const int at = Lds<D>::value(row, column >> 3) + (column & 7) * 2;
@@ -193,32 +196,48 @@ __device__ __forceinline__ bf16x8_t value_fragment(const char* v, int db, int ts
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// Values that are not finite, in steps where a mask hides positions from some
-// rows: a weight of 0 times such a value would be NaN.  Takes them out of the
-// fragment; *code: 1 for +inf, 2^8 for -inf, 2^16 for NaN in their place.
-__device__ __forceinline__ uint32_t mark_of(uint32_t bits) {
-  return bits == 0x7F80u ? 0x3F80u : bits == 0xFF80u ? 0x4380u : 0x4780u;
-}
-__device__ __forceinline__ bool take_out(bf16x8_t& v, bf16x8_t& code) {
-  u32x4 w = __builtin_bit_cast(u32x4, v), c;
-  bool any = false;
+// In steps where a mask hides positions from some rows, a value that is not finite
+// would make NaN of its weight of 0: whether there are any among `ROWS` rows.
+template <int D, int ROWS>
+__device__ __forceinline__ bool any_special(const char* v) {
+  const int lane = opaque_lane();
+  uint32_t bad = 0;
+#pragma unroll 4
+  for (int i = 0; i < ROWS * Lds<D>::kRowBytes / (16 * kWave); ++i) {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(v + (i * kWave + lane) * 16);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const bool lo = (w[e] & 0x7F80u) == 0x7F80u, hi = (w[e] & 0x7F800000u) == 0x7F800000u;
-    c[e] = (lo ? mark_of(w[e] & 0xFFFFu) : 0u) | (hi ? mark_of(w[e] >> 16) << 16 : 0u);
-    w[e] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
-    any = any || lo || hi;
+    for (int e = 0; e < 4; ++e)  // bit 31 or 15: an exponent of all ones
+      bad |= ((w[e] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
   }
-  v = __builtin_bit_cast(bf16x8_t, w);
-  code = __builtin_bit_cast(bf16x8_t, c);
-  return any;
+  return __builtin_amdgcn_ballot_w64(bad != 0) != 0;
 }
-// What the marks of a row's visible positions make of its output.
-__device__ __forceinline__ float marked(float o, float marks) {
-  const int n = static_cast<int>(marks);
-  const bool pos = (n & 0xFF) != 0, neg = (n & 0xFF00) != 0, nan = n >= 1 << 16;
-  if (nan || (pos && neg)) return __builtin_nanf("");
-  return pos ? o + __builtin_inff() : neg ? o - __builtin_inff() : o;
+// 0 in their place.
+__device__ __forceinline__ bf16x8_t without_special(bf16x8_t v) {
+  u32x4 w = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    w[e] &= ((w[e] & 0x7F80u) == 0x7F80u ? 0u : 0xFFFFu) |
+            ((w[e] & 0x7F800000u) == 0x7F800000u ? 0u : 0xFFFF0000u);
+  return __builtin_bit_cast(bf16x8_t, w);
+}
+// Adds them to the outputs of the rows that see them, whatever their weight.
+template <int D, int ROWS>
+__device__ __forceinline__ void add_special(State<D>& s, const char* v, int j0, int low,
+                                            int last) {
+#pragma unroll 1
+  for (int r = 0; r < ROWS; ++r) {
+    const int lane = opaque_lane();
+    const bool seen = j0 + r >= low && j0 + r <= last;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int column = 32 * db + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+        const uint16_t bits = *reinterpret_cast<const uint16_t*>(
+            v + Lds<D>::value(r, column >> 3) + (column & 7) * 2);
+        s.o[db][i] += seen && (bits & 0x7F80u) == 0x7F80u ? bf16_to_f32(bits) : 0.0f;
+      }
+  }
 }
 
 // One step: NB blocks of 32 positions from j0 on, keys at k, values at v in LDS.
@@ -226,7 +245,7 @@ __device__ __forceinline__ float marked(float o, float marks) {
 template <int D, int NB, bool MASKED>
 __device__ __forceinline__ void step(State<D>& s, const bf16x8_t (&q)[D / 16], const char* k,
                                      const char* v, int j0, int low, int last, float scale_log2) {
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  const int lane = opaque_lane();
   f32x16 x[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -284,46 +303,22 @@ __device__ __forceinline__ void step(State<D>& s, const bf16x8_t (&q)[D / 16], c
       p[2 * nb + h] = __builtin_bit_cast(bf16x8_t, w);
     }
   s.l += sum;
-  bool bad = false;
+  const bool special = MASKED && any_special<D, 32 * NB>(v);
+  if (!special) {
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db)
+    for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-    for (int ts = 0; ts < 2 * NB; ++ts) {
-      bf16x8_t f = value_fragment<D>(v, db, ts);
-      if constexpr (MASKED) {
-        bf16x8_t code;
-        bad = take_out(f, code) || bad;
-      }
-      s.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, p[ts], s.o[db], 0, 0, 0);
-    }
-  if constexpr (MASKED) {
-    if (__builtin_amdgcn_ballot_w64(bad) == 0) return;
-    bf16x8_t seen[2 * NB];  // 1 where the row sees the position
+      for (int ts = 0; ts < 2 * NB; ++ts)
+        s.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_fragment<D>(v, lane, db, ts), p[ts],
+                                                          s.o[db], 0, 0, 0);
+  } else {
 #pragma unroll
-    for (int ts = 0; ts < 2 * NB; ++ts) {
-      u32x4 w;
+    for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = j0 + 16 * ts + 8 * (e >> 1) + 4 * (lane >> 5) + 2 * (e & 1);
-        w[e] = (j >= low && j <= last ? 0x3F80u : 0u) |
-               (j + 1 >= low && j + 1 <= last ? 0x3F800000u : 0u);
-      }
-      seen[ts] = __builtin_bit_cast(bf16x8_t, w);
-    }
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db) {
-      f32x16 marks;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) marks[i] = 0.0f;
-#pragma unroll
-      for (int ts = 0; ts < 2 * NB; ++ts) {
-        bf16x8_t f = value_fragment<D>(v, db, ts), code;
-        take_out(f, code);
-        marks = __builtin_amdgcn_mfma_f32_32x32x16_bf16(code, seen[ts], marks, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s.o[db][i] = marked(s.o[db][i], marks[i]);
-    }
+      for (int ts = 0; ts < 2 * NB; ++ts)
+        s.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            without_special(value_fragment<D>(v, lane, db, ts)), p[ts], s.o[db], 0, 0, 0);
+    add_special<D, 32 * NB>(s, v, j0, low, last);
   }
 }
 
@@ -453,6 +448,95 @@ struct Loader {
   }
 };
 
+// One LDS-direct load: 16 bytes a lane from offset `off` of the resource to LDS at
+// `lds` + 16 lane.  In inline assembly, as the compiler would wait for every such
+// load before any read of LDS; the waits are those written below.  s_nop covers
+// the write of M0, which nothing else here reads.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void load_to_lds(buffer_rsrc_t rsrc, uint32_t off, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %0, %1, 0 offen lds"
+      :
+      : "v"(off), "s"(rsrc), "s"(lds)
+      : "memory", "m0");
+}
+#pragma clang diagnostic pop
+// s_waitcnt vmcnt(N), the other counters at their maxima.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(((N >> 4) << 14) | (0xF << 8) | (0x7 << 4) | (N & 15));
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+// Every read of LDS has returned.
+__device__ __forceinline__ void wait_reads() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+// Keys of pages that are not there: NaN.
+__device__ const u32x4 kNoKeys = {0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+
+typedef const __attribute__((address_space(4))) int32_t* scalar_i32_t;
+
+// The same step without registers, where the kRows rows of a wave's load lie in one
+// page (page_size a multiple of kRows): its address is uniform, and rows behind
+// `end`, or of a page that is not there, are out of the resource's bounds, which
+// makes them 0.
+template <int D, int ROWS, int W>
+struct Direct {
+  static constexpr int kRows = kWave / Lds<D>::kChunks;  // of a load
+  static constexpr int kPer = ROWS / kRows / W;          // loads a wave, of keys or values
+  int page[kPer];
+
+  // The pages of the step at j0, ahead of its loads.
+  __device__ __forceinline__ void look_up(const Args& a, const int32_t* pages, int j0, int end,
+                                          int wave) {
+    const scalar_i32_t table = (scalar_i32_t)(reinterpret_cast<uintptr_t>(pages));
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      page[i] = table[divide(min(j0 + (i * W + wave) * kRows, end - 1), a.by_page)];
+  }
+  __device__ __forceinline__ void load(const Args& a, int head, int j0, int end, int wave,
+                                       uint32_t lds) const {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int in_row = lane / Lds<D>::kChunks, place = lane % Lds<D>::kChunks;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int r0 = (i * W + wave) * kRows;
+      const int j = min(j0 + r0, end - 1);
+      const int n = min(max(end - (j0 + r0), 0), kRows);  // rows that are read
+      const bool there = page[i] >= 0 && page[i] < a.n_pages;
+      const int64_t at = there ? page[i] : 0;
+      const int64_t slot = j - divide(j, a.by_page) * a.page_size;
+      const int r = r0 + in_row;
+      const int ck = Lds<D>::key(r, place) - r * Lds<D>::kRowBytes;  // bytes of a row
+      const int cv = Lds<D>::value(r, place) - r * Lds<D>::kRowBytes;
+      const uint32_t bytes = static_cast<uint32_t>(a.dim) * 2u;
+      const auto offset = [&](int c, const Cache& cache) {
+        return static_cast<uint32_t>(c) < bytes
+                   ? static_cast<uint32_t>(in_row * static_cast<int>(cache.slot) * 2 + c)
+                   : 0xFFFFFFF0u;
+      };
+      const auto extent = [&](const Cache& cache) {
+        return n > 0 ? static_cast<uint32_t>((n - 1) * static_cast<int>(cache.slot)) * 2u + bytes
+                     : 0u;
+      };
+      const uint16_t* k = a.k.data + at * a.k.page + slot * a.k.slot + head * a.k.head;
+      const uint16_t* v = a.v.data + at * a.v.page + slot * a.v.slot + head * a.v.head;
+      const uint32_t to = lds + static_cast<uint32_t>((i * W + wave) * 1024);
+      load_to_lds(there ? make_rsrc(k, extent(a.k)) : make_rsrc(&kNoKeys, 16u),
+                  there ? offset(ck, a.k) : 0u, to);
+      load_to_lds(make_rsrc(v, there ? extent(a.v) : 0u), offset(cv, a.v),
+                  to + ROWS * Lds<D>::kRowBytes);
+    }
+  }
+};
+
 // The steps of a part: [first, last) of those of `keys` positions, and how many
 // parts have any.
 struct Range {
@@ -507,8 +591,9 @@ __device__ __forceinline__ Work work_of(const Args& a) {
 
 constexpr int kKeys = attention::kKeys;
 
-template <int D>
-__global__ __launch_bounds__(kThreads) void paged_attention_many_kernel(const Args a) {
+template <int D, bool DIRECT>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_many_kernel(
+    const Args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ uint32_t shared;
   constexpr int kStage = 2 * kKeys * Lds<D>::kRowBytes;
@@ -536,26 +621,48 @@ __global__ __launch_bounds__(kThreads) void paged_attention_many_kernel(const Ar
   State<D> s;
   clear(s);
   const int32_t* pages = a.pages + t.b * a.pages_ld;
-  Loader<D, kKeys, kNW> loader;
-  const int thread = static_cast<int>(threadIdx.x);
-  if (r.first < r.last) {
-    loader.load(a, pages, w.head, r.first * kKeys, r.end, thread);
-    loader.put(smem, smem + kStage / 2, thread);
-  }
-  for (int i = r.first; i < r.last; ++i) {
-    __syncthreads();
-    const char* k = smem + ((i - r.first) & 1) * kStage;
-    char* next = smem + ((i - r.first + 1) & 1) * kStage;
-    const bool more = i + 1 < r.last;
-    if (more) loader.load(a, pages, w.head, (i + 1) * kKeys, r.end, thread);
+  const auto compute = [&](int i, const char* k) {
     const int j0 = i * kKeys;
-    if (j0 <= any_last && j0 + kKeys > any_low) {
-      if (j0 + kKeys - 1 <= all_last && j0 >= all_low)
-        step<D, kKeys / 32, false>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
-      else
-        step<D, kKeys / 32, true>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
+    if (j0 > any_last || j0 + kKeys <= any_low) return;
+    if (j0 + kKeys - 1 <= all_last && j0 >= all_low)
+      step<D, kKeys / 32, false>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
+    else
+      step<D, kKeys / 32, true>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
+  };
+  if constexpr (DIRECT) {
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
+    Direct<D, kKeys, kNW> loads;
+    if (r.first < r.last) {
+      loads.look_up(a, pages, r.first * kKeys, r.end, wave);
+      loads.load(a, w.head, r.first * kKeys, r.end, wave, lds);
+      loads.look_up(a, pages, min(r.first + 1, r.last - 1) * kKeys, r.end, wave);
     }
-    if (more) loader.put(next, next + kStage / 2, thread);
+    for (int i = r.first; i < r.last; ++i) {
+      const int stage = (i - r.first) & 1;
+      // This step's loads have landed; every wave has read the step before.
+      wait_loads<0>();
+      lds_barrier();
+      if (i + 1 < r.last) {
+        loads.load(a, w.head, (i + 1) * kKeys, r.end, wave, lds + (stage ^ 1) * kStage);
+        loads.look_up(a, pages, min(i + 2, r.last - 1) * kKeys, r.end, wave);
+      }
+      compute(i, smem + stage * kStage);
+    }
+  } else {
+    Loader<D, kKeys, kNW> loader;
+    const int thread = static_cast<int>(threadIdx.x);
+    if (r.first < r.last) {
+      loader.load(a, pages, w.head, r.first * kKeys, r.end, thread);
+      loader.put(smem, smem + kStage / 2, thread);
+    }
+    for (int i = r.first; i < r.last; ++i) {
+      __syncthreads();
+      char* next = smem + ((i - r.first + 1) & 1) * kStage;
+      const bool more = i + 1 < r.last;
+      if (more) loader.load(a, pages, w.head, (i + 1) * kKeys, r.end, thread);
+      compute(i, smem + ((i - r.first) & 1) * kStage);
+      if (more) loader.put(next, next + kStage / 2, thread);
+    }
   }
   s.l += other_half(s.l);
   const int tile = w.tile * a.kv_heads + w.head;
@@ -582,10 +689,12 @@ __device__ __forceinline__ void wave_fence() {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
-// Positions of a wave's step.
+// Positions of a wave's step, and its stages in LDS: two where four waves' fit.
 constexpr int kFewKeys = 32;
-
 template <int D>
+constexpr int kFewStages = D <= 128 ? 2 : 1;
+
+template <int D, bool DIRECT>
 __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(const Args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ uint32_t shared;
@@ -611,21 +720,56 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(const Arg
   State<D> s;
   clear(s);
   const int32_t* pages = a.pages + t.b * a.pages_ld;
-  Loader<D, kFewKeys, 1> loader;
-  char* own = smem + wave * kStage;
-  int i = r.first + wave;
-  if (i < r.last) loader.load(a, pages, w.head, i * kFewKeys, r.end, lane);
-  for (; i < r.last; i += kNW) {
-    loader.put(own, own + kStage / 2, lane);
-    wave_fence();
-    if (i + kNW < r.last)
-      loader.load(a, pages, w.head, (i + kNW) * kFewKeys, r.end, lane);
+  char* own = smem + wave * kFewStages<D> * kStage;
+  const auto compute = [&](int i, const char* k) {
     const int j0 = i * kFewKeys;
     if (j0 + kFewKeys - 1 <= all_last && j0 >= all_low)
-      step<D, kFewKeys / 32, false>(s, q, own, own + kStage / 2, j0, low, last, a.scale_log2);
+      step<D, kFewKeys / 32, false>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
     else
-      step<D, kFewKeys / 32, true>(s, q, own, own + kStage / 2, j0, low, last, a.scale_log2);
-    wave_fence();
+      step<D, kFewKeys / 32, true>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
+  };
+  if constexpr (DIRECT) {
+    const uint32_t lds = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
+        static_cast<int>((uint32_t)(uintptr_t)(lds_ptr_t)own)));
+    Direct<D, kFewKeys, 1> loads;
+    int i = r.first + wave;
+    if (i < r.last) {
+      loads.look_up(a, pages, i * kFewKeys, r.end, 0);
+      loads.load(a, w.head, i * kFewKeys, r.end, 0, lds);
+      loads.look_up(a, pages, min(i + kNW, r.last - 1) * kFewKeys, r.end, 0);
+    }
+    for (int stage = 0; i < r.last; i += kNW) {
+      const bool more = i + kNW < r.last;
+      if (kFewStages<D> == 2 && more) {
+        // The other stage's step was read before this one's wait.
+        wait_reads();
+        loads.load(a, w.head, (i + kNW) * kFewKeys, r.end, 0, lds + (stage ^ 1) * kStage);
+        loads.look_up(a, pages, min(i + 2 * kNW, r.last - 1) * kFewKeys, r.end, 0);
+        wait_loads<2 * Direct<D, kFewKeys, 1>::kPer>();
+      } else {
+        wait_loads<0>();
+      }
+      compute(i, own + stage * kStage);
+      if (kFewStages<D> == 2) {
+        stage ^= 1;
+      } else if (more) {
+        wait_reads();
+        loads.load(a, w.head, (i + kNW) * kFewKeys, r.end, 0, lds);
+        loads.look_up(a, pages, min(i + 2 * kNW, r.last - 1) * kFewKeys, r.end, 0);
+      }
+    }
+  } else {
+    Loader<D, kFewKeys, 1> loader;
+    int i = r.first + wave;
+    if (i < r.last) loader.load(a, pages, w.head, i * kFewKeys, r.end, lane);
+    for (; i < r.last; i += kNW) {
+      loader.put(own, own + kStage / 2, lane);
+      wave_fence();
+      if (i + kNW < r.last)
+        loader.load(a, pages, w.head, (i + kNW) * kFewKeys, r.end, lane);
+      compute(i, own);
+      wave_fence();
+    }
   }
   s.l += other_half(s.l);
   // The waves' results, in their order.
@@ -689,27 +833,37 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(const Arg
 
 // ------------------------------------------------------------------- host --
 
-template <int D>
-int launch(const Args& a, int rows, hipStream_t stream) {
+// A kernel with more dynamic LDS than the default limit: allowed once per process
+// and kernel (the attribute belongs to the kernel, not to a device).
+template <auto KERNEL>
+int launch_with(const Args& a, size_t lds, hipStream_t stream, const char* name) {
+  static const hipError_t err =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+  CREDIT_HIP(err);
   const dim3 grid(static_cast<unsigned>(a.tiles) * static_cast<unsigned>(a.parts) *
                   static_cast<unsigned>(a.kv_heads));
+  KERNEL<<<grid, kThreads, lds, stream>>>(a);
+  return check_launch(name);
+}
+template <int D>
+int launch(const Args& a, int rows, hipStream_t stream) {
+  // Rows of a load in one page, and their offsets within 31 bits.
+  constexpr int kRows = Direct<D, kKeys, kNW>::kRows;
+  const int64_t most = int64_t{1} << 28;
+  const bool direct = a.page_size % kRows == 0 && a.k.slot < most / kRows * 2 &&
+                      a.v.slot < most / kRows * 2;
   if (rows == kFew) {
-    constexpr size_t kBytes =
-        std::max<size_t>(size_t{kNW} * 2 * kFewKeys * Lds<D>::kRowBytes, kNW * 16 * kWave * 4);
-    static const hipError_t err = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(paged_attention_few_kernel<D>),
-        hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBytes));
-    CREDIT_HIP(err);
-    paged_attention_few_kernel<D><<<grid, kThreads, kBytes, stream>>>(a);
-    return check_launch("paged_attention_few_kernel");
+    constexpr const char* kName = "paged_attention_few_kernel";
+    constexpr size_t kBytes = std::max<size_t>(
+        size_t{kNW} * kFewStages<D> * 2 * kFewKeys * Lds<D>::kRowBytes, kNW * 16 * kWave * 4);
+    return direct ? launch_with<paged_attention_few_kernel<D, true>>(a, kBytes, stream, kName)
+                  : launch_with<paged_attention_few_kernel<D, false>>(a, kBytes, stream, kName);
   }
+  constexpr const char* kName = "paged_attention_many_kernel";
   constexpr size_t kBytes = size_t{4} * kKeys * Lds<D>::kRowBytes;
-  static const hipError_t err =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attention_many_kernel<D>),
-                          hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBytes));
-  CREDIT_HIP(err);
-  paged_attention_many_kernel<D><<<grid, kThreads, kBytes, stream>>>(a);
-  return check_launch("paged_attention_many_kernel");
+  return direct ? launch_with<paged_attention_many_kernel<D, true>>(a, kBytes, stream, kName)
+                : launch_with<paged_attention_many_kernel<D, false>>(a, kBytes, stream, kName);
 }
 
 int check_vectors(const Place& p, const char* name) {
