@@ -67,13 +67,14 @@ struct Args {
   uint16_t* out;
   int64_t out_token, out_head;
   float* lse;  // [tokens, heads] or nullptr
-  float* partial;
+  float* partial;      // parts' results, a unit and key head each; nullptr: no parts
   uint32_t* arrived;
   int64_t tokens;
   int batch, heads, kv_heads, group, dim;
   int page_size, n_pages, positions;  // positions: most that a row of pages holds
   Divisor by_page, by_group;
-  int window, parts, tiles;
+  int window, units, tiles;
+  int most_parts, least_steps, share;  // of a tile; of a part; units that all steps are dealt to
   float scale, scale_log2;  // scale, scale log2(e)
 };
 
@@ -89,38 +90,137 @@ struct Tile {
   int rows, row0;
   int kv, ahead;
 };
+// The value of any lane of a wave that all hold one.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 __device__ __forceinline__ int64_t start_of(const Args& a, int b) {
   const int64_t s = a.q_start[b];
   return s < 0 ? 0 : s < a.tokens ? s : a.tokens;
 }
-// False: no rows here.
+__device__ __forceinline__ int rows_of(const Args& a, int b) {
+  const int64_t n = start_of(a, b + 1) - start_of(a, b);
+  return n > 0 ? static_cast<int>(n * a.group) : 0;
+}
+__device__ __forceinline__ int positions_of(const Args& a, int b) {
+  return min(max(a.kv_len[b], 0), a.positions);
+}
+
+// A workgroup's work: part `part` of the tile's, which are `each` steps of its
+// positions; unit0: the number of its part 0 among all units.
+struct Work {
+  Tile t;
+  int head, part, each, unit0;
+};
 template <int ROWS>
-__device__ __forceinline__ bool find_tile(Tile& t, const Args& a, int index) {
+__device__ __forceinline__ void tile_of(Work& w, const Args& a, int b, int tile) {
+  Tile& t = w.t;
+  t.b = uniform(b);
+  t.first = uniform(static_cast<int>(start_of(a, t.b)));
+  t.rows = uniform(rows_of(a, t.b));
+  t.row0 = uniform(tile) * ROWS;
+  t.kv = uniform(positions_of(a, t.b));
+  t.ahead = t.kv - divide(t.rows, a.by_group);
+}
+
+// Without parts: units are the tiles' slots, sequence b's from
+// floor(first row / ROWS) + b on, found by a search.
+template <int ROWS>
+__device__ __forceinline__ bool find_tile(Work& w, const Args& a, int unit) {
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   int lo = 0, n = a.batch;
   while (n > 1) {
     const int step = (n + kWave - 1) / kWave;
     const int b = lo + lane * step;
-    const bool at = lane * step < n &&
-                    start_of(a, b) * a.group / ROWS + b <= static_cast<int64_t>(index);
+    const bool at =
+        lane * step < n && start_of(a, b) * a.group / ROWS + b <= static_cast<int64_t>(unit);
     const int count = __builtin_popcountll(__builtin_amdgcn_ballot_w64(at));
     if (count == 0) return false;
     const int skip = (count - 1) * step;
     lo += skip;
     n = min(step, n - skip);
   }
-  t.b = __builtin_amdgcn_readfirstlane(lo);
-  t.first = start_of(a, t.b);
-  const int64_t slot = t.first * a.group / ROWS + t.b;
-  const int64_t rows = (start_of(a, t.b + 1) - t.first) * a.group;
-  const int64_t row0 = (index - slot) * ROWS;
-  if (row0 < 0 || row0 >= rows) return false;
-  t.rows = static_cast<int>(rows);
-  t.row0 = static_cast<int>(row0);
-  const int kv = a.kv_len[t.b];
-  t.kv = kv < 0 ? 0 : kv < a.positions ? kv : a.positions;
-  t.ahead = t.kv - t.rows / a.group;
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  const int64_t slot = start_of(a, lo) * a.group / ROWS + lo;
+  if (unit < slot) return false;
+  const int64_t row0 = (unit - slot) * ROWS;
+  if (row0 >= rows_of(a, lo)) return false;
+  tile_of<ROWS>(w, a, lo, static_cast<int>(unit - slot));
+  w.part = 0;
+  w.each = 1 << 30;
+  w.unit0 = unit;
   return true;
+}
+
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) v = max(v, __shfl_xor(v, d));
+  return v;
+}
+// With parts: all sequences' steps are dealt to about a.share units of one length,
+// so that sequences of unlike lengths keep the device busy alike; each wave counts
+// them through and finds its unit.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ bool find_part(Work& w, const Args& a, int unit) {
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  const auto tiles_of = [&](int b) {
+    return b < a.batch ? (rows_of(a, b) + ROWS - 1) / ROWS : 0;
+  };
+  const auto steps_of = [&](int b) {
+    if (b >= a.batch) return 0;
+    const int kv = positions_of(a, b);
+    if (a.window == 0) return (kv + KEYS - 1) / KEYS;
+    const int64_t seen = static_cast<int64_t>(a.window) + divide(rows_of(a, b), a.by_group);
+    return static_cast<int>(min(static_cast<int64_t>(kv), seen) + KEYS - 1) / KEYS + 1;
+  };
+  double total = 0.0, all = 0.0;
+  int longest = 0;
+  for (int b = lane; b - lane < a.batch; b += kWave) {
+    const int tiles = tiles_of(b), steps = steps_of(b);
+    all += tiles;
+    total += static_cast<double>(tiles) * steps;
+    if (tiles > 0) longest = max(longest, steps);
+  }
+  // More tiles than the rows make: q_start does not rise.  Nothing is done.
+  if (wave_reduce_sum_f64(all) > a.tiles) return false;
+  total = wave_reduce_sum_f64(total);
+  longest = wave_max(longest);
+  w.each = uniform(max(max(a.least_steps, static_cast<int>(total / a.share) + 1),
+                       (longest + a.most_parts - 1) / a.most_parts));
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kWave) {
+    const int b = b0 + lane;
+    const int tiles = tiles_of(b);
+    const int parts = max(1, (steps_of(b) + w.each - 1) / w.each);
+    int upto = tiles * parts;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+      const int v = __shfl_up(upto, d);
+      if (lane >= d) upto += v;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(unit < before + upto);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      const int p = __builtin_amdgcn_readlane(parts, at);
+      const int first = uniform(before + __builtin_amdgcn_readlane(upto - tiles * parts, at));
+      const int tile = (unit - first) / p;
+      tile_of<ROWS>(w, a, b0 + at, tile);
+      w.part = uniform(unit - first - tile * p);
+      w.unit0 = unit - w.part;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, kWave - 1);
+  }
+  return false;
+}
+// Key heads next to each other: the dies take workgroups in turn, so that tiles of
+// one head's keys tend to share one die's L2.  Later tiles, which see more, first.
+// False: no work here.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ bool find_work(Work& w, const Args& a) {
+  const int i = static_cast<int>(blockIdx.x);
+  w.head = i % a.kv_heads;
+  const int unit = a.units - 1 - i / a.kv_heads;
+  return a.partial != nullptr ? find_part<ROWS, KEYS>(w, a, unit) : find_tile<ROWS>(w, a, unit);
 }
 
 // Layout of a step's keys and values in LDS: rows of D elements, 16-byte chunk c
@@ -322,84 +422,109 @@ __device__ __forceinline__ void step(State<D>& s, const bf16x8_t (&q)[D / 16], c
   }
 }
 
-// The rows' outputs from o, l (of all lanes' halves) and m.
-template <int D>
-__device__ __forceinline__ void finish(const State<D>& s, const Args& a, const Tile& t, int row,
-                                       int kv_head, int from, int to) {
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  if (row >= t.rows) return;
+__device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+// l = 0: nothing was seen.
+__device__ __forceinline__ float lse_of(const Args& a, float m, float l) {
+  return l == 0.0f ? kNegInf : base_of(m) * a.scale + logf(l);
+}
+// What scales a wave's or part's results to the maximum m of all (nothing seen: its
+// sums are 0, or NaN).
+__device__ __forceinline__ float weight_of(const Args& a, float own, float m) {
+  return own == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((own - base_of(m)) * a.scale_log2);
+}
+// Head and token of a row; its place in an array of rows.
+struct Row {
+  int64_t token;
+  int head;
+};
+__device__ __forceinline__ Row row_of(const Args& a, const Work& w, int row) {
   const int token = divide(row, a.by_group);
-  const int head = kv_head * a.group + row - token * a.group;
-  const float inv = s.l == 0.0f ? 0.0f : 1.0f / s.l;
-  uint16_t* p = a.out + (t.first + token) * a.out_token + head * a.out_head;
+  return {w.t.first + token, w.head * a.group + row - token * a.group};
+}
+
+// A wave's rows, finished.
+template <int D>
+__device__ __forceinline__ void finish(const State<D>& s, const Args& a, const Work& w, int row) {
+  const int lane = opaque_lane();
+  if (row >= w.t.rows) return;
+  const Row r = row_of(a, w, row);
+  const float inv = inverse_of(s.l);
+  uint16_t* p = a.out + r.token * a.out_token + r.head * a.out_head;
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db) {
-    if (db < from || db >= to) continue;
+  for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int d = 32 * db + 8 * i + 4 * (lane >> 5);
-      // l = 0: nothing was seen and o is 0.
       const uint32_t lo = pack_bf16x2(s.o[db][4 * i] * inv, s.o[db][4 * i + 1] * inv);
       const uint32_t hi = pack_bf16x2(s.o[db][4 * i + 2] * inv, s.o[db][4 * i + 3] * inv);
       if (d < a.dim)
         *reinterpret_cast<uint64_t*>(p + d) = lo | static_cast<uint64_t>(hi) << 32;
     }
-  }
-  if (a.lse != nullptr && lane < 32 && from == 0)
-    a.lse[(t.first + token) * a.heads + head] =
-        s.l == 0.0f ? kNegInf : base_of(s.m) * a.scale + logf(s.l);
+  if (a.lse != nullptr && lane < 32) a.lse[r.token * a.heads + r.head] = lse_of(a, s.m, s.l);
 }
 
-// A part's results in the workspace: per 32 rows, o in the order of its lanes, then
-// m and l.
-template <int D>
-__device__ __forceinline__ float* part_at(const Args& a, int tile, int part, int block, int rows) {
-  return a.partial + ((static_cast<int64_t>(tile) * a.parts + part) * rows + block * 32) *
-                         (D + 2);
+// A part's results in the workspace: ROWS rows of D outputs, then the rows' maxima
+// and sums.
+template <int D, int ROWS>
+__device__ __forceinline__ float* part_at(const Args& a, const Work& w, int part) {
+  return a.partial + (static_cast<int64_t>(w.unit0 + part) * a.kv_heads + w.head) * ROWS * (D + 2);
 }
-template <int D>
-__device__ __forceinline__ void leave(float* at, const State<D>& s, int db) {
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2_t v = {s.o[db][2 * i], s.o[db][2 * i + 1]};
-    publish(reinterpret_cast<double*>(at) + (db * 8 + i) * kWave + lane,
-            __builtin_bit_cast(double, v));
-  }
+// Stores and loads of a part's results at device scope (sc1: past the die's own
+// L2), 16 bytes each; `part`: its resource.
+constexpr int kDeviceScope = 16;
+__device__ __forceinline__ void publish_quad(buffer_rsrc_t part, int at, f32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, at * 4, 0,
+                                         kDeviceScope);
 }
-// All of the tile's parts joined: those of the 32 rows at block, column blocks
-// from .. to.
-template <int D>
-__device__ __forceinline__ void join(State<D>& s, const Args& a, int tile, int parts, int block,
-                                     int rows, int from, int to) {
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  clear(s);
-  for (int part = 0; part < parts; ++part) {
-    const float* at = part_at<D>(a, tile, part, block, rows);
-    const float m = fetch(at + 32 * D + (lane & 31));
-    s.m = fmaxf(s.m, m);
+__device__ __forceinline__ f32x4 fetch_quad(buffer_rsrc_t part, int at) {
+  return __builtin_bit_cast(
+      f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, at * 4, 0, kDeviceScope));
+}
+template <int D, int ROWS>
+__device__ __forceinline__ buffer_rsrc_t part_rsrc(float* at) {
+  return make_rsrc(at, ROWS * (D + 2) * sizeof(float));
+}
+
+// All parts of a tile joined by its workgroup, in their order: the rows' maxima and
+// sums by way of LDS, then four columns a thread, eight parts at a time.
+template <int D, int ROWS>
+__device__ __forceinline__ void join(const Args& a, const Work& w, int parts, char* smem) {
+  float* weight = reinterpret_cast<float*>(smem);  // [parts + 1][ROWS]
+  float* sum = weight + (parts + 1) * ROWS;        // [parts][ROWS]
+  const int thread = static_cast<int>(threadIdx.x);
+  const int rows = min(ROWS, w.t.rows - w.t.row0);
+#pragma unroll 4
+  for (int i = thread; i < parts * ROWS; i += kThreads) {
+    const float* at = part_at<D, ROWS>(a, w, i / ROWS) + ROWS * D + i % ROWS;
+    weight[i] = fetch(at);
+    sum[i] = fetch(at + ROWS);
   }
-  const float base = base_of(s.m);
-  for (int part = 0; part < parts; ++part) {
-    const float* at = part_at<D>(a, tile, part, block, rows);
-    const float m = fetch(at + 32 * D + (lane & 31));
-    const float l = fetch(at + 32 * D + 32 + (lane & 31));
-    // A part that saw nothing has m = -inf and l = 0.
-    const float w = m == kNegInf ? 0.0f
-                                 : __builtin_amdgcn_exp2f((m - base) * a.scale_log2);
-    s.l += m == kNegInf ? l : l * w;
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db) {
-      if (db < from || db >= to) continue;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2_t v = __builtin_bit_cast(
-            float2_t,
-            fetch(reinterpret_cast<const double*>(at) + (db * 8 + i) * kWave + lane));
-        s.o[db][2 * i] += m == kNegInf ? v.x : v.x * w;
-        s.o[db][2 * i + 1] += m == kNegInf ? v.y : v.y * w;
-      }
+  __syncthreads();
+  if (thread < rows) {
+    float m = kNegInf, l = 0.0f;
+    for (int p = 0; p < parts; ++p) m = fmaxf(m, weight[p * ROWS + thread]);
+    for (int p = 0; p < parts; ++p) {
+      const float f = weight_of(a, weight[p * ROWS + thread], m);
+      l += f * sum[p * ROWS + thread];
+      weight[p * ROWS + thread] = f;
     }
+    const Row r = row_of(a, w, w.t.row0 + thread);
+    if (a.lse != nullptr) a.lse[r.token * a.heads + r.head] = lse_of(a, m, l);
+    weight[parts * ROWS + thread] = inverse_of(l);
+  }
+  __syncthreads();
+  for (int i = thread; i < rows * (D / 4); i += kThreads) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    if (d >= a.dim) continue;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p)
+      o += fetch_quad(part_rsrc<D, ROWS>(part_at<D, ROWS>(a, w, p)), row * D + d) *
+           weight[p * ROWS + row];
+    o *= weight[parts * ROWS + row];
+    const Row r = row_of(a, w, w.t.row0 + row);
+    *reinterpret_cast<uint64_t*>(a.out + r.token * a.out_token + r.head * a.out_head + d) =
+        pack_bf16x2(o[0], o[1]) | static_cast<uint64_t>(pack_bf16x2(o[2], o[3])) << 32;
   }
 }
 
@@ -449,19 +574,20 @@ struct Loader {
 };
 
 // One LDS-direct load: 16 bytes a lane from offset `off` of the resource to LDS at
-// `lds` + 16 lane.  In inline assembly, as the compiler would wait for every such
-// load before any read of LDS; the waits are those written below.  s_nop covers
+// `lds` + AT + 16 lane.  In inline assembly, as the compiler would wait for every
+// such load before any read of LDS; the waits are those written below.  s_nop covers
 // the write of M0, which nothing else here reads.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+template <uint32_t AT>
 __device__ __forceinline__ void load_to_lds(buffer_rsrc_t rsrc, uint32_t off, uint32_t lds) {
   asm volatile(
-      "s_mov_b32 m0, %2\n\t"
+      "s_add_u32 m0, %2, %3\n\t"
       "s_nop 0\n\t"
       "buffer_load_dwordx4 %0, %1, 0 offen lds"
       :
-      : "v"(off), "s"(rsrc), "s"(lds)
-      : "memory", "m0");
+      : "v"(off), "s"(rsrc), "s"(lds), "i"(AT)
+      : "memory", "m0", "scc");
 }
 #pragma clang diagnostic pop
 // s_waitcnt vmcnt(N), the other counters at their maxima.
@@ -483,83 +609,111 @@ __device__ const u32x4 kNoKeys = {0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07
 
 typedef const __attribute__((address_space(4))) int32_t* scalar_i32_t;
 
-// The same step without registers, where the kRows rows of a wave's load lie in one
-// page (page_size a multiple of kRows): its address is uniform, and rows behind
-// `end`, or of a page that is not there, are out of the resource's bounds, which
-// makes them 0.
-template <int D, int ROWS, int W>
+// fn(integral_constant 0 .. N - 1).
+template <int N, int I = 0, class Fn>
+__device__ __forceinline__ void unrolled(Fn&& fn) {
+  if constexpr (I < N) {
+    fn(std::integral_constant<int, I>{});
+    unrolled<N, I + 1>(fn);
+  }
+}
+
+// The same step without registers, where whole pieces of PIECE rows lie in one page
+// (page_size a multiple of PIECE): a piece's address is uniform, and rows behind
+// `end`, or of a page that is not there, are out of its resource's bounds, which
+// makes them 0.  A wave loads ROWS / W consecutive rows.
+template <int D, int ROWS, int W, int PIECE>
 struct Direct {
   static constexpr int kRows = kWave / Lds<D>::kChunks;  // of a load
-  static constexpr int kPer = ROWS / kRows / W;          // loads a wave, of keys or values
-  int page[kPer];
+  static constexpr int kMine = ROWS / W;                 // of a wave
+  static constexpr int kPieces = kMine / PIECE;
+  static constexpr int kLoads = PIECE / kRows;  // of a piece, of keys or values
+  static constexpr int kPer = kMine / kRows;    // of a step, of keys or values
+  // Loads apart whose rows swizzle alike.
+  static constexpr int kTurn = kPer < 16 / kRows ? kPer : 16 / kRows;
+  int page[kPieces];
+  uint32_t k_off[kTurn], v_off[kTurn];
 
+  // Byte offsets of the lanes' loads within a piece: row and the chunk that lands
+  // at the lane's place.
+  __device__ __forceinline__ void init(const Args& a, int wave) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int in_row = lane / Lds<D>::kChunks, place = lane % Lds<D>::kChunks;
+    const uint32_t bytes = static_cast<uint32_t>(a.dim) * 2u;
+#pragma unroll
+    for (int i = 0; i < kTurn; ++i) {
+      const int r = wave * kMine + i * kRows + in_row;
+      const uint32_t ck = Lds<D>::key(r, place) - r * Lds<D>::kRowBytes;
+      const uint32_t cv = Lds<D>::value(r, place) - r * Lds<D>::kRowBytes;
+      const uint32_t row = static_cast<uint32_t>(i % kLoads * kRows + in_row) * 2u;
+      k_off[i] = ck < bytes ? row * static_cast<uint32_t>(a.k.slot) + ck : 0xFFFFFFF0u;
+      v_off[i] = cv < bytes ? row * static_cast<uint32_t>(a.v.slot) + cv : 0xFFFFFFF0u;
+    }
+  }
   // The pages of the step at j0, ahead of its loads.
   __device__ __forceinline__ void look_up(const Args& a, const int32_t* pages, int j0, int end,
                                           int wave) {
     const scalar_i32_t table = (scalar_i32_t)(reinterpret_cast<uintptr_t>(pages));
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      page[i] = table[divide(min(j0 + (i * W + wave) * kRows, end - 1), a.by_page)];
+    for (int i = 0; i < kPieces; ++i)
+      page[i] = table[divide(min(j0 + wave * kMine + i * PIECE, end - 1), a.by_page)];
   }
+  // lds: of the wave's first row of keys.
   __device__ __forceinline__ void load(const Args& a, int head, int j0, int end, int wave,
                                        uint32_t lds) const {
-    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-    const int in_row = lane / Lds<D>::kChunks, place = lane % Lds<D>::kChunks;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int r0 = (i * W + wave) * kRows;
-      const int j = min(j0 + r0, end - 1);
-      const int n = min(max(end - (j0 + r0), 0), kRows);  // rows that are read
+    unrolled<kPieces>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      const int j = j0 + wave * kMine + i * PIECE;
+      const int n = min(max(end - j, 0), PIECE);  // rows that are read
       const bool there = page[i] >= 0 && page[i] < a.n_pages;
       const int64_t at = there ? page[i] : 0;
-      const int64_t slot = j - divide(j, a.by_page) * a.page_size;
-      const int r = r0 + in_row;
-      const int ck = Lds<D>::key(r, place) - r * Lds<D>::kRowBytes;  // bytes of a row
-      const int cv = Lds<D>::value(r, place) - r * Lds<D>::kRowBytes;
-      const uint32_t bytes = static_cast<uint32_t>(a.dim) * 2u;
-      const auto offset = [&](int c, const Cache& cache) {
-        return static_cast<uint32_t>(c) < bytes
-                   ? static_cast<uint32_t>(in_row * static_cast<int>(cache.slot) * 2 + c)
-                   : 0xFFFFFFF0u;
-      };
-      const auto extent = [&](const Cache& cache) {
-        return n > 0 ? static_cast<uint32_t>((n - 1) * static_cast<int>(cache.slot)) * 2u + bytes
+      const int in_page = j - divide(j, a.by_page) * a.page_size;
+      const auto extent = [&](const Cache& c) {
+        return n > 0 ? static_cast<uint32_t>(n - 1) * static_cast<uint32_t>(c.slot) * 2u +
+                           static_cast<uint32_t>(a.dim) * 2u
                      : 0u;
       };
-      const uint16_t* k = a.k.data + at * a.k.page + slot * a.k.slot + head * a.k.head;
-      const uint16_t* v = a.v.data + at * a.v.page + slot * a.v.slot + head * a.v.head;
-      const uint32_t to = lds + static_cast<uint32_t>((i * W + wave) * 1024);
-      load_to_lds(there ? make_rsrc(k, extent(a.k)) : make_rsrc(&kNoKeys, 16u),
-                  there ? offset(ck, a.k) : 0u, to);
-      load_to_lds(make_rsrc(v, there ? extent(a.v) : 0u), offset(cv, a.v),
-                  to + ROWS * Lds<D>::kRowBytes);
-    }
+      const auto first = [&](const Cache& c) {
+        return c.data + at * c.page + static_cast<int64_t>(in_page) * c.slot + head * c.head;
+      };
+      const buffer_rsrc_t k = make_rsrc(there ? static_cast<const void*>(first(a.k)) : &kNoKeys,
+                                        there ? extent(a.k) : 16u);
+      const buffer_rsrc_t v = make_rsrc(first(a.v), there ? extent(a.v) : 0u);
+      unrolled<kLoads>([&](auto lc) {
+        constexpr int l = i * kLoads + decltype(lc)::value;
+        constexpr uint32_t kAt = l * 1024;
+        load_to_lds<kAt>(k, there ? k_off[l % kTurn] : 0u, lds);
+        load_to_lds<kAt + ROWS * Lds<D>::kRowBytes>(v, v_off[l % kTurn], lds);
+      });
+    });
   }
 };
 
 // The steps of a part: [first, last) of those of `keys` positions, and how many
-// parts have any.
+// parts the tile has.
 struct Range {
   int first, last, parts;
   int end;  // positions that any row sees end here
 };
-__device__ __forceinline__ Range range_of(const Args& a, const Tile& t, int rows, int part,
-                                          int keys) {
-  const int last_row = min(t.row0 + rows, t.rows) - 1;
-  const int last = t.ahead + divide(last_row, a.by_group);
+__device__ __forceinline__ Range range_of(const Args& a, const Work& w, int rows, int keys) {
+  const Tile& t = w.t;
+  const int last = t.ahead + divide(min(t.row0 + rows, t.rows) - 1, a.by_group);
   int low = 0;
   if (a.window > 0) low = max(0, t.ahead + divide(t.row0, a.by_group) - a.window + 1);
   Range r;
   r.end = last + 1;
   const int from = low / keys, to = last < 0 ? 0 : last / keys + 1;
   const int n = max(0, to - from);
-  const int each = max(1, (n + a.parts - 1) / a.parts);
-  r.parts = max(1, (n + each - 1) / each);
-  r.first = from + part * each;
-  r.last = min(to, r.first + each);
+  r.parts = max(1, (n + w.each - 1) / w.each);
+  r.first = from + w.part * w.each;
+  r.last = min(to, r.first + min(w.each, n));
   return r;
 }
 
+__device__ __forceinline__ uint32_t* counter_of(const Args& a, const Work& w) {
+  return a.arrived +
+         (static_cast<int64_t>(w.unit0) * a.kv_heads + w.head) * kGroupCounterStride;
+}
 // Whether this workgroup is the last of the tile's parts; its own results are
 // published.
 __device__ __forceinline__ bool last_of(uint32_t* counter, int parts, uint32_t* shared) {
@@ -574,33 +728,18 @@ __device__ __forceinline__ bool last_of(uint32_t* counter, int parts, uint32_t* 
   return *shared + 1 == static_cast<uint32_t>(parts);
 }
 
-struct Work {
-  int tile, part, head;
-};
-// Key heads next to each other: the dies take workgroups in turn, so that tiles of
-// one head's keys tend to share one die's L2.  Later tiles, which see more, first.
-__device__ __forceinline__ Work work_of(const Args& a) {
-  const int i = static_cast<int>(blockIdx.x);
-  Work w;
-  w.head = i % a.kv_heads;
-  const int j = i / a.kv_heads;
-  w.part = j % a.parts;
-  w.tile = a.tiles - 1 - j / a.parts;
-  return w;
-}
-
 constexpr int kKeys = attention::kKeys;
 
-template <int D, bool DIRECT>
+template <int D, int PIECE>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_many_kernel(
     const Args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ uint32_t shared;
   constexpr int kStage = 2 * kKeys * Lds<D>::kRowBytes;
-  const Work w = work_of(a);
-  Tile t;
-  if (!find_tile<kMany>(t, a, w.tile)) return;
-  const Range r = range_of(a, t, kMany, w.part, kKeys);
+  Work w;
+  if (!find_work<kMany, kKeys>(w, a)) return;
+  const Tile& t = w.t;
+  const Range r = range_of(a, w, kMany, kKeys);
   if (w.part >= r.parts) return;
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
@@ -629,9 +768,12 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_ma
     else
       step<D, kKeys / 32, true>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
   };
-  if constexpr (DIRECT) {
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
-    Direct<D, kKeys, kNW> loads;
+  if constexpr (PIECE > 0) {
+    const uint32_t lds = static_cast<uint32_t>(
+        uniform(static_cast<int>((uint32_t)(uintptr_t)(lds_ptr_t)smem) +
+                wave * (kKeys / kNW) * Lds<D>::kRowBytes));
+    Direct<D, kKeys, kNW, PIECE> loads;
+    loads.init(a, wave);
     if (r.first < r.last) {
       loads.look_up(a, pages, r.first * kKeys, r.end, wave);
       loads.load(a, w.head, r.first * kKeys, r.end, wave, lds);
@@ -665,20 +807,28 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_ma
     }
   }
   s.l += other_half(s.l);
-  const int tile = w.tile * a.kv_heads + w.head;
-  if (r.parts > 1) {
-    float* at = part_at<D>(a, tile, w.part, wave, kMany);
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db) leave(at, s, db);
-    if (lane < 32) {
-      publish(at + 32 * D + lane, s.m);
-      publish(at + 32 * D + 32 + lane, s.l);
-    }
-    if (!last_of(a.arrived + static_cast<int64_t>(tile) * kGroupCounterStride, r.parts, &shared))
-      return;
-    join(s, a, tile, r.parts, wave, kMany, 0, D / 32);
+  if (r.parts == 1) {
+    finish(s, a, w, row);
+    return;
   }
-  finish(s, a, t, row, w.head, 0, D / 32);
+  float* at = part_at<D, kMany>(a, w, w.part);
+  const buffer_rsrc_t part = part_rsrc<D, kMany>(at);
+  const int in_tile = 32 * wave + (lane & 31);
+  if (row < t.rows) {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        publish_quad(part, in_tile * D + 32 * db + 8 * i + 4 * (lane >> 5),
+                     f32x4{s.o[db][4 * i], s.o[db][4 * i + 1], s.o[db][4 * i + 2],
+                           s.o[db][4 * i + 3]});
+  }
+  if (lane < 32) {
+    publish(at + kMany * D + in_tile, s.m);
+    publish(at + kMany * (D + 1) + in_tile, s.l);
+  }
+  if (last_of(counter_of(a, w), r.parts, &shared))
+    join<D, kMany>(a, w, r.parts, smem);
 }
 
 // A wave's LDS operations run in order; this keeps the compiler to it where lanes
@@ -690,20 +840,20 @@ __device__ __forceinline__ void wave_fence() {
 }
 
 // Positions of a wave's step, and its stages in LDS: two where four waves' fit.
-constexpr int kFewKeys = 32;
+using attention::kFewKeys;
 template <int D>
 constexpr int kFewStages = D <= 128 ? 2 : 1;
 
-template <int D, bool DIRECT>
+template <int D, int PIECE>
 __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(const Args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ uint32_t shared;
-  __shared__ float ms[kNW][32], ls[kNW][32];
+  __shared__ float ms[kNW][kFew], ls[kNW][kFew];
   constexpr int kStage = 2 * kFewKeys * Lds<D>::kRowBytes;
-  const Work w = work_of(a);
-  Tile t;
-  if (!find_tile<kFew>(t, a, w.tile)) return;
-  const Range r = range_of(a, t, kFew, w.part, kFewKeys);
+  Work w;
+  if (!find_work<kFew, kFewKeys>(w, a)) return;
+  const Tile& t = w.t;
+  const Range r = range_of(a, w, kFew, kFewKeys);
   if (w.part >= r.parts) return;
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
@@ -728,10 +878,11 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(const Arg
     else
       step<D, kFewKeys / 32, true>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
   };
-  if constexpr (DIRECT) {
+  if constexpr (PIECE > 0) {
     const uint32_t lds = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
         static_cast<int>((uint32_t)(uintptr_t)(lds_ptr_t)own)));
-    Direct<D, kFewKeys, 1> loads;
+    Direct<D, kFewKeys, 1, PIECE> loads;
+    loads.init(a, 0);
     int i = r.first + wave;
     if (i < r.last) {
       loads.look_up(a, pages, i * kFewKeys, r.end, 0);
@@ -745,7 +896,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(const Arg
         wait_reads();
         loads.load(a, w.head, (i + kNW) * kFewKeys, r.end, 0, lds + (stage ^ 1) * kStage);
         loads.look_up(a, pages, min(i + 2 * kNW, r.last - 1) * kFewKeys, r.end, 0);
-        wait_loads<2 * Direct<D, kFewKeys, 1>::kPer>();
+        wait_loads<2 * Direct<D, kFewKeys, 1, PIECE>::kPer>();
       } else {
         wait_loads<0>();
       }
@@ -772,63 +923,72 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(const Arg
     }
   }
   s.l += other_half(s.l);
-  // The waves' results, in their order.
+  // The waves' results, added in their order: rows of D and four more floats, which
+  // spreads a column of rows over the banks.
+  constexpr int kPitch = D + 4;
+  float* sums = reinterpret_cast<float*>(smem);  // [waves][kFew][kPitch]
   if (lane < 32) {
     ms[wave][lane] = s.m;
     ls[wave][lane] = s.l;
   }
   __syncthreads();
-  float m = kNegInf, l = 0.0f;
+  float m = kNegInf;
 #pragma unroll
   for (int v = 0; v < kNW; ++v) m = fmaxf(m, ms[v][lane & 31]);
-  const float base = base_of(m);
-#pragma unroll
-  for (int v = 0; v < kNW; ++v) {
-    const float mv = ms[v][lane & 31];
-    l += mv == kNegInf ? ls[v][lane & 31]
-                       : ls[v][lane & 31] * __builtin_amdgcn_exp2f((mv - base) * a.scale_log2);
-  }
-  const float factor = s.m == kNegInf ? 1.0f
-                                      : __builtin_amdgcn_exp2f((s.m - base) * a.scale_log2);
-  float* sums = reinterpret_cast<float*>(smem);  // [waves][16][64] of one column block
-  s.m = m;
-  s.l = l;
-#pragma unroll
-  for (int db = 0; db < D / 32; ++db) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) sums[(wave * 16 + e) * kWave + lane] = s.o[db][e] * factor;
-    __syncthreads();
-    if (db % kNW == wave) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float v = 0.0f;
-#pragma unroll
-        for (int n = 0; n < kNW; ++n) v += sums[(n * 16 + e) * kWave + lane];
-        s.o[db][e] = v;
-      }
-    }
-    __syncthreads();
-  }
-  const int tile = w.tile * a.kv_heads + w.head;
-  const bool parted = r.parts > 1;
-  if (parted) {
-    float* at = part_at<D>(a, tile, w.part, 0, kFew);
+  const float factor = weight_of(a, s.m, m);
+  if (row < t.rows) {
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
-      if (db % kNW == wave) leave(at, s, db);
-    if (wave == 0 && lane < 32) {
-      publish(at + 32 * D + lane, s.m);
-      publish(at + 32 * D + 32 + lane, s.l);
-    }
-    if (!last_of(a.arrived + static_cast<int64_t>(tile) * kGroupCounterStride, r.parts, &shared))
-      return;
-  }
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-    if (db % kNW == wave) {
-      if (parted) join(s, a, tile, r.parts, 0, kFew, db, db + 1);
-      finish(s, a, t, row, w.head, db, db + 1);
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(sums + (wave * kFew + (lane & 31)) * kPitch + 32 * db + 8 * i +
+                                  4 * (lane >> 5)) =
+            f32x4{s.o[db][4 * i], s.o[db][4 * i + 1], s.o[db][4 * i + 2], s.o[db][4 * i + 3]} *
+            factor;
+  }
+  __syncthreads();
+  const int rows = min(kFew, t.rows - t.row0);
+  const bool parted = r.parts > 1;
+  float* at = parted ? part_at<D, kFew>(a, w, w.part) : nullptr;
+  const auto sum_of = [&](int in_tile, float& most) {
+    most = kNegInf;
+#pragma unroll
+    for (int v = 0; v < kNW; ++v) most = fmaxf(most, ms[v][in_tile]);
+    float l = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kNW; ++v) l += ls[v][in_tile] * weight_of(a, ms[v][in_tile], most);
+    return l;
+  };
+  for (int i = static_cast<int>(threadIdx.x); i < rows * (D / 4); i += kThreads) {
+    const int in_tile = i / (D / 4), d = i % (D / 4) * 4;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < kNW; ++n)
+      v += *reinterpret_cast<const f32x4*>(sums + (n * kFew + in_tile) * kPitch + d);
+    if (parted) {
+      publish_quad(part_rsrc<D, kFew>(at), in_tile * D + d, v);
+    } else if (d < a.dim) {
+      float most;
+      v *= inverse_of(sum_of(in_tile, most));
+      const Row r0 = row_of(a, w, t.row0 + in_tile);
+      *reinterpret_cast<uint64_t*>(a.out + r0.token * a.out_token + r0.head * a.out_head + d) =
+          pack_bf16x2(v[0], v[1]) | static_cast<uint64_t>(pack_bf16x2(v[2], v[3])) << 32;
     }
+  }
+  if (static_cast<int>(threadIdx.x) < kFew) {
+    const int in_tile = static_cast<int>(threadIdx.x);
+    float most;
+    const float l = sum_of(in_tile, most);
+    if (parted) {
+      publish(at + kFew * D + in_tile, most);
+      publish(at + kFew * (D + 1) + in_tile, l);
+    } else if (in_tile < rows && a.lse != nullptr) {
+      const Row r0 = row_of(a, w, t.row0 + in_tile);
+      a.lse[r0.token * a.heads + r0.head] = lse_of(a, most, l);
+    }
+  }
+  if (parted && last_of(counter_of(a, w), r.parts, &shared))
+    join<D, kFew>(a, w, r.parts, smem);
 }
 
 // ------------------------------------------------------------------- host --
@@ -841,29 +1001,35 @@ int launch_with(const Args& a, size_t lds, hipStream_t stream, const char* name)
       hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL),
                           hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
   CREDIT_HIP(err);
-  const dim3 grid(static_cast<unsigned>(a.tiles) * static_cast<unsigned>(a.parts) *
-                  static_cast<unsigned>(a.kv_heads));
+  const dim3 grid(static_cast<unsigned>(a.units) * static_cast<unsigned>(a.kv_heads));
   KERNEL<<<grid, kThreads, lds, stream>>>(a);
   return check_launch(name);
 }
 template <int D>
 int launch(const Args& a, int rows, hipStream_t stream) {
-  // Rows of a load in one page, and their offsets within 31 bits.
-  constexpr int kRows = Direct<D, kKeys, kNW>::kRows;
-  const int64_t most = int64_t{1} << 28;
-  const bool direct = a.page_size % kRows == 0 && a.k.slot < most / kRows * 2 &&
-                      a.v.slot < most / kRows * 2;
-  if (rows == kFew) {
-    constexpr const char* kName = "paged_attention_few_kernel";
-    constexpr size_t kBytes = std::max<size_t>(
-        size_t{kNW} * kFewStages<D> * 2 * kFewKeys * Lds<D>::kRowBytes, kNW * 16 * kWave * 4);
-    return direct ? launch_with<paged_attention_few_kernel<D, true>>(a, kBytes, stream, kName)
-                  : launch_with<paged_attention_few_kernel<D, false>>(a, kBytes, stream, kName);
-  }
-  constexpr const char* kName = "paged_attention_many_kernel";
-  constexpr size_t kBytes = size_t{4} * kKeys * Lds<D>::kRowBytes;
-  return direct ? launch_with<paged_attention_many_kernel<D, true>>(a, kBytes, stream, kName)
-                : launch_with<paged_attention_many_kernel<D, false>>(a, kBytes, stream, kName);
+  // Pieces of 16 rows, of a load's, or through registers where pages hold no whole
+  // number of them or a piece's offsets pass 31 bits.
+  constexpr int kRows = Direct<D, kKeys, kNW, 16>::kRows;
+  constexpr int64_t kMost = int64_t{1} << 25;
+  const bool near = a.k.slot < kMost && a.v.slot < kMost;
+  const auto choose = [&](auto&& with) {
+    if (near && a.page_size % 16 == 0) return with(std::integral_constant<int, 16>{});
+    if (near && a.page_size % kRows == 0) return with(std::integral_constant<int, kRows>{});
+    return with(std::integral_constant<int, 0>{});
+  };
+  if (rows == kFew)
+    return choose([&](auto piece) {
+      constexpr size_t kBytes = std::max<size_t>(
+          size_t{kNW} * kFewStages<D> * 2 * kFewKeys * Lds<D>::kRowBytes,
+          size_t{kNW} * kFew * (D + 4) * sizeof(float));
+      return launch_with<paged_attention_few_kernel<D, decltype(piece)::value>>(
+          a, kBytes, stream, "paged_attention_few_kernel");
+    });
+  return choose([&](auto piece) {
+    constexpr size_t kBytes = size_t{4} * kKeys * Lds<D>::kRowBytes;
+    return launch_with<paged_attention_many_kernel<D, decltype(piece)::value>>(
+        a, kBytes, stream, "paged_attention_many_kernel");
+  });
 }
 
 int check_vectors(const Place& p, const char* name) {
@@ -958,19 +1124,20 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
   a.scale = scale;
   a.scale_log2 = static_cast<float>(1.44269504088896340736 * static_cast<double>(scale));
   const int rows = attention::tile_rows(tokens, batch, a.group);
-  const int64_t tiles = attention::tiles(tokens, batch, a.group, rows);
-  int64_t parts =
-      attention::parts(tokens, batch, a.heads, a.kv_heads, a.positions);
+  a.tiles = static_cast<int>(attention::tiles(tokens, batch, a.group, rows));
+  attention::Parts parts = attention::parts(tokens, batch, a.heads, a.kv_heads, a.positions);
   hipStream_t stream = cfg_stream(cfg);
-  if (tiles * a.kv_heads > kMaxGroupsPerLaunch) parts = 1;
-  if (parts > 1 && (cfg == nullptr || cfg->workspace == nullptr) && !keeps_scratch(stream))
-    parts = 1;
-  if (tiles * parts * a.kv_heads > (int64_t{1} << 23))
-    return set_error(CREDIT_ERR_BAD_SHAPE, "%lld tiles of %d key heads are too many for a launch",
-                     static_cast<long long>(tiles), a.kv_heads);
-  a.parts = static_cast<int>(parts);
-  a.tiles = static_cast<int>(tiles);
-  if (parts > 1) {
+  if (static_cast<int64_t>(parts.units) * a.kv_heads > kMaxGroupsPerLaunch ||
+      ((cfg == nullptr || cfg->workspace == nullptr) && !keeps_scratch(stream)))
+    parts.most = 1;
+  a.units = parts.most > 1 ? parts.units : a.tiles;
+  if (static_cast<int64_t>(a.units) * a.kv_heads > (int64_t{1} << 23))
+    return set_error(CREDIT_ERR_BAD_SHAPE, "%d tiles of %d key heads are too many for a launch",
+                     a.units, a.kv_heads);
+  if (parts.most > 1) {
+    a.most_parts = parts.most;
+    a.least_steps = parts.least_steps;
+    a.share = parts.share;
     char* base = nullptr;
     CREDIT_TRY(acquire_workspace(
         cfg, attention::workspace(tokens, batch, a.heads, a.kv_heads, dim, a.positions), &base));

@@ -14,8 +14,10 @@ namespace attention {
 constexpr int kMaxDim = 256;
 constexpr int kFew = 32;     // query rows (tokens times heads of a group) of a small tile
 constexpr int kMany = 128;   // of a large one
-constexpr int kKeys = 64;    // positions of a step
+constexpr int kKeys = 64;    // positions of a step of large tiles
+constexpr int kFewKeys = 32; // of small ones
 constexpr int kMaxParts = 128;
+constexpr int kMaxBatch = 1024;     // sequences that a wave counts through
 
 // Small tiles serve where a sequence has no more rows than one.
 inline int tile_rows(int64_t tokens, int64_t batch, int64_t group) {
@@ -29,15 +31,28 @@ inline int64_t tiles(int64_t tokens, int64_t batch, int64_t group, int rows) {
   return tokens * group / rows + batch;
 }
 
-// Parts that the positions of a tile are cut into.
-inline int64_t parts(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
-                     int64_t positions) {
+// Parts that the positions of tiles are cut into: all tiles' steps, as they turn
+// out on the device, are dealt to about `share` units (of each key head) of one
+// length, at least least_steps, a tile to at most `most` of them; `units` bounds
+// their number.  most 1: none are cut.
+struct Parts {
+  int most, least_steps, share, units;
+};
+inline Parts parts(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
+                   int64_t positions) {
   const int64_t group = heads / kv_heads;
   const int rows = tile_rows(tokens, batch, group);
-  const int64_t work = std::max<int64_t>(1, tiles(tokens, batch, group, rows) * kv_heads);
-  const int64_t longest = (positions + kKeys - 1) / kKeys;
-  return std::max<int64_t>(
-      1, std::min<int64_t>({kMaxParts, (512 + work - 1) / work, (longest + 3) / 4}));
+  const int64_t all = tiles(tokens, batch, group, rows);
+  const int keys = rows == kFew ? kFewKeys : kKeys;
+  const int64_t least = rows == kFew ? 8 : 16;
+  const int64_t longest = (positions + keys - 1) / keys;
+  const int64_t share =
+      std::max<int64_t>(1, ((rows == kFew ? 1024 : 512) + kv_heads - 1) / kv_heads);
+  const int64_t most = std::min<int64_t>({rows == kFew ? kMaxParts : kMaxParts / 4,
+                                          (longest + least - 1) / least, share});
+  if (most < 2 || batch > kMaxBatch || all > 4 * share) return {1, 0, 0, 0};
+  return {static_cast<int>(most), static_cast<int>(least), static_cast<int>(share),
+          static_cast<int>(share + all)};
 }
 
 inline int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
@@ -49,13 +64,11 @@ inline int64_t part_floats(int rows, int dim) {
 
 inline size_t workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int dim,
                         int64_t positions) {
-  const int64_t n = parts(tokens, batch, heads, kv_heads, positions);
-  if (n < 2) return 0;
+  const Parts p = parts(tokens, batch, heads, kv_heads, positions);
+  if (p.most < 2) return 0;
   const int64_t group = heads / kv_heads;
   const int rows = tile_rows(tokens, batch, group);
-  return static_cast<size_t>(tiles(tokens, batch, group, rows) * kv_heads * n *
-                             part_floats(rows, dim)) *
-         sizeof(float);
+  return static_cast<size_t>(p.units * kv_heads * part_floats(rows, dim)) * sizeof(float);
 }
 
 // n / d for n < 2^31 as (mulhi(n, mul) + n) >> shift.
