@@ -93,6 +93,13 @@ struct Tile {
 // The value of any lane of a wave that all hold one.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+__device__ __forceinline__ const void* uniform(const void* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = static_cast<uint32_t>(uniform(static_cast<int>(v)));
+  const uint32_t hi = static_cast<uint32_t>(uniform(static_cast<int>(v >> 32)));
+  return reinterpret_cast<const void*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 __device__ __forceinline__ int64_t start_of(const Args& a, int b) {
   const int64_t s = a.q_start[b];
   return s < 0 ? 0 : s < a.tokens ? s : a.tokens;
@@ -151,10 +158,20 @@ __device__ __forceinline__ bool find_tile(Work& w, const Args& a, int unit) {
   return true;
 }
 
-__device__ __forceinline__ int wave_max(int v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) v = max(v, __shfl_xor(v, d));
-  return v;
+// A sequence's tiles and steps as find_part counts them.
+struct Count {
+  int tiles, steps;
+};
+template <int ROWS, int KEYS>
+__device__ __forceinline__ Count count_of(const Args& a, int b) {
+  if (b >= a.batch) return {0, 0};
+  const int rows = rows_of(a, b), kv = positions_of(a, b);
+  Count c{(rows + ROWS - 1) / ROWS, (kv + KEYS - 1) / KEYS};
+  if (a.window > 0) {  // those in front of the window are not walked
+    const int64_t seen = static_cast<int64_t>(a.window) + divide(rows, a.by_group);
+    c.steps = static_cast<int>(min(static_cast<int64_t>(kv), seen) + KEYS - 1) / KEYS + 1;
+  }
+  return c;
 }
 // With parts: all sequences' steps are dealt to about a.share units of one length,
 // so that sequences of unlike lengths keep the device busy alike; each wave counts
@@ -162,36 +179,28 @@ __device__ __forceinline__ int wave_max(int v) {
 template <int ROWS, int KEYS>
 __device__ __forceinline__ bool find_part(Work& w, const Args& a, int unit) {
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  const auto tiles_of = [&](int b) {
-    return b < a.batch ? (rows_of(a, b) + ROWS - 1) / ROWS : 0;
-  };
-  const auto steps_of = [&](int b) {
-    if (b >= a.batch) return 0;
-    const int kv = positions_of(a, b);
-    if (a.window == 0) return (kv + KEYS - 1) / KEYS;
-    const int64_t seen = static_cast<int64_t>(a.window) + divide(rows_of(a, b), a.by_group);
-    return static_cast<int>(min(static_cast<int64_t>(kv), seen) + KEYS - 1) / KEYS + 1;
-  };
-  double total = 0.0, all = 0.0;
-  int longest = 0;
-  for (int b = lane; b - lane < a.batch; b += kWave) {
-    const int tiles = tiles_of(b), steps = steps_of(b);
-    all += tiles;
-    total += static_cast<double>(tiles) * steps;
-    if (tiles > 0) longest = max(longest, steps);
+  Count c = count_of<ROWS, KEYS>(a, lane);
+  constexpr double kTile = 1ull << 39;  // tiles and steps summed as one number
+  double sum = c.tiles * (kTile + c.steps);
+  int longest = c.tiles > 0 ? c.steps : 0;
+  for (int b = lane + kWave; b - lane < a.batch; b += kWave) {
+    const Count more = count_of<ROWS, KEYS>(a, b);
+    sum += more.tiles * (kTile + more.steps);
+    if (more.tiles > 0) longest = max(longest, more.steps);
   }
+  sum = wave_reduce_sum_f64(sum);
+  longest = uniform(static_cast<int>(
+      wave_reduce(static_cast<float>((longest + 63) / 64), MaxOp()))) * 64;  // at least it
+  const double tiles = __builtin_floor(sum / kTile);
   // More tiles than the rows make: q_start does not rise.  Nothing is done.
-  if (wave_reduce_sum_f64(all) > a.tiles) return false;
-  total = wave_reduce_sum_f64(total);
-  longest = wave_max(longest);
-  w.each = uniform(max(max(a.least_steps, static_cast<int>(total / a.share) + 1),
+  if (tiles > a.tiles) return false;
+  w.each = uniform(max(max(a.least_steps, static_cast<int>((sum - tiles * kTile) / a.share) + 1),
                        (longest + a.most_parts - 1) / a.most_parts));
   int before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kWave) {
-    const int b = b0 + lane;
-    const int tiles = tiles_of(b);
-    const int parts = max(1, (steps_of(b) + w.each - 1) / w.each);
-    int upto = tiles * parts;
+    if (b0 > 0) c = count_of<ROWS, KEYS>(a, b0 + lane);
+    const int parts = max(1, (c.steps + w.each - 1) / w.each);
+    int upto = c.tiles * parts;
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) {
       const int v = __shfl_up(upto, d);
@@ -201,7 +210,7 @@ __device__ __forceinline__ bool find_part(Work& w, const Args& a, int unit) {
     if (past != 0) {
       const int at = __builtin_ctzll(past);
       const int p = __builtin_amdgcn_readlane(parts, at);
-      const int first = uniform(before + __builtin_amdgcn_readlane(upto - tiles * parts, at));
+      const int first = uniform(before + __builtin_amdgcn_readlane(upto - c.tiles * parts, at));
       const int tile = (unit - first) / p;
       tile_of<ROWS>(w, a, b0 + at, tile);
       w.part = uniform(unit - first - tile * p);
@@ -341,10 +350,12 @@ __device__ __forceinline__ void add_special(State<D>& s, const char* v, int j0, 
 }
 
 // One step: NB blocks of 32 positions from j0 on, keys at k, values at v in LDS.
-// MASKED: a row sees those in [low, last] alone.
-template <int D, int NB, bool MASKED>
+// MASKED: a row sees those in [low, last] alone.  scored() runs once the keys have
+// been read, ready() before the values are.
+template <int D, int NB, bool MASKED, class Scored, class Ready>
 __device__ __forceinline__ void step(State<D>& s, const bf16x8_t (&q)[D / 16], const char* k,
-                                     const char* v, int j0, int low, int last, float scale_log2) {
+                                     const char* v, int j0, int low, int last, float scale_log2,
+                                     Scored&& scored, Ready&& ready) {
   const int lane = opaque_lane();
   f32x16 x[NB];
 #pragma unroll
@@ -359,6 +370,7 @@ __device__ __forceinline__ void step(State<D>& s, const bf16x8_t (&q)[D / 16], c
       x[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, q[ks], x[nb], 0, 0, 0);
     }
   }
+  scored();
   float m = kNegInf;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -403,6 +415,7 @@ __device__ __forceinline__ void step(State<D>& s, const bf16x8_t (&q)[D / 16], c
       p[2 * nb + h] = __builtin_bit_cast(bf16x8_t, w);
     }
   s.l += sum;
+  ready();
   const bool special = MASKED && any_special<D, 32 * NB>(v);
   if (!special) {
 #pragma unroll
@@ -485,44 +498,30 @@ __device__ __forceinline__ buffer_rsrc_t part_rsrc(float* at) {
   return make_rsrc(at, ROWS * (D + 2) * sizeof(float));
 }
 
-// All parts of a tile joined by its workgroup, in their order: the rows' maxima and
-// sums by way of LDS, then four columns a thread, eight parts at a time.
+// All parts of a tile joined by its workgroup, in their order: four columns of a row
+// a thread, whose reads of eight parts are in flight together.
 template <int D, int ROWS>
-__device__ __forceinline__ void join(const Args& a, const Work& w, int parts, char* smem) {
-  float* weight = reinterpret_cast<float*>(smem);  // [parts + 1][ROWS]
-  float* sum = weight + (parts + 1) * ROWS;        // [parts][ROWS]
-  const int thread = static_cast<int>(threadIdx.x);
+__device__ __forceinline__ void join(const Args& a, const Work& w, int parts) {
   const int rows = min(ROWS, w.t.rows - w.t.row0);
-#pragma unroll 4
-  for (int i = thread; i < parts * ROWS; i += kThreads) {
-    const float* at = part_at<D, ROWS>(a, w, i / ROWS) + ROWS * D + i % ROWS;
-    weight[i] = fetch(at);
-    sum[i] = fetch(at + ROWS);
-  }
-  __syncthreads();
-  if (thread < rows) {
-    float m = kNegInf, l = 0.0f;
-    for (int p = 0; p < parts; ++p) m = fmaxf(m, weight[p * ROWS + thread]);
-    for (int p = 0; p < parts; ++p) {
-      const float f = weight_of(a, weight[p * ROWS + thread], m);
-      l += f * sum[p * ROWS + thread];
-      weight[p * ROWS + thread] = f;
-    }
-    const Row r = row_of(a, w, w.t.row0 + thread);
-    if (a.lse != nullptr) a.lse[r.token * a.heads + r.head] = lse_of(a, m, l);
-    weight[parts * ROWS + thread] = inverse_of(l);
-  }
-  __syncthreads();
-  for (int i = thread; i < rows * (D / 4); i += kThreads) {
+  for (int i = static_cast<int>(threadIdx.x); i < rows * (D / 4); i += kThreads) {
     const int row = i / (D / 4), d = i % (D / 4) * 4;
-    if (d >= a.dim) continue;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = kNegInf, l = 0.0f;
 #pragma unroll 8
-    for (int p = 0; p < parts; ++p)
-      o += fetch_quad(part_rsrc<D, ROWS>(part_at<D, ROWS>(a, w, p)), row * D + d) *
-           weight[p * ROWS + row];
-    o *= weight[parts * ROWS + row];
+    for (int p = 0; p < parts; ++p) {
+      float* at = part_at<D, ROWS>(a, w, p);
+      const f32x4 po = fetch_quad(part_rsrc<D, ROWS>(at), row * D + d);
+      const float pm = fetch(at + ROWS * D + row), pl = fetch(at + ROWS * (D + 1) + row);
+      const float both = fmaxf(m, pm);
+      const float f = weight_of(a, m, both), pf = weight_of(a, pm, both);
+      o = o * f + po * pf;
+      l = l * f + pl * pf;
+      m = both;
+    }
     const Row r = row_of(a, w, w.t.row0 + row);
+    if (a.lse != nullptr && d == 0) a.lse[r.token * a.heads + r.head] = lse_of(a, m, l);
+    if (d >= a.dim) continue;
+    o *= inverse_of(l);
     *reinterpret_cast<uint64_t*>(a.out + r.token * a.out_token + r.head * a.out_head + d) =
         pack_bf16x2(o[0], o[1]) | static_cast<uint64_t>(pack_bf16x2(o[2], o[3])) << 32;
   }
@@ -579,15 +578,25 @@ struct Loader {
 // the write of M0, which nothing else here reads.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-template <uint32_t AT>
+// NT: with the nontemporal hint.
+template <uint32_t AT, bool NT>
 __device__ __forceinline__ void load_to_lds(buffer_rsrc_t rsrc, uint32_t off, uint32_t lds) {
-  asm volatile(
-      "s_add_u32 m0, %2, %3\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %0, %1, 0 offen lds"
-      :
-      : "v"(off), "s"(rsrc), "s"(lds), "i"(AT)
-      : "memory", "m0", "scc");
+  if constexpr (NT)
+    asm volatile(
+        "s_add_u32 m0, %2, %3\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %0, %1, 0 offen nt lds"
+        :
+        : "v"(off), "s"(rsrc), "s"(lds), "i"(AT)
+        : "memory", "m0", "scc");
+  else
+    asm volatile(
+        "s_add_u32 m0, %2, %3\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %0, %1, 0 offen lds"
+        :
+        : "v"(off), "s"(rsrc), "s"(lds), "i"(AT)
+        : "memory", "m0", "scc");
 }
 #pragma clang diagnostic pop
 // s_waitcnt vmcnt(N), the other counters at their maxima.
@@ -658,7 +667,8 @@ struct Direct {
     for (int i = 0; i < kPieces; ++i)
       page[i] = table[divide(min(j0 + wave * kMine + i * PIECE, end - 1), a.by_page)];
   }
-  // lds: of the wave's first row of keys.
+  // KEYS: the keys, else the values.  lds: of the wave's first row of them.
+  template <bool KEYS, bool NT>
   __device__ __forceinline__ void load(const Args& a, int head, int j0, int end, int wave,
                                        uint32_t lds) const {
     unrolled<kPieces>([&](auto ic) {
@@ -668,22 +678,22 @@ struct Direct {
       const bool there = page[i] >= 0 && page[i] < a.n_pages;
       const int64_t at = there ? page[i] : 0;
       const int in_page = j - divide(j, a.by_page) * a.page_size;
-      const auto extent = [&](const Cache& c) {
-        return n > 0 ? static_cast<uint32_t>(n - 1) * static_cast<uint32_t>(c.slot) * 2u +
-                           static_cast<uint32_t>(a.dim) * 2u
-                     : 0u;
-      };
-      const auto first = [&](const Cache& c) {
-        return c.data + at * c.page + static_cast<int64_t>(in_page) * c.slot + head * c.head;
-      };
-      const buffer_rsrc_t k = make_rsrc(there ? static_cast<const void*>(first(a.k)) : &kNoKeys,
-                                        there ? extent(a.k) : 16u);
-      const buffer_rsrc_t v = make_rsrc(first(a.v), there ? extent(a.v) : 0u);
+      const Cache& c = KEYS ? a.k : a.v;
+      const uint32_t extent = n > 0 ? static_cast<uint32_t>(n - 1) *
+                                              static_cast<uint32_t>(c.slot) * 2u +
+                                          static_cast<uint32_t>(a.dim) * 2u
+                                    : 0u;
+      const void* first =
+          c.data + at * c.page + static_cast<int64_t>(in_page) * c.slot + head * c.head;
+      const bool keys_gone = KEYS && !there;
+      const buffer_rsrc_t rsrc =
+          make_rsrc(uniform(keys_gone ? static_cast<const void*>(&kNoKeys) : first),
+                    static_cast<uint32_t>(uniform(
+                        static_cast<int>(keys_gone ? 16u : there ? extent : 0u))));
       unrolled<kLoads>([&](auto lc) {
         constexpr int l = i * kLoads + decltype(lc)::value;
-        constexpr uint32_t kAt = l * 1024;
-        load_to_lds<kAt>(k, there ? k_off[l % kTurn] : 0u, lds);
-        load_to_lds<kAt + ROWS * Lds<D>::kRowBytes>(v, v_off[l % kTurn], lds);
+        const uint32_t off = KEYS ? (there ? k_off[l % kTurn] : 0u) : v_off[l % kTurn];
+        load_to_lds<l * 1024, NT>(rsrc, off, static_cast<uint32_t>(uniform(static_cast<int>(lds))));
       });
     });
   }
@@ -760,13 +770,16 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_ma
   State<D> s;
   clear(s);
   const int32_t* pages = a.pages + t.b * a.pages_ld;
+  const auto none = [] {};
   const auto compute = [&](int i, const char* k) {
     const int j0 = i * kKeys;
     if (j0 > any_last || j0 + kKeys <= any_low) return;
     if (j0 + kKeys - 1 <= all_last && j0 >= all_low)
-      step<D, kKeys / 32, false>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
+      step<D, kKeys / 32, false>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2, none,
+                                 none);
     else
-      step<D, kKeys / 32, true>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
+      step<D, kKeys / 32, true>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2, none,
+                                 none);
   };
   if constexpr (PIECE > 0) {
     const uint32_t lds = static_cast<uint32_t>(
@@ -774,9 +787,13 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_ma
                 wave * (kKeys / kNW) * Lds<D>::kRowBytes));
     Direct<D, kKeys, kNW, PIECE> loads;
     loads.init(a, wave);
+    const auto load = [&](int i, uint32_t at) {
+      loads.template load<true, false>(a, w.head, i * kKeys, r.end, wave, at);
+      loads.template load<false, false>(a, w.head, i * kKeys, r.end, wave, at + kStage / 2);
+    };
     if (r.first < r.last) {
       loads.look_up(a, pages, r.first * kKeys, r.end, wave);
-      loads.load(a, w.head, r.first * kKeys, r.end, wave, lds);
+      load(r.first, lds);
       loads.look_up(a, pages, min(r.first + 1, r.last - 1) * kKeys, r.end, wave);
     }
     for (int i = r.first; i < r.last; ++i) {
@@ -785,7 +802,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_ma
       wait_loads<0>();
       lds_barrier();
       if (i + 1 < r.last) {
-        loads.load(a, w.head, (i + 1) * kKeys, r.end, wave, lds + (stage ^ 1) * kStage);
+        load(i + 1, lds + (stage ^ 1) * kStage);
         loads.look_up(a, pages, min(i + 2, r.last - 1) * kKeys, r.end, wave);
       }
       compute(i, smem + stage * kStage);
@@ -828,7 +845,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_ma
     publish(at + kMany * (D + 1) + in_tile, s.l);
   }
   if (last_of(counter_of(a, w), r.parts, &shared))
-    join<D, kMany>(a, w, r.parts, smem);
+    join<D, kMany>(a, w, r.parts);
 }
 
 // A wave's LDS operations run in order; this keeps the compiler to it where lanes
@@ -839,13 +856,10 @@ __device__ __forceinline__ void wave_fence() {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
-// Positions of a wave's step, and its stages in LDS: two where four waves' fit.
-using attention::kFewKeys;
-template <int D>
-constexpr int kFewStages = D <= 128 ? 2 : 1;
+using attention::kFewKeys;  // positions of a wave's step
 
 template <int D, int PIECE>
-__global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_few_kernel(const Args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ uint32_t shared;
   __shared__ float ms[kNW][kFew], ls[kNW][kFew];
@@ -870,43 +884,56 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(const Arg
   State<D> s;
   clear(s);
   const int32_t* pages = a.pages + t.b * a.pages_ld;
-  char* own = smem + wave * kFewStages<D> * kStage;
-  const auto compute = [&](int i, const char* k) {
+  char* own = smem + wave * kStage;
+  const auto compute = [&](int i, auto&& scored, auto&& ready) {
     const int j0 = i * kFewKeys;
     if (j0 + kFewKeys - 1 <= all_last && j0 >= all_low)
-      step<D, kFewKeys / 32, false>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
+      step<D, kFewKeys / 32, false>(s, q, own, own + kStage / 2, j0, low, last, a.scale_log2,
+                                    scored, ready);
     else
-      step<D, kFewKeys / 32, true>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2);
+      step<D, kFewKeys / 32, true>(s, q, own, own + kStage / 2, j0, low, last, a.scale_log2,
+                                   scored, ready);
   };
   if constexpr (PIECE > 0) {
-    const uint32_t lds = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
-        static_cast<int>((uint32_t)(uintptr_t)(lds_ptr_t)own)));
+    const uint32_t lds = static_cast<uint32_t>(
+        uniform(static_cast<int>((uint32_t)(uintptr_t)(lds_ptr_t)own)));
     Direct<D, kFewKeys, 1, PIECE> loads;
+    constexpr int kPer = Direct<D, kFewKeys, 1, PIECE>::kPer;
     loads.init(a, 0);
+    const auto load_keys = [&](int i) {
+      loads.template load<true, true>(a, w.head, i * kFewKeys, r.end, 0, lds);
+    };
+    const auto load_values = [&](int i) {
+      loads.template load<false, true>(a, w.head, i * kFewKeys, r.end, 0, lds + kStage / 2);
+      // Of the step after this one.
+      loads.look_up(a, pages, min(i + kNW, r.last - 1) * kFewKeys, r.end, 0);
+    };
     int i = r.first + wave;
     if (i < r.last) {
       loads.look_up(a, pages, i * kFewKeys, r.end, 0);
-      loads.load(a, w.head, i * kFewKeys, r.end, 0, lds);
-      loads.look_up(a, pages, min(i + kNW, r.last - 1) * kFewKeys, r.end, 0);
+      load_keys(i);
+      load_values(i);
     }
-    for (int stage = 0; i < r.last; i += kNW) {
+    // In flight at the loop's start: this step's keys, then its values.  The next
+    // step's keys are loaded once this one's have been read, its values likewise.
+    for (; i < r.last; i += kNW) {
       const bool more = i + kNW < r.last;
-      if (kFewStages<D> == 2 && more) {
-        // The other stage's step was read before this one's wait.
+      wait_loads<kPer>();
+      compute(
+          i,
+          [&] {
+            wait_reads();
+            if (more) load_keys(i + kNW);
+          },
+          [&] {
+            if (more)
+              wait_loads<kPer>();
+            else
+              wait_loads<0>();
+          });
+      if (more) {
         wait_reads();
-        loads.load(a, w.head, (i + kNW) * kFewKeys, r.end, 0, lds + (stage ^ 1) * kStage);
-        loads.look_up(a, pages, min(i + 2 * kNW, r.last - 1) * kFewKeys, r.end, 0);
-        wait_loads<2 * Direct<D, kFewKeys, 1, PIECE>::kPer>();
-      } else {
-        wait_loads<0>();
-      }
-      compute(i, own + stage * kStage);
-      if (kFewStages<D> == 2) {
-        stage ^= 1;
-      } else if (more) {
-        wait_reads();
-        loads.load(a, w.head, (i + kNW) * kFewKeys, r.end, 0, lds);
-        loads.look_up(a, pages, min(i + 2 * kNW, r.last - 1) * kFewKeys, r.end, 0);
+        load_values(i + kNW);
       }
     }
   } else {
@@ -918,7 +945,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(const Arg
       wave_fence();
       if (i + kNW < r.last)
         loader.load(a, pages, w.head, (i + kNW) * kFewKeys, r.end, lane);
-      compute(i, own);
+      compute(i, [] {}, [] {});
       wave_fence();
     }
   }
@@ -988,7 +1015,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(const Arg
     }
   }
   if (parted && last_of(counter_of(a, w), r.parts, &shared))
-    join<D, kFew>(a, w, r.parts, smem);
+    join<D, kFew>(a, w, r.parts);
 }
 
 // ------------------------------------------------------------------- host --
@@ -1020,7 +1047,7 @@ int launch(const Args& a, int rows, hipStream_t stream) {
   if (rows == kFew)
     return choose([&](auto piece) {
       constexpr size_t kBytes = std::max<size_t>(
-          size_t{kNW} * kFewStages<D> * 2 * kFewKeys * Lds<D>::kRowBytes,
+          size_t{kNW} * 2 * kFewKeys * Lds<D>::kRowBytes,
           size_t{kNW} * kFew * (D + 4) * sizeof(float));
       return launch_with<paged_attention_few_kernel<D, decltype(piece)::value>>(
           a, kBytes, stream, "paged_attention_few_kernel");

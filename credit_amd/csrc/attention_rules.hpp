@@ -46,8 +46,8 @@ inline Parts parts(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
   const int keys = rows == kFew ? kFewKeys : kKeys;
   const int64_t least = rows == kFew ? 8 : 16;
   const int64_t longest = (positions + keys - 1) / keys;
-  const int64_t share =
-      std::max<int64_t>(1, ((rows == kFew ? 1024 : 512) + kv_heads - 1) / kv_heads);
+  const int64_t share = rows == kFew ? std::max<int64_t>(1, (2048 + kv_heads - 1) / kv_heads)
+                                     : std::max<int64_t>(1, 512 / kv_heads - all);
   const int64_t most = std::min<int64_t>({rows == kFew ? kMaxParts : kMaxParts / 4,
                                           (longest + least - 1) / least, share});
   if (most < 2 || batch > kMaxBatch || all > 4 * share) return {1, 0, 0, 0};
