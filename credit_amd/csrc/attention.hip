@@ -67,14 +67,14 @@ struct Args {
   uint16_t* out;
   int64_t out_token, out_head;
   float* lse;  // [tokens, heads] or nullptr
-  float* partial;      // parts' results, a unit and key head each; nullptr: no parts
+  float* partial;      // parts' results, two a workgroup; nullptr: no parts
   uint32_t* arrived;
   int64_t tokens;
   int batch, heads, kv_heads, group, dim;
   int page_size, n_pages, positions;  // positions: most that a row of pages holds
   Divisor by_page, by_group;
-  int window, units, tiles;
-  int most_parts, least_steps, share;  // of a tile; of a part; units that all steps are dealt to
+  int window, units, tiles;  // units: workgroups a key head
+  int least_steps;           // of a unit
   float scale, scale_log2;  // scale, scale log2(e)
 };
 
@@ -82,6 +82,10 @@ __device__ __forceinline__ int divide(int n, const Divisor& d) {
   return static_cast<int>(
       (__umulhi(static_cast<uint32_t>(n), d.mul) + static_cast<uint32_t>(n)) >> d.shift);
 }
+
+// The lane, opaque to the compiler: what is derived from it within a step is not
+// kept in registers from step to step.
+__device__ __forceinline__ int opaque_lane() { return opaque_lane_index() & (kWave - 1); }
 
 // A tile: rows row0 .. of sequence b, whose token i sees positions up to ahead + i.
 struct Tile {
@@ -112,11 +116,11 @@ __device__ __forceinline__ int positions_of(const Args& a, int b) {
   return min(max(a.kv_len[b], 0), a.positions);
 }
 
-// A workgroup's work: part `part` of the tile's, which are `each` steps of its
-// positions; unit0: the number of its part 0 among all units.
+// Work on a tile: `take` of its steps from the skip-th on, which is part `part` of
+// `parts`; unit: the one with part 0, inside: whether the tile begins within it.
 struct Work {
   Tile t;
-  int head, part, each, unit0;
+  int head, skip, take, part, parts, unit, inside;
 };
 template <int ROWS>
 __device__ __forceinline__ void tile_of(Work& w, const Args& a, int b, int tile) {
@@ -129,36 +133,7 @@ __device__ __forceinline__ void tile_of(Work& w, const Args& a, int b, int tile)
   t.ahead = t.kv - divide(t.rows, a.by_group);
 }
 
-// Without parts: units are the tiles' slots, sequence b's from
-// floor(first row / ROWS) + b on, found by a search.
-template <int ROWS>
-__device__ __forceinline__ bool find_tile(Work& w, const Args& a, int unit) {
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  int lo = 0, n = a.batch;
-  while (n > 1) {
-    const int step = (n + kWave - 1) / kWave;
-    const int b = lo + lane * step;
-    const bool at =
-        lane * step < n && start_of(a, b) * a.group / ROWS + b <= static_cast<int64_t>(unit);
-    const int count = __builtin_popcountll(__builtin_amdgcn_ballot_w64(at));
-    if (count == 0) return false;
-    const int skip = (count - 1) * step;
-    lo += skip;
-    n = min(step, n - skip);
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  const int64_t slot = start_of(a, lo) * a.group / ROWS + lo;
-  if (unit < slot) return false;
-  const int64_t row0 = (unit - slot) * ROWS;
-  if (row0 >= rows_of(a, lo)) return false;
-  tile_of<ROWS>(w, a, lo, static_cast<int>(unit - slot));
-  w.part = 0;
-  w.each = 1 << 30;
-  w.unit0 = unit;
-  return true;
-}
-
-// A sequence's tiles and steps as find_part counts them.
+// A sequence's tiles and the steps of each, at least one.
 struct Count {
   int tiles, steps;
 };
@@ -166,71 +141,121 @@ template <int ROWS, int KEYS>
 __device__ __forceinline__ Count count_of(const Args& a, int b) {
   if (b >= a.batch) return {0, 0};
   const int rows = rows_of(a, b), kv = positions_of(a, b);
-  Count c{(rows + ROWS - 1) / ROWS, (kv + KEYS - 1) / KEYS};
+  Count c{(rows + ROWS - 1) / ROWS, max(1, (kv + KEYS - 1) / KEYS)};
   if (a.window > 0) {  // those in front of the window are not walked
     const int64_t seen = static_cast<int64_t>(a.window) + divide(rows, a.by_group);
     c.steps = static_cast<int>(min(static_cast<int64_t>(kv), seen) + KEYS - 1) / KEYS + 1;
   }
   return c;
 }
-// With parts: all sequences' steps are dealt to about a.share units of one length,
-// so that sequences of unlike lengths keep the device busy alike; each wave counts
-// them through and finds its unit.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ bool find_part(Work& w, const Args& a, int unit) {
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  Count c = count_of<ROWS, KEYS>(a, lane);
-  constexpr double kTile = 1ull << 39;  // tiles and steps summed as one number
-  double sum = c.tiles * (kTile + c.steps);
-  int longest = c.tiles > 0 ? c.steps : 0;
-  for (int b = lane + kWave; b - lane < a.batch; b += kWave) {
-    const Count more = count_of<ROWS, KEYS>(a, b);
-    sum += more.tiles * (kTile + more.steps);
-    if (more.tiles > 0) longest = max(longest, more.steps);
-  }
-  sum = wave_reduce_sum_f64(sum);
-  longest = uniform(static_cast<int>(
-      wave_reduce(static_cast<float>((longest + 63) / 64), MaxOp()))) * 64;  // at least it
-  const double tiles = __builtin_floor(sum / kTile);
-  // More tiles than the rows make: q_start does not rise.  Nothing is done.
-  if (tiles > a.tiles) return false;
-  w.each = uniform(max(max(a.least_steps, static_cast<int>((sum - tiles * kTile) / a.share) + 1),
-                       (longest + a.most_parts - 1) / a.most_parts));
-  int before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kWave) {
-    if (b0 > 0) c = count_of<ROWS, KEYS>(a, b0 + lane);
-    const int parts = max(1, (c.steps + w.each - 1) / w.each);
-    int upto = c.tiles * parts;
+
+// What a workgroup does, tile by tile.  Key heads lie next to each other in the
+// grid: the dies take workgroups in turn, so that tiles of one head's keys tend to
+// share one die's L2.
+//
+// With parts: the steps of all tiles of a key head, one sequence behind the other,
+// are dealt to its units in runs of one length, whatever the sequences' lengths:
+// the device is busy evenly to the end, and only a run's first and last tile can be
+// shared with other units.  Each wave counts the sequences through.
+// Without: a unit is a tile's slot, sequence b's from floor(first row / ROWS) + b
+// on, found by a search; later tiles, which see more, first.
+template <int ROWS, int KEYS, bool PARTS>
+struct Cursor {
+  int head, unit, each;
+  int64_t at, end;  // steps of the unit's run, -1: without parts
+  int upto;         // of this lane's sequence among the first 64: steps up to its end
+  Count count;
+
+  __device__ __forceinline__ static int scan(int v) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) {
-      const int v = __shfl_up(upto, d);
-      if (lane >= d) upto += v;
+      const int u = __shfl_up(v, d);
+      if (lane >= d) v += u;
     }
-    const uint64_t past = __builtin_amdgcn_ballot_w64(unit < before + upto);
-    if (past != 0) {
-      const int at = __builtin_ctzll(past);
-      const int p = __builtin_amdgcn_readlane(parts, at);
-      const int first = uniform(before + __builtin_amdgcn_readlane(upto - c.tiles * parts, at));
-      const int tile = (unit - first) / p;
-      tile_of<ROWS>(w, a, b0 + at, tile);
-      w.part = uniform(unit - first - tile * p);
-      w.unit0 = unit - w.part;
+    return v;
+  }
+  __device__ __forceinline__ void start(const Args& a) {
+    const int i = static_cast<int>(blockIdx.x);
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    head = i % a.kv_heads;
+    unit = i / a.kv_heads;
+    at = end = -1;
+    if constexpr (!PARTS) return;
+    count = count_of<ROWS, KEYS>(a, lane);
+    upto = scan(count.tiles * count.steps);
+    constexpr double kTile = 1ull << 39;  // tiles and steps summed as one number
+    double sum = count.tiles * (kTile + count.steps);
+    for (int b = lane + kWave; b - lane < a.batch; b += kWave) {
+      const Count more = count_of<ROWS, KEYS>(a, b);
+      sum += more.tiles * (kTile + more.steps);
+    }
+    sum = wave_reduce_sum_f64(sum);
+    const double tiles = __builtin_floor(sum / kTile);
+    // More tiles than the rows make: q_start does not rise.  Nothing is done.
+    const int all = tiles > a.tiles ? 0 : uniform(static_cast<int>(sum - tiles * kTile));
+    each = max(a.least_steps, (all + a.units - 1) / a.units);
+    at = static_cast<int64_t>(unit) * each;
+    end = min(at + each, static_cast<int64_t>(all));
+  }
+  // The next tile's work; false: none.
+  __device__ __forceinline__ bool next(Work& w, const Args& a) {
+    w.head = head;
+    if constexpr (!PARTS) return search(w, a, a.units - 1 - unit);
+    if (at >= end) return false;
+    const int now = uniform(static_cast<int>(at));
+    int before = 0, to = upto;
+    Count c = count;
+    for (int b0 = 0;; b0 += kWave) {
+      if (b0 > 0) {
+        c = count_of<ROWS, KEYS>(a, b0 + static_cast<int>(threadIdx.x & (kWave - 1)));
+        to = scan(c.tiles * c.steps);
+      }
+      const uint64_t past = __builtin_amdgcn_ballot_w64(now < before + to);
+      if (past == 0) {  // ends: now is less than the last sequence's
+        before += __builtin_amdgcn_readlane(to, kWave - 1);
+        continue;
+      }
+      const int in = __builtin_ctzll(past);
+      const int steps = __builtin_amdgcn_readlane(c.steps, in);
+      const int first = before + __builtin_amdgcn_readlane(to - c.tiles * c.steps, in);
+      const int tile = (now - first) / steps;
+      const int from = first + tile * steps;
+      tile_of<ROWS>(w, a, b0 + in, tile);
+      w.skip = now - from;
+      w.take = min(static_cast<int>(end) - now, steps - w.skip);
+      w.unit = from / each;
+      w.inside = from != w.unit * each;
+      w.parts = (from + steps - 1) / each - w.unit + 1;
+      w.part = unit - w.unit;
+      at += w.take;
       return true;
     }
-    before += __builtin_amdgcn_readlane(upto, kWave - 1);
   }
-  return false;
-}
-// Key heads next to each other: the dies take workgroups in turn, so that tiles of
-// one head's keys tend to share one die's L2.  Later tiles, which see more, first.
-// False: no work here.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ bool find_work(Work& w, const Args& a) {
-  const int i = static_cast<int>(blockIdx.x);
-  w.head = i % a.kv_heads;
-  const int unit = a.units - 1 - i / a.kv_heads;
-  return a.partial != nullptr ? find_part<ROWS, KEYS>(w, a, unit) : find_tile<ROWS>(w, a, unit);
-}
+  __device__ __forceinline__ static bool search(Work& w, const Args& a, int slot) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    int lo = 0, n = a.batch;
+    while (n > 1) {
+      const int step = (n + kWave - 1) / kWave;
+      const int b = lo + lane * step;
+      const bool at =
+          lane * step < n && start_of(a, b) * a.group / ROWS + b <= static_cast<int64_t>(slot);
+      const int count = __builtin_popcountll(__builtin_amdgcn_ballot_w64(at));
+      if (count == 0) return false;
+      const int skip = (count - 1) * step;
+      lo += skip;
+      n = min(step, n - skip);
+    }
+    lo = uniform(lo);
+    const int64_t first = start_of(a, lo) * a.group / ROWS + lo;
+    if (slot < first || (slot - first) * ROWS >= rows_of(a, lo)) return false;
+    tile_of<ROWS>(w, a, lo, static_cast<int>(slot - first));
+    w.skip = w.part = 0;
+    w.take = 1 << 30;
+    w.parts = 1;
+    return true;
+  }
+};
 
 // Layout of a step's keys and values in LDS: rows of D elements, 16-byte chunk c
 // of row r at place c ^ swizzle(r), so that the reads below meet no bank twice:
@@ -268,18 +293,13 @@ __device__ __forceinline__ void clear(State<D>& s) {
 // are 0.
 __device__ __forceinline__ float base_of(float m) { return m == kNegInf ? 0.0f : m; }
 
-// The lane, opaque to the compiler: what is derived from it within a step is not
-// kept in registers from step to step.
-__device__ __forceinline__ int opaque_lane() { return opaque_lane_index() & (kWave - 1); }
-
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
 // The queries of a wave's rows: lane l holds elements 16 ks + 8 (l / 32) .. + 7 of
 // row l % 32.
 template <int D>
 __device__ __forceinline__ void load_queries(bf16x8_t (&q)[D / 16], const Args& a, const Tile& t,
-                                             int row, int kv_head) {
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+                                             int lane, int row, int kv_head) {
   const int token = divide(row, a.by_group), head = row - token * a.group;
   const uint16_t* p = a.q + (t.first + token) * a.q_token +
                       static_cast<int64_t>(kv_head * a.group + head) * a.q_head;
@@ -480,7 +500,10 @@ __device__ __forceinline__ void finish(const State<D>& s, const Args& a, const W
 // and sums.
 template <int D, int ROWS>
 __device__ __forceinline__ float* part_at(const Args& a, const Work& w, int part) {
-  return a.partial + (static_cast<int64_t>(w.unit0 + part) * a.kv_heads + w.head) * ROWS * (D + 2);
+  // A unit's first place is for the tile that it begins in, its second for the one
+  // that begins within it.
+  const int64_t place = 2 * static_cast<int64_t>(w.unit + part) + (part == 0 ? w.inside : 0);
+  return a.partial + (place * a.kv_heads + w.head) * ROWS * (D + 2);
 }
 // Stores and loads of a part's results at device scope (sc1: past the die's own
 // L2), 16 bytes each; `part`: its resource.
@@ -501,14 +524,14 @@ __device__ __forceinline__ buffer_rsrc_t part_rsrc(float* at) {
 // All parts of a tile joined by its workgroup, in their order: four columns of a row
 // a thread, whose reads of eight parts are in flight together.
 template <int D, int ROWS>
-__device__ __forceinline__ void join(const Args& a, const Work& w, int parts) {
+__device__ __forceinline__ void join(const Args& a, const Work& w) {
   const int rows = min(ROWS, w.t.rows - w.t.row0);
   for (int i = static_cast<int>(threadIdx.x); i < rows * (D / 4); i += kThreads) {
     const int row = i / (D / 4), d = i % (D / 4) * 4;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     float m = kNegInf, l = 0.0f;
 #pragma unroll 8
-    for (int p = 0; p < parts; ++p) {
+    for (int p = 0; p < w.parts; ++p) {
       float* at = part_at<D, ROWS>(a, w, p);
       const f32x4 po = fetch_quad(part_rsrc<D, ROWS>(at), row * D + d);
       const float pm = fetch(at + ROWS * D + row), pl = fetch(at + ROWS * (D + 1) + row);
@@ -645,8 +668,7 @@ struct Direct {
 
   // Byte offsets of the lanes' loads within a piece: row and the chunk that lands
   // at the lane's place.
-  __device__ __forceinline__ void init(const Args& a, int wave) {
-    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  __device__ __forceinline__ void init(const Args& a, int lane, int wave) {
     const int in_row = lane / Lds<D>::kChunks, place = lane % Lds<D>::kChunks;
     const uint32_t bytes = static_cast<uint32_t>(a.dim) * 2u;
 #pragma unroll
@@ -699,10 +721,9 @@ struct Direct {
   }
 };
 
-// The steps of a part: [first, last) of those of `keys` positions, and how many
-// parts the tile has.
+// The steps [first, last) of a tile's work.
 struct Range {
-  int first, last, parts;
+  int first, last;
   int end;  // positions that any row sees end here
 };
 __device__ __forceinline__ Range range_of(const Args& a, const Work& w, int rows, int keys) {
@@ -710,19 +731,12 @@ __device__ __forceinline__ Range range_of(const Args& a, const Work& w, int rows
   const int last = t.ahead + divide(min(t.row0 + rows, t.rows) - 1, a.by_group);
   int low = 0;
   if (a.window > 0) low = max(0, t.ahead + divide(t.row0, a.by_group) - a.window + 1);
-  Range r;
-  r.end = last + 1;
   const int from = low / keys, to = last < 0 ? 0 : last / keys + 1;
-  const int n = max(0, to - from);
-  r.parts = max(1, (n + w.each - 1) / w.each);
-  r.first = from + w.part * w.each;
-  r.last = min(to, r.first + min(w.each, n));
-  return r;
+  return {from + w.skip, min(to, from + w.skip + w.take), last + 1};
 }
 
 __device__ __forceinline__ uint32_t* counter_of(const Args& a, const Work& w) {
-  return a.arrived +
-         (static_cast<int64_t>(w.unit0) * a.kv_heads + w.head) * kGroupCounterStride;
+  return a.arrived + (static_cast<int64_t>(w.unit) * a.kv_heads + w.head) * kGroupCounterStride;
 }
 // Whether this workgroup is the last of the tile's parts; its own results are
 // published.
@@ -740,19 +754,14 @@ __device__ __forceinline__ bool last_of(uint32_t* counter, int parts, uint32_t* 
 
 constexpr int kKeys = attention::kKeys;
 
-template <int D, int PIECE>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_many_kernel(
-    const Args a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ uint32_t shared;
+template <int D, int PIECE, bool PARTS>
+__device__ __forceinline__ void work_on_many(const Args& a, const Work& w, char* smem,
+                                             uint32_t* shared) {
   constexpr int kStage = 2 * kKeys * Lds<D>::kRowBytes;
-  Work w;
-  if (!find_work<kMany, kKeys>(w, a)) return;
   const Tile& t = w.t;
   const Range r = range_of(a, w, kMany, kKeys);
-  if (w.part >= r.parts) return;
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  const int lane = opaque_lane();
+  const int wave = uniform(opaque_lane_index() / kWave);
   const int row = t.row0 + 32 * wave + (lane & 31);
   const int last = row < t.rows ? t.ahead + divide(row, a.by_group) : -1;
   const int low = a.window > 0 ? last - a.window + 1 : 0;
@@ -766,7 +775,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_ma
   const int any_low =
       a.window > 0 ? t.ahead + divide(min(wave_row, t.rows - 1), a.by_group) - a.window + 1 : 0;
   bf16x8_t q[D / 16];
-  load_queries<D>(q, a, t, row, w.head);
+  load_queries<D>(q, a, t, lane, row, w.head);
   State<D> s;
   clear(s);
   const int32_t* pages = a.pages + t.b * a.pages_ld;
@@ -786,7 +795,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_ma
         uniform(static_cast<int>((uint32_t)(uintptr_t)(lds_ptr_t)smem) +
                 wave * (kKeys / kNW) * Lds<D>::kRowBytes));
     Direct<D, kKeys, kNW, PIECE> loads;
-    loads.init(a, wave);
+    loads.init(a, lane, wave);
     const auto load = [&](int i, uint32_t at) {
       loads.template load<true, false>(a, w.head, i * kKeys, r.end, wave, at);
       loads.template load<false, false>(a, w.head, i * kKeys, r.end, wave, at + kStage / 2);
@@ -824,7 +833,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_ma
     }
   }
   s.l += other_half(s.l);
-  if (r.parts == 1) {
+  if (!PARTS || w.parts == 1) {
     finish(s, a, w, row);
     return;
   }
@@ -844,8 +853,25 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_ma
     publish(at + kMany * D + in_tile, s.m);
     publish(at + kMany * (D + 1) + in_tile, s.l);
   }
-  if (last_of(counter_of(a, w), r.parts, &shared))
-    join<D, kMany>(a, w, r.parts);
+  if (last_of(counter_of(a, w), w.parts, shared)) join<D, kMany>(a, w);
+}
+
+template <int D, int PIECE, bool PARTS>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_many_kernel(
+    const Args a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ uint32_t shared;
+  Cursor<kMany, kKeys, PARTS> cursor;
+  Work w;
+  cursor.start(a);
+  if constexpr (PARTS) {
+    while (cursor.next(w, a)) {
+      work_on_many<D, PIECE, true>(a, w, smem, &shared);
+      __syncthreads();
+    }
+  } else if (cursor.next(w, a)) {
+    work_on_many<D, PIECE, false>(a, w, smem, &shared);
+  }
 }
 
 // A wave's LDS operations run in order; this keeps the compiler to it where lanes
@@ -858,19 +884,15 @@ __device__ __forceinline__ void wave_fence() {
 
 using attention::kFewKeys;  // positions of a wave's step
 
-template <int D, int PIECE>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_few_kernel(const Args a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ uint32_t shared;
-  __shared__ float ms[kNW][kFew], ls[kNW][kFew];
+template <int D, int PIECE, bool PARTS>
+__device__ __forceinline__ void work_on_few(const Args& a, const Work& w, char* smem,
+                                            float (&ms)[kNW][kFew], float (&ls)[kNW][kFew],
+                                            uint32_t* shared) {
   constexpr int kStage = 2 * kFewKeys * Lds<D>::kRowBytes;
-  Work w;
-  if (!find_work<kFew, kFewKeys>(w, a)) return;
   const Tile& t = w.t;
   const Range r = range_of(a, w, kFew, kFewKeys);
-  if (w.part >= r.parts) return;
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  const int lane = opaque_lane();
+  const int wave = uniform(opaque_lane_index() / kWave);
   const int row = t.row0 + (lane & 31);
   const int last = row < t.rows ? t.ahead + divide(row, a.by_group) : -1;
   const int low = a.window > 0 ? last - a.window + 1 : 0;
@@ -880,7 +902,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_fe
   const int all_low =
       a.window > 0 ? t.ahead + divide(last_row, a.by_group) - a.window + 1 : 0;
   bf16x8_t q[D / 16];
-  load_queries<D>(q, a, t, row, w.head);
+  load_queries<D>(q, a, t, lane, row, w.head);
   State<D> s;
   clear(s);
   const int32_t* pages = a.pages + t.b * a.pages_ld;
@@ -899,7 +921,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_fe
         uniform(static_cast<int>((uint32_t)(uintptr_t)(lds_ptr_t)own)));
     Direct<D, kFewKeys, 1, PIECE> loads;
     constexpr int kPer = Direct<D, kFewKeys, 1, PIECE>::kPer;
-    loads.init(a, 0);
+    loads.init(a, lane, 0);
     const auto load_keys = [&](int i) {
       loads.template load<true, true>(a, w.head, i * kFewKeys, r.end, 0, lds);
     };
@@ -975,7 +997,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_fe
   }
   __syncthreads();
   const int rows = min(kFew, t.rows - t.row0);
-  const bool parted = r.parts > 1;
+  const bool parted = PARTS && w.parts > 1;
   float* at = parted ? part_at<D, kFew>(a, w, w.part) : nullptr;
   const auto sum_of = [&](int in_tile, float& most) {
     most = kNegInf;
@@ -1014,8 +1036,27 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_fe
       a.lse[r0.token * a.heads + r0.head] = lse_of(a, most, l);
     }
   }
-  if (parted && last_of(counter_of(a, w), r.parts, &shared))
-    join<D, kFew>(a, w, r.parts);
+  if constexpr (PARTS)
+    if (parted && last_of(counter_of(a, w), w.parts, shared)) join<D, kFew>(a, w);
+}
+
+template <int D, int PIECE, bool PARTS>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_few_kernel(
+    const Args a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ uint32_t shared;
+  __shared__ float ms[kNW][kFew], ls[kNW][kFew];
+  Cursor<kFew, kFewKeys, PARTS> cursor;
+  Work w;
+  cursor.start(a);
+  if constexpr (PARTS) {
+    while (cursor.next(w, a)) {
+      work_on_few<D, PIECE, true>(a, w, smem, ms, ls, &shared);
+      __syncthreads();
+    }
+  } else if (cursor.next(w, a)) {
+    work_on_few<D, PIECE, false>(a, w, smem, ms, ls, &shared);
+  }
 }
 
 // ------------------------------------------------------------------- host --
@@ -1040,21 +1081,26 @@ int launch(const Args& a, int rows, hipStream_t stream) {
   constexpr int64_t kMost = int64_t{1} << 25;
   const bool near = a.k.slot < kMost && a.v.slot < kMost;
   const auto choose = [&](auto&& with) {
-    if (near && a.page_size % 16 == 0) return with(std::integral_constant<int, 16>{});
-    if (near && a.page_size % kRows == 0) return with(std::integral_constant<int, kRows>{});
-    return with(std::integral_constant<int, 0>{});
+    const auto parts = [&](auto piece) {
+      return a.partial != nullptr ? with(piece, std::true_type{}) : with(piece, std::false_type{});
+    };
+    if (near && a.page_size % 16 == 0) return parts(std::integral_constant<int, 16>{});
+    if (near && a.page_size % kRows == 0) return parts(std::integral_constant<int, kRows>{});
+    return parts(std::integral_constant<int, 0>{});
   };
   if (rows == kFew)
-    return choose([&](auto piece) {
+    return choose([&](auto piece, auto parts) {
       constexpr size_t kBytes = std::max<size_t>(
           size_t{kNW} * 2 * kFewKeys * Lds<D>::kRowBytes,
           size_t{kNW} * kFew * (D + 4) * sizeof(float));
-      return launch_with<paged_attention_few_kernel<D, decltype(piece)::value>>(
+      return launch_with<paged_attention_few_kernel<D, decltype(piece)::value,
+                                                    decltype(parts)::value>>(
           a, kBytes, stream, "paged_attention_few_kernel");
     });
-  return choose([&](auto piece) {
+  return choose([&](auto piece, auto parts) {
     constexpr size_t kBytes = size_t{4} * kKeys * Lds<D>::kRowBytes;
-    return launch_with<paged_attention_many_kernel<D, decltype(piece)::value>>(
+    return launch_with<paged_attention_many_kernel<D, decltype(piece)::value,
+                                                    decltype(parts)::value>>(
         a, kBytes, stream, "paged_attention_many_kernel");
   });
 }
@@ -1156,15 +1202,13 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
   hipStream_t stream = cfg_stream(cfg);
   if (static_cast<int64_t>(parts.units) * a.kv_heads > kMaxGroupsPerLaunch ||
       ((cfg == nullptr || cfg->workspace == nullptr) && !keeps_scratch(stream)))
-    parts.most = 1;
-  a.units = parts.most > 1 ? parts.units : a.tiles;
+    parts.units = 0;
+  a.units = parts.units > 0 ? parts.units : a.tiles;
   if (static_cast<int64_t>(a.units) * a.kv_heads > (int64_t{1} << 23))
     return set_error(CREDIT_ERR_BAD_SHAPE, "%d tiles of %d key heads are too many for a launch",
                      a.units, a.kv_heads);
-  if (parts.most > 1) {
-    a.most_parts = parts.most;
+  if (parts.units > 0) {
     a.least_steps = parts.least_steps;
-    a.share = parts.share;
     char* base = nullptr;
     CREDIT_TRY(acquire_workspace(
         cfg, attention::workspace(tokens, batch, a.heads, a.kv_heads, dim, a.positions), &base));

@@ -16,8 +16,8 @@ constexpr int kFew = 32;     // query rows (tokens times heads of a group) of a 
 constexpr int kMany = 128;   // of a large one
 constexpr int kKeys = 64;    // positions of a step of large tiles
 constexpr int kFewKeys = 32; // of small ones
-constexpr int kMaxParts = 128;
-constexpr int kMaxBatch = 1024;     // sequences that a wave counts through
+constexpr int kMaxBatch = 1024;  // sequences that a wave counts through
+constexpr int kResident = 512;   // workgroups: two a CU
 
 // Small tiles serve where a sequence has no more rows than one.
 inline int tile_rows(int64_t tokens, int64_t batch, int64_t group) {
@@ -31,12 +31,11 @@ inline int64_t tiles(int64_t tokens, int64_t batch, int64_t group, int rows) {
   return tokens * group / rows + batch;
 }
 
-// Parts that the positions of tiles are cut into: all tiles' steps, as they turn
-// out on the device, are dealt to about `share` units (of each key head) of one
-// length, at least least_steps, a tile to at most `most` of them; `units` bounds
-// their number.  most 1: none are cut.
+// How a call's steps are dealt out: to `units` workgroups a key head, in runs of one
+// length of at least least_steps, whose first and last tile may be parts of theirs.
+// units 0: a workgroup a tile, none in parts.
 struct Parts {
-  int most, least_steps, share, units;
+  int units, least_steps;
 };
 inline Parts parts(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
                    int64_t positions) {
@@ -46,13 +45,13 @@ inline Parts parts(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
   const int keys = rows == kFew ? kFewKeys : kKeys;
   const int64_t least = rows == kFew ? 8 : 16;
   const int64_t longest = (positions + keys - 1) / keys;
-  const int64_t share = rows == kFew ? std::max<int64_t>(1, (2048 + kv_heads - 1) / kv_heads)
-                                     : std::max<int64_t>(1, 512 / kv_heads - all);
-  const int64_t most = std::min<int64_t>({rows == kFew ? kMaxParts : kMaxParts / 4,
-                                          (longest + least - 1) / least, share});
-  if (most < 2 || batch > kMaxBatch || all > 4 * share) return {1, 0, 0, 0};
-  return {static_cast<int>(most), static_cast<int>(least), static_cast<int>(share),
-          static_cast<int>(share + all)};
+  const int64_t units = std::max<int64_t>(1, kResident / kv_heads);
+  // Many tiles of a few steps, and long prompts, are dealt by the dispatcher.
+  if (longest <= least || batch > kMaxBatch || all * longest >= (int64_t{1} << 31) ||
+      (rows == kMany && all > units))
+    return {0, 0};
+  return {static_cast<int>(std::min(units, (all * longest + least - 1) / least)),
+          static_cast<int>(least)};
 }
 
 inline int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
@@ -65,10 +64,8 @@ inline int64_t part_floats(int rows, int dim) {
 inline size_t workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int dim,
                         int64_t positions) {
   const Parts p = parts(tokens, batch, heads, kv_heads, positions);
-  if (p.most < 2) return 0;
-  const int64_t group = heads / kv_heads;
-  const int rows = tile_rows(tokens, batch, group);
-  return static_cast<size_t>(p.units * kv_heads * part_floats(rows, dim)) * sizeof(float);
+  const int rows = tile_rows(tokens, batch, heads / kv_heads);
+  return static_cast<size_t>(2 * p.units * kv_heads * part_floats(rows, dim)) * sizeof(float);
 }
 
 // n / d for n < 2^31 as (mulhi(n, mul) + n) >> shift.
