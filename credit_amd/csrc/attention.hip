@@ -10,8 +10,9 @@
 // weights, packed to bf16, are already the other product's operand, O^T = V^T P^T,
 // whose V^T comes from row-major LDS through transposing reads.  Products are
 // exact and summed in fp32; the weights' rounding to bf16 (2^-8 of each, sums are
-// taken before it) is what matrix units of this rate take.  m is raised only where
-// a score passes it by 2^8, so that the usual step rescales nothing.
+// taken before it) is what matrix units of this rate take.  m is that of the first
+// step, raised only where a score passes it by 2^16: floating point keeps the same
+// relative precision wherever it lies, and the usual step rescales nothing.
 //
 // Large tiles: four waves of 32 rows share every step's keys and values in LDS.
 // Small tiles (few rows, decode): four waves share the rows and take steps of the
@@ -37,7 +38,7 @@ using heads::Place;
 constexpr int kThreads = 256;
 constexpr int kNW = kThreads / kWave;
 constexpr float kNegInf = -__builtin_inff();
-constexpr float kRaise = 8.0f;  // log2 of the weights' largest value
+constexpr float kRaise = 16.0f;  // log2 of the weights' largest value
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
@@ -45,11 +46,20 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4_t;
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
+// LDS by its own 32-bit addresses: those of a step's reads differ in bits that an
+// exclusive or sets, one instruction each.  The kernels' LDS is one dynamic array,
+// which begins at address 0; its steps lie at multiples of 1 KiB.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(lds_ptr_t)(const_cast<void*>(p));
+}
+template <class T>
+__device__ __forceinline__ T lds_read(uint32_t at) {
+  return *(__attribute__((address_space(3))) const T*)(uintptr_t)at;
+}
 // Four positions of one element (column) for each lane of a group of 16: lane j of
 // it addresses row j / 4, columns 4 (j % 4) .. + 3, and gets column j of the rows.
-__device__ __forceinline__ bf16x4_t read_transposed(const char* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-      reinterpret_cast<lds_bf16x4_t*>((lds_ptr_t)(const_cast<char*>(p))));
+__device__ __forceinline__ bf16x4_t read_transposed(uint32_t at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(uintptr_t)at);
 }
 
 struct Cache {
@@ -68,6 +78,7 @@ struct Args {
   int64_t out_token, out_head;
   float* lse;  // [tokens, heads] or nullptr
   float* partial;      // parts' results, two a workgroup; nullptr: no parts
+  uint32_t partial_bytes;
   uint32_t* arrived;
   int64_t tokens;
   int batch, heads, kv_heads, group, dim;
@@ -293,7 +304,13 @@ __device__ __forceinline__ void clear(State<D>& s) {
 // are 0.
 __device__ __forceinline__ float base_of(float m) { return m == kNegInf ? 0.0f : m; }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+// Of lane l and lane l ^ 32: both values, in some order.
+__device__ __forceinline__ float2_t both_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
+                                                  __builtin_bit_cast(uint32_t, v), false, false);
+  const uint32_t a = r[0], b = r[1];  // a bit_cast of r[1] itself takes r[0]
+  return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
+}
 
 // The queries of a wave's rows: lane l holds elements 16 ks + 8 (l / 32) .. + 7 of
 // row l % 32.
@@ -312,28 +329,40 @@ __device__ __forceinline__ void load_queries(bf16x8_t (&q)[D / 16], const Args& 
   }
 }
 
+// A lane's places in a step's keys and values.  Its first chunk of keys (row l % 32,
+// chunk l / 32); those of elements 16 ks on are 32 ks away by exclusive or, those of
+// row 32 nb + l % 32 32 nb rows on.  Of the values the row and columns that it
+// addresses for a fragment of columns 0 .. 31; those of columns 32 db on are 64 db
+// away by exclusive or.
+struct Places {
+  uint32_t key, value;
+};
+template <int D>
+__device__ __forceinline__ Places places_of(int lane) {
+  const int row = 4 * (lane >> 5) + ((lane & 15) >> 2);
+  const int column = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  return {static_cast<uint32_t>(Lds<D>::key(lane & 31, lane >> 5)),
+          static_cast<uint32_t>(Lds<D>::value(row, column >> 3) + (column & 7) * 2)};
+}
 // A fragment of V^T: column 32 db + l % 32 of the 16 positions from 16 ts on, in
 // the weights' order (element e: position 16 ts + 8 (e / 4) + 4 (l / 32) + e % 4).
 template <int D>
-__device__ __forceinline__ bf16x8_t value_fragment(const char* v, int lane, int db, int ts) {
-  const int row = 16 * ts + 4 * (lane >> 5) + ((lane & 15) >> 2);
-  const int column = 32 * db + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-  const int at = Lds<D>::value(row, column >> 3) + (column & 7) * 2;
-  const bf16x4_t lo = read_transposed(v + at);
-  // 8 rows on: the swizzle is the same.
-  const bf16x4_t hi = read_transposed(v + at + 8 * Lds<D>::kRowBytes);
+__device__ __forceinline__ bf16x8_t value_fragment(uint32_t v, int db, int ts) {
+  const uint32_t at = (v ^ (64u * db)) + 16 * ts * Lds<D>::kRowBytes;
+  const bf16x4_t lo = read_transposed(at);
+  const bf16x4_t hi = read_transposed(at + 8 * Lds<D>::kRowBytes);
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // In steps where a mask hides positions from some rows, a value that is not finite
 // would make NaN of its weight of 0: whether there are any among `ROWS` rows.
 template <int D, int ROWS>
-__device__ __forceinline__ bool any_special(const char* v) {
-  const int lane = opaque_lane();
+__device__ __forceinline__ bool any_special(uint32_t v) {
+  const uint32_t own = v + static_cast<uint32_t>(opaque_lane()) * 16;
   uint32_t bad = 0;
 #pragma unroll 4
   for (int i = 0; i < ROWS * Lds<D>::kRowBytes / (16 * kWave); ++i) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(v + (i * kWave + lane) * 16);
+    const u32x4 w = lds_read<u32x4>(own + i * kWave * 16);
 #pragma unroll
     for (int e = 0; e < 4; ++e)  // bit 31 or 15: an exponent of all ones
       bad |= ((w[e] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
@@ -351,8 +380,7 @@ __device__ __forceinline__ bf16x8_t without_special(bf16x8_t v) {
 }
 // Adds them to the outputs of the rows that see them, whatever their weight.
 template <int D, int ROWS>
-__device__ __forceinline__ void add_special(State<D>& s, const char* v, int j0, int low,
-                                            int last) {
+__device__ __forceinline__ void add_special(State<D>& s, uint32_t v, int j0, int low, int last) {
 #pragma unroll 1
   for (int r = 0; r < ROWS; ++r) {
     const int lane = opaque_lane();
@@ -362,61 +390,71 @@ __device__ __forceinline__ void add_special(State<D>& s, const char* v, int j0, 
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int column = 32 * db + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-        const uint16_t bits = *reinterpret_cast<const uint16_t*>(
-            v + Lds<D>::value(r, column >> 3) + (column & 7) * 2);
+        const uint16_t bits =
+            lds_read<uint16_t>(v + Lds<D>::value(r, column >> 3) + (column & 7) * 2);
         s.o[db][i] += seen && (bits & 0x7F80u) == 0x7F80u ? bf16_to_f32(bits) : 0.0f;
       }
   }
 }
 
-// One step: NB blocks of 32 positions from j0 on, keys at k, values at v in LDS.
-// MASKED: a row sees those in [low, last] alone.  scored() runs once the keys have
-// been read, ready() before the values are.
-template <int D, int NB, bool MASKED, class Scored, class Ready>
-__device__ __forceinline__ void step(State<D>& s, const bf16x8_t (&q)[D / 16], const char* k,
-                                     const char* v, int j0, int low, int last, float scale_log2,
-                                     Scored&& scored, Ready&& ready) {
-  const int lane = opaque_lane();
-  f32x16 x[NB];
+// A step: NB blocks of 32 positions from j0 on, keys at k, values at v in LDS;
+// masked: a row sees those in [low, last] alone.
+struct Step {
+  uint32_t k, v;
+  int j0;
+  bool masked;
+  int low, last;
+};
+// What a step came to.  kRaise, kSpecial: nothing yet; the rows' maxima have to be
+// raised first, or the values hold what the mask must be kept from.  The loops over
+// the steps leave such steps to code behind them: a second way to the outputs inside
+// costs a copy of them in every step (64 registers; a prompt of 8192 tokens 602 us
+// against 470 without).
+enum class Outcome { kDone, kRaise, kSpecial };
+
+template <int D, int NB>
+__device__ __forceinline__ void scores(f32x16 (&x)[NB], const bf16x8_t (&q)[D / 16],
+                                       const Places& places, const Step& at) {
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[nb][i] = 0.0f;
+  const uint32_t key = places.key + at.k;
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      const int row = 32 * nb + (lane & 31);
-      const bf16x8_t f = *reinterpret_cast<const bf16x8_t*>(
-          k + Lds<D>::key(row, 2 * ks + (lane >> 5)));
-      x[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, q[ks], x[nb], 0, 0, 0);
-    }
-  }
-  scored();
-  float m = kNegInf;
+  for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+      x[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+          lds_read<bf16x8_t>((key ^ (32u * ks)) + 32 * nb * Lds<D>::kRowBytes), q[ks], x[nb], 0, 0,
+          0);
+}
+template <int NB>
+__device__ __forceinline__ void hide(f32x16 (&x)[NB], const Step& at) {
+  const int j0 = at.j0 + 4 * (opaque_lane() >> 5);
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      if constexpr (MASKED) {
-        const int j = j0 + 32 * nb + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-        x[nb][i] = j >= low && j <= last ? x[nb][i] : kNegInf;
-      }
-      m = fmaxf(m, x[nb][i]);
+      const int j = j0 + 32 * nb + 8 * (i >> 2) + (i & 3);
+      x[nb][i] = j >= at.low && j <= at.last ? x[nb][i] : kNegInf;
     }
-  m = fmaxf(m, other_half(m));
-  if (__builtin_amdgcn_ballot_w64((m - s.m) * scale_log2 > kRaise ||
-                                  (s.m == kNegInf && m != kNegInf)) != 0) {
-    const float raised = fmaxf(s.m, m);
-    const float by = __builtin_amdgcn_exp2f((s.m - base_of(raised)) * scale_log2);
-    const float factor = s.m == kNegInf ? 0.0f : by;
-    s.m = raised;
-    s.l *= factor;
+}
+// The scores' maximum of each row; NaN makes its row NaN.
+template <int NB>
+__device__ __forceinline__ float most(const f32x16 (&x)[NB]) {
+  float m = fmax_nan(x[0][0], x[0][1]);
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s.o[db][i] *= factor;
-  }
-  const float base = base_of(s.m) * scale_log2;
-  bf16x8_t p[2 * NB];
+    for (int i = nb == 0 ? 2 : 0; i < 16; ++i) m = fmax_nan(m, x[nb][i]);
+  const float2_t ms = both_halves(m);
+  return fmax_nan(ms.x, ms.y);
+}
+// The weights, as the other product's operand, and their sum.
+template <int NB>
+__device__ __forceinline__ float weights(bf16x8_t (&p)[2 * NB], const f32x16 (&x)[NB], float m,
+                                         float scale_log2) {
+  const float base = base_of(m) * scale_log2;
   float sum = 0.0f;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -434,24 +472,110 @@ __device__ __forceinline__ void step(State<D>& s, const bf16x8_t (&q)[D / 16], c
       }
       p[2 * nb + h] = __builtin_bit_cast(bf16x8_t, w);
     }
-  s.l += sum;
+  return sum;
+}
+// Whether a row's maximum has to be raised for a step's m; the first is taken as it
+// is, while o and l are 0 (or NaN).
+template <int D>
+__device__ __forceinline__ bool to_raise(State<D>& s, float m, float scale_log2) {
+  s.m = s.m == kNegInf ? m : s.m;
+  return __builtin_amdgcn_ballot_w64((m - s.m) * scale_log2 > kRaise) != 0;
+}
+// scored() runs once the keys have been read, ready() before the values are.
+template <int D, int NB, class Scored, class Ready>
+__device__ __forceinline__ Outcome step(State<D>& s, const bf16x8_t (&q)[D / 16],
+                                        const Places& places, const Step& at, float scale_log2,
+                                        Scored&& scored, Ready&& ready) {
+  if (at.masked) {
+    ready();
+    if (any_special<D, 32 * NB>(at.v)) return Outcome::kSpecial;
+  }
+  f32x16 x[NB];
+  scores<D, NB>(x, q, places, at);
+  if (at.masked) hide<NB>(x, at);
+  const float m = most<NB>(x);
+  if (to_raise(s, m, scale_log2)) return Outcome::kRaise;
+  scored();
+  bf16x8_t p[2 * NB];
+  s.l += weights<NB>(p, x, s.m, scale_log2);
   ready();
-  const bool special = MASKED && any_special<D, 32 * NB>(v);
-  if (!special) {
+  const uint32_t value = places.value + at.v;
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
+  for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-      for (int ts = 0; ts < 2 * NB; ++ts)
-        s.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_fragment<D>(v, lane, db, ts), p[ts],
-                                                          s.o[db], 0, 0, 0);
-  } else {
+    for (int ts = 0; ts < 2 * NB; ++ts)
+      s.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_fragment<D>(value, db, ts), p[ts],
+                                                        s.o[db], 0, 0, 0);
+  return Outcome::kDone;
+}
+// Raises the maxima of the rows to those of the step.
+template <int D, int NB>
+__device__ __forceinline__ void raise(State<D>& s, const bf16x8_t (&q)[D / 16],
+                                      const Places& places, const Step& at, float scale_log2) {
+  f32x16 x[NB];
+  scores<D, NB>(x, q, places, at);
+  if (at.masked) hide<NB>(x, at);
+  const float raised = fmax_nan(s.m, most<NB>(x));
+  const float factor =
+      s.m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((s.m - raised) * scale_log2);
+  s.m = raised;
+  s.l *= factor;
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
+  for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-      for (int ts = 0; ts < 2 * NB; ++ts)
-        s.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            without_special(value_fragment<D>(v, lane, db, ts)), p[ts], s.o[db], 0, 0, 0);
-    add_special<D, 32 * NB>(s, v, j0, low, last);
+    for (int i = 0; i < 16; ++i) s.o[db][i] *= factor;
+}
+// A masked step over values that are not finite; the same bits as step()'s where
+// they are hidden.
+template <int D, int NB>
+__device__ __forceinline__ void special_step(State<D>& s, const bf16x8_t (&q)[D / 16],
+                                             const Places& places, const Step& at,
+                                             float scale_log2) {
+  f32x16 x[NB];
+  scores<D, NB>(x, q, places, at);
+  hide<NB>(x, at);
+  if (to_raise(s, most<NB>(x), scale_log2)) raise<D, NB>(s, q, places, at, scale_log2);
+  bf16x8_t p[2 * NB];
+  s.l += weights<NB>(p, x, s.m, scale_log2);
+  const uint32_t value = places.value + at.v;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int ts = 0; ts < 2 * NB; ++ts)
+      s.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+          without_special(value_fragment<D>(value, db, ts)), p[ts], s.o[db], 0, 0, 0);
+  add_special<D, 32 * NB>(s, at.v, at.j0, at.low, at.last);
+}
+// The steps first, first + by, .. below last: at(i) gives one, begin(i) runs before
+// each, scored(i) and ready(i) as in step(), end(i) behind each.
+template <int D, int NB, class At, class Begin, class Scored, class Ready, class End>
+__device__ __forceinline__ void walk(State<D>& s, const bf16x8_t (&q)[D / 16],
+                                     const Places& places, float scale_log2, int first, int last,
+                                     int by, At&& at, Begin&& begin, Scored&& scored,
+                                     Ready&& ready, End&& end) {
+  int i = first;
+  if (i >= last) return;
+  begin(i);
+  while (true) {
+    Outcome out;
+    while (true) {
+      out = step<D, NB>(s, q, places, at(i), scale_log2, [&] { scored(i); }, [&] { ready(i); });
+      if (out != Outcome::kDone) break;
+      end(i);
+      i += by;
+      if (i >= last) return;
+      begin(i);
+    }
+    if (out == Outcome::kRaise) {
+      raise<D, NB>(s, q, places, at(i), scale_log2);
+      continue;
+    }
+    special_step<D, NB>(s, q, places, at(i), scale_log2);
+    scored(i);
+    end(i);
+    i += by;
+    if (i >= last) return;
+    begin(i);
   }
 }
 
@@ -497,57 +621,107 @@ __device__ __forceinline__ void finish(const State<D>& s, const Args& a, const W
 }
 
 // A part's results in the workspace: ROWS rows of D outputs, then the rows' maxima
-// and sums.
+// and sums; its first float.  A unit's first place is for the tile that it begins
+// in, its second for the one that begins within it.
 template <int D, int ROWS>
-__device__ __forceinline__ float* part_at(const Args& a, const Work& w, int part) {
-  // A unit's first place is for the tile that it begins in, its second for the one
-  // that begins within it.
-  const int64_t place = 2 * static_cast<int64_t>(w.unit + part) + (part == 0 ? w.inside : 0);
-  return a.partial + (place * a.kv_heads + w.head) * ROWS * (D + 2);
+__device__ __forceinline__ uint32_t part_at(const Args& a, const Work& w, int part) {
+  const uint32_t place = 2u * (w.unit + part) + (part == 0 ? w.inside : 0);
+  return (place * a.kv_heads + w.head) * (ROWS * (D + 2));
 }
-// Stores and loads of a part's results at device scope (sc1: past the die's own
-// L2), 16 bytes each; `part`: its resource.
+// Stores and loads of them at device scope (sc1: past the die's own L2).
 constexpr int kDeviceScope = 16;
-__device__ __forceinline__ void publish_quad(buffer_rsrc_t part, int at, f32x4 v) {
-  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, at * 4, 0,
+__device__ __forceinline__ buffer_rsrc_t parts_rsrc(const Args& a) {
+  return make_rsrc(a.partial, a.partial_bytes);
+}
+__device__ __forceinline__ void publish_quad(buffer_rsrc_t parts, uint32_t at, f32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), parts, at * 4, 0,
                                          kDeviceScope);
 }
-__device__ __forceinline__ f32x4 fetch_quad(buffer_rsrc_t part, int at) {
+__device__ __forceinline__ f32x4 fetch_quad(buffer_rsrc_t parts, uint32_t at) {
   return __builtin_bit_cast(
-      f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, at * 4, 0, kDeviceScope));
-}
-template <int D, int ROWS>
-__device__ __forceinline__ buffer_rsrc_t part_rsrc(float* at) {
-  return make_rsrc(at, ROWS * (D + 2) * sizeof(float));
+      f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, at * 4, 0, kDeviceScope));
 }
 
+// Four columns of a tile's row, finished.
+__device__ __forceinline__ void write_quad(const Args& a, const Work& w, int row, int d, f32x4 o,
+                                           float m, float l) {
+  const Row r = row_of(a, w, w.t.row0 + row);
+  if (a.lse != nullptr && d == 0) a.lse[r.token * a.heads + r.head] = lse_of(a, m, l);
+  if (d >= a.dim) return;
+  o *= inverse_of(l);
+  *reinterpret_cast<uint64_t*>(a.out + r.token * a.out_token + r.head * a.out_head + d) =
+      pack_bf16x2(o[0], o[1]) | static_cast<uint64_t>(pack_bf16x2(o[2], o[3])) << 32;
+}
 // All parts of a tile joined by its workgroup, in their order: four columns of a row
-// a thread, whose reads of eight parts are in flight together.
+// a thread and turn, the reads of kTurns turns and two parts in flight together; of
+// few rows the parts are dealt to several threads, which meet in LDS.
 template <int D, int ROWS>
-__device__ __forceinline__ void join(const Args& a, const Work& w) {
-  const int rows = min(ROWS, w.t.rows - w.t.row0);
-  for (int i = static_cast<int>(threadIdx.x); i < rows * (D / 4); i += kThreads) {
-    const int row = i / (D / 4), d = i % (D / 4) * 4;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    float m = kNegInf, l = 0.0f;
-#pragma unroll 8
-    for (int p = 0; p < w.parts; ++p) {
-      float* at = part_at<D, ROWS>(a, w, p);
-      const f32x4 po = fetch_quad(part_rsrc<D, ROWS>(at), row * D + d);
-      const float pm = fetch(at + ROWS * D + row), pl = fetch(at + ROWS * (D + 1) + row);
-      const float both = fmaxf(m, pm);
-      const float f = weight_of(a, m, both), pf = weight_of(a, pm, both);
-      o = o * f + po * pf;
-      l = l * f + pl * pf;
-      m = both;
+__device__ __forceinline__ void join(const Args& a, const Work& w, char* smem) {
+  const buffer_rsrc_t all = parts_rsrc(a);
+  constexpr int kQuads = D / 4;
+  constexpr int kTurns = ROWS == kFew ? 1 : 4;
+  const int rows = min(ROWS, w.t.rows - w.t.row0), items = rows * kQuads;
+  const int thread = static_cast<int>(threadIdx.x);
+  // Threads of a (row, quad).
+  const int several = items * 2 > kThreads ? 1 : kThreads / items;
+  const int which = several > 1 ? thread / items : 0;
+  for (int i0 = several > 1 ? thread % items : thread; i0 < items; i0 += kTurns * kThreads) {
+    f32x4 o[kTurns];
+    float m[kTurns], l[kTurns];
+    int row[kTurns], quad[kTurns];
+#pragma unroll
+    for (int n = 0; n < kTurns; ++n) {
+      const int i = min(i0 + n * kThreads, items - 1);
+      row[n] = i / kQuads;
+      quad[n] = i % kQuads;
+      o[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      m[n] = kNegInf;
+      l[n] = 0.0f;
     }
-    const Row r = row_of(a, w, w.t.row0 + row);
-    if (a.lse != nullptr && d == 0) a.lse[r.token * a.heads + r.head] = lse_of(a, m, l);
-    if (d >= a.dim) continue;
-    o *= inverse_of(l);
-    *reinterpret_cast<uint64_t*>(a.out + r.token * a.out_token + r.head * a.out_head + d) =
-        pack_bf16x2(o[0], o[1]) | static_cast<uint64_t>(pack_bf16x2(o[2], o[3])) << 32;
+    const int end = which < several ? w.parts : 0;
+#pragma unroll(ROWS == kFew ? 8 : 2)
+    for (int p = which; p < end; p += several) {
+      const uint32_t at = part_at<D, ROWS>(a, w, p);
+#pragma unroll
+      for (int n = 0; n < kTurns; ++n) {
+        const f32x4 po = fetch_quad(all, at + row[n] * D + 4 * quad[n]);
+        const float pm = fetch(a.partial + at + ROWS * D + row[n]);
+        const float pl = fetch(a.partial + at + ROWS * (D + 1) + row[n]);
+        const float both = fmax_nan(m[n], pm);
+        const float f = weight_of(a, m[n], both), pf = weight_of(a, pm, both);
+        o[n] = o[n] * f + po * pf;
+        l[n] = l[n] * f + pl * pf;
+        m[n] = both;
+      }
+    }
+    if (several > 1) {  // one turn
+      f32x4* os = reinterpret_cast<f32x4*>(smem);  // [thread]
+      float2_t* mls = reinterpret_cast<float2_t*>(os + kThreads);
+      os[thread] = o[0];
+      mls[thread] = float2_t{m[0], l[0]};
+    }
+    if (several == 1) {
+#pragma unroll
+      for (int n = 0; n < kTurns; ++n)
+        if (i0 + n * kThreads < items) write_quad(a, w, row[n], 4 * quad[n], o[n], m[n], l[n]);
+    }
   }
+  if (several == 1) return;
+  __syncthreads();
+  if (thread >= items) return;
+  const f32x4* os = reinterpret_cast<const f32x4*>(smem);
+  const float2_t* mls = reinterpret_cast<const float2_t*>(os + kThreads);
+  f32x4 o = os[thread];
+  float m = mls[thread].x, l = mls[thread].y;
+  for (int n = 1; n < min(several, w.parts); ++n) {
+    const float2_t ml = mls[n * items + thread];
+    const float both = fmax_nan(m, ml.x);
+    const float f = weight_of(a, m, both), pf = weight_of(a, ml.x, both);
+    o = o * f + os[n * items + thread] * pf;
+    l = l * f + ml.y * pf;
+    m = both;
+  }
+  write_quad(a, w, thread / kQuads, thread % kQuads * 4, o, m, l);
 }
 
 // Steps of a wave or workgroup: positions through registers into LDS.  W waves
@@ -740,23 +914,24 @@ __device__ __forceinline__ uint32_t* counter_of(const Args& a, const Work& w) {
 }
 // Whether this workgroup is the last of the tile's parts; its own results are
 // published.
-__device__ __forceinline__ bool last_of(uint32_t* counter, int parts, uint32_t* shared) {
+__device__ __forceinline__ bool last_of(uint32_t* counter, int parts, char* smem) {
   publish_wait();
-  __syncthreads();
+  __syncthreads();  // smem is free, too
+  uint32_t* before = reinterpret_cast<uint32_t*>(smem);
   if (threadIdx.x == 0) {
-    const uint32_t before = arrive(counter);
-    *shared = before;
-    if (before + 1 == static_cast<uint32_t>(parts)) counter_reset(counter);
+    *before = arrive(counter);
+    if (*before + 1 == static_cast<uint32_t>(parts)) counter_reset(counter);
   }
   __syncthreads();
-  return *shared + 1 == static_cast<uint32_t>(parts);
+  const bool last = *before + 1 == static_cast<uint32_t>(parts);
+  __syncthreads();
+  return last;
 }
 
 constexpr int kKeys = attention::kKeys;
 
 template <int D, int PIECE, bool PARTS>
-__device__ __forceinline__ void work_on_many(const Args& a, const Work& w, char* smem,
-                                             uint32_t* shared) {
+__device__ __forceinline__ void work_on_many(const Args& a, const Work& w, char* smem) {
   constexpr int kStage = 2 * kKeys * Lds<D>::kRowBytes;
   const Tile& t = w.t;
   const Range r = range_of(a, w, kMany, kKeys);
@@ -765,57 +940,49 @@ __device__ __forceinline__ void work_on_many(const Args& a, const Work& w, char*
   const int row = t.row0 + 32 * wave + (lane & 31);
   const int last = row < t.rows ? t.ahead + divide(row, a.by_group) : -1;
   const int low = a.window > 0 ? last - a.window + 1 : 0;
-  // Of the wave's rows: what all of them see and what any does.
+  // What all of the wave's rows see.
   const int wave_row = t.row0 + 32 * wave;
   // Rows that are not there need no mask: nothing of theirs is written.
   const int all_last = wave_row < t.rows ? t.ahead + divide(wave_row, a.by_group) : -1;
   const int any_last =
       wave_row < t.rows ? t.ahead + divide(min(wave_row + 31, t.rows - 1), a.by_group) : -1;
   const int all_low = a.window > 0 ? any_last - a.window + 1 : 0;
-  const int any_low =
-      a.window > 0 ? t.ahead + divide(min(wave_row, t.rows - 1), a.by_group) - a.window + 1 : 0;
   bf16x8_t q[D / 16];
   load_queries<D>(q, a, t, lane, row, w.head);
   State<D> s;
   clear(s);
   const int32_t* pages = a.pages + t.b * a.pages_ld;
-  const auto none = [] {};
-  const auto compute = [&](int i, const char* k) {
+  const Places places = places_of<D>(lane);
+  const uint32_t lds = static_cast<uint32_t>(uniform(static_cast<int>(lds_address(smem))));
+  const auto step_at = [&](int i) {
+    const uint32_t k = lds + ((i - r.first) & 1) * kStage;
     const int j0 = i * kKeys;
-    if (j0 > any_last || j0 + kKeys <= any_low) return;
-    if (j0 + kKeys - 1 <= all_last && j0 >= all_low)
-      step<D, kKeys / 32, false>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2, none,
-                                 none);
-    else
-      step<D, kKeys / 32, true>(s, q, k, k + kStage / 2, j0, low, last, a.scale_log2, none,
-                                 none);
+    return Step{k, k + kStage / 2, j0, j0 + kKeys - 1 > all_last || j0 < all_low, low, last};
   };
+  const auto none = [](int) {};
   if constexpr (PIECE > 0) {
-    const uint32_t lds = static_cast<uint32_t>(
-        uniform(static_cast<int>((uint32_t)(uintptr_t)(lds_ptr_t)smem) +
-                wave * (kKeys / kNW) * Lds<D>::kRowBytes));
+    const uint32_t own = lds + wave * (kKeys / kNW) * Lds<D>::kRowBytes;
     Direct<D, kKeys, kNW, PIECE> loads;
     loads.init(a, lane, wave);
-    const auto load = [&](int i, uint32_t at) {
-      loads.template load<true, false>(a, w.head, i * kKeys, r.end, wave, at);
-      loads.template load<false, false>(a, w.head, i * kKeys, r.end, wave, at + kStage / 2);
+    const auto load = [&](int i) {
+      const uint32_t to = own + ((i - r.first) & 1) * kStage;
+      loads.template load<true, false>(a, w.head, i * kKeys, r.end, wave, to);
+      loads.template load<false, false>(a, w.head, i * kKeys, r.end, wave, to + kStage / 2);
+      loads.look_up(a, pages, min(i + 1, r.last - 1) * kKeys, r.end, wave);
     };
     if (r.first < r.last) {
       loads.look_up(a, pages, r.first * kKeys, r.end, wave);
-      load(r.first, lds);
-      loads.look_up(a, pages, min(r.first + 1, r.last - 1) * kKeys, r.end, wave);
+      load(r.first);
     }
-    for (int i = r.first; i < r.last; ++i) {
-      const int stage = (i - r.first) & 1;
-      // This step's loads have landed; every wave has read the step before.
-      wait_loads<0>();
-      lds_barrier();
-      if (i + 1 < r.last) {
-        load(i + 1, lds + (stage ^ 1) * kStage);
-        loads.look_up(a, pages, min(i + 2, r.last - 1) * kKeys, r.end, wave);
-      }
-      compute(i, smem + stage * kStage);
-    }
+    walk<D, kKeys / 32>(
+        s, q, places, a.scale_log2, r.first, r.last, 1, step_at,
+        [&](int i) {
+          // This step's loads have landed; every wave has read the step before.
+          wait_loads<0>();
+          lds_barrier();
+          if (i + 1 < r.last) load(i + 1);
+        },
+        none, none, none);
   } else {
     Loader<D, kKeys, kNW> loader;
     const int thread = static_cast<int>(threadIdx.x);
@@ -823,54 +990,57 @@ __device__ __forceinline__ void work_on_many(const Args& a, const Work& w, char*
       loader.load(a, pages, w.head, r.first * kKeys, r.end, thread);
       loader.put(smem, smem + kStage / 2, thread);
     }
-    for (int i = r.first; i < r.last; ++i) {
-      __syncthreads();
-      char* next = smem + ((i - r.first + 1) & 1) * kStage;
-      const bool more = i + 1 < r.last;
-      if (more) loader.load(a, pages, w.head, (i + 1) * kKeys, r.end, thread);
-      compute(i, smem + ((i - r.first) & 1) * kStage);
-      if (more) loader.put(next, next + kStage / 2, thread);
-    }
+    walk<D, kKeys / 32>(
+        s, q, places, a.scale_log2, r.first, r.last, 1, step_at,
+        [&](int i) {
+          __syncthreads();
+          if (i + 1 < r.last) loader.load(a, pages, w.head, (i + 1) * kKeys, r.end, thread);
+        },
+        none, none,
+        [&](int i) {
+          char* next = smem + ((i - r.first + 1) & 1) * kStage;
+          if (i + 1 < r.last) loader.put(next, next + kStage / 2, thread);
+        });
   }
-  s.l += other_half(s.l);
+  const float2_t halves = both_halves(s.l);
+  s.l = halves.x + halves.y;
   if (!PARTS || w.parts == 1) {
     finish(s, a, w, row);
     return;
   }
-  float* at = part_at<D, kMany>(a, w, w.part);
-  const buffer_rsrc_t part = part_rsrc<D, kMany>(at);
+  const uint32_t at = part_at<D, kMany>(a, w, w.part);
+  const buffer_rsrc_t all = parts_rsrc(a);
   const int in_tile = 32 * wave + (lane & 31);
   if (row < t.rows) {
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        publish_quad(part, in_tile * D + 32 * db + 8 * i + 4 * (lane >> 5),
+        publish_quad(all, at + in_tile * D + 32 * db + 8 * i + 4 * (lane >> 5),
                      f32x4{s.o[db][4 * i], s.o[db][4 * i + 1], s.o[db][4 * i + 2],
                            s.o[db][4 * i + 3]});
   }
   if (lane < 32) {
-    publish(at + kMany * D + in_tile, s.m);
-    publish(at + kMany * (D + 1) + in_tile, s.l);
+    publish(a.partial + at + kMany * D + in_tile, s.m);
+    publish(a.partial + at + kMany * (D + 1) + in_tile, s.l);
   }
-  if (last_of(counter_of(a, w), w.parts, shared)) join<D, kMany>(a, w);
+  if (last_of(counter_of(a, w), w.parts, smem)) join<D, kMany>(a, w, smem);
 }
 
 template <int D, int PIECE, bool PARTS>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_many_kernel(
     const Args a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ uint32_t shared;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
   Cursor<kMany, kKeys, PARTS> cursor;
   Work w;
   cursor.start(a);
   if constexpr (PARTS) {
     while (cursor.next(w, a)) {
-      work_on_many<D, PIECE, true>(a, w, smem, &shared);
+      work_on_many<D, PIECE, true>(a, w, smem);
       __syncthreads();
     }
   } else if (cursor.next(w, a)) {
-    work_on_many<D, PIECE, false>(a, w, smem, &shared);
+    work_on_many<D, PIECE, false>(a, w, smem);
   }
 }
 
@@ -884,10 +1054,16 @@ __device__ __forceinline__ void wave_fence() {
 
 using attention::kFewKeys;  // positions of a wave's step
 
+// LDS of a workgroup's steps, where its waves' results meet behind them.
+template <int D>
+constexpr size_t kFewBytes = std::max<size_t>(size_t{kNW} * 2 * kFewKeys * Lds<D>::kRowBytes,
+                                              size_t{kNW} * kFew * (D + 4) * sizeof(float));
+
 template <int D, int PIECE, bool PARTS>
-__device__ __forceinline__ void work_on_few(const Args& a, const Work& w, char* smem,
-                                            float (&ms)[kNW][kFew], float (&ls)[kNW][kFew],
-                                            uint32_t* shared) {
+__device__ __forceinline__ void work_on_few(const Args& a, const Work& w, char* smem) {
+  using Rows = float[kNW][kFew];
+  Rows& ms = *reinterpret_cast<Rows*>(smem + kFewBytes<D>);  // the waves' maxima, sums
+  Rows& ls = *reinterpret_cast<Rows*>(smem + kFewBytes<D> + sizeof(Rows));
   constexpr int kStage = 2 * kFewKeys * Lds<D>::kRowBytes;
   const Tile& t = w.t;
   const Range r = range_of(a, w, kFew, kFewKeys);
@@ -907,18 +1083,15 @@ __device__ __forceinline__ void work_on_few(const Args& a, const Work& w, char* 
   clear(s);
   const int32_t* pages = a.pages + t.b * a.pages_ld;
   char* own = smem + wave * kStage;
-  const auto compute = [&](int i, auto&& scored, auto&& ready) {
+  const Places places = places_of<D>(lane);
+  const uint32_t lds = static_cast<uint32_t>(uniform(static_cast<int>(lds_address(own))));
+  const auto step_at = [&](int i) {
     const int j0 = i * kFewKeys;
-    if (j0 + kFewKeys - 1 <= all_last && j0 >= all_low)
-      step<D, kFewKeys / 32, false>(s, q, own, own + kStage / 2, j0, low, last, a.scale_log2,
-                                    scored, ready);
-    else
-      step<D, kFewKeys / 32, true>(s, q, own, own + kStage / 2, j0, low, last, a.scale_log2,
-                                   scored, ready);
+    return Step{lds, lds + kStage / 2, j0, j0 + kFewKeys - 1 > all_last || j0 < all_low, low,
+                last};
   };
+  const auto none = [](int) {};
   if constexpr (PIECE > 0) {
-    const uint32_t lds = static_cast<uint32_t>(
-        uniform(static_cast<int>((uint32_t)(uintptr_t)(lds_ptr_t)own)));
     Direct<D, kFewKeys, 1, PIECE> loads;
     constexpr int kPer = Direct<D, kFewKeys, 1, PIECE>::kPer;
     loads.init(a, lane, 0);
@@ -930,48 +1103,48 @@ __device__ __forceinline__ void work_on_few(const Args& a, const Work& w, char* 
       // Of the step after this one.
       loads.look_up(a, pages, min(i + kNW, r.last - 1) * kFewKeys, r.end, 0);
     };
-    int i = r.first + wave;
-    if (i < r.last) {
-      loads.look_up(a, pages, i * kFewKeys, r.end, 0);
-      load_keys(i);
-      load_values(i);
+    const int first = r.first + wave;
+    if (first < r.last) {
+      loads.look_up(a, pages, first * kFewKeys, r.end, 0);
+      load_keys(first);
+      load_values(first);
     }
-    // In flight at the loop's start: this step's keys, then its values.  The next
-    // step's keys are loaded once this one's have been read, its values likewise.
-    for (; i < r.last; i += kNW) {
-      const bool more = i + kNW < r.last;
-      wait_loads<kPer>();
-      compute(
-          i,
-          [&] {
-            wait_reads();
-            if (more) load_keys(i + kNW);
-          },
-          [&] {
-            if (more)
-              wait_loads<kPer>();
-            else
-              wait_loads<0>();
-          });
-      if (more) {
-        wait_reads();
-        load_values(i + kNW);
-      }
-    }
+    // In flight as a step begins: its keys, then its values.  The next step's keys
+    // are loaded once its own have been read, the values likewise.
+    walk<D, kFewKeys / 32>(
+        s, q, places, a.scale_log2, first, r.last, kNW, step_at,
+        [&](int) { wait_loads<kPer>(); },
+        [&](int i) {
+          wait_reads();
+          if (i + kNW < r.last) load_keys(i + kNW);
+        },
+        [&](int i) {
+          // A masked step waits for its values before the next keys are loaded.
+          if (i + kNW < r.last && !step_at(i).masked)
+            wait_loads<kPer>();
+          else
+            wait_loads<0>();
+        },
+        [&](int i) {
+          wait_reads();
+          if (i + kNW < r.last) load_values(i + kNW);
+        });
   } else {
     Loader<D, kFewKeys, 1> loader;
-    int i = r.first + wave;
-    if (i < r.last) loader.load(a, pages, w.head, i * kFewKeys, r.end, lane);
-    for (; i < r.last; i += kNW) {
-      loader.put(own, own + kStage / 2, lane);
-      wave_fence();
-      if (i + kNW < r.last)
-        loader.load(a, pages, w.head, (i + kNW) * kFewKeys, r.end, lane);
-      compute(i, [] {}, [] {});
-      wave_fence();
-    }
+    const int first = r.first + wave;
+    if (first < r.last) loader.load(a, pages, w.head, first * kFewKeys, r.end, lane);
+    walk<D, kFewKeys / 32>(
+        s, q, places, a.scale_log2, first, r.last, kNW, step_at,
+        [&](int i) {
+          loader.put(own, own + kStage / 2, lane);
+          wave_fence();
+          if (i + kNW < r.last)
+            loader.load(a, pages, w.head, (i + kNW) * kFewKeys, r.end, lane);
+        },
+        none, none, [&](int) { wave_fence(); });
   }
-  s.l += other_half(s.l);
+  const float2_t halves = both_halves(s.l);
+  s.l = halves.x + halves.y;
   // The waves' results, added in their order: rows of D and four more floats, which
   // spreads a column of rows over the banks.
   constexpr int kPitch = D + 4;
@@ -998,7 +1171,7 @@ __device__ __forceinline__ void work_on_few(const Args& a, const Work& w, char* 
   __syncthreads();
   const int rows = min(kFew, t.rows - t.row0);
   const bool parted = PARTS && w.parts > 1;
-  float* at = parted ? part_at<D, kFew>(a, w, w.part) : nullptr;
+  const uint32_t at = parted ? part_at<D, kFew>(a, w, w.part) : 0;
   const auto sum_of = [&](int in_tile, float& most) {
     most = kNegInf;
 #pragma unroll
@@ -1015,7 +1188,7 @@ __device__ __forceinline__ void work_on_few(const Args& a, const Work& w, char* 
     for (int n = 0; n < kNW; ++n)
       v += *reinterpret_cast<const f32x4*>(sums + (n * kFew + in_tile) * kPitch + d);
     if (parted) {
-      publish_quad(part_rsrc<D, kFew>(at), in_tile * D + d, v);
+      publish_quad(parts_rsrc(a), at + in_tile * D + d, v);
     } else if (d < a.dim) {
       float most;
       v *= inverse_of(sum_of(in_tile, most));
@@ -1029,33 +1202,31 @@ __device__ __forceinline__ void work_on_few(const Args& a, const Work& w, char* 
     float most;
     const float l = sum_of(in_tile, most);
     if (parted) {
-      publish(at + kFew * D + in_tile, most);
-      publish(at + kFew * (D + 1) + in_tile, l);
+      publish(a.partial + at + kFew * D + in_tile, most);
+      publish(a.partial + at + kFew * (D + 1) + in_tile, l);
     } else if (in_tile < rows && a.lse != nullptr) {
       const Row r0 = row_of(a, w, t.row0 + in_tile);
       a.lse[r0.token * a.heads + r0.head] = lse_of(a, most, l);
     }
   }
   if constexpr (PARTS)
-    if (parted && last_of(counter_of(a, w), w.parts, shared)) join<D, kFew>(a, w);
+    if (parted && last_of(counter_of(a, w), w.parts, smem)) join<D, kFew>(a, w, smem);
 }
 
 template <int D, int PIECE, bool PARTS>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_few_kernel(
     const Args a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ uint32_t shared;
-  __shared__ float ms[kNW][kFew], ls[kNW][kFew];
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
   Cursor<kFew, kFewKeys, PARTS> cursor;
   Work w;
   cursor.start(a);
   if constexpr (PARTS) {
     while (cursor.next(w, a)) {
-      work_on_few<D, PIECE, true>(a, w, smem, ms, ls, &shared);
+      work_on_few<D, PIECE, true>(a, w, smem);
       __syncthreads();
     }
   } else if (cursor.next(w, a)) {
-    work_on_few<D, PIECE, false>(a, w, smem, ms, ls, &shared);
+    work_on_few<D, PIECE, false>(a, w, smem);
   }
 }
 
@@ -1090,9 +1261,7 @@ int launch(const Args& a, int rows, hipStream_t stream) {
   };
   if (rows == kFew)
     return choose([&](auto piece, auto parts) {
-      constexpr size_t kBytes = std::max<size_t>(
-          size_t{kNW} * 2 * kFewKeys * Lds<D>::kRowBytes,
-          size_t{kNW} * kFew * (D + 4) * sizeof(float));
+      constexpr size_t kBytes = kFewBytes<D> + 2 * sizeof(float[kNW][kFew]);
       return launch_with<paged_attention_few_kernel<D, decltype(piece)::value,
                                                     decltype(parts)::value>>(
           a, kBytes, stream, "paged_attention_few_kernel");
@@ -1210,8 +1379,10 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
   if (parts.units > 0) {
     a.least_steps = parts.least_steps;
     char* base = nullptr;
-    CREDIT_TRY(acquire_workspace(
-        cfg, attention::workspace(tokens, batch, a.heads, a.kv_heads, dim, a.positions), &base));
+    const size_t bytes =
+        attention::workspace(tokens, batch, a.heads, a.kv_heads, dim, a.positions);
+    CREDIT_TRY(acquire_workspace(cfg, bytes, &base));
+    a.partial_bytes = static_cast<uint32_t>(bytes);
     a.partial = reinterpret_cast<float*>(ws_scratch(base));
     a.arrived = ws_counters(base) + kGroupCounterBase;
   }

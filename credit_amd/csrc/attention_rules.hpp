@@ -48,6 +48,7 @@ inline Parts parts(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
   const int64_t units = std::max<int64_t>(1, kResident / kv_heads);
   // Many tiles of a few steps, and long prompts, are dealt by the dispatcher.
   if (longest <= least || batch > kMaxBatch || all * longest >= (int64_t{1} << 31) ||
+      kv_heads > kResident ||  // places lie within 32-bit offsets
       (rows == kMany && all > units))
     return {0, 0};
   return {static_cast<int>(std::min(units, (all * longest + least - 1) / least)),
