@@ -62,6 +62,15 @@ __device__ __forceinline__ bf16x4_t read_transposed(uint32_t at) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(uintptr_t)at);
 }
 
+// The kernel's arguments, opaque to the compiler: read again where they are used
+// instead of kept in scalar registers over a loop that has none to spare.
+template <class A>
+__device__ __forceinline__ const A& arguments() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  __asm__ volatile("" : "+s"(p));
+  return *(const A*)p;
+}
+
 struct Cache {
   const uint16_t* data;
   int64_t page, slot, head;  // strides
@@ -409,7 +418,7 @@ struct Step {
 // raised first, or the values hold what the mask must be kept from.  The loops over
 // the steps leave such steps to code behind them: a second way to the outputs inside
 // costs a copy of them in every step (64 registers; a prompt of 8192 tokens 602 us
-// against 470 without).
+// against 575).
 enum class Outcome { kDone, kRaise, kSpecial };
 
 template <int D, int NB>
@@ -724,50 +733,35 @@ __device__ __forceinline__ void join(const Args& a, const Work& w, char* smem) {
   write_quad(a, w, thread / kQuads, thread % kQuads * 4, o, m, l);
 }
 
-// Steps of a wave or workgroup: positions through registers into LDS.  W waves
-// load one step of ROWS positions together.
+// A step's positions through registers into LDS, for pages of any size: W waves
+// copy ROWS positions from j0 on.  Those from `end` on are not read: their values are
+// 0, as those of pages outside the cache, whose keys are NaN.
 template <int D, int ROWS, int W>
-struct Loader {
-  static constexpr int kPer = ROWS * Lds<D>::kChunks / (kWave * W);  // 16-byte loads a lane
-  u32x4 k[kPer], v[kPer];
-
-  // Positions j0 + r, r < ROWS; those from `end` on are not read: their values
-  // are 0, as those of pages outside the cache, whose keys are NaN.
-  __device__ __forceinline__ void load(const Args& a, const int32_t* pages, int head, int j0,
-                                       int end, int thread) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int at = thread + i * kWave * W;
-      const int row = at / Lds<D>::kChunks, chunk = at % Lds<D>::kChunks;
-      const int j = j0 + row;
-      u32x4 kv = {0, 0, 0, 0}, vv = kv;
-      if (j < end && chunk * 8 < a.dim) {
-        const int column = divide(j, a.by_page);
-        const int page = pages[column];
-        if (page >= 0 && page < a.n_pages) {
-          const int64_t slot = j - column * a.page_size;
-          kv = *reinterpret_cast<const u32x4*>(a.k.data + page * a.k.page + slot * a.k.slot +
-                                               head * a.k.head + chunk * 8);
-          vv = *reinterpret_cast<const u32x4*>(a.v.data + page * a.v.page + slot * a.v.slot +
-                                               head * a.v.head + chunk * 8);
-        } else {
-          kv = u32x4{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
-        }
+__device__ __forceinline__ void copy_step(const Args& a, const int32_t* pages, int head, int j0,
+                                          int end, int thread, char* key, char* value) {
+#pragma unroll 2
+  for (int i = 0; i < ROWS * Lds<D>::kChunks / (kWave * W); ++i) {
+    const int at = thread + i * kWave * W;
+    const int row = at / Lds<D>::kChunks, chunk = at % Lds<D>::kChunks;
+    const int j = j0 + row;
+    u32x4 k = {0, 0, 0, 0}, v = k;
+    if (j < end && chunk * 8 < a.dim) {
+      const int column = divide(j, a.by_page);
+      const int page = pages[column];
+      if (page >= 0 && page < a.n_pages) {
+        const int64_t slot = j - column * a.page_size;
+        k = *reinterpret_cast<const u32x4*>(a.k.data + page * a.k.page + slot * a.k.slot +
+                                            head * a.k.head + chunk * 8);
+        v = *reinterpret_cast<const u32x4*>(a.v.data + page * a.v.page + slot * a.v.slot +
+                                            head * a.v.head + chunk * 8);
+      } else {
+        k = u32x4{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
       }
-      k[i] = kv;
-      v[i] = vv;
     }
+    *reinterpret_cast<u32x4*>(key + Lds<D>::key(row, chunk)) = k;
+    *reinterpret_cast<u32x4*>(value + Lds<D>::value(row, chunk)) = v;
   }
-  __device__ __forceinline__ void put(char* key, char* value, int thread) const {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int at = thread + i * kWave * W;
-      const int row = at / Lds<D>::kChunks, chunk = at % Lds<D>::kChunks;
-      *reinterpret_cast<u32x4*>(key + Lds<D>::key(row, chunk)) = k[i];
-      *reinterpret_cast<u32x4*>(value + Lds<D>::value(row, chunk)) = v[i];
-    }
-  }
-};
+}
 
 // One LDS-direct load: 16 bytes a lane from offset `off` of the resource to LDS at
 // `lds` + AT + 16 lane.  In inline assembly, as the compiler would wait for every
@@ -984,23 +978,15 @@ __device__ __forceinline__ void work_on_many(const Args& a, const Work& w, char*
         },
         none, none, none);
   } else {
-    Loader<D, kKeys, kNW> loader;
-    const int thread = static_cast<int>(threadIdx.x);
-    if (r.first < r.last) {
-      loader.load(a, pages, w.head, r.first * kKeys, r.end, thread);
-      loader.put(smem, smem + kStage / 2, thread);
-    }
     walk<D, kKeys / 32>(
         s, q, places, a.scale_log2, r.first, r.last, 1, step_at,
         [&](int i) {
+          char* to = smem + ((i - r.first) & 1) * kStage;
+          copy_step<D, kKeys, kNW>(a, pages, w.head, i * kKeys, r.end,
+                                   static_cast<int>(threadIdx.x), to, to + kStage / 2);
           __syncthreads();
-          if (i + 1 < r.last) loader.load(a, pages, w.head, (i + 1) * kKeys, r.end, thread);
         },
-        none, none,
-        [&](int i) {
-          char* next = smem + ((i - r.first + 1) & 1) * kStage;
-          if (i + 1 < r.last) loader.put(next, next + kStage / 2, thread);
-        });
+        none, none, none);
   }
   const float2_t halves = both_halves(s.l);
   s.l = halves.x + halves.y;
@@ -1035,8 +1021,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_ma
   Work w;
   cursor.start(a);
   if constexpr (PARTS) {
-    while (cursor.next(w, a)) {
-      work_on_many<D, PIECE, true>(a, w, smem);
+    while (cursor.next(w, arguments<Args>())) {
+      work_on_many<D, PIECE, true>(arguments<Args>(), w, smem);
       __syncthreads();
     }
   } else if (cursor.next(w, a)) {
@@ -1130,18 +1116,15 @@ __device__ __forceinline__ void work_on_few(const Args& a, const Work& w, char* 
           if (i + kNW < r.last) load_values(i + kNW);
         });
   } else {
-    Loader<D, kFewKeys, 1> loader;
-    const int first = r.first + wave;
-    if (first < r.last) loader.load(a, pages, w.head, first * kFewKeys, r.end, lane);
     walk<D, kFewKeys / 32>(
-        s, q, places, a.scale_log2, first, r.last, kNW, step_at,
+        s, q, places, a.scale_log2, r.first + wave, r.last, kNW, step_at,
         [&](int i) {
-          loader.put(own, own + kStage / 2, lane);
           wave_fence();
-          if (i + kNW < r.last)
-            loader.load(a, pages, w.head, (i + kNW) * kFewKeys, r.end, lane);
+          copy_step<D, kFewKeys, 1>(a, pages, w.head, i * kFewKeys, r.end, lane, own,
+                                    own + kStage / 2);
+          wave_fence();
         },
-        none, none, [&](int) { wave_fence(); });
+        none, none, none);
   }
   const float2_t halves = both_halves(s.l);
   s.l = halves.x + halves.y;
@@ -1221,8 +1204,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void paged_attention_fe
   Work w;
   cursor.start(a);
   if constexpr (PARTS) {
-    while (cursor.next(w, a)) {
-      work_on_few<D, PIECE, true>(a, w, smem);
+    while (cursor.next(w, arguments<Args>())) {
+      work_on_few<D, PIECE, true>(arguments<Args>(), w, smem);
       __syncthreads();
     }
   } else if (cursor.next(w, a)) {
