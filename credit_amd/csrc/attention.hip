@@ -651,86 +651,126 @@ __device__ __forceinline__ f32x4 fetch_quad(buffer_rsrc_t parts, uint32_t at) {
       f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, at * 4, 0, kDeviceScope));
 }
 
-// Four columns of a tile's row, finished.
-__device__ __forceinline__ void write_quad(const Args& a, const Work& w, int row, int d, f32x4 o,
-                                           float m, float l) {
-  const Row r = row_of(a, w, w.t.row0 + row);
-  if (a.lse != nullptr && d == 0) a.lse[r.token * a.heads + r.head] = lse_of(a, m, l);
-  if (d >= a.dim) return;
-  o *= inverse_of(l);
-  *reinterpret_cast<uint64_t*>(a.out + r.token * a.out_token + r.head * a.out_head + d) =
-      pack_bf16x2(o[0], o[1]) | static_cast<uint64_t>(pack_bf16x2(o[2], o[3])) << 32;
-}
-// All parts of a tile joined by its workgroup, in their order: four columns of a row
-// a thread and turn, the reads of kTurns turns and two parts in flight together; of
-// few rows the parts are dealt to several threads, which meet in LDS.
+// All parts of a tile joined by its workgroup, in their order: first the rows'
+// maxima and sums over all parts, then, kMost parts at a time, each part's weight of
+// each row into LDS and four columns of a row a thread and turn, the reads of kTurns
+// turns and kParts parts in flight together.  Of few rows the parts are dealt to
+// several threads, which meet in LDS.
 template <int D, int ROWS>
 __device__ __forceinline__ void join(const Args& a, const Work& w, char* smem) {
   const buffer_rsrc_t all = parts_rsrc(a);
   constexpr int kQuads = D / 4;
-  constexpr int kTurns = ROWS == kFew ? 1 : 4;
+  constexpr int kTurns = ROWS == kFew ? 1 : 4, kParts = ROWS == kFew ? 8 : 4;
+  constexpr int kMost = ROWS == kFew ? kWave : 16;
   const int rows = min(ROWS, w.t.rows - w.t.row0), items = rows * kQuads;
   const int thread = static_cast<int>(threadIdx.x);
+  const int lane = thread & (kWave - 1), wave = thread / kWave;
+  float* weight = reinterpret_cast<float*>(smem);           // [kMost][ROWS]
+  float2_t* total = reinterpret_cast<float2_t*>(weight + kMost * ROWS);  // maximum, 1 / sum
+  f32x4* meet = reinterpret_cast<f32x4*>(total + ROWS);     // [kThreads]
+  const auto most_of = [&](int part, int row) {
+    return fetch(a.partial + part_at<D, ROWS>(a, w, part) + ROWS * D + row);
+  };
+  const auto sum_of = [&](int part, int row) {
+    return fetch(a.partial + part_at<D, ROWS>(a, w, part) + ROWS * (D + 1) + row);
+  };
+  const auto finished = [&](int row, float m, float l) {
+    total[row] = float2_t{m, inverse_of(l)};
+    const Row r = row_of(a, w, w.t.row0 + row);
+    if (a.lse != nullptr) a.lse[r.token * a.heads + r.head] = lse_of(a, m, l);
+  };
+  if constexpr (ROWS == kFew) {  // a lane a part
+#pragma unroll 1
+    for (int row = wave; row < rows; row += kNW) {
+      float m = kNegInf, l = 0.0f;
+#pragma unroll 1
+      for (int p = lane; p < w.parts; p += kWave) {
+        const float own = most_of(p, row), sum = sum_of(p, row);
+        const float raised = fmax_nan(m, own);
+        l = l * weight_of(a, m, raised) + sum * weight_of(a, own, raised);
+        m = raised;
+      }
+      const float raised = wave_reduce(m, MaxOp());
+      l = wave_reduce(l * weight_of(a, m, raised), SumOp());
+      if (lane == 0) finished(row, raised, l);
+    }
+  } else if (thread < rows) {  // a thread a row
+    float m = kNegInf, l = 0.0f;
+#pragma unroll 4
+    for (int p = 0; p < w.parts; ++p) {
+      const float own = most_of(p, thread), sum = sum_of(p, thread);
+      const float raised = fmax_nan(m, own);
+      l = l * weight_of(a, m, raised) + sum * weight_of(a, own, raised);
+      m = raised;
+    }
+    finished(thread, m, l);
+  }
+  __syncthreads();
   // Threads of a (row, quad).
   const int several = items * 2 > kThreads ? 1 : kThreads / items;
   const int which = several > 1 ? thread / items : 0;
-  for (int i0 = several > 1 ? thread % items : thread; i0 < items; i0 += kTurns * kThreads) {
+  const int own = several > 1 ? thread - which * items : thread;
+#pragma unroll 1
+  for (int turn = 0; turn * kThreads < items; turn += kTurns) {
     f32x4 o[kTurns];
-    float m[kTurns], l[kTurns];
-    int row[kTurns], quad[kTurns];
+    int item[kTurns];
 #pragma unroll
     for (int n = 0; n < kTurns; ++n) {
-      const int i = min(i0 + n * kThreads, items - 1);
-      row[n] = i / kQuads;
-      quad[n] = i % kQuads;
       o[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      m[n] = kNegInf;
-      l[n] = 0.0f;
+      item[n] = min(own + (several > 1 ? 0 : (turn + n) * kThreads), items - 1);
     }
-    const int end = which < several ? w.parts : 0;
-#pragma unroll(ROWS == kFew ? 8 : 2)
-    for (int p = which; p < end; p += several) {
-      const uint32_t at = part_at<D, ROWS>(a, w, p);
+#pragma unroll 1
+    for (int p0 = 0; p0 < w.parts; p0 += kMost) {
+      const int parts = min(kMost, w.parts - p0);
+      if (turn == 0 || w.parts > kMost) {
+        __syncthreads();
+#pragma unroll 2
+        for (int i = thread; i < parts * rows; i += kThreads) {
+          const int p = i / rows, row = i - p * rows;
+          const float2_t of = total[row];
+          weight[p * ROWS + row] = weight_of(a, most_of(p0 + p, row), of.x) * of.y;
+        }
+        __syncthreads();
+      }
+#pragma unroll 1
+      for (int p1 = which; p1 < parts; p1 += several * kParts) {
+        f32x4 v[kParts][kTurns];
 #pragma unroll
-      for (int n = 0; n < kTurns; ++n) {
-        const f32x4 po = fetch_quad(all, at + row[n] * D + 4 * quad[n]);
-        const float pm = fetch(a.partial + at + ROWS * D + row[n]);
-        const float pl = fetch(a.partial + at + ROWS * (D + 1) + row[n]);
-        const float both = fmax_nan(m[n], pm);
-        const float f = weight_of(a, m[n], both), pf = weight_of(a, pm, both);
-        o[n] = o[n] * f + po * pf;
-        l[n] = l[n] * f + pl * pf;
-        m[n] = both;
+        for (int p = 0; p < kParts; ++p) {
+          const uint32_t at = part_at<D, ROWS>(a, w, p0 + min(p1 + p * several, parts - 1));
+#pragma unroll
+          for (int n = 0; n < kTurns; ++n) v[p][n] = fetch_quad(all, at + 4 * item[n]);
+        }
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+          const int part = p1 + p * several;
+#pragma unroll
+          for (int n = 0; n < kTurns; ++n) {
+            const float f = weight[min(part, parts - 1) * ROWS + item[n] / kQuads];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o[n][e] = part < parts ? __builtin_fmaf(v[p][n][e], f, o[n][e]) : o[n][e];
+          }
+        }
       }
     }
-    if (several > 1) {  // one turn
-      f32x4* os = reinterpret_cast<f32x4*>(smem);  // [thread]
-      float2_t* mls = reinterpret_cast<float2_t*>(os + kThreads);
-      os[thread] = o[0];
-      mls[thread] = float2_t{m[0], l[0]};
+    if (several > 1) {
+      meet[thread] = o[0];
+      __syncthreads();
+      for (int n = 1; n < several && which == 0; ++n) o[0] += meet[n * items + own];
     }
-    if (several == 1) {
 #pragma unroll
-      for (int n = 0; n < kTurns; ++n)
-        if (i0 + n * kThreads < items) write_quad(a, w, row[n], 4 * quad[n], o[n], m[n], l[n]);
+    for (int n = 0; n < kTurns; ++n) {
+      const int i = own + (several > 1 ? 0 : (turn + n) * kThreads);
+      if (i >= items || (several > 1 && (n > 0 || which > 0))) continue;
+      const int row = i / kQuads, d = i % kQuads * 4;
+      if (d >= a.dim) continue;
+      const Row r = row_of(a, w, w.t.row0 + row);
+      *reinterpret_cast<uint64_t*>(a.out + r.token * a.out_token + r.head * a.out_head + d) =
+          pack_bf16x2(o[n][0], o[n][1]) |
+          static_cast<uint64_t>(pack_bf16x2(o[n][2], o[n][3])) << 32;
     }
   }
-  if (several == 1) return;
-  __syncthreads();
-  if (thread >= items) return;
-  const f32x4* os = reinterpret_cast<const f32x4*>(smem);
-  const float2_t* mls = reinterpret_cast<const float2_t*>(os + kThreads);
-  f32x4 o = os[thread];
-  float m = mls[thread].x, l = mls[thread].y;
-  for (int n = 1; n < min(several, w.parts); ++n) {
-    const float2_t ml = mls[n * items + thread];
-    const float both = fmax_nan(m, ml.x);
-    const float f = weight_of(a, m, both), pf = weight_of(a, ml.x, both);
-    o = o * f + os[n * items + thread] * pf;
-    l = l * f + ml.y * pf;
-    m = both;
-  }
-  write_quad(a, w, thread / kQuads, thread % kQuads * 4, o, m, l);
 }
 
 // A step's positions through registers into LDS, for pages of any size: W waves
