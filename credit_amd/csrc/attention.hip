@@ -1269,9 +1269,8 @@ int launch_with(const Args& a, size_t lds, hipStream_t stream, const char* name)
 }
 template <int D>
 int launch(const Args& a, int rows, hipStream_t stream) {
-  // Pieces of 16 rows, of a load's, or through registers where pages hold no whole
-  // number of them or a piece's offsets pass 31 bits.
-  constexpr int kRows = Direct<D, kKeys, kNW, 16>::kRows;
+  // Pieces of 16 rows or 8, or through registers where pages hold no whole number of
+  // them or a piece's offsets pass 31 bits.
   constexpr int64_t kMost = int64_t{1} << 25;
   const bool near = a.k.slot < kMost && a.v.slot < kMost;
   const auto choose = [&](auto&& with) {
@@ -1279,7 +1278,7 @@ int launch(const Args& a, int rows, hipStream_t stream) {
       return a.partial != nullptr ? with(piece, std::true_type{}) : with(piece, std::false_type{});
     };
     if (near && a.page_size % 16 == 0) return parts(std::integral_constant<int, 16>{});
-    if (near && a.page_size % kRows == 0) return parts(std::integral_constant<int, kRows>{});
+    if (near && a.page_size % 8 == 0) return parts(std::integral_constant<int, 8>{});
     return parts(std::integral_constant<int, 0>{});
   };
   if (rows == kFew)
