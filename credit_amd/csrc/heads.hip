@@ -26,7 +26,6 @@ using heads::kMaxDim;
 using heads::Place;
 
 constexpr int kThreads = 256;
-constexpr int64_t kMaxGrid = int64_t{1} << 23;  // a grid's threads fit 32 bits
 
 template <class T, int N>
 using Raw = T __attribute__((ext_vector_type(N)));
@@ -45,11 +44,13 @@ __device__ __forceinline__ float widen(T v) {
   else
     return bf16_to_f32(v);
 }
-template <class T, int N>
+template <class T, int N, bool NT = false>
 __device__ __forceinline__ Unit<T, N> load_unit(const T* p) {
   Unit<T, N> u;
   if constexpr (N == 1)
     u.v = *p;
+  else if constexpr (NT)
+    u.v = __builtin_nontemporal_load(reinterpret_cast<const Raw<T, N>*>(p));
   else
     u.v = *reinterpret_cast<const Raw<T, N>*>(p);
   return u;
@@ -83,10 +84,12 @@ __device__ __forceinline__ Unit<T, N> narrow_unit(const float (&f)[N]) {
   }
   return u;
 }
-template <class T, int N>
+template <class T, int N, bool NT = false>
 __device__ __forceinline__ void store_unit(T* p, const Unit<T, N>& u) {
   if constexpr (N == 1)
     *p = u.v;
+  else if constexpr (NT)
+    __builtin_nontemporal_store(u.v, reinterpret_cast<Raw<T, N>*>(p));
   else
     *reinterpret_cast<Raw<T, N>*>(p) = u.v;
 }
@@ -103,14 +106,12 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// sin and cos of position * freq radians.  The angle in turns, its nearest
-// quarter taken off, in 64 bits: of positions up to 2^31 more than 20 bits behind
-// the point stay.  What is left lies in +-pi/4, where the Taylor polynomials of
-// degree 9 and 10 are within 2e-9 and 1e-10 of the functions.
-__device__ __forceinline__ void sincos_at(double position, float freq, float& s, float& c) {
-  constexpr double kInv2Pi = 0.15915494309189533576888;
+// sin and cos of an angle of `turns`, its nearest quarter taken off in 64 bits: of
+// positions up to 2^31 more than 20 bits behind the point stay.  What is left lies in
+// +-pi/4, where the Taylor polynomials of degree 9 and 10 are within 2e-9 and 1e-10 of
+// the functions.
+__device__ __forceinline__ void sincos_of(double turns, float& s, float& c) {
   constexpr float k2Pi = 6.28318530717958647692528f;
-  const double turns = position * (static_cast<double>(freq) * kInv2Pi);
   const double part = turns - __builtin_rint(turns);  // [-1/2, 1/2]
   const double quarter = __builtin_rint(4.0 * part);
   const float x = static_cast<float>(__builtin_fma(quarter, -0.25, part)) * k2Pi;
@@ -139,6 +140,7 @@ struct Rotation {
   int interleaved;
   float magnitude;
   float sign;  // of the angle: -1 for the transposed
+  int whole;   // every element is turned
 };
 
 // The two units of lane `p` of a head and what turns them.
@@ -165,24 +167,47 @@ __device__ __forceinline__ Seat<N> seat_of(int p, int dim, const Rotation& r) {
   s.turn_b = s.eb < r.rot;
   return s;
 }
+// Turns a position of lane p's pairs.
 template <int N>
-__device__ __forceinline__ void angles_of(float (&c)[N], float (&s)[N], int p, int64_t token,
-                                          const Rotation& r) {
-  const double position = p * N < r.rot / 2 ? static_cast<double>(r.positions[token]) : 0.0;
+__device__ __forceinline__ void turns_of(double (&f)[N], int p, const Rotation& r) {
+  constexpr double kInv2Pi = 0.15915494309189533576888;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    f[j] = p * N + j < r.rot / 2 ? static_cast<double>(r.inv_freq[p * N + j]) * kInv2Pi : 0.0;
+}
+template <int N>
+__device__ __forceinline__ void angles_of(float (&c)[N], float (&s)[N], const double (&f)[N],
+                                          int64_t token, const Rotation& r) {
+  const double position = static_cast<double>(r.positions[token]);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int i = p * N + j;
-    const float f = i < r.rot / 2 ? r.inv_freq[i] : 0.0f;
-    sincos_at(position, f, s[j], c[j]);
+    sincos_of(position * f[j], s[j], c[j]);
     c[j] *= r.magnitude;
     s[j] *= r.magnitude * r.sign;
   }
 }
+// v^(-1/2): the instruction's, within a step, and one step of Newton's method.  The
+// instruction takes subnormal numbers for 0, so small ones are raised by 2^64.
+__device__ __forceinline__ float inverse_root(float v) {
+  const bool small = v < 0x1p-64f;
+  const float u = small ? v * 0x1p64f : v;
+  float r = __builtin_amdgcn_rsqf(u);
+  if (u > 0.0f && u < __builtin_inff())
+    r = __builtin_fmaf(0.5f * r, __builtin_fmaf(-u * r, r, 1.0f), r);
+  return small ? r * 0x1p32f : r;
+}
 // Units without a rotated pair keep their elements, whatever the other holds.
 template <int N>
 __device__ __forceinline__ void turn(float (&a)[N], float (&b)[N], const float (&c)[N],
-                                     const float (&s)[N], const Seat<N>& seat, bool interleaved) {
-  if (N == 1 || !interleaved) {
+                                     const float (&s)[N], const Seat<N>& seat, const Rotation& r) {
+  if (r.whole != 0 && (N == 1 || r.interleaved == 0)) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float x = a[j], y = b[j];
+      a[j] = __builtin_fmaf(x, c[j], -(y * s[j]));
+      b[j] = __builtin_fmaf(y, c[j], x * s[j]);
+    }
+  } else if (N == 1 || r.interleaved == 0) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float x = a[j], y = b[j];
@@ -229,7 +254,10 @@ struct ForwardArgs {
   float eps;
 };
 
-template <class T, int N, int G, int U, int RUN>
+// WHOLE: lanes, units and heads go evenly: dim = 2 N G, and every unit has RUN
+// heads.  NT: loads and stores with the nontemporal hint.  Workgroups loop over
+// units.
+template <class T, int N, int G, int U, int RUN, bool WHOLE, bool NT>
 __global__ __launch_bounds__(kThreads) void heads_fwd_kernel(const ForwardArgs<T> a) {
   int which = 0;
   if (a.sides > 1 && blockIdx.x >= a.side[1].first_block) which = 1;
@@ -240,30 +268,46 @@ __global__ __launch_bounds__(kThreads) void heads_fwd_kernel(const ForwardArgs<T
       side.first_block;
   const int lane = static_cast<int>(threadIdx.x) % G;
   const int groups = 1 << side.groups_log;
+  const bool turned = a.r.rot > 0 && side.plain == 0;
   Seat<N> seat[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) seat[u] = seat_of<N>(lane + G * u, a.dim, a.r);
+  double freq[U][N];
   float wa[U][N], wb[U][N];
   const bool norm = side.w != nullptr;
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+  for (int u = 0; u < U; ++u) {
+    seat[u] = seat_of<N>(lane + G * u, a.dim, a.r);
+    if constexpr (WHOLE) seat[u].has_a = seat[u].has_b = true;
 #pragma unroll
     for (int j = 0; j < N; ++j) wa[u][j] = wb[u][j] = 0.0f;
-  if (norm) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
+    if (norm) {
       if (seat[u].has_a) widen_unit<T, N>(wa[u], load_unit<T, N>(side.w + seat[u].ea));
       if (seat[u].has_b) widen_unit<T, N>(wb[u], load_unit<T, N>(side.w + seat[u].eb));
     }
+    if (turned) turns_of<N>(freq[u], lane + G * u, a.r);
   }
+  const float inv_dim = 1.0f / static_cast<float>(a.dim);
   for (int64_t unit = (blockIdx.x - side.first_block) * (kThreads / G) +
                       static_cast<int>(threadIdx.x) / G;
        unit < side.units; unit += blocks * (kThreads / G)) {
     const int64_t token = unit >> side.groups_log;
     const int first = static_cast<int>(unit & (groups - 1));
-    if (first >= side.heads) continue;
-    const T* x = side.x + token * side.x_token;
-    T* y = side.y;
+    if (!WHOLE && first >= side.heads) continue;
+    const T* x = side.x + token * side.x_token + first * side.x_head;
+    const int64_t x_step = groups * side.x_head, y_step = groups * side.y_head;
+    // On their way while the angles are taken.
+    Unit<T, N> ra[RUN][U], rb[RUN][U];
+#pragma unroll
+    for (int k = 0; k < RUN; ++k) {
+      const T* p = x + (WHOLE || first + k * groups < side.heads ? k : 0) * x_step;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        ra[k][u].v = 0;
+        rb[k][u].v = 0;
+        if (seat[u].has_a) ra[k][u] = load_unit<T, N, NT>(p + seat[u].ea);
+        if (seat[u].has_b) rb[k][u] = load_unit<T, N, NT>(p + seat[u].eb);
+      }
+    }
+    T* y = side.y + first * side.y_head;
     bool keep = true;
     if (side.slots != nullptr) {
       const int64_t slot = side.slots[token];
@@ -273,58 +317,41 @@ __global__ __launch_bounds__(kThreads) void heads_fwd_kernel(const ForwardArgs<T
     } else {
       y += token * side.y_token;
     }
-    float c[U][N], s[U][N];
-    if (a.r.rot > 0 && side.plain == 0) {
+    if (side.plain != 0) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) angles_of<N>(c[u], s[u], lane + G * u, token, a.r);
-    } else {
+      for (int k = 0; k < RUN; ++k) {
+        if (!keep || (!WHOLE && first + k * groups >= side.heads)) break;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          c[u][j] = 1.0f;
-          s[u][j] = 0.0f;
+        for (int u = 0; u < U; ++u) {
+          if (seat[u].has_a) store_unit<T, N, NT>(y + k * y_step + seat[u].ea, ra[k][u]);
+          if (seat[u].has_b) store_unit<T, N, NT>(y + k * y_step + seat[u].eb, rb[k][u]);
         }
-    }
-    Unit<T, N> ra[RUN][U], rb[RUN][U];
-#pragma unroll
-    for (int k = 0; k < RUN; ++k) {
-      const int h = min(first + k * groups, side.heads - 1);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const T* p = x + h * side.x_head;
-        ra[k][u].v = 0;
-        rb[k][u].v = 0;
-        if (seat[u].has_a) ra[k][u] = load_unit<T, N>(p + seat[u].ea);
-        if (seat[u].has_b) rb[k][u] = load_unit<T, N>(p + seat[u].eb);
       }
+      continue;
+    }
+    float c[U][N], s[U][N];
+    if (turned) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) angles_of<N>(c[u], s[u], freq[u], token, a.r);
     }
 #pragma unroll
     for (int k = 0; k < RUN; ++k) {
       const int h = first + k * groups;
-      if (h >= side.heads) break;
-      T* q = y + h * side.y_head;
-      if (side.plain != 0) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (keep && seat[u].has_a) store_unit<T, N>(q + seat[u].ea, ra[k][u]);
-          if (keep && seat[u].has_b) store_unit<T, N>(q + seat[u].eb, rb[k][u]);
-        }
-        continue;
-      }
+      if (!WHOLE && h >= side.heads) break;
       float fa[U][N], fb[U][N];
       float sum = 0.0f;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         widen_unit<T, N>(fa[u], ra[k][u]);
         widen_unit<T, N>(fb[u], rb[k][u]);
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          sum = __builtin_fmaf(fa[u][j], fa[u][j], __builtin_fmaf(fb[u][j], fb[u][j], sum));
       }
       if (norm) {
-        const float r =
-            1.0f / __builtin_sqrtf(group_sum<G>(sum) / static_cast<float>(a.dim) + a.eps);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            sum = __builtin_fmaf(fa[u][j], fa[u][j], __builtin_fmaf(fb[u][j], fb[u][j], sum));
+        const float r = inverse_root(__builtin_fmaf(group_sum<G>(sum), inv_dim, a.eps));
         if (side.rstd != nullptr && lane == 0) side.rstd[token * side.rstd_token + h] = r;
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -336,9 +363,12 @@ __global__ __launch_bounds__(kThreads) void heads_fwd_kernel(const ForwardArgs<T
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        turn<N>(fa[u], fb[u], c[u], s[u], seat[u], a.r.interleaved != 0);
-        if (keep && seat[u].has_a) store_unit<T, N>(q + seat[u].ea, narrow_unit<T, N>(fa[u]));
-        if (keep && seat[u].has_b) store_unit<T, N>(q + seat[u].eb, narrow_unit<T, N>(fb[u]));
+        if (turned) turn<N>(fa[u], fb[u], c[u], s[u], seat[u], a.r);
+        T* q = y + k * y_step;
+        if (keep && seat[u].has_a)
+          store_unit<T, N, NT>(q + seat[u].ea, narrow_unit<T, N>(fa[u]));
+        if (keep && seat[u].has_b)
+          store_unit<T, N, NT>(q + seat[u].eb, narrow_unit<T, N>(fb[u]));
       }
     }
   }
@@ -368,7 +398,7 @@ struct GradArgs {
 
 // Workgroups loop over tokens with the weight's gradient in registers and leave
 // one partial row each.
-template <class T, int N, int G, int U, int RUN>
+template <class T, int N, int G, int U, int RUN, bool WHOLE, bool NT>
 __global__ __launch_bounds__(kThreads) void heads_bwd_kernel(const GradArgs<T> a) {
   __shared__ float rows[kThreads / G][2 * N * U * G];
   const GradSide<T>& side = a.side[blockIdx.x >= a.side[1].first_block ? 1 : 0];
@@ -376,58 +406,57 @@ __global__ __launch_bounds__(kThreads) void heads_bwd_kernel(const GradArgs<T> a
   const int lane = static_cast<int>(threadIdx.x) % G;
   const int groups = 1 << side.groups_log;
   const float inv_dim = 1.0f / static_cast<float>(a.dim);
+  const bool turned = a.r.rot > 0;
   Seat<N> seat[U];
+  double freq[U][N];
   float wa[U][N], wb[U][N], da[U][N], db[U][N];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     seat[u] = seat_of<N>(lane + G * u, a.dim, a.r);
+    if constexpr (WHOLE) seat[u].has_a = seat[u].has_b = true;
 #pragma unroll
     for (int j = 0; j < N; ++j) wa[u][j] = wb[u][j] = da[u][j] = db[u][j] = 0.0f;
     if (seat[u].has_a) widen_unit<T, N>(wa[u], load_unit<T, N>(side.w + seat[u].ea));
     if (seat[u].has_b) widen_unit<T, N>(wb[u], load_unit<T, N>(side.w + seat[u].eb));
+    if (turned) turns_of<N>(freq[u], lane + G * u, a.r);
   }
   for (int64_t unit = block * (kThreads / G) + static_cast<int>(threadIdx.x) / G;
        unit < side.units; unit += side.blocks * (kThreads / G)) {
     const int64_t token = unit >> side.groups_log;
     const int first = static_cast<int>(unit & (groups - 1));
-    if (first >= side.heads) continue;
-    float c[U][N], s[U][N];
-    if (a.r.rot > 0) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) angles_of<N>(c[u], s[u], lane + G * u, token, a.r);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          c[u][j] = 1.0f;
-          s[u][j] = 0.0f;
-        }
-    }
+    if (!WHOLE && first >= side.heads) continue;
+    const T* x = side.x + token * side.x_token + first * side.x_head;
+    const T* dy = side.dy + token * side.dy_token + first * side.dy_head;
+    T* dx = side.dx + token * side.dx_token + first * side.dx_head;
+    // On their way while the angles are taken.
     Unit<T, N> xa[RUN][U], xb[RUN][U], ga[RUN][U], gb[RUN][U];
     float rstd[RUN];
 #pragma unroll
     for (int k = 0; k < RUN; ++k) {
-      const int h = min(first + k * groups, side.heads - 1);
-      rstd[k] = side.rstd[token * a.rstd_token + h];
-      const T* px = side.x + token * side.x_token + h * side.x_head;
-      const T* pg = side.dy + token * side.dy_token + h * side.dy_head;
+      const int step = (WHOLE || first + k * groups < side.heads ? k : 0) * groups;
+      const T* px = x + step * side.x_head;
+      const T* pg = dy + step * side.dy_head;
+      rstd[k] = side.rstd[token * a.rstd_token + first + step];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         xa[k][u].v = 0;
         xb[k][u].v = 0;
         ga[k][u].v = 0;
         gb[k][u].v = 0;
-        if (seat[u].has_a) xa[k][u] = load_unit<T, N>(px + seat[u].ea);
-        if (seat[u].has_b) xb[k][u] = load_unit<T, N>(px + seat[u].eb);
-        if (seat[u].has_a) ga[k][u] = load_unit<T, N>(pg + seat[u].ea);
-        if (seat[u].has_b) gb[k][u] = load_unit<T, N>(pg + seat[u].eb);
+        if (seat[u].has_a) xa[k][u] = load_unit<T, N, NT>(px + seat[u].ea);
+        if (seat[u].has_b) xb[k][u] = load_unit<T, N, NT>(px + seat[u].eb);
+        if (seat[u].has_a) ga[k][u] = load_unit<T, N, NT>(pg + seat[u].ea);
+        if (seat[u].has_b) gb[k][u] = load_unit<T, N, NT>(pg + seat[u].eb);
       }
+    }
+    float c[U][N], s[U][N];
+    if (turned) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) angles_of<N>(c[u], s[u], freq[u], token, a.r);
     }
 #pragma unroll
     for (int k = 0; k < RUN; ++k) {
-      const int h = first + k * groups;
-      if (h >= side.heads) break;
+      if (!WHOLE && first + k * groups >= side.heads) break;
       float na[U][N], nb[U][N], fa[U][N], fb[U][N];
       float dot = 0.0f;
 #pragma unroll
@@ -436,7 +465,7 @@ __global__ __launch_bounds__(kThreads) void heads_bwd_kernel(const GradArgs<T> a
         widen_unit<T, N>(nb[u], xb[k][u]);
         widen_unit<T, N>(fa[u], ga[k][u]);
         widen_unit<T, N>(fb[u], gb[k][u]);
-        turn<N>(fa[u], fb[u], c[u], s[u], seat[u], a.r.interleaved != 0);
+        if (turned) turn<N>(fa[u], fb[u], c[u], s[u], seat[u], a.r);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           na[u][j] *= rstd[k];
@@ -449,7 +478,7 @@ __global__ __launch_bounds__(kThreads) void heads_bwd_kernel(const GradArgs<T> a
         }
       }
       const float mean = group_sum<G>(dot) * inv_dim;
-      T* q = side.dx + token * side.dx_token + h * side.dx_head;
+      T* q = dx + k * groups * side.dx_head;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -457,8 +486,8 @@ __global__ __launch_bounds__(kThreads) void heads_bwd_kernel(const GradArgs<T> a
           fa[u][j] = rstd[k] * __builtin_fmaf(-mean, na[u][j], fa[u][j]);
           fb[u][j] = rstd[k] * __builtin_fmaf(-mean, nb[u][j], fb[u][j]);
         }
-        if (seat[u].has_a) store_unit<T, N>(q + seat[u].ea, narrow_unit<T, N>(fa[u]));
-        if (seat[u].has_b) store_unit<T, N>(q + seat[u].eb, narrow_unit<T, N>(fb[u]));
+        if (seat[u].has_a) store_unit<T, N, NT>(q + seat[u].ea, narrow_unit<T, N>(fa[u]));
+        if (seat[u].has_b) store_unit<T, N, NT>(q + seat[u].eb, narrow_unit<T, N>(fb[u]));
       }
     }
   }
@@ -514,7 +543,7 @@ int check_own(const Place& out, const char* name, const Place& in, const char* i
 }
 int check_rotation(const credit_rotation* r, int64_t tokens, int dim, bool transposed,
                    Rotation* out) {
-  *out = Rotation{nullptr, nullptr, 0, 0, 1.0f, 1.0f};
+  *out = Rotation{nullptr, nullptr, 0, 0, 1.0f, 1.0f, 0};
   if (r == nullptr) return CREDIT_OK;
   if (r->rot < 0 || r->rot > dim || r->rot % 2 != 0)
     return set_error(CREDIT_ERR_BAD_SHAPE, "rot %d is not an even number in [0, %d]", r->rot, dim);
@@ -526,7 +555,7 @@ int check_rotation(const credit_rotation* r, int64_t tokens, int dim, bool trans
   if (!__builtin_isfinite(r->magnitude))
     return set_error(CREDIT_ERR_BAD_CONFIG, "magnitude %g is not finite", r->magnitude);
   *out = Rotation{r->positions, r->inv_freq, r->rot, r->interleaved != 0, r->magnitude,
-                  transposed ? -1.0f : 1.0f};
+                  transposed ? -1.0f : 1.0f, r->rot == dim};
   return CREDIT_OK;
 }
 int check_eps(float eps) {
@@ -578,33 +607,80 @@ void with_units(const Shape& shape, Fn&& fn) {
 
 int log2_of(int v) { return 31 - __builtin_clz(static_cast<unsigned>(v)); }
 
+// Units of a side, its groups and workgroups: as many as its share, by heads, of
+// kBlocks, which loop over them.
+struct Deal {
+  int groups, run;
+  int64_t units, blocks;
+};
+inline Deal deal(int64_t tokens, int side_heads, int64_t all_heads, int lanes, int most,
+                 int64_t blocks) {
+  Deal d;
+  d.groups = heads::groups_of(tokens, side_heads, lanes, most);
+  d.run = (side_heads + d.groups - 1) / d.groups;
+  d.units = tokens * d.groups;
+  const int64_t share = std::max<int64_t>(1, blocks * side_heads / all_heads);
+  const int64_t per = kThreads / lanes;
+  d.blocks = std::min(share, (d.units + per - 1) / per);
+  return d;
+}
+
+// fn(RUN, WHOLE, NT) of heads a group takes at once.  Beyond what the last-level
+// cache holds (256 MiB) nothing that is written is found there again: nontemporal.
+// us, without -> with, turned alone: 16384 tokens of 32 + 8 heads of 128 in bf16 (320
+// MiB) 79 -> 67, 2048 in fp32 (80 MiB) 19 -> 27; 8192 tokens into a cache (192 MiB) 42
+// -> 46.
+template <int U, int MOST, class Fn>
+void with_run(int run, bool even, int64_t bytes, Fn&& fn) {
+  using std::integral_constant;
+  if constexpr (U > 1) {
+    fn(integral_constant<int, 1>{}, std::false_type{}, std::false_type{});
+  } else {
+    const auto go = [&](auto n) {
+      if (!even) return fn(n, std::false_type{}, std::false_type{});
+      if constexpr (decltype(n)::value == MOST)
+        if (bytes > int64_t{256} << 20) return fn(n, std::true_type{}, std::true_type{});
+      fn(n, std::true_type{}, std::false_type{});
+    };
+    if (run == 1) return go(integral_constant<int, 1>{});
+    if constexpr (MOST > 2)
+      if (run > 2) return go(integral_constant<int, MOST>{});
+    go(integral_constant<int, 2>{});
+  }
+}
+
+// Workgroups of the forward's launch: more than the device holds at once, so that one
+// ends while another begins, each with a few units over which its lanes keep weights
+// and frequencies.  us at 1024 / 2048 / 4096 / one a unit: norm and rotation of 16384
+// tokens of 32 + 8 heads of 128 in bf16 71 / 66 / 65 / 67, of 131072 tokens of 2 + 1
+// heads 43 / 42 / 44 / 49, 8192 tokens into a cache 44 / 38 / 38 / 38.
+constexpr int64_t kForwardBlocks = 4096;
+
 template <class T>
 int launch_forward(ForwardArgs<T>& a, int64_t tokens, const Shape& shape, hipStream_t stream) {
   with_units<T>(shape, [&](auto n, auto g, auto u) {
     constexpr int N = decltype(n)::value, G = decltype(g)::value, U = decltype(u)::value;
     constexpr int kMost = U == 1 ? 4 : 1;
-    int64_t blocks = 0;
+    int64_t blocks = 0, all = 0, bytes = 0;
     int run = 1;
+    for (int i = 0; i < a.sides; ++i) all += a.side[i].heads;
+    bool even = a.dim == 2 * N * G;
     for (int i = 0; i < a.sides; ++i) {
       Side<T>& s = a.side[i];
-      const int groups = heads::groups_of(tokens, s.heads, G, kMost);
-      s.groups_log = log2_of(groups);
-      run = std::max(run, (s.heads + groups - 1) / groups);
-      s.units = tokens * groups;
+      const Deal d = deal(tokens, s.heads, all, G, kMost, kForwardBlocks);
+      s.groups_log = log2_of(d.groups);
+      run = std::max(run, d.run);
+      s.units = d.units;
       s.first_block = blocks;
-      blocks += std::min(kMaxGrid / 4, (s.units + kThreads / G - 1) / (kThreads / G));
+      blocks += d.blocks;
+      bytes += 2 * tokens * s.heads * a.dim * static_cast<int64_t>(sizeof(T));
     }
+    for (int i = 0; i < a.sides; ++i) even = even && a.side[i].heads == run << a.side[i].groups_log;
     const dim3 grid(static_cast<unsigned>(blocks));
-    if constexpr (kMost == 1) {
-      heads_fwd_kernel<T, N, G, U, 1><<<grid, kThreads, 0, stream>>>(a);
-    } else {
-      if (run == 1)
-        heads_fwd_kernel<T, N, G, U, 1><<<grid, kThreads, 0, stream>>>(a);
-      else if (run == 2)
-        heads_fwd_kernel<T, N, G, U, 2><<<grid, kThreads, 0, stream>>>(a);
-      else
-        heads_fwd_kernel<T, N, G, U, 4><<<grid, kThreads, 0, stream>>>(a);
-    }
+    with_run<U, kMost>(run, even, bytes, [&](auto r, auto whole, auto nt) {
+      heads_fwd_kernel<T, N, G, U, decltype(r)::value, decltype(whole)::value,
+                       decltype(nt)::value><<<grid, kThreads, 0, stream>>>(a);
+    });
   });
   return check_launch("heads_fwd_kernel");
 }
@@ -765,14 +841,12 @@ int norm_rope_bwd(const credit_heads* q, const credit_heads* k, const T* q_weigh
       s.dx_token = dx[i]->token_stride;
       s.dx_head = dx[i]->head_stride;
       s.heads = x[i]->heads;
-      const int groups = heads::groups_of(tokens, s.heads, G, kMost);
-      s.groups_log = log2_of(groups);
-      run = std::max(run, (s.heads + groups - 1) / groups);
-      s.units = tokens * groups;
+      const Deal d = deal(tokens, s.heads, all, G, kMost, kMaxGradBlocks - 1);
+      s.groups_log = log2_of(d.groups);
+      run = std::max(run, d.run);
+      s.units = d.units;
       s.first_block = blocks;
-      // Its share of the workgroups, by its heads.
-      const int64_t share = std::max<int64_t>(1, (kMaxGradBlocks - 1) * s.heads / all);
-      s.blocks = std::min(share, (s.units + kThreads / G - 1) / (kThreads / G));
+      s.blocks = d.blocks;
       s.partial = reinterpret_cast<float*>(ws_scratch(base)) + blocks * dim;
       blocks += s.blocks;
       sum.partial[i] = s.partial;
@@ -780,15 +854,15 @@ int norm_rope_bwd(const credit_heads* q, const credit_heads* k, const T* q_weigh
       sum.rows[i] = s.blocks;
     }
     if (blocks == 0) return;
+    bool even = dim == 2 * N * G;
+    for (const GradSide<T>& s : a.side) even = even && s.heads == run << s.groups_log;
     const dim3 grid(static_cast<unsigned>(blocks));
-    if constexpr (kMost == 1) {
-      heads_bwd_kernel<T, N, G, U, 1><<<grid, kThreads, 0, stream>>>(a);
-    } else {
-      if (run == 1)
-        heads_bwd_kernel<T, N, G, U, 1><<<grid, kThreads, 0, stream>>>(a);
-      else
-        heads_bwd_kernel<T, N, G, U, 2><<<grid, kThreads, 0, stream>>>(a);
-    }
+    with_run<U, kMost>(run, even, 3 * tokens * all * dim * static_cast<int64_t>(sizeof(T)),
+                       [&](auto r, auto whole, auto nt) {
+                         heads_bwd_kernel<T, N, G, U, decltype(r)::value,
+                                          decltype(whole)::value, decltype(nt)::value>
+                             <<<grid, kThreads, 0, stream>>>(a);
+                       });
   });
   CREDIT_TRY(check_launch("heads_bwd_kernel"));
   heads_dw_kernel<<<dim3(static_cast<unsigned>((dim + kSumCols - 1) / kSumCols), 2),
