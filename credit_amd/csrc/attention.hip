@@ -277,13 +277,14 @@ struct Cursor {
   }
 };
 
-// Layout of a step's keys and values in LDS: rows of D elements, 16-byte chunk c
-// of row r at place c ^ swizzle(r), so that the reads below meet no bank twice:
-// of the keys 16 rows' same chunk, of the values 4 rows' 64 bytes.
+// Layout of a step's keys and values in LDS: rows of D elements, or the power of two
+// above, 16-byte chunk c of row r at place c ^ swizzle(r), so that the reads below
+// meet no bank twice: of the keys 16 rows' same chunk, of the values 4 rows' 64 bytes.
 template <int D>
 struct Lds {
-  static constexpr int kChunks = D / 8;
-  static constexpr int kRowBytes = D * 2;
+  static constexpr int kWidth = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+  static constexpr int kChunks = kWidth / 8;
+  static constexpr int kRowBytes = kWidth * 2;
   __device__ static int key(int row, int chunk) {
     const int s = D == 64 ? (row >> 1) & 7 : row & 15;
     return row * kRowBytes + (chunk ^ s) * 16;
@@ -1411,8 +1412,12 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
   switch (attention::padded_dim(dim)) {
     case 64:
       return launch<64>(a, rows, stream);
+    case 96:
+      return launch<96>(a, rows, stream);
     case 128:
       return launch<128>(a, rows, stream);
+    case 192:
+      return launch<192>(a, rows, stream);
     default:
       return launch<256>(a, rows, stream);
   }

@@ -55,7 +55,10 @@ inline Parts parts(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_head
           static_cast<int>(least)};
 }
 
-inline int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+// Columns that the products take.
+inline int padded_dim(int dim) {
+  return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
+}
 
 // Floats that a part of a tile leaves: its rows' outputs, maxima and sums.
 inline int64_t part_floats(int rows, int dim) {

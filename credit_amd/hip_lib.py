@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 import threading
 from dataclasses import dataclass
 from pathlib import Path
@@ -143,9 +144,12 @@ _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
 _F = ctypes.c_float
 _CFG = ctypes.POINTER(CreditCfg)
-_HEADS = ctypes.POINTER(CreditHeads)
-_ROTATION = ctypes.POINTER(CreditRotation)
-_PAGES = ctypes.POINTER(CreditPages)
+# Addresses of these structs: the calls here pass them packed, which takes a third of
+# the time of a ctypes structure's.
+_HEADS = _ROTATION = _PAGES = ctypes.c_void_p
+_pack_heads = struct.Struct("@Pqqi4x").pack
+_pack_rotation = struct.Struct("@PPiif4x").pack
+_pack_pages = struct.Struct("@Pqqqqii").pack
 
 # name -> argument types (return type is int unless listed in _RESTYPES).
 SIGNATURES: dict[str, list] = {
@@ -817,25 +821,24 @@ def topk_distill_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher: t
 # ---------------------------------------------------- operators on heads --
 
 
-def _heads(t: torch.Tensor, name: str, dtype: torch.dtype, tokens: int, dim: int, device: int):
-    """A [tokens, heads, dim] tensor whose heads' elements are contiguous."""
-    if t.dim() != 3:
-        raise ValueError(f"{name}: expected [tokens, heads, dim], got shape {tuple(t.shape)}")
-    n, heads, d = t.shape
+def _heads(t: torch.Tensor, name: str, dtype: torch.dtype, tokens: int, dim: int,
+           device: int) -> bytes:
+    """credit_heads of a [tokens, heads, dim] tensor whose heads' elements are
+    contiguous."""
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name}: expected [tokens, heads, dim], got shape {tuple(shape)}")
+    n, heads, d = shape
     token, head, one = t.stride()
     if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     if n != tokens or d != dim:
-        raise ValueError(f"{name}: expected [{tokens}, heads, {dim}], got {tuple(t.shape)}")
+        raise ValueError(f"{name}: expected [{tokens}, heads, {dim}], got {tuple(shape)}")
     if one != 1 and d > 1:
         raise ValueError(f"{name}: the elements of a head must be contiguous")
     if t.get_device() != device:
-        raise ValueError(f"{name}: expected a tensor on {_device_name(device)}, got {t.device}")
-    return ctypes.byref(CreditHeads(t.data_ptr(), token, head, heads))
-
-
-def _device_name(device: int) -> str:
-    return f"cuda:{device}"
+        raise ValueError(f"{name}: expected a tensor on cuda:{device}, got {t.device}")
+    return _pack_heads(t.data_ptr(), token, head, heads)
 
 
 def _heads_call(op: str, q: torch.Tensor, name: str) -> tuple[int, int, int, Callable[..., int]]:
@@ -843,14 +846,15 @@ def _heads_call(op: str, q: torch.Tensor, name: str) -> tuple[int, int, int, Cal
     suffix = _LOGITS_TYPES.get(q.dtype)
     if suffix is None:
         raise TypeError(f"{name}: expected torch.float32 or torch.bfloat16, got {q.dtype}")
-    if q.dim() != 3:
-        raise ValueError(f"{name}: expected [tokens, heads, dim], got shape {tuple(q.shape)}")
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name}: expected [tokens, heads, dim], got shape {tuple(shape)}")
     device = q.get_device()
     if device < 0:
         raise ValueError(f"{name}: tensor must be on a GPU, got {q.device}")
-    if device != torch.cuda.current_device():
+    if device != torch._C._cuda_getDevice():
         raise ValueError(f"{name}: on {q.device}, which is not the current device")
-    return q.shape[0], q.shape[2], device, getattr(load_library(), op + suffix)
+    return shape[0], shape[2], device, getattr(load_library(), op + suffix)
 
 
 _LAYOUTS = {"half": 0, "interleaved": 1}
@@ -866,10 +870,10 @@ def _rotation(positions: torch.Tensor | None, inv_freq: torch.Tensor | None, lay
     if positions is None:
         return None
     pairs = inv_freq.shape[0] if inv_freq.dim() == 1 else -1
-    return ctypes.byref(CreditRotation(
+    return _pack_rotation(
         _operand(positions, "positions", torch.int64, (tokens,), device, "the queries'"),
         _operand(inv_freq, "inv_freq", torch.float32, (pairs,), device, "the queries'"),
-        2 * pairs, interleaved, magnitude))
+        2 * pairs, interleaved, magnitude)
 
 
 def rope_frequencies(rot: int, base: float = 10000.0, scaling: str | None = None,
@@ -984,22 +988,24 @@ def qk_norm_rope_bwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
         check(status, fn.__name__)
 
 
-def _pages(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int, device: int):
-    """A cache [pages, slots of a page, heads, dim], at any strides but the last."""
-    if t.dim() != 4:
+def _pages(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int, device: int) -> bytes:
+    """credit_pages of a cache [pages, slots of a page, heads, dim], at any strides but
+    the last."""
+    shape = t.shape
+    if len(shape) != 4:
         raise ValueError(f"{name}: expected [pages, page size, heads, dim], "
-                         f"got shape {tuple(t.shape)}")
-    pages, size, heads, d = t.shape
+                         f"got shape {tuple(shape)}")
+    pages, size, heads, d = shape
     page, slot, head, one = t.stride()
     if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     if d != dim:
-        raise ValueError(f"{name}: expected heads of {dim}, got {tuple(t.shape)}")
+        raise ValueError(f"{name}: expected heads of {dim}, got {tuple(shape)}")
     if one != 1 and d > 1:
         raise ValueError(f"{name}: the elements of a head must be contiguous")
     if t.get_device() != device:
-        raise ValueError(f"{name}: expected a tensor on {_device_name(device)}, got {t.device}")
-    return ctypes.byref(CreditPages(t.data_ptr(), page, slot, head, pages, size, heads))
+        raise ValueError(f"{name}: expected a tensor on cuda:{device}, got {t.device}")
+    return _pack_pages(t.data_ptr(), page, slot, head, pages, size, heads)
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
@@ -1037,6 +1043,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
     if status:
         check(status, fn.__name__)
 
+
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                     pages: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
                     out: torch.Tensor, lse: torch.Tensor | None = None,
@@ -1064,7 +1071,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if one != 1 and cols > 1:
         raise ValueError("pages: the entries of a sequence must be contiguous")
     if pages.get_device() != dev:
-        raise ValueError(f"pages: expected a tensor on {_device_name(dev)}, got {pages.device}")
+        raise ValueError(f"pages: expected a tensor on cuda:{dev}, got {pages.device}")
     status = fn(_heads(q, "q", dt, tokens, dim, dev), _pages(k_cache, "k_cache", dt, dim, dev),
                 _pages(v_cache, "v_cache", dt, dim, dev), pages.data_ptr(),
                 ld if batch > 1 else cols, cols,
