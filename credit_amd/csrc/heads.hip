@@ -357,8 +357,8 @@ __global__ __launch_bounds__(kThreads) void heads_fwd_kernel(const ForwardArgs<T
         for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            fa[u][j] *= r * wa[u][j];
-            fb[u][j] *= r * wb[u][j];
+            fa[u][j] = fa[u][j] * r * wa[u][j];
+            fb[u][j] = fb[u][j] * r * wb[u][j];
           }
       }
 #pragma unroll

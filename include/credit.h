@@ -530,8 +530,8 @@ int credit_paged_append_bf16(const credit_heads* k, const credit_heads* v,
 /* Attention of a batch's new tokens over a paged cache.  Sequence b has kv_len[b]
  * positions in the cache, position j in slot j % page_size of page
  * pages[b pages_ld + j / page_size], its new tokens among them as the last: tokens
- * q_start[b] .. q_start[b + 1] - 1 of q (q_start [batch + 1] rising from row to
- * row).  Token i of n new ones sees positions j <= kv_len[b] - n + i, with window
+ * q_start[b] .. q_start[b + 1] - 1 of q (q_start [batch + 1] never falling; the
+ * values of a batch where it does are open, its accesses in bounds).  Token i of n new ones sees positions j <= kv_len[b] - n + i, with window
  * > 0 only the last window of those:
  *   out = sum_j p_j v_j, p = softmax(scale q k_j), lse = ln sum_j e^(scale q k_j)
  * (lse [tokens, q heads] fp32; NULL: not wanted), head h of q with key head
