@@ -987,6 +987,18 @@ __device__ __forceinline__ bool last_of(uint32_t* counter, int parts, char* smem
 
 constexpr int kKeys = attention::kKeys;
 
+// A tile of 128 rows: 32 a wave, keys and values of 64 positions in one of two stages
+// of LDS, the next step's on their way into the other (64 KiB for heads up to 128: two
+// workgroups a CU, so that one's products run under the other's exponentials).  Bound
+// by the matrix units and what stands between their products: a wave's step of heads
+// of 128 is 32 products of 32 x 32 x 16 and the exponentials of 2048 scores.
+// Measured, 32 heads over 8 key heads of 128: a prompt of 8192 550-560 us (990
+// TFLOP/s; a large product alone 1268), of 2048 62; 4 chunks of 1024 tokens over 8192
+// positions 505 (1020), 512 tokens over 8192 in parts 88-93; heads of 64, a prompt of
+// 4096 89 us (774), of 192 (16 heads) 150 (687), of 256 377 (365: the registers of a
+// wave alone on its SIMD do not hold it all); chunks of 6 sequences of up to 500 tokens
+// over 6000 positions, 14 heads of 80 over 2 key heads, pages of 24, a window of 4096
+// 80-88.
 template <int D, int PIECE, bool PARTS>
 __device__ __forceinline__ void work_on_many(const Args& a, const Work& w, char* smem) {
   constexpr int kStage = 2 * kKeys * Lds<D>::kRowBytes;
@@ -1102,6 +1114,16 @@ __device__ __forceinline__ void wave_fence() {
 }
 
 using attention::kFewKeys;  // positions of a wave's step
+
+// A tile of up to 32 rows: each wave takes every fourth step of 32 positions, with a
+// stage of LDS of its own and no barrier; its keys are replaced by the next step's as
+// soon as they are read, the values likewise, so that loads never stop.  Bound by HBM
+// where there are steps enough, else by a chain of latencies: find the work, the first
+// keys, the meeting of the waves and of the parts.  Nothing is read twice: nontemporal.
+// Measured, 32 heads over 8 key heads of 128: one token over 32 positions 6.1 us, 8192
+// 13.3, 131072 98 (5.5 TB/s); 64 sequences of 8192 345-357 us (6.0-6.2 TB/s of the 7.1
+// that reads alone reach), of up to 16384 390 (5.8); one key head, 512 sequences of
+// 8192 344 (6.2); 128 with heads of 64 402 (5.3).
 
 // LDS of a workgroup's steps, where its waves' results meet behind them.
 template <int D>
@@ -1293,7 +1315,9 @@ int launch_with(const Args& a, size_t lds, hipStream_t stream, const char* name)
 template <int D>
 int launch(const Args& a, int rows, hipStream_t stream) {
   // Pieces of 16 rows or 8, or through registers where pages hold no whole number of
-  // them or a piece's offsets pass 31 bits.
+  // them or a piece's offsets pass 31 bits.  us with pages of 16 / 8 / 12 positions: 64
+  // sequences of 8192, one token each 343 / 346 / 602, 4 chunks of 1024 over 8192
+  // 514 / 539 / 871.
   constexpr int64_t kMost = int64_t{1} << 25;
   const bool near = a.k.slot < kMost && a.v.slot < kMost;
   const auto choose = [&](auto&& with) {
