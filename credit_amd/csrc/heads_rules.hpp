@@ -58,19 +58,26 @@ inline bool same(const Place& a, const Place& b) {
          (a.count <= 1 || a.step == b.step);
 }
 
-// Groups of lanes (a power of two of them) that share a token's heads, group g
-// taking heads g, g + groups, ...: as many as the heads where that leaves the
-// device short of waves, fewer where a group's angles then serve up to `most`
-// heads.  `group_lanes`: lanes of a group.  us, a head a group -> `most` of them: 16384
-// tokens of 32 + 8 heads of 128 in bf16, norm and rotation 89 -> 66, their gradients
-// 125 -> 106; 64 tokens, which stay at a head a group, 4.8.
-inline int groups_of(int64_t tokens, int heads, int group_lanes, int most) {
+// Heads that a group of lanes takes of each tensor of a launch, a power of two up to
+// `most`: one where that leaves the device short of waves (four a SIMD), more where a
+// group's angles then serve them all.  `all`: heads of a token in all tensors,
+// `widest`: of the one with the most.  us, a
+// head a group -> `most` of them: 16384 tokens of 32 + 8 heads of 128 in bf16, norm and
+// rotation 89 -> 66, their gradients 125 -> 106; 64 tokens, which stay at a head a
+// group, 4.8.
+inline int run_of(int64_t tokens, int64_t all, int widest, int group_lanes, int most) {
+  constexpr double kLanes = 64.0 * 4096.0;
+  int run = most;
+  while (run > 1 && (run / 2 >= widest ||
+                     static_cast<double>(tokens) * all * group_lanes < kLanes * run))
+    run /= 2;
+  return run;
+}
+// Groups (a power of two of them) that share a token's heads, group g taking heads g,
+// g + groups, ...
+inline int groups_of(int heads, int run) {
   int groups = 1;
-  while (groups < heads) groups *= 2;
-  constexpr int64_t kLanes = int64_t{64} * 4096;  // four waves a SIMD
-  while (groups > 1 && groups / 2 * most >= heads &&
-         tokens * (groups / 2) * group_lanes >= kLanes)
-    groups /= 2;
+  while (groups * run < heads) groups *= 2;
   return groups;
 }
 

@@ -15,9 +15,10 @@ extern "C" {
 int heads_apart(const int64_t* a, const int64_t* b) { return heads::apart(place(a), place(b)); }
 int heads_apart_within(const int64_t* a) { return heads::apart_within(place(a)); }
 int heads_same(const int64_t* a, const int64_t* b) { return heads::same(place(a), place(b)); }
-int heads_groups_of(int64_t tokens, int n, int lanes, int most) {
-  return heads::groups_of(tokens, n, lanes, most);
+int heads_run_of(int64_t tokens, int64_t all, int widest, int lanes, int most) {
+  return heads::run_of(tokens, all, widest, lanes, most);
 }
+int heads_groups_of(int n, int run) { return heads::groups_of(n, run); }
 int attention_tile_rows(int64_t tokens, int64_t batch, int64_t group) {
   return attention::tile_rows(tokens, batch, group);
 }

@@ -27,7 +27,8 @@ def rules(tmp_path_factory):
     place = I64 * 6
     for name, args, result in (
             ("heads_apart", [place, place], INT), ("heads_apart_within", [place], INT),
-            ("heads_same", [place, place], INT), ("heads_groups_of", [I64, INT, INT, INT], INT),
+            ("heads_same", [place, place], INT), ("heads_run_of", [I64, I64, INT, INT, INT], INT),
+            ("heads_groups_of", [INT, INT], INT),
             ("attention_tile_rows", [I64] * 3, INT), ("attention_tiles", [I64] * 3 + [INT], I64),
             ("attention_units", [I64] * 5, INT),
             ("attention_workspace", [I64] * 4 + [INT, I64], SIZE),
@@ -78,15 +79,18 @@ def test_places_apart_share_no_byte(rules):
 
 
 def test_groups_cover_the_heads(rules):
-    for tokens in (1, 64, 1000, 4096, 1 << 20, 1 << 40):
+    for most in (1, 2, 4):
+        for tokens in (1, 64, 1000, 4096, 1 << 20, 1 << 40):
+            for lanes in (4, 8, 64):
+                assert rules.heads_run_of(tokens, 40, 32, lanes, most) in (1, 2, 4)[:most]
         for n in (1, 2, 3, 8, 14, 32, 127, 1000):
-            for lanes in (2, 8, 64):
-                for most in (1, 2, 4):
-                    groups = rules.heads_groups_of(tokens, n, lanes, most)
-                    assert groups & (groups - 1) == 0 and groups < 2 * n
-                    assert -(-n // groups) <= most
-    assert rules.heads_groups_of(1, 32, 8, 4) == 32  # a token's heads side by side
-    assert rules.heads_groups_of(1 << 20, 32, 8, 4) == 8
+            groups = rules.heads_groups_of(n, most)
+            assert groups & (groups - 1) == 0 and groups * most >= n
+            assert groups == 1 or groups // 2 * most < n
+    assert rules.heads_run_of(1, 48, 32, 8, 4) == 1  # a token's heads side by side
+    assert rules.heads_run_of(8192, 48, 32, 8, 4) == 4
+    assert rules.heads_run_of(16384, 40, 32, 8, 2) == 2
+    assert rules.heads_run_of(1 << 20, 3, 2, 8, 4) == 2  # no more than there are
 
 
 def test_tiles_hold_every_sequence(rules):
