@@ -262,7 +262,7 @@ struct ForwardArgs {
 //
 // Measured in bf16, heads of 128 (a copy reaches 5.16 TB/s): norm, rotation and rstd
 // of 16384 tokens of 32 + 8 heads 65 us (5.2 TB/s), rotation alone 62 (5.4), 8192
-// tokens of 32 queries, 8 keys and values into a cache 38 (5.4); in fp32 8192 tokens
+// tokens of 32 queries, 8 keys and values into a cache 41 (4.9); in fp32 8192 tokens
 // normed and turned 61 (5.5).  64 tokens 4.8 us, one 4.3, a cache's 64 5.0: launch,
 // loads, sines and stores one behind the other.
 template <class T, int N, int G, int U, int RUN, bool WHOLE, bool NT>
@@ -651,11 +651,13 @@ inline Deal deal(int64_t tokens, int side_heads, int64_t all_heads, int lanes, i
   return d;
 }
 
-// fn(RUN, WHOLE, NT) of heads a group takes at once.  Beyond what the last-level
-// cache holds (256 MiB) nothing that is written is found there again: nontemporal.
-// us, without -> with, turned alone: 16384 tokens of 32 + 8 heads of 128 in bf16 (320
-// MiB) 79 -> 67, 2048 in fp32 (80 MiB) 19 -> 27; 8192 tokens into a cache (192 MiB) 42
-// -> 46.
+// fn(RUN, WHOLE, NT) of heads a group takes at once.  Nontemporal where a call's
+// tensors take more than a third of the last-level cache (256 MiB): among the others
+// of a step they are not found there again.  us, without -> with, norm and rotation in
+// bf16, calls on 1 / 3 / 8 sets of tensors in turn: 81 MiB 21 / 21 / 27 -> 20 / 21 / 21,
+// 161 MiB 33 / 42 / 43 -> 36 / 36 / 37, 320 MiB 79 -> 65; rotation in fp32 of strided
+// tensors, 80 MiB 17 / 17 / 21 -> 19 / 20 / 20; 192 MiB into a cache 37 / 48 / 48 -> 40 /
+// 41 / 42; gradients, 121 MiB 29 / 37 / 37 -> 33 / 34 / 35.
 template <int U, int MOST, class Fn>
 void with_run(int run, bool even, int64_t bytes, Fn&& fn) {
   using std::integral_constant;
@@ -665,7 +667,7 @@ void with_run(int run, bool even, int64_t bytes, Fn&& fn) {
     const auto go = [&](auto n) {
       if (!even) return fn(n, std::false_type{}, std::false_type{});
       if constexpr (decltype(n)::value == MOST)
-        if (bytes > int64_t{256} << 20) return fn(n, std::true_type{}, std::true_type{});
+        if (bytes > (int64_t{256} << 20) / 3) return fn(n, std::true_type{}, std::true_type{});
       fn(n, std::true_type{}, std::false_type{});
     };
     if (run == 1) return go(integral_constant<int, 1>{});
