@@ -995,8 +995,7 @@ constexpr int kKeys = attention::kKeys;
 // Measured, 32 heads over 8 key heads of 128: a prompt of 8192 550-560 us (990
 // TFLOP/s; a large product alone 1268), of 2048 62; 4 chunks of 1024 tokens over 8192
 // positions 505 (1020), 512 tokens over 8192 in parts 88-93; heads of 64, a prompt of
-// 4096 89 us (774), of 192 (16 heads) 150 (687), of 256 377 (365: the registers of a
-// wave alone on its SIMD do not hold it all); chunks of 6 sequences of up to 500 tokens
+// 4096 89 us (774), of 192 (16 heads) 150 (687); chunks of 6 sequences of up to 500 tokens
 // over 6000 positions, 14 heads of 80 over 2 key heads, pages of 24, a window of 4096
 // 80-88.
 template <int D, int PIECE, bool PARTS>
@@ -1123,7 +1122,9 @@ using attention::kFewKeys;  // positions of a wave's step
 // Measured, 32 heads over 8 key heads of 128: one token over 32 positions 6.1 us, 8192
 // 13.3, 131072 98 (5.5 TB/s); 64 sequences of 8192 345-357 us (6.0-6.2 TB/s of the 7.1
 // that reads alone reach), of up to 16384 390 (5.8); one key head, 512 sequences of
-// 8192 344 (6.2); 128 with heads of 64 402 (5.3).
+// 8192 344 (6.2); 128 with heads of 64 402 (5.3).  Prompts with heads of 256, 4096
+// tokens and 16 heads, 344 us (399 TFLOP/s): a wave's keys and outputs leave no registers
+// to read ahead.
 
 // LDS of a workgroup's steps, where its waves' results meet behind them.
 template <int D>
@@ -1335,12 +1336,14 @@ int launch(const Args& a, int rows, hipStream_t stream) {
                                                     decltype(parts)::value>>(
           a, kBytes, stream, "paged_attention_few_kernel");
     });
-  return choose([&](auto piece, auto parts) {
-    constexpr size_t kBytes = size_t{4} * kKeys * Lds<D>::kRowBytes;
-    return launch_with<paged_attention_many_kernel<D, decltype(piece)::value,
-                                                    decltype(parts)::value>>(
-        a, kBytes, stream, "paged_attention_many_kernel");
-  });
+  if constexpr (D <= attention::kManyDim)
+    return choose([&](auto piece, auto parts) {
+      constexpr size_t kBytes = size_t{4} * kKeys * Lds<D>::kRowBytes;
+      return launch_with<paged_attention_many_kernel<D, decltype(piece)::value,
+                                                      decltype(parts)::value>>(
+          a, kBytes, stream, "paged_attention_many_kernel");
+    });
+  return set_error(CREDIT_ERR_UNSUPPORTED, "tiles of %d rows with heads of %d", rows, D);
 }
 
 int check_vectors(const Place& p, const char* name) {
@@ -1434,9 +1437,11 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
   a.window = window;
   a.scale = scale;
   a.scale_log2 = static_cast<float>(1.44269504088896340736 * static_cast<double>(scale));
-  const int rows = attention::tile_rows(tokens, batch, a.group);
+  const int rows =
+      attention::tile_rows(tokens, batch, a.heads, a.kv_heads, dim, a.positions);
   a.tiles = static_cast<int>(attention::tiles(tokens, batch, a.group, rows));
-  attention::Parts parts = attention::parts(tokens, batch, a.heads, a.kv_heads, a.positions);
+  attention::Parts parts = attention::parts(tokens, batch, a.heads, a.kv_heads, dim,
+                                             a.positions, window);
   hipStream_t stream = cfg_stream(cfg);
   if (static_cast<int64_t>(parts.units) * a.kv_heads > kMaxGroupsPerLaunch ||
       ((cfg == nullptr || cfg->workspace == nullptr) && !keeps_scratch(stream)))
@@ -1449,7 +1454,7 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
     a.least_steps = parts.least_steps;
     char* base = nullptr;
     const size_t bytes =
-        attention::workspace(tokens, batch, a.heads, a.kv_heads, dim, a.positions);
+        attention::workspace(tokens, batch, a.heads, a.kv_heads, dim, a.positions, window);
     CREDIT_TRY(acquire_workspace(cfg, bytes, &base));
     a.partial_bytes = static_cast<uint32_t>(bytes);
     a.partial = reinterpret_cast<float*>(ws_scratch(base));
@@ -1492,7 +1497,7 @@ size_t credit_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int
       dim <= 0 || dim > attention::kMaxDim || positions <= 0)
     return 0;
   const size_t body =
-      attention::workspace(tokens, batch, q_heads, kv_heads, dim, positions);
+      attention::workspace(tokens, batch, q_heads, kv_heads, dim, positions, 0);
   return body == 0 ? 0 : kScratchOffset + body;
 }
 

@@ -12,6 +12,7 @@ namespace credit {
 namespace attention {
 
 constexpr int kMaxDim = 256;
+constexpr int kManyDim = 192;  // of large tiles
 constexpr int kFew = 32;     // query rows (tokens times heads of a group) of a small tile
 constexpr int kMany = 128;   // of a large one
 constexpr int kKeys = 64;    // positions of a step of large tiles
@@ -19,12 +20,25 @@ constexpr int kFewKeys = 32; // of small ones
 constexpr int kMaxBatch = 1024;  // sequences that a wave counts through
 constexpr int kResident = 512;   // workgroups: two a CU
 
-// Small tiles serve where a sequence has no more rows than one.  us, small / large,
-// 32 heads over 8 key heads of 128, 8 sequences of 8192 positions: 8 new tokens each
-// (32 rows) 60 / 68, 16 tokens 83 / 75, 32 tokens 128 / 80; 64 sequences, one token
-// each 355 / 448.
-inline int tile_rows(int64_t tokens, int64_t batch, int64_t group) {
-  return tokens * group <= kFew * batch ? kFew : kMany;
+// Columns that the products take: 80 of 96 instead of 128 were 90 us against 102 (six
+// sequences of up to 500 new tokens), 192 instead of 256 169 against 406.
+inline int padded_dim(int dim) {
+  return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
+}
+
+// Small tiles serve where a sequence has no more rows than one; where they leave each
+// a CU of its own and the positions are few, as there is not work enough to share; and
+// for the widest heads, of which a large tile's wave has no registers for.  us, small /
+// large, 32 heads over 8 key heads of 128: 8 sequences of 8192 positions with 8 new
+// tokens each (32 rows) 60 / 68, with 16 82 / 72, with 32 128 / 80; 64 sequences with one
+// 355 / 448; one sequence, 40 tokens over 500 positions 10.9 / 26, 64 over 2048 23 / 28,
+// 128 over 8192 55 / 47.  16 heads over 4 of 256: 13 tokens each of 9 sequences over
+// 10818 172 / 278, 2048 tokens over 4096 308 / 426.
+inline int tile_rows(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int dim,
+                     int64_t positions) {
+  const int64_t rows = tokens * (heads / kv_heads);
+  if (rows <= kFew * batch || padded_dim(dim) > kManyDim) return kFew;
+  return positions <= 2048 && (rows / kFew + batch) * kv_heads <= kResident / 2 ? kFew : kMany;
 }
 
 // Tiles of a call whose sequences may lie anywhere: sequence b's begin at slot
@@ -42,35 +56,41 @@ inline int64_t tiles(int64_t tokens, int64_t batch, int64_t group, int rows) {
 // of 512 positions 11.6 us in parts, 9.5 whole; of 1024 11.7 / 14.0, of 8192 13.3 / 83.
 // 64 ragged sequences of up to 16384 390 / 493, 512 tokens over 8192 positions 93 /
 // 194.  A run of at least 8 small steps: 4 / 8 / 16 of them 15.1 / 13.3 / 14.2 us at
-// 8192 positions (10.5 / 11.7 / 14.0 at 1024), and of at least 16 large ones: 8 / 16 /
-// 32 of them 51 / 42 / 60 us, 256 tokens over 4096 positions.
-// More large tiles than there are units go whole, a prompt's later ones, which see
-// more, first: a prompt of 8192 549 us whole, 785 in parts, of 4096 160 / 222, 4 chunks
+// 8192 positions (10.5 / 11.7 / 14.0 at 1024).  Of large ones at least 16: 8 / 16 / 32
+// of them 51 / 42 / 60 us, 256 tokens over 4096 positions; but where that leaves units
+// idle, one a CU with as few as 4: 13 tokens each of 9 sequences over 10818 positions
+// 372 -> 278, 10 each of 9 over 1024 39 -> 18.
+// More tiles than there are units, of sequences with several, go whole, a prompt's
+// later ones, which see more, first: a prompt of 8192 549 us whole, 785 in parts, of 4096 160 / 222, 4 chunks
 // of 1024 over 8192 505 / 521.
 struct Parts {
   int units, least_steps;
 };
-inline Parts parts(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
-                   int64_t positions) {
+inline Parts parts(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int dim,
+                   int64_t positions, int64_t window) {
   const int64_t group = heads / kv_heads;
-  const int rows = tile_rows(tokens, batch, group);
+  const int rows = tile_rows(tokens, batch, heads, kv_heads, dim, positions);
   const int64_t all = tiles(tokens, batch, group, rows);
   const int keys = rows == kFew ? kFewKeys : kKeys;
-  const int64_t least = rows == kFew ? 8 : 16;
-  const int64_t longest = (positions + keys - 1) / keys;
-  const int64_t units = std::max<int64_t>(1, kResident / kv_heads);
-  if (longest <= 16 || batch > kMaxBatch || all * longest >= (int64_t{1} << 31) ||
-      kv_heads > kResident ||  // places lie within 32-bit offsets
-      (rows == kMany && all > units))
+  // Whether there are parts does not depend on a window but where it makes them few.
+  int64_t longest = (positions + keys - 1) / keys;
+  const bool countable = all * longest < (int64_t{1} << 31);
+  if (window > 0) longest = std::min(longest, (window + rows + keys - 1) / keys + 1);
+  int64_t units = std::max<int64_t>(1, kResident / kv_heads);
+  if (longest <= (rows == kFew ? 16 : 8) || batch > kMaxBatch || !countable ||
+      kv_heads > kResident ||  // offsets within 32 bits
+      (tokens * group > kFew * batch && all > units))
     return {0, 0};
+  int64_t least = 8;
+  if (rows == kMany) {
+    least = 16;
+    if (all * longest < least * units) {
+      least = 4;
+      units = std::max<int64_t>(1, units / 2);
+    }
+  }
   return {static_cast<int>(std::min(units, (all * longest + least - 1) / least)),
           static_cast<int>(least)};
-}
-
-// Columns that the products take: 80 of 96 instead of 128 were 90 us against 102 (six
-// sequences of up to 500 new tokens), 192 instead of 256 169 against 406.
-inline int padded_dim(int dim) {
-  return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
 }
 
 // Floats that a part of a tile leaves: its rows' outputs, maxima and sums.
@@ -79,9 +99,9 @@ inline int64_t part_floats(int rows, int dim) {
 }
 
 inline size_t workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int dim,
-                        int64_t positions) {
-  const Parts p = parts(tokens, batch, heads, kv_heads, positions);
-  const int rows = tile_rows(tokens, batch, heads / kv_heads);
+                        int64_t positions, int64_t window) {
+  const Parts p = parts(tokens, batch, heads, kv_heads, dim, positions, window);
+  const int rows = tile_rows(tokens, batch, heads, kv_heads, dim, positions);
   return static_cast<size_t>(2 * p.units * kv_heads * part_floats(rows, dim)) * sizeof(float);
 }
 

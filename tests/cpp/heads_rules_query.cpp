@@ -19,18 +19,20 @@ int heads_run_of(int64_t tokens, int64_t all, int widest, int lanes, int most) {
   return heads::run_of(tokens, all, widest, lanes, most);
 }
 int heads_groups_of(int n, int run) { return heads::groups_of(n, run); }
-int attention_tile_rows(int64_t tokens, int64_t batch, int64_t group) {
-  return attention::tile_rows(tokens, batch, group);
+int attention_tile_rows(int64_t tokens, int64_t batch, int64_t n, int64_t kv, int dim,
+                        int64_t positions) {
+  return attention::tile_rows(tokens, batch, n, kv, dim, positions);
 }
 int64_t attention_tiles(int64_t tokens, int64_t batch, int64_t group, int rows) {
   return attention::tiles(tokens, batch, group, rows);
 }
-int attention_units(int64_t tokens, int64_t batch, int64_t n, int64_t kv, int64_t positions) {
-  return attention::parts(tokens, batch, n, kv, positions).units;
+int attention_units(int64_t tokens, int64_t batch, int64_t n, int64_t kv, int dim,
+                    int64_t positions, int64_t window) {
+  return attention::parts(tokens, batch, n, kv, dim, positions, window).units;
 }
 size_t attention_workspace(int64_t tokens, int64_t batch, int64_t n, int64_t kv, int dim,
-                           int64_t positions) {
-  return attention::workspace(tokens, batch, n, kv, dim, positions);
+                           int64_t positions, int64_t window) {
+  return attention::workspace(tokens, batch, n, kv, dim, positions, window);
 }
 int attention_padded_dim(int dim) { return attention::padded_dim(dim); }
 uint32_t attention_divide(uint32_t n, uint32_t d) {

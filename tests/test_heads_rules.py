@@ -29,9 +29,9 @@ def rules(tmp_path_factory):
             ("heads_apart", [place, place], INT), ("heads_apart_within", [place], INT),
             ("heads_same", [place, place], INT), ("heads_run_of", [I64, I64, INT, INT, INT], INT),
             ("heads_groups_of", [INT, INT], INT),
-            ("attention_tile_rows", [I64] * 3, INT), ("attention_tiles", [I64] * 3 + [INT], I64),
-            ("attention_units", [I64] * 5, INT),
-            ("attention_workspace", [I64] * 4 + [INT, I64], SIZE),
+            ("attention_tile_rows", [I64] * 4 + [INT, I64], INT), ("attention_tiles", [I64] * 3 + [INT], I64),
+            ("attention_units", [I64] * 4 + [INT, I64, I64], INT),
+            ("attention_workspace", [I64] * 4 + [INT, I64, I64], SIZE),
             ("attention_padded_dim", [INT], INT),
             ("attention_divide", [ctypes.c_uint32] * 2, ctypes.c_uint32)):
         fn = getattr(lib, name)
@@ -103,7 +103,7 @@ def test_tiles_hold_every_sequence(rules):
                    for _ in range(batch)]
         lead, tail = rng.randrange(40), rng.randrange(40)
         tokens = lead + sum(lengths) + tail
-        rows = rules.attention_tile_rows(tokens, batch, group)
+        rows = rules.attention_tile_rows(tokens, batch, group, 1, 128, rng.choice((100, 9000)))
         assert rows in (FEW, MANY)
         at, free = lead, 0
         for b, n in enumerate(lengths):
@@ -114,20 +114,39 @@ def test_tiles_hold_every_sequence(rules):
         assert free <= rules.attention_tiles(tokens, batch, group, rows)
 
 
+def test_tile_rows(rules):
+    rows = rules.attention_tile_rows
+    assert rows(64, 64, 32, 8, 128, 8192) == rows(8, 1, 32, 8, 128, 8192) == FEW
+    assert rows(9, 1, 32, 8, 128, 8192) == MANY  # 36 rows over many positions
+    assert rows(9, 1, 32, 8, 128, 2048) == FEW and rows(9, 1, 32, 8, 128, 2049) == MANY
+    assert rows(248, 1, 32, 8, 128, 2048) == FEW and rows(256, 1, 32, 8, 128, 2048) == MANY
+    assert rows(8192, 1, 16, 4, 200, 8192) == FEW and rows(8192, 1, 16, 4, 192, 8192) == MANY
+
+
 def test_parts(rules):
     # Short sequences, long prompts and too many sequences to count through: whole tiles.
-    assert rules.attention_units(1, 1, 32, 8, 256) == 0
-    assert rules.attention_units(8192, 1, 32, 8, 8192) == 0
-    assert rules.attention_units(2000, 2000, 32, 8, 8192) == 0
-    assert rules.attention_units(1, 1, 32, 8, 8192) == 32  # 1 tile of 256 steps, 8 each
+    units, workspace = rules.attention_units, rules.attention_workspace
+    assert units(1, 1, 32, 8, 128, 512, 0) == 0
+    assert units(8192, 1, 32, 8, 128, 8192, 0) == units(8192, 1, 32, 8, 256, 8192, 0) == 0
+    assert units(2000, 2000, 32, 8, 128, 8192, 0) == 0
+    assert units(1, 1, 32, 8, 128, 8192, 0) == 32  # 1 tile of 256 steps, 8 each
+    assert units(1, 1, 32, 8, 128, 8192, 100) == 0  # 6 steps
+    assert units(512, 1, 32, 8, 128, 8192, 0) == 64  # 17 tiles of 128 steps
+    assert units(40, 1, 32, 8, 128, 8192, 0) == 32  # 2 of 128, one unit a CU
+    assert units(40, 4, 8, 8, 128, 3000, 0) == 59  # 5 small tiles of 94
+    assert units(33, 1, 8, 8, 128, 3000, 0) == 12  # 1 large one of 47, 4 each
     for heads, kv in ((32, 8), (8, 1), (14, 2), (64, 64), (1024, 1024), (600, 600)):
-        for tokens, batch in ((1, 1), (64, 64), (512, 1), (300, 7)):
-            for positions in (1, 300, 8192, 1 << 20, 1 << 30):
-                units = rules.attention_units(tokens, batch, heads, kv, positions)
-                assert units * kv <= max(RESIDENT, kv)
-                size = rules.attention_workspace(tokens, batch, heads, kv, 256, positions)
-                # Two places a unit, offsets within 32 bits.
-                assert (size == 0) == (units == 0) and size < 1 << 31
+        for tokens, batch in ((1, 1), (64, 64), (512, 1), (300, 7), (40, 1)):
+            for positions in (1, 300, 2048, 8192, 1 << 20, 1 << 30):
+                for dim in (128, 256):
+                    n = units(tokens, batch, heads, kv, dim, positions, 0)
+                    assert n * kv <= max(RESIDENT, kv)
+                    size = workspace(tokens, batch, heads, kv, dim, positions, 0)
+                    # Two places a unit, offsets within 32 bits.
+                    assert (size == 0) == (n == 0) and size < 1 << 31
+                    # What is asked for without a window serves with any.
+                    for window in (1, 100, 1000, 5000, 1 << 30):
+                        assert size >= workspace(tokens, batch, heads, kv, dim, positions, window)
 
 
 def test_divisors(rules):
@@ -149,7 +168,7 @@ def test_padded_dims(rules):
 def test_workspace_bytes_of_the_library(rules, lib):
     for tokens, batch, heads, kv, dim, positions in (
             (1, 1, 32, 8, 128, 8192), (64, 64, 32, 8, 80, 16384), (512, 1, 8, 8, 200, 9000)):
-        body = rules.attention_workspace(tokens, batch, heads, kv, dim, positions)
+        body = rules.attention_workspace(tokens, batch, heads, kv, dim, positions, 0)
         assert hip_lib.paged_attention_workspace_bytes(
             tokens, batch, heads, kv, dim, positions) == body + (5 << 20) + 256
     assert hip_lib.paged_attention_workspace_bytes(8192, 1, 32, 8, 128, 8192) == 0
