@@ -1329,21 +1329,22 @@ int launch(const Args& a, int rows, hipStream_t stream) {
     if (near && a.page_size % 8 == 0) return parts(std::integral_constant<int, 8>{});
     return parts(std::integral_constant<int, 0>{});
   };
-  if (rows == kFew)
-    return choose([&](auto piece, auto parts) {
-      constexpr size_t kBytes = kFewBytes<D> + 2 * sizeof(float[kNW][kFew]);
-      return launch_with<paged_attention_few_kernel<D, decltype(piece)::value,
-                                                    decltype(parts)::value>>(
-          a, kBytes, stream, "paged_attention_few_kernel");
-    });
-  if constexpr (D <= attention::kManyDim)
-    return choose([&](auto piece, auto parts) {
-      constexpr size_t kBytes = size_t{4} * kKeys * Lds<D>::kRowBytes;
-      return launch_with<paged_attention_many_kernel<D, decltype(piece)::value,
-                                                      decltype(parts)::value>>(
-          a, kBytes, stream, "paged_attention_many_kernel");
-    });
-  return set_error(CREDIT_ERR_UNSUPPORTED, "tiles of %d rows with heads of %d", rows, D);
+  const auto few = [&](auto piece, auto parts) {
+    constexpr size_t kBytes = kFewBytes<D> + 2 * sizeof(float[kNW][kFew]);
+    return launch_with<
+        paged_attention_few_kernel<D, decltype(piece)::value, decltype(parts)::value>>(
+        a, kBytes, stream, "paged_attention_few_kernel");
+  };
+  if constexpr (D <= attention::kManyDim) {
+    if (rows == kMany)
+      return choose([&](auto piece, auto parts) {
+        constexpr size_t kBytes = size_t{4} * kKeys * Lds<D>::kRowBytes;
+        return launch_with<
+            paged_attention_many_kernel<D, decltype(piece)::value, decltype(parts)::value>>(
+            a, kBytes, stream, "paged_attention_many_kernel");
+      });
+  }
+  return choose(few);
 }
 
 int check_vectors(const Place& p, const char* name) {

@@ -17,10 +17,14 @@ def parted(args) -> bool:
     return workspace(args)[1] > 0
 
 
+# New tokens and positions: a tile a sequence, several small ones, large ones.
+SHAPES = {"few": ([1, 1, 2], [700, 90, 1500]), "several": ([60, 1, 130], [1500, 30, 700]),
+          "large": ([60, 1, 130], [2300, 30, 2100])}
+
+
 @pytest.mark.parametrize("page", [16, 8, 12])
 @pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
-@pytest.mark.parametrize("shape", [([1, 1, 2], [700, 90, 1500]), ([60, 1, 130], [1500, 30, 700])],
-                         ids=["few", "many"])
+@pytest.mark.parametrize("shape", SHAPES.values(), ids=SHAPES)
 def test_widths_and_pages(gpu, shape, dim, page):
     args = make(*shape, 2, 1, dim, page, seed=dim + page)
     assert parted(args)
@@ -31,8 +35,22 @@ def test_widths_and_pages(gpu, shape, dim, page):
     check(short)
 
 
+@pytest.mark.parametrize("page", [64, 8, 5])
+@pytest.mark.parametrize("dim", [64, 96, 128, 192])
+def test_large_tiles_whole(gpu, dim, page):
+    """Of more key heads than small tiles would have a CU each, and few steps; of more
+    rows than there are units."""
+    args = make([300, 200, 1, 0], [400, 510, 30, 9], 16, 16, dim, page, seed=dim + page)
+    assert not parted(args)
+    check(args, window=0 if page == 8 else 77)
+    args = make([700, 700], [700, 800], 64, 64, dim, page) if dim == 64 else args
+    assert not parted(args)
+    check(args)
+
+
 @pytest.mark.parametrize("dim", [8, 72, 80, 104, 136, 200])
-@pytest.mark.parametrize("shape", [([2], [900]), ([90], [1300])], ids=["few", "many"])
+@pytest.mark.parametrize("shape", [([2], [900]), ([90], [1300]), ([90], [2200])],
+                         ids=["few", "several", "large"])
 def test_dims_between_the_widths(gpu, shape, dim):
     args = make(*shape, 3, 1, dim, 16, seed=dim)
     assert parted(args)
@@ -78,19 +96,20 @@ def test_many_parts_of_a_tile(gpu, new):
 
 
 @pytest.mark.parametrize("window", [1, 33, 64, 65, 1000, 2 ** 31 - 1])
-@pytest.mark.parametrize("shape", [([1, 3], [3000, 800]), ([70, 200], [2000, 900])],
-                         ids=["few", "many"])
+@pytest.mark.parametrize("shape", [([1, 3], [3000, 800]), ([70, 200], [2000, 900]),
+                                   ([70, 200], [2400, 900])], ids=["few", "several", "large"])
 def test_windows(gpu, shape, window):
     args = make(*shape, 7, 1, 64, 16)
     assert parted(args)
     check(args, window)
 
 
+@pytest.mark.parametrize("longest", [2000, 2500])  # small tiles, large ones
 @pytest.mark.parametrize("value", [math.nan, math.inf])
-def test_hidden_values_in_parts(gpu, value):
-    """Garbage behind the last position and in front of a window, where a step is
-    shared by rows that see it and rows that do not."""
-    args = make([3, 40], [2000, 1500], 4, 2, 128, 16)
+def test_hidden_values_in_parts(gpu, value, longest):
+    """Garbage in front of a window, where a step is shared by rows that see it and
+    rows that do not."""
+    args = make([3, 40], [longest, 1500], 4, 2, 128, 16)
     want = call(args, 100)
     table, page = args[3], 16
     for b, js in ((0, (5, 1000, 1896)), (1, (0, 1359))):
