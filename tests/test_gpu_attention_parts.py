@@ -43,7 +43,7 @@ def test_large_tiles_whole(gpu, dim, page):
     args = make([300, 200, 1, 0], [400, 510, 30, 9], 16, 16, dim, page, seed=dim + page)
     assert not parted(args)
     check(args, window=0 if page == 8 else 77)
-    args = make([700, 700], [700, 800], 64, 64, dim, page) if dim == 64 else args
+    args = make([60] * 8, [600] + [100] * 7, 64, 64, dim, page, seed=dim)
     assert not parted(args)
     check(args)
 
