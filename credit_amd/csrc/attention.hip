@@ -1435,7 +1435,10 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
   a.positions = static_cast<int>(pages_cols * k_cache->page_size);
   a.by_page = attention::divisor(a.page_size);
   a.by_group = attention::divisor(a.group);
-  a.window = window;
+  // A window of at least the positions that there may be hides none of them.  Those
+  // left are below 2^30, as are rows: a border of theirs lies within 32 bits, also
+  // where a sequence has fewer positions than new tokens.
+  a.window = window = window < a.positions ? window : 0;
   a.scale = scale;
   a.scale_log2 = static_cast<float>(1.44269504088896340736 * static_cast<double>(scale));
   const int rows =
