@@ -271,16 +271,15 @@ int wide_layernorm_fwd(const uint16_t* x, const uint16_t* gamma, const uint16_t*
                        float eps, bool vec, const credit_cfg* cfg, bool* taken);
 
 // Arguments of the operators on heads, checked (heads.hip): their sizes, a tensor
-// by tokens and heads, an output like its input, a paged cache (the places of its
-// pages and of the slots of one), two tensors that may share no element, and a
-// call without variants.
+// by tokens and heads, an output like its input, a paged cache, two tensors that may
+// share no element, and a call without variants.
 int check_tokens(int64_t tokens, int32_t dim, int32_t max_dim);
 int check_heads(const credit_heads* h, const char* name, int64_t tokens, int dim, size_t elem,
                 heads::Place* place);
 int check_output(const credit_heads* h, const char* name, const credit_heads* in, int64_t tokens,
                  int dim, size_t elem, heads::Place* place);
 int check_cache(const credit_pages* cache, const char* name, int dim, size_t elem,
-                heads::Place* pages, heads::Place* slots);
+                heads::Place* place);
 int check_places_apart(const heads::Place& out, const char* name, const heads::Place& other,
                        const char* other_name);
 int check_only_auto(const credit_cfg* cfg);

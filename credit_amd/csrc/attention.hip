@@ -1348,7 +1348,7 @@ int launch(const Args& a, int rows, hipStream_t stream) {
 }
 
 int check_vectors(const Place& p, const char* name) {
-  if (p.at % 16 == 0 && p.run % 16 == 0 && p.step % 16 == 0) return CREDIT_OK;
+  if (p.at % 16 == 0 && p.run % 16 == 0 && p.step % 16 == 0 && p.lead % 16 == 0) return CREDIT_OK;
   return set_error(CREDIT_ERR_ALIGNMENT, "%s: address and strides are not all multiples of 16 bytes",
                    name);
 }
@@ -1364,11 +1364,11 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
   if (batch < 0 || batch > (1 << 20))
     return set_error(CREDIT_ERR_BAD_SHAPE, "batch %lld outside [0, 2^20]",
                      static_cast<long long>(batch));
-  Place pq, po, kc, vc, kslots, vslots;
+  Place pq, po, kc, vc;
   CREDIT_TRY(check_heads(q, "q", tokens, dim, kElem, &pq));
   CREDIT_TRY(check_output(out, "out", q, tokens, dim, kElem, &po));
-  CREDIT_TRY(check_cache(k_cache, "k_cache", dim, kElem, &kc, &kslots));
-  CREDIT_TRY(check_cache(v_cache, "v_cache", dim, kElem, &vc, &vslots));
+  CREDIT_TRY(check_cache(k_cache, "k_cache", dim, kElem, &kc));
+  CREDIT_TRY(check_cache(v_cache, "v_cache", dim, kElem, &vc));
   if (k_cache->pages != v_cache->pages || k_cache->page_size != v_cache->page_size ||
       k_cache->heads != v_cache->heads)
     return set_error(CREDIT_ERR_BAD_SHAPE, "k_cache and v_cache have different pages");
@@ -1400,9 +1400,7 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
   CREDIT_TRY(check_vectors(pq, "q"));
   CREDIT_TRY(check_vectors(po, "out"));
   CREDIT_TRY(check_vectors(kc, "k_cache"));
-  CREDIT_TRY(check_vectors(kslots, "k_cache"));
   CREDIT_TRY(check_vectors(vc, "v_cache"));
-  CREDIT_TRY(check_vectors(vslots, "v_cache"));
   CREDIT_TRY(check_places_apart(po, "out", pq, "q"));
   CREDIT_TRY(check_places_apart(po, "out", kc, "k_cache"));
   CREDIT_TRY(check_places_apart(po, "out", vc, "v_cache"));

@@ -599,7 +599,7 @@ struct Shape {
 
   void add(const Place& p) {
     addresses |= p.at;
-    strides |= p.run | p.step;
+    strides |= p.run | p.step | p.lead;
   }
   bool serves(int n, size_t elem) const {
     const int border = r->interleaved != 0 ? r->rot : r->rot / 2;
@@ -901,13 +901,12 @@ int norm_rope_bwd(const credit_heads* q, const credit_heads* k, const T* q_weigh
 }
 
 int check_pages(const credit_pages* c, const char* name, const credit_heads* in, int dim,
-                size_t elem, Place* pages, Place* slots) {
+                size_t elem, Place* place) {
   CREDIT_TRY(check_ptr(c, name));
   if (c->heads != in->heads)
     return set_error(CREDIT_ERR_BAD_SHAPE, "%s: %d heads, its input has %d", name, c->heads,
                      in->heads);
-  (void)dim;
-  return check_cache(c, name, dim, elem, pages, slots);
+  return check_cache(c, name, dim, elem, place);
 }
 
 int append(const credit_heads* k, const credit_heads* v, const credit_heads* q,
@@ -922,11 +921,11 @@ int append(const credit_heads* k, const credit_heads* v, const credit_heads* q,
   CREDIT_TRY(check_rotation(rotation, tokens, dim, false, &a.r));
   Shape shape{dim, &a.r};
   const bool queries = q != nullptr || q_out != nullptr;
-  Place pk, pv, pq, po, kc, vc, kslots, vslots;
+  Place pk, pv, pq, po, kc, vc;
   CREDIT_TRY(check_heads(k, "k", tokens, dim, kElem, &pk));
   CREDIT_TRY(check_heads(v, "v", tokens, dim, kElem, &pv));
-  CREDIT_TRY(check_pages(k_cache, "k_cache", k, dim, kElem, &kc, &kslots));
-  CREDIT_TRY(check_pages(v_cache, "v_cache", v, dim, kElem, &vc, &vslots));
+  CREDIT_TRY(check_pages(k_cache, "k_cache", k, dim, kElem, &kc));
+  CREDIT_TRY(check_pages(v_cache, "v_cache", v, dim, kElem, &vc));
   if (queries) {
     CREDIT_TRY(check_heads(q, "q", tokens, dim, kElem, &pq));
     CREDIT_TRY(check_output(q_out, "q_out", q, tokens, dim, kElem, &po));
@@ -972,7 +971,7 @@ int append(const credit_heads* k, const credit_heads* v, const credit_heads* q,
   if (queries) a.side[a.sides++] = side_of<T>(q, q_out, q_weight);
   into(k, k_cache, k_weight, false);
   into(v, v_cache, nullptr, true);
-  for (const Place* p : {&pk, &pv, &pq, &po, &kc, &vc, &kslots, &vslots}) shape.add(*p);
+  for (const Place* p : {&pk, &pv, &pq, &po, &kc, &vc}) shape.add(*p);
   shape.addresses |= reinterpret_cast<uintptr_t>(k_weight) | reinterpret_cast<uintptr_t>(q_weight);
   return launch_forward<T>(a, tokens, shape, cfg_stream(cfg));
 }
@@ -1032,9 +1031,7 @@ int check_only_auto(const credit_cfg* cfg) {
   return CREDIT_OK;
 }
 
-// A cache's two levels: pages of heads, slots of heads.
-int check_cache(const credit_pages* c, const char* name, int dim, size_t elem, Place* pages,
-                Place* slots) {
+int check_cache(const credit_pages* c, const char* name, int dim, size_t elem, Place* place) {
   CREDIT_TRY(check_ptr(c, name));
   if (c->pages < 0 || c->pages > (int64_t{1} << 31) - 1 || c->page_size < 1 ||
       c->page_size > (1 << 20) || c->heads < 1 || c->heads > (1 << 20))
@@ -1050,15 +1047,10 @@ int check_cache(const credit_pages* c, const char* name, int dim, size_t elem, P
   if (c->page_stride < 0 || c->slot_stride < 0 || c->head_stride < 0 ||
       bytes > static_cast<double>(kMaxBytes))
     return set_error(CREDIT_ERR_BAD_SHAPE, "%s: strides negative or too large", name);
-  *slots = Place{reinterpret_cast<uintptr_t>(c->data), c->slot_stride * e, c->head_stride * e,
-                 c->page_size, c->heads, dim * e};
-  if (!heads::apart_within(*slots))
+  *place = Place{reinterpret_cast<uintptr_t>(c->data), c->slot_stride * e, c->head_stride * e,
+                 c->page_size, c->heads, dim * e, c->page_stride * e, c->pages};
+  if (!heads::apart_within(*place))
     return set_error(CREDIT_ERR_BAD_SHAPE, "%s: its slots overlap each other", name);
-  // A page as one run of its bytes; pages may be interleaved with another cache's.
-  *pages = Place{reinterpret_cast<uintptr_t>(c->data), c->page_stride * e, slots->span(), c->pages,
-                 1, slots->span()};
-  if (c->pages > 1 && pages->run < pages->width)
-    return set_error(CREDIT_ERR_BAD_SHAPE, "%s: its pages overlap each other", name);
   return CREDIT_OK;
 }
 size_t qk_norm_rope_bwd_workspace(int64_t dim) {

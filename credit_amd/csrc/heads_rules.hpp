@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <iterator>
 
 namespace credit {
 namespace heads {
@@ -14,43 +15,65 @@ namespace heads {
 constexpr int kMaxDim = 512;
 
 // Vectors that are `step` bytes apart, `count` of them in each of `outer` runs
-// that are `run` bytes apart, `width` bytes each.
+// that are `run` bytes apart, `width` bytes each; a cache's pages: `leads` of these,
+// `lead` bytes apart.  Any of the distances may be the largest.
 struct Place {
   uintptr_t at = 0;
   int64_t run = 0, step = 0;
   int64_t outer = 0, count = 0, width = 0;
+  int64_t lead = 0, leads = 1;
 
-  bool empty() const { return outer == 0 || count == 0 || width == 0; }
+  bool empty() const { return outer == 0 || count == 0 || width == 0 || leads == 0; }
   // Bytes from the first to behind the last.
-  int64_t span() const { return empty() ? 0 : (outer - 1) * run + (count - 1) * step + width; }
-  // Of one run.
-  int64_t extent() const { return (count - 1) * step + width; }
+  int64_t span() const {
+    return empty() ? 0 : (leads - 1) * lead + (outer - 1) * run + (count - 1) * step + width;
+  }
+  // Bytes from the first vector's to behind the last one's, counted modulo `distance`,
+  // of which the levels at its multiples take no part.
+  int64_t extent(int64_t distance) const {
+    const auto own = [&](int64_t stride, int64_t n) {
+      return n == 1 || stride % distance == 0 ? 0 : (n - 1) * stride;
+    };
+    return own(lead, leads) + own(run, outer) + own(step, count) + width;
+  }
 };
 
-// Whether no byte of a tensor belongs to two of its vectors.
+// Whether no byte of a tensor belongs to two of its vectors: each level's distance
+// holds all that lies within it.
 inline bool apart_within(const Place& p) {
   if (p.empty()) return true;
-  const int64_t step = p.count == 1 ? p.width : p.step, run = p.outer == 1 ? p.span() : p.run;
-  if (step >= p.width && run >= (p.count - 1) * step + p.width) return true;
-  return run >= p.width && step >= (p.outer - 1) * run + p.width;
+  struct Level {
+    int64_t stride, n;
+  } levels[] = {{p.lead, p.leads}, {p.run, p.outer}, {p.step, p.count}};
+  std::sort(std::begin(levels), std::end(levels),
+            [](const Level& a, const Level& b) { return a.stride < b.stride; });
+  int64_t within = p.width;
+  for (const Level& l : levels) {
+    if (l.n == 1) continue;
+    if (l.stride < within) return false;
+    within += (l.n - 1) * l.stride;
+  }
+  return true;
 }
 
-// Whether two tensors share no byte, as far as can be told: spans apart, or
-// vectors or whole runs of one distance that lie between each other's (heads or
-// column ranges of one buffer).
-inline bool between(uintptr_t a, int64_t wa, uintptr_t b, int64_t wb, int64_t distance) {
-  if (distance <= 0 || wa > distance || wb > distance) return false;
-  const int64_t d = b >= a ? static_cast<int64_t>(b - a) : -static_cast<int64_t>(a - b);
+// Whether two tensors share no byte, as far as can be told: spans apart, or all of
+// each one's bytes between the other's modulo one of their distances (heads, slots,
+// pages or column ranges of one buffer).
+inline bool between(const Place& a, const Place& b, int64_t distance) {
+  if (distance <= 0) return false;
+  const int64_t wa = a.extent(distance), wb = b.extent(distance);
+  if (wa > distance || wb > distance) return false;
+  const int64_t d = b.at >= a.at ? static_cast<int64_t>(b.at - a.at)
+                                 : -static_cast<int64_t>(a.at - b.at);
   const int64_t after = ((d % distance) + distance) % distance;
   return after >= wa && after + wb <= distance;
 }
 inline bool apart(const Place& a, const Place& b) {
   if (a.empty() || b.empty()) return true;
   if (a.at >= b.at + b.span() || b.at >= a.at + a.span()) return true;
-  if (a.run == b.run && between(a.at, a.extent(), b.at, b.extent(), a.run)) return true;
-  const auto whole = [](const Place& p) { return p.outer == 1 || p.run % p.step == 0; };
-  return a.step == b.step && a.step > 0 && whole(a) && whole(b) &&
-         between(a.at, a.width, b.at, b.width, a.step);
+  for (const int64_t distance : {a.lead, a.run, a.step, b.lead, b.run, b.step})
+    if (between(a, b, distance)) return true;
+  return false;
 }
 
 inline bool same(const Place& a, const Place& b) {

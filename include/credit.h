@@ -446,7 +446,9 @@ typedef struct credit_rotation {
 } credit_rotation;
 
 /* A paged cache of keys or values: head h of slot s of page p at
- * data + p page_stride + s slot_stride + h head_stride (elements). */
+ * data + p page_stride + s slot_stride + h head_stride (elements), any of the
+ * strides the largest; keys and values may lie in one buffer, by pages, slots or
+ * heads in turn. */
 typedef struct credit_pages {
   void* data;
   int64_t page_stride;
