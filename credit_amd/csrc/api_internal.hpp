@@ -7,6 +7,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "../../include/credit.h"
 #include "heads_rules.hpp"
 #include "split_plan.hpp"
@@ -282,6 +284,21 @@ int check_cache(const credit_pages* cache, const char* name, int dim, size_t ele
                 heads::Place* place);
 int check_places_apart(const heads::Place& out, const char* name, const heads::Place& other,
                        const char* other_name);
+// Outputs that may share no element with each other or with any of the others.
+struct NamedPlace {
+  heads::Place place;
+  const char* name;
+};
+int check_outputs_apart(std::initializer_list<NamedPlace> outs,
+                        std::initializer_list<NamedPlace> others);
+// A contiguous tensor of n elements of `elem` bytes; NULL: none.
+inline heads::Place flat_place(const void* p, int64_t n, size_t elem) {
+  heads::Place place;
+  place.at = reinterpret_cast<uintptr_t>(p);
+  place.outer = place.count = 1;
+  place.width = p == nullptr ? 0 : n * static_cast<int64_t>(elem);
+  return place;
+}
 int check_only_auto(const credit_cfg* cfg);
 
 // CU count of the current device, or 256 (MI355X) when none is visible.

@@ -1404,6 +1404,15 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
   CREDIT_TRY(check_places_apart(po, "out", pq, "q"));
   CREDIT_TRY(check_places_apart(po, "out", kc, "k_cache"));
   CREDIT_TRY(check_places_apart(po, "out", vc, "v_cache"));
+  const NamedPlace table{Place{reinterpret_cast<uintptr_t>(pages), pages_ld * 4, 0, batch, 1,
+                               pages_cols * 4},
+                         "pages"};
+  const NamedPlace starts{flat_place(q_start, batch + 1, 4), "q_start"};
+  const NamedPlace lengths{flat_place(kv_len, batch, 4), "kv_len"};
+  CREDIT_TRY(check_outputs_apart({{po, "out"}}, {table, starts, lengths}));
+  CREDIT_TRY(check_outputs_apart(
+      {{flat_place(lse, tokens * q->heads, sizeof(float)), "lse"}},
+      {{pq, "q"}, {po, "out"}, {kc, "k_cache"}, {vc, "v_cache"}, table, starts, lengths}));
   Args a{};
   a.q = static_cast<const uint16_t*>(q->data);
   a.q_token = q->token_stride;

@@ -729,9 +729,12 @@ Side<T> side_of(const credit_heads* in, const credit_heads* out, const T* w) {
   s.heads = in->heads;
   return s;
 }
-Place weight_place(const void* w, int dim, size_t elem) {
-  return Place{reinterpret_cast<uintptr_t>(w), 0, 0, 1, 1,
-               static_cast<int64_t>(dim) * static_cast<int64_t>(elem)};
+// The small inputs of a call's rotation (none: empty).
+NamedPlace positions_of(const Rotation& r, int64_t tokens) {
+  return {flat_place(r.positions, tokens, sizeof(int64_t)), "positions"};
+}
+NamedPlace frequencies_of(const Rotation& r) {
+  return {flat_place(r.inv_freq, r.rot / 2, sizeof(float)), "inv_freq"};
 }
 
 // Both forwards without a cache; no weights: the rotation alone.
@@ -771,6 +774,16 @@ int rotate(const credit_heads* q, const credit_heads* k, const T* q_weight, cons
     CREDIT_TRY(check_places_apart(out[1], "k_out", in[0], "q"));
     CREDIT_TRY(check_places_apart(out[0], "q_out", out[1], "k_out"));
   }
+  const NamedPlace wq{flat_place(q_weight, dim, kElem), "q_weight"};
+  const NamedPlace wk{flat_place(k_weight, dim, kElem), "k_weight"};
+  const NamedPlace pos = positions_of(a.r, tokens), freq = frequencies_of(a.r);
+  CREDIT_TRY(check_outputs_apart({{out[0], "q_out"}}, {wq, wk, pos, freq}));
+  CREDIT_TRY(check_outputs_apart({{out[1], "k_out"}}, {wq, wk, pos, freq}));
+  if (rstd != nullptr)
+    CREDIT_TRY(check_outputs_apart(
+        {{flat_place(rstd, tokens * (static_cast<int64_t>(q->heads) + k->heads), sizeof(float)),
+          "rstd"}},
+        {{in[0], "q"}, {in[1], "k"}, {out[0], "q_out"}, {out[1], "k_out"}, wq, wk, pos, freq}));
   a.sides = keys ? 2 : 1;
   a.dim = dim;
   a.eps = eps;
@@ -838,6 +851,18 @@ int norm_rope_bwd(const credit_heads* q, const credit_heads* k, const T* q_weigh
     CREDIT_TRY(check_places_apart(pd[i], kNames[2][i], py[1 - i], kNames[1][1 - i]));
   }
   if (tokens > 0) CREDIT_TRY(check_places_apart(pd[0], "dq", pd[1], "dk"));
+  const NamedPlace wq{flat_place(q_weight, dim, kElem), "q_weight"};
+  const NamedPlace wk{flat_place(k_weight, dim, kElem), "k_weight"};
+  const NamedPlace pos = positions_of(a.r, tokens), freq = frequencies_of(a.r);
+  const NamedPlace norms{
+      flat_place(rstd, tokens * (static_cast<int64_t>(q->heads) + k->heads), sizeof(float)),
+      "rstd"};
+  CREDIT_TRY(check_outputs_apart({{pd[0], "dq"}, {pd[1], "dk"}}, {wq, wk, pos, freq, norms}));
+  CREDIT_TRY(check_outputs_apart({{flat_place(dq_weight, dim, sizeof(float)), "dq_weight"},
+                                  {flat_place(dk_weight, dim, sizeof(float)), "dk_weight"}},
+                                 {{px[0], "q"}, {px[1], "k"}, {py[0], "dq_out"},
+                                  {py[1], "dk_out"}, {pd[0], "dq"}, {pd[1], "dk"}, wq, wk, pos,
+                                  freq, norms}));
   hipStream_t stream = cfg_stream(cfg);
   if ((cfg == nullptr || cfg->workspace == nullptr) && !keeps_scratch(stream))
     return set_error(CREDIT_ERR_WORKSPACE,
@@ -956,6 +981,11 @@ int append(const credit_heads* k, const credit_heads* v, const credit_heads* q,
     CREDIT_TRY(check_places_apart(po, "q_out", pk, "k"));
     CREDIT_TRY(check_places_apart(po, "q_out", pv, "v"));
   }
+  CREDIT_TRY(check_outputs_apart({{kc, "k_cache"}, {vc, "v_cache"}, {po, "q_out"}},
+                                 {{flat_place(k_weight, dim, kElem), "k_weight"},
+                                  {flat_place(q_weight, dim, kElem), "q_weight"},
+                                  positions_of(a.r, tokens), frequencies_of(a.r),
+                                  {flat_place(slots, tokens, sizeof(int64_t)), "slots"}}));
   a.dim = dim;
   a.eps = eps;
   const auto into = [&](const credit_heads* in, const credit_pages* c, const T* w, bool plain) {
@@ -1015,6 +1045,16 @@ int check_output(const credit_heads* h, const char* name, const credit_heads* in
 int check_places_apart(const Place& out, const char* name, const Place& other, const char* other_name) {
   if (heads::apart(out, other)) return CREDIT_OK;
   return set_error(CREDIT_ERR_BAD_CONFIG, "%s overlaps %s", name, other_name);
+}
+int check_outputs_apart(std::initializer_list<NamedPlace> outs,
+                        std::initializer_list<NamedPlace> others) {
+  for (const NamedPlace* out = outs.begin(); out != outs.end(); ++out) {
+    for (const NamedPlace* next = out + 1; next != outs.end(); ++next)
+      CREDIT_TRY(check_places_apart(out->place, out->name, next->place, next->name));
+    for (const NamedPlace& other : others)
+      CREDIT_TRY(check_places_apart(out->place, out->name, other.place, other.name));
+  }
+  return CREDIT_OK;
 }
 int check_tokens(int64_t tokens, int32_t dim, int32_t max_dim) {
   if (tokens < 0 || tokens > (int64_t{1} << 31) - 1)

@@ -494,6 +494,7 @@ int credit_qk_norm_rope_fwd_bf16(const credit_heads* q, const credit_heads* k,
  *   dq = r (d w - n mean(d w n)),  dq_weight [dim] = sum of d n over all tokens
  * and heads (fp32, in an order that is the same from call to call), and the same
  * for the keys.  dq may be dq_out or q, dk dk_out or k (same data and strides).
+ * dq_weight and dk_weight are arrays of their own, as rstd and lse are.
  * credit_workspace_bytes(CREDIT_OP_QK_NORM_ROPE_BWD, tokens, dim, ...) gives its
  * workspace; under capture and on hipStreamPerThread cfg->workspace has to be
  * set (CREDIT_ERR_WORKSPACE).  Variants: AUTO. */

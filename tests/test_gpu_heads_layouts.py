@@ -49,3 +49,53 @@ def test_every_order(gpu, order, page):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert all(torch.equal(a, b) for a, b in zip(caches, usual))
     assert (buffer[..., DIM:] == 3).all()
+
+
+def test_tensors_next_to_each_other(gpu):
+    """All tensors of the gradients, of norm and rotation and of an attention one behind
+    the other in one buffer: none overlaps, none is refused, the values are those of
+    tensors of their own."""
+    tokens, qh, kh = 7, 6, 2
+    g = torch.Generator().manual_seed(1)
+    arena, at = torch.zeros(1 << 20, dtype=torch.uint8, device=gpu), 0
+
+    def put(t):
+        nonlocal at
+        n = t.numel() * t.element_size()
+        here = arena[at:at + n].view(t.dtype).view(t.shape)
+        at += n
+        here.copy_(t)
+        return here
+
+    def both(f):
+        own = f(lambda t: t.to(gpu))
+        for a, b in zip(f(put), own):
+            assert torch.equal(a, b)
+
+    xs, dys = ([torch.randn((tokens, h, DIM), generator=g).to(BF16) for h in (qh, kh)]
+               for _ in "xy")
+    ws = [torch.randn(DIM, generator=g).to(BF16) for _ in "qk"]
+    pos, freq = torch.arange(tokens + 1), hip_lib.rope_frequencies(DIM)[0]  # 16-byte units
+    rstd = torch.zeros((tokens, qh + kh))
+
+    def training(at):
+        q, k, wq, wk, p, f, r, *more = (at(t) for t in (
+            *xs, *ws, pos, freq, rstd, *xs, *dys, *xs, *(torch.zeros(DIM) for _ in "qk")))
+        p = p[:tokens]
+        hip_lib.qk_norm_rope_fwd(q, k, wq, wk, p, f, more[0], more[1], r)
+        hip_lib.qk_norm_rope_bwd(q, k, wq, wk, p, f, r, *more[2:])
+        return r, *more
+
+    def serving(at):
+        q, k_cache, v_cache, table, start, lengths, out, lse = (at(t) for t in (
+            xs[0], *(torch.randn((4, 4, kh, DIM), generator=g.manual_seed(2)).to(BF16)
+                     for _ in "kv"),
+            torch.tensor([[3, 1, 2, 0]], dtype=torch.int32),
+            torch.tensor([0, tokens, tokens, tokens], dtype=torch.int32),
+            torch.tensor([14, 0, 0, 0], dtype=torch.int32), torch.zeros_like(xs[0]),
+            torch.zeros((tokens, qh))))
+        hip_lib.paged_attention(q, k_cache, v_cache, table, start[:2], lengths[:1], out, lse)
+        return out, lse
+
+    both(training)
+    both(serving)
