@@ -1080,8 +1080,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                 _heads(out, "out", dt, tokens, dim, dev),
                 None if lse is None else _operand(lse, "lse", torch.float32,
                                                   (tokens, q.shape[1]), dev, "the queries'"),
-                tokens, batch, dim, 1.0 / math.sqrt(dim) if scale is None else scale, window,
-                _cfg_ref(cfg, dev))
+                tokens, batch, dim, 1.0 / math.sqrt(dim) if scale is None else scale,
+                # Beyond 32 bits it stays what it is: no window, or a refused one.
+                max(-1, min(window, 0x7FFFFFFF)), _cfg_ref(cfg, dev))
     if status:
         check(status, fn.__name__)
 

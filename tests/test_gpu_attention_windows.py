@@ -2,6 +2,7 @@
 as there are and of more, where sequences have fewer positions than new tokens."""
 import pytest
 
+from credit_amd import hip_lib
 from tests.heads_rules_lib import FEW, MANY, build, way
 from tests.test_gpu_paged_attention import call, check, make
 
@@ -31,3 +32,15 @@ def test_fewer_positions_than_new_tokens(gpu, rules, which, window):
     if window >= longest:  # hides nothing
         whole, whole_lse = call(args)
         assert (out == whole).all() and (lse == whole_lse).all()
+
+
+def test_windows_beyond_32_bits(gpu):
+    """They are none, or negative; their low 32 bits say nothing."""
+    args = make([3, 20], [50, 80], 4, 2, 64, 16)
+    want, want_lse = call(args)
+    for window in (2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 70 + 5):
+        out, lse = call(args, window)
+        assert (out == want).all() and (lse == want_lse).all()
+    for window in (-1, -2 ** 31 - 1, -2 ** 32 + 5):
+        with pytest.raises(hip_lib.CreditError, match="window"):
+            call(args, window)
