@@ -1347,6 +1347,10 @@ int launch(const Args& a, int rows, hipStream_t stream) {
   return choose(few);
 }
 
+// Largest calls: rows are tokens times query heads, positions those of a row of pages.
+constexpr int64_t kMaxRows = int64_t{1} << 30, kMaxPositions = int64_t{1} << 30;
+constexpr int64_t kMaxSequences = int64_t{1} << 20;
+
 int check_vectors(const Place& p, const char* name) {
   if (p.at % 16 == 0 && p.run % 16 == 0 && p.step % 16 == 0 && p.lead % 16 == 0) return CREDIT_OK;
   return set_error(CREDIT_ERR_ALIGNMENT, "%s: address and strides are not all multiples of 16 bytes",
@@ -1361,7 +1365,7 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
   CREDIT_TRY(check_tokens(tokens, dim, attention::kMaxDim));
   if (dim % 8 != 0)
     return set_error(CREDIT_ERR_BAD_SHAPE, "dim %d is not a multiple of 8", dim);
-  if (batch < 0 || batch > (1 << 20))
+  if (batch < 0 || batch > kMaxSequences)
     return set_error(CREDIT_ERR_BAD_SHAPE, "batch %lld outside [0, 2^20]",
                      static_cast<long long>(batch));
   Place pq, po, kc, vc;
@@ -1376,12 +1380,12 @@ int attend(const credit_heads* q, const credit_pages* k_cache, const credit_page
     return set_error(CREDIT_ERR_BAD_SHAPE, "%d query heads are not a multiple of %d key heads",
                      q->heads, k_cache->heads);
   if (pages_cols < 0 || pages_ld < pages_cols || pages_ld > (int64_t{1} << 40) ||
-      static_cast<double>(pages_cols) * k_cache->page_size > static_cast<double>(1 << 30))
+      static_cast<double>(pages_cols) * k_cache->page_size > static_cast<double>(kMaxPositions))
     return set_error(CREDIT_ERR_BAD_SHAPE,
                      "pages: rows of %lld entries, %lld apart, of %d positions each",
                      static_cast<long long>(pages_cols), static_cast<long long>(pages_ld),
                      k_cache->page_size);
-  if (static_cast<double>(tokens) * q->heads > static_cast<double>(1 << 30))
+  if (static_cast<double>(tokens) * q->heads > static_cast<double>(kMaxRows))
     return set_error(CREDIT_ERR_BAD_SHAPE, "%lld tokens of %d heads are more than 2^30 rows",
                      static_cast<long long>(tokens), q->heads);
   const int64_t sequences = tokens == 0 ? 0 : batch;
@@ -1504,8 +1508,10 @@ int credit_paged_attention_bf16(const credit_heads* q, const credit_pages* k_cac
 
 size_t credit_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int32_t q_heads,
                                               int32_t kv_heads, int32_t dim, int64_t positions) {
-  if (tokens <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 ||
-      dim <= 0 || dim > attention::kMaxDim || positions <= 0)
+  // What the call refuses takes none, and sizes of its range keep the rules in theirs.
+  if (tokens <= 0 || tokens > kMaxRows || batch <= 0 || batch > kMaxSequences || q_heads <= 0 ||
+      kv_heads <= 0 || q_heads % kv_heads != 0 || tokens * q_heads > kMaxRows || dim <= 0 ||
+      dim > attention::kMaxDim || dim % 8 != 0 || positions <= 0 || positions > kMaxPositions)
     return 0;
   const size_t body =
       attention::workspace(tokens, batch, q_heads, kv_heads, dim, positions, 0);

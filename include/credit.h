@@ -562,7 +562,7 @@ int credit_paged_attention_bf16(const credit_heads* q, const credit_pages* k_cac
                                 int64_t tokens, int64_t batch, int32_t dim, float scale,
                                 int32_t window, const credit_cfg* cfg);
 /* Bytes of a cfg->workspace with which the call above takes parts as it does
- * without one (0: it takes none).  Plumbing of this ABI. */
+ * without one (0: it takes none, or refuses these sizes).  Plumbing of this ABI. */
 size_t credit_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int32_t q_heads,
                                               int32_t kv_heads, int32_t dim, int64_t positions);
 
