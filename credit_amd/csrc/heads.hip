@@ -18,6 +18,7 @@
 #include "api_internal.hpp"
 #include "common.hpp"
 #include "heads_rules.hpp"
+#include "workspace_cache.hpp"
 
 namespace credit {
 namespace {
@@ -803,6 +804,26 @@ int rotate(const credit_heads* q, const credit_heads* k, const T* q_weight, cons
 // Workgroups of the gradients' launch at most: four a CU of the largest device.
 constexpr int64_t kMaxGradBlocks = 1024;
 
+// Where they leave their partial rows: the caller's workspace, else a buffer that only
+// they use, one for each (device, stream).  In the library's workspace another thread's
+// call of another operator on the stream, between the two launches, would write over them.
+int partial_rows(const credit_cfg* cfg, int dim, float** rows) {
+  const size_t bytes = qk_norm_rope_bwd_workspace(dim);
+  char* base = nullptr;
+  if (cfg != nullptr && cfg->workspace != nullptr) {
+    CREDIT_TRY(acquire_workspace(cfg, bytes, &base));
+    base = ws_scratch(base);
+  } else {
+    static auto* buffers = new WorkspaceCache<ScratchAlloc>();
+    int device = 0;
+    CREDIT_HIP(hipGetDevice(&device));
+    if (buffers->get(device, cfg_stream(cfg), bytes, &base) != CREDIT_OK)
+      return set_error(CREDIT_ERR_HIP, "no memory for %zu bytes of partial rows", bytes);
+  }
+  *rows = reinterpret_cast<float*>(base);
+  return CREDIT_OK;
+}
+
 template <class T>
 int norm_rope_bwd(const credit_heads* q, const credit_heads* k, const T* q_weight,
                   const T* k_weight, const credit_rotation* rotation, const float* rstd,
@@ -870,8 +891,8 @@ int norm_rope_bwd(const credit_heads* q, const credit_heads* k, const T* q_weigh
   // The two launches of a call stay together when threads share a stream.
   static std::mutex* mu = new std::mutex();
   std::lock_guard<std::mutex> lock(*mu);
-  char* base = nullptr;
-  CREDIT_TRY(acquire_workspace(cfg, qk_norm_rope_bwd_workspace(dim), &base));
+  float* partial = nullptr;
+  CREDIT_TRY(partial_rows(cfg, dim, &partial));
   a.dim = dim;
   a.rstd_token = static_cast<int64_t>(q->heads) + k->heads;
   SumArgs sum{};
@@ -902,7 +923,7 @@ int norm_rope_bwd(const credit_heads* q, const credit_heads* k, const T* q_weigh
       s.units = d.units;
       s.first_block = blocks;
       s.blocks = d.blocks;
-      s.partial = reinterpret_cast<float*>(ws_scratch(base)) + blocks * dim;
+      s.partial = partial + blocks * dim;
       blocks += s.blocks;
       sum.partial[i] = s.partial;
       sum.dw[i] = s.dw;
