@@ -992,10 +992,10 @@ constexpr int kKeys = attention::kKeys;
 // workgroups a CU, so that one's products run under the other's exponentials).  Bound
 // by the matrix units and what stands between their products: a wave's step of heads
 // of 128 is 32 products of 32 x 32 x 16 and the exponentials of 2048 scores.
-// Measured, 32 heads over 8 key heads of 128: a prompt of 8192 550-560 us (990
-// TFLOP/s; a large product alone 1268), of 2048 62; 4 chunks of 1024 tokens over 8192
-// positions 505 (1020), 512 tokens over 8192 in parts 88-93; heads of 64, a prompt of
-// 4096 89 us (774), of 192 (16 heads) 150 (687); chunks of 6 sequences of up to 500 tokens
+// Measured, 32 heads over 8 key heads of 128: a prompt of 8192 550-570 us (960-1000
+// TFLOP/s; a large product alone 1268), of 2048 59-62; 4 chunks of 1024 tokens over 8192
+// positions 505-520 (990-1020), 512 tokens over 8192 in parts 88-93; heads of 64, a prompt
+// of 4096 88 us (780), of 192 (16 heads) 146-150 (690-705); chunks of 6 sequences of up to 500 tokens
 // over 6000 positions, 14 heads of 80 over 2 key heads, pages of 24, a window of 4096
 // 80-88.
 template <int D, int PIECE, bool PARTS>
@@ -1119,12 +1119,13 @@ using attention::kFewKeys;  // positions of a wave's step
 // soon as they are read, the values likewise, so that loads never stop.  Bound by HBM
 // where there are steps enough, else by a chain of latencies: find the work, the first
 // keys, the meeting of the waves and of the parts.  Nothing is read twice: nontemporal.
-// Measured, 32 heads over 8 key heads of 128: one token over 32 positions 6.1 us, 8192
-// 13.3, 131072 98 (5.5 TB/s); 64 sequences of 8192 345-357 us (6.0-6.2 TB/s of the 7.1
-// that reads alone reach), of up to 16384 390 (5.8); one key head, 512 sequences of
+// Measured, 32 heads over 8 key heads of 128: one token over 32 positions 5.3-6.1 us, 8192
+// 13.3-14.7, 131072 94-98 (5.5-5.7 TB/s); 64 sequences of 8192 327-357 us (6.0-6.6 TB/s of
+// the 7.1 that reads alone reach), of up to 16384 355-363 (6.2-6.4); one key head, 512 sequences of
 // 8192 344 (6.2); 128 with heads of 64 402 (5.3).  Prompts with heads of 256, 4096
-// tokens and 16 heads, 344 us (399 TFLOP/s): a wave's keys and outputs leave no registers
-// to read ahead.
+// tokens and 16 heads, 346 us (397 TFLOP/s): 20 to 46 of a wave's registers spill, as the
+// code behind its loop has copies of the outputs and 64 hold queries; and 32 rows share a
+// read of keys and values.
 
 // LDS of a workgroup's steps, where its waves' results meet behind them.
 template <int D>

@@ -30,10 +30,17 @@ inline int padded_dim(int dim) {
 // a CU of its own and the positions are few, as there is not work enough to share; and
 // for the widest heads, of which a large tile's wave has no registers for.  us, small /
 // large, 32 heads over 8 key heads of 128: 8 sequences of 8192 positions with 8 new
-// tokens each (32 rows) 60 / 68, with 16 82 / 72, with 32 128 / 80; 64 sequences with one
-// 355 / 448; one sequence, 40 tokens over 500 positions 10.9 / 26, 64 over 2048 23 / 28,
-// 128 over 8192 55 / 47.  16 heads over 4 of 256: 13 tokens each of 9 sequences over
-// 10818 172 / 278, 2048 tokens over 4096 308 / 426.
+// tokens each (32 rows) 61 / 68, with 16 84 / 74, with 32 124 / 85; 64 sequences with one
+// 327 / 425; one sequence, 40 tokens over 500 positions 10.2 / 26, 64 over 2048 24 / 27,
+// 128 over 8192 59 / 45; against the rule 10 tokens each of 9 sequences over 1024 31 / 26.
+// 16 heads over 4 of 256: 13 tokens each of 9 sequences over 10818 171 / 292, 2048
+// tokens over 4096 244 / 436.
+//
+// Lengths are on the device: `positions` is what a row of the table of pages holds, and
+// the figures here and below are of tables as wide as the longest sequence (in a graph,
+// three sets of inputs in turn).  A wider one is taken for longer sequences: 40 tokens
+// over 500 positions 10.2 us with 512 in a row, 18.5 with 2048, 22 with 8192, 38 with
+// 131072; 500 tokens over 500 26, 23, 38, 38; one over 500 9.2, then 11.1.
 inline int tile_rows(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int dim,
                      int64_t positions) {
   const int64_t rows = tokens * (heads / kv_heads);
@@ -53,16 +60,22 @@ inline int64_t tiles(int64_t tokens, int64_t batch, int64_t group, int rows) {
 // units 0: a workgroup a tile, none in parts.
 //
 // Meeting costs some 4 us, which a tile of up to 16 steps takes by itself: one sequence
-// of 512 positions 11.6 us in parts, 9.5 whole; of 1024 11.7 / 14.0, of 8192 13.3 / 83.
-// 64 ragged sequences of up to 16384 390 / 493, 512 tokens over 8192 positions 93 /
-// 194.  A run of at least 8 small steps: 4 / 8 / 16 of them 15.1 / 13.3 / 14.2 us at
-// 8192 positions (10.5 / 11.7 / 14.0 at 1024).  Of large ones at least 16: 8 / 16 / 32
-// of them 51 / 42 / 60 us, 256 tokens over 4096 positions; but where that leaves units
-// idle, one a CU with as few as 4: 13 tokens each of 9 sequences over 10818 positions
-// 372 -> 278, 10 each of 9 over 1024 39 -> 18.
+// of 512 positions 10.8 us in parts, 8.7 whole; of 1024 10.8 / 13.2, of 8192 14.7 / 102.
+// 64 ragged sequences of up to 16384 357 / 459, 512 tokens over 8192 positions 90 /
+// 197.  A run of at least 8 small steps: 4 / 8 / 16 of them 16.1 / 14.7 / 16.6 us at
+// 8192 positions (9.7 / 10.8 / 13.2 at 1024).  Of large ones at least 16, which counts
+// where a row of pages holds more than the sequences have: 8 / 16 / 32 of them 55 / 61 /
+// 90 us, 100 tokens each of 3 over 3000 positions of 16384; 53 / 52 / 69, 300 each of 4
+// over 1000 of 16384.
+// Where even whole rows of pages would leave units idle with that, one a CU with as few
+// as 4.  us, so / at least 16 / at least 8, one a CU: 40 tokens over 4096 37 / 46 / 32, 16
+// each of 4 over 4096 36 / 49 / 35, 100 over 3000 43 / 45 / 40, 50 each of 3 over 2500
+// with 16 heads over 2 34 / 46 / 33, 128 over 4096 with 32 heads of 64 27 / 31 / 26; where
+// there is more to do it loses, 128 over 8192 48 / 46 / 45, 256 over 4096 42 / 41 / 40, 64
+// over 8192 with 8 heads over 1 68 / 42 / 42.
 // More tiles than there are units, of sequences with several, go whole, a prompt's
-// later ones, which see more, first: a prompt of 8192 549 us whole, 785 in parts, of 4096 160 / 222, 4 chunks
-// of 1024 over 8192 505 / 521.
+// later ones, which see more, first: a prompt of 8192 555 us whole, 795 in parts, of 4096
+// 153 / 210, 4 chunks of 1024 over 8192 516 / 528.
 struct Parts {
   int units, least_steps;
 };

@@ -3,7 +3,7 @@
 // its gradients (credit_qk_norm_rope_*), and the same on the way into a paged
 // cache (credit_paged_append_*).
 //
-// A head is held by a group of lanes (2 to 64 of them), each with two units of N
+// A head is held by a group of lanes (4 to 64 of them), each with two units of N
 // consecutive elements: units p and p + rot/2N of the rotated part where pairs
 // are half of it apart, so that a pair never leaves its lane, else neighbours.
 // The only exchange is the head's sum of squares.  A group's lanes take the sines

@@ -886,8 +886,10 @@ def rope_frequencies(rot: int, base: float = 10000.0, scaling: str | None = None
     interpolated); "ntk" takes the base to base factor^(rot/(rot-2)), which keeps
     the shortest wave and stretches the longest by the factor; "yarn" divides those
     that turn fewer than `low` times in original_length positions, keeps those that
-    turn more than `high` times and blends linearly in between, with a magnitude of
-    1 + ln(factor)/10."""
+    turn more than `high` times and blends linearly in their turns in between, with a
+    magnitude of 1 + ln(factor)/10.  Checkpoints trained with a blend that is linear in
+    the pairs' index, or with borders rounded to pairs, bring frequencies of their own:
+    pass those."""
     if rot < 2 or rot % 2:
         raise ValueError(f"rot must be an even number of at least 2, got {rot}")
     if not (base > 0.0 and factor > 0.0):
@@ -1057,7 +1059,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     [batch] (positions in the cache, the new tokens' among them).  lse [tokens, q
     heads] fp32, where given, gets the log-sums.  scale: 1 / sqrt(dim) unless given.
     window > 0: a token sees the last `window` positions up to its own.  Rows that
-    see nothing get 0 and -inf, tokens of no sequence are left as they are."""
+    see nothing get 0 and -inf, tokens of no sequence are left as they are.  How the
+    work is cut goes by the width of pages: of a table for longer contexts give the
+    columns that the longest sequence needs, pages[:, :n]."""
     if q.dtype is not torch.bfloat16:
         raise TypeError(f"q: expected torch.bfloat16, got {q.dtype}")
     tokens, dim, dev, fn = _heads_call("credit_paged_attention_", q, "q")

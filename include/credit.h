@@ -534,8 +534,9 @@ int credit_paged_append_bf16(const credit_heads* k, const credit_heads* v,
  * positions in the cache, position j in slot j % page_size of page
  * pages[b pages_ld + j / page_size], its new tokens among them as the last: tokens
  * q_start[b] .. q_start[b + 1] - 1 of q (q_start [batch + 1] never falling; the
- * values of a batch where it does are open, its accesses in bounds).  Token i of n new ones sees positions j <= kv_len[b] - n + i, with window
- * > 0 only the last window of those:
+ * values of a batch where it does are open, its accesses in bounds).  Token i of n new
+ * ones sees positions j <= kv_len[b] - n + i, with window > 0 only the last window of
+ * those:
  *   out = sum_j p_j v_j, p = softmax(scale q k_j), lse = ln sum_j e^(scale q k_j)
  * (lse [tokens, q heads] fp32; NULL: not wanted), head h of q with key head
  * h / (q heads / key heads).  A row that sees nothing (kv_len[b] < n), or only
@@ -545,9 +546,13 @@ int credit_paged_append_bf16(const credit_heads* k, const credit_heads* v,
  * cache's pages) become NaN.  kv_len beyond pages_cols page_size counts as that;
  * tokens of no sequence are left as they are.
  * Scores, maxima, sums and outputs are held in fp32, the weights rounded to bf16
- * for their product with v, out once more.  dim: a multiple of 8 up to 256;
+ * for their product with v, out once more.  Weights of up to 2^16 are summed before the
+ * division: values beyond 1e24 may overflow, as products of q and k beyond 1e38 do.  dim: a multiple of 8 up to 256;
  * addresses and strides of q, out and the caches: multiples of 16 bytes
  * (CREDIT_ERR_ALIGNMENT).  out shares nothing with q or the caches.
+ * The size of tiles and the cut into parts go by pages_cols page_size, as lengths are
+ * read on the device alone: no more columns than the longest sequence needs (of a
+ * wider table, its first ones) are faster.
  * Few rows over many positions are cut into parts whose results meet in the
  * workspace, credit_paged_attention_workspace_bytes(tokens, batch, q heads, key
  * heads, dim, pages_cols page_size) bytes; under capture and on
