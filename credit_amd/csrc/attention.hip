@@ -995,9 +995,9 @@ constexpr int kKeys = attention::kKeys;
 // Measured, 32 heads over 8 key heads of 128: a prompt of 8192 550-570 us (960-1000
 // TFLOP/s; a large product alone 1268), of 2048 59-62; 4 chunks of 1024 tokens over 8192
 // positions 505-520 (990-1020), 512 tokens over 8192 in parts 88-93; heads of 64, a prompt
-// of 4096 88 us (780), of 192 (16 heads) 146-150 (690-705); chunks of 6 sequences of up to 500 tokens
-// over 6000 positions, 14 heads of 80 over 2 key heads, pages of 24, a window of 4096
-// 80-88.
+// of 4096 88 us (780), of 192 (16 heads) 146-150 (690-705); chunks of 6 sequences of up
+// to 500 tokens over 6000 positions, 14 heads of 80 over 2 key heads, pages of 24, a window
+// of 4096 80-88.
 template <int D, int PIECE, bool PARTS>
 __device__ __forceinline__ void work_on_many(const Args& a, const Work& w, char* smem) {
   constexpr int kStage = 2 * kKeys * Lds<D>::kRowBytes;
@@ -1121,8 +1121,8 @@ using attention::kFewKeys;  // positions of a wave's step
 // keys, the meeting of the waves and of the parts.  Nothing is read twice: nontemporal.
 // Measured, 32 heads over 8 key heads of 128: one token over 32 positions 5.3-6.1 us, 8192
 // 13.3-14.7, 131072 94-98 (5.5-5.7 TB/s); 64 sequences of 8192 327-357 us (6.0-6.6 TB/s of
-// the 7.1 that reads alone reach), of up to 16384 355-363 (6.2-6.4); one key head, 512 sequences of
-// 8192 344 (6.2); 128 with heads of 64 402 (5.3).  Prompts with heads of 256, 4096
+// the 7.1 that reads alone reach), of up to 16384 355-363 (6.2-6.4); one key head, 512
+// sequences of 8192 344 (6.2); 128 with heads of 64 402 (5.3).  Prompts with heads of 256, 4096
 // tokens and 16 heads, 346 us (397 TFLOP/s): 20 to 46 of a wave's registers spill, as the
 // code behind its loop has copies of the outputs and 64 hold queries; and 32 rows share a
 // read of keys and values.
@@ -1353,7 +1353,7 @@ constexpr int64_t kMaxRows = int64_t{1} << 30, kMaxPositions = int64_t{1} << 30;
 constexpr int64_t kMaxSequences = int64_t{1} << 20;
 
 int check_vectors(const Place& p, const char* name) {
-  if (p.at % 16 == 0 && p.run % 16 == 0 && p.step % 16 == 0 && p.lead % 16 == 0) return CREDIT_OK;
+  if (p.at % 16 == 0 && (p.run | p.step | p.lead) % 16 == 0) return CREDIT_OK;
   return set_error(CREDIT_ERR_ALIGNMENT, "%s: address and strides are not all multiples of 16 bytes",
                    name);
 }

@@ -30,8 +30,8 @@ inline int padded_dim(int dim) {
 // a CU of its own and the positions are few, as there is not work enough to share; and
 // for the widest heads, of which a large tile's wave has no registers for.  us, small /
 // large, 32 heads over 8 key heads of 128: 8 sequences of 8192 positions with 8 new
-// tokens each (32 rows) 61 / 68, with 16 84 / 74, with 32 124 / 85; 64 sequences with one
-// 327 / 425; one sequence, 40 tokens over 500 positions 10.2 / 26, 64 over 2048 24 / 27,
+// tokens each (32 rows) 61 / 68, with 16 84 / 75, with 32 124 / 85; 64 sequences with one
+// 327 / 426; one sequence, 40 tokens over 500 positions 10.2 / 26, 64 over 2048 24 / 27,
 // 128 over 8192 59 / 45; against the rule 10 tokens each of 9 sequences over 1024 31 / 26.
 // 16 heads over 4 of 256: 13 tokens each of 9 sequences over 10818 171 / 292, 2048
 // tokens over 4096 244 / 436.

@@ -547,9 +547,10 @@ int credit_paged_append_bf16(const credit_heads* k, const credit_heads* v,
  * tokens of no sequence are left as they are.
  * Scores, maxima, sums and outputs are held in fp32, the weights rounded to bf16
  * for their product with v, out once more.  Weights of up to 2^16 are summed before the
- * division: values beyond 1e24 may overflow, as products of q and k beyond 1e38 do.  dim: a multiple of 8 up to 256;
- * addresses and strides of q, out and the caches: multiples of 16 bytes
- * (CREDIT_ERR_ALIGNMENT).  out shares nothing with q or the caches.
+ * division: values beyond 1e24 may overflow, as products of q and k beyond 1e38 do.
+ * dim: a multiple of 8 up to 256; addresses and strides of q, out and the caches:
+ * multiples of 16 bytes (CREDIT_ERR_ALIGNMENT).  out and lse share nothing with each
+ * other or with an input.
  * The size of tiles and the cut into parts go by pages_cols page_size, as lengths are
  * read on the device alone: no more columns than the longest sequence needs (of a
  * wider table, its first ones) are faster.
